@@ -1,0 +1,530 @@
+// Attention of one new token per request over a paged cache, which also adds to each cached key's score the weights that it got.
+//
+//   s[h, k] = c(scale q_h . K_k),  lse_h = log(sum_k e^s[h, k] + e^sink_h),  out_h = sum_k e^(s[h, k] - lse_h) V_k
+//   scores[b, g, k] += sum over the query heads h of kv head g of e^(s[h, k] - lse_h)
+//
+// A weight is known when the last key has been seen, so there are two kernels.  The first reads keys and values once, leaves the scores s in a
+// workspace (4 bytes a query head and key, beside 4 D bytes of the key and its value: 6 % more for 4 heads of 128, written and read in L2) and
+// a running maximum, sum and output per part of a request's keys.  The second joins the parts, writes the output and adds
+// the weights.
+//
+// First kernel: rows are pairs (request, kv head); all their tiles of 64 keys, in order, are dealt to the CTAs in equal runs, so that ragged and
+// few long requests keep all SMs as busy as many equal ones.  In a run a warp takes every eighth strip of 16 keys through
+// S^T = K Q^T (m16n8k16: keys are rows, the at most 16 query heads columns), an own running maximum and O^T += V^T P^T; its strips
+// come by asynchronous copies of its own, STAGES of them on their way across the borders of rows, so warps meet only where a row
+// ends.  Weights enter the second product as two 16-bit parts, P = hi + lo: the output is then as exact as its own rounding.
+// Decode is bound by the bytes of the cache; a tcgen05 product (128 keys x 16) would take the scores through tensor memory and
+// barriers between roles for products that are a few percent of the time.
+#include "attention_prompt.cuh"
+
+namespace sdec {
+
+constexpr int TILE = 64, STRIP = 16;
+constexpr int MAX_REQUESTS = 1024;          // of a launch: their first tiles lie in shared memory
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Params {
+  const void* q;
+  const void* cache;
+  const int* block_table;
+  const int* seq_lens;
+  void* out;
+  float* scores;
+  const float* sinks;
+  float* raw;              // [tile of a row][64][G]: scores in powers of two
+  float* part;             // [segment][G][D + 2]: output, maximum, sum
+  int64_t q_stride, out_stride, bt_stride, sc_req, sc_head;
+  int64_t num_blocks;
+  int B, Hkv, G, D, BS, max_rows, ctas, chunks;      // chunks: of at most 16 query heads of a kv head
+  float scale_log2, ku, c2;
+};
+
+VB_DEVICE int rows_of(const Params& p, int b) { return min(max(p.seq_lens[b], 0), p.max_rows); }
+
+// first[b]: tiles of all rows in front of request b, as if each request had one kv head; first[B]: of all
+VB_DEVICE void scan_tiles(const Params& p, int* first, int* warp_sums) {
+  const int n_threads = blockDim.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = n_threads >> 5;
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += n_threads) {
+    const int b = b0 + threadIdx.x;
+    const int mine = b < p.B ? (rows_of(p, b) + TILE - 1) / TILE : 0;
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[w] = x;
+    __syncthreads();
+    int before = base;
+    for (int i = 0; i < nw; ++i) {
+      if (i < w) before += warp_sums[i];
+      base += warp_sums[i];
+    }
+    if (b < p.B) first[b] = before + x - mine;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first[p.B] = base;
+  __syncthreads();
+}
+
+// A row: request, kv head, chunk of query heads; its tiles are [begin, end) of the order of all
+struct Row {
+  int index, b, hc, begin, end;
+};
+VB_DEVICE void row_at(const int* first, int B, int H, int tile, Row& r) {      // the row that has this tile
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] * H <= tile) lo = mid; else hi = mid - 1;
+  }
+  const int n = first[lo + 1] - first[lo];               // > 0: the last request that begins at or in front of the tile
+  r.b = lo;
+  r.hc = (tile - first[lo] * H) / n;
+  r.index = lo * H + r.hc;
+  r.begin = first[lo] * H + r.hc * n;
+  r.end = r.begin + n;
+}
+VB_DEVICE void next_row(const int* first, int H, Row& r) {                     // behind it there is one more
+  if (++r.hc == H) {
+    r.hc = 0;
+    do { ++r.b; } while (first[r.b + 1] == first[r.b]);
+  }
+  r.index = r.b * H + r.hc;
+  r.begin = r.end;
+  r.end = r.begin + first[r.b + 1] - first[r.b];
+}
+
+VB_DEVICE void cp_async16(uint32_t dst, const void* src, bool real) {
+  const int n = real ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+VB_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> VB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+VB_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+VB_DEVICE void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T> VB_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> VB_DEVICE void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> VB_DEVICE void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of 16-bit values, two to a lane, with rows and columns exchanged
+VB_DEVICE uint32_t turn8(uint32_t x) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x)); return r; }
+
+// DP: head size, rounded up to 64, 128 or 256 (what is behind it is zeros in shared memory); NT: groups of eight query heads
+template <int DP_> struct Form {
+  static constexpr int DP = DP_, WARPS = DP == 256 ? 4 : 8, THREADS = WARPS * 32;
+  static constexpr int STRIP_BYTES = STRIP * DP * 2;                       // of keys; values behind them
+  static constexpr int STAGES = DP == 64 ? 6 : 3;
+  static constexpr int RING = WARPS * STAGES * 2 * STRIP_BYTES;
+  static constexpr int REGS = DP / 16 * 4 + 4;                             // of a group of heads: output, maxima, sums
+  static constexpr int SMEM = RING + WARPS / 2 * REGS * 128 + (MAX_REQUESTS + 1 + 32) * 4;
+};
+
+template <typename T, int DP, int NT, bool VT, bool CAP>
+__global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Params p) {
+  using F = Form<DP>;
+  // The reference of a head's weights is its largest score less SHIFT, or up to 8 below that.  fp16 has no values under 2^-24: as multiples of 2^-32 of the
+  // largest weight the tail of a long request is not lost.
+  constexpr float SHIFT = sizeof(T) == 2 && DTypeOf<T>::v == DT_F16 ? 7.f : 0.f;
+  constexpr int WARPS = F::WARPS, STAGES = F::STAGES, KD = DP / 16, CH = DP / 8;           // CH: 16-byte pieces of a key
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* exch = reinterpret_cast<float*>(smem + F::RING);
+  int* first = reinterpret_cast<int*>(smem + F::RING + WARPS / 2 * F::REGS * 128);
+  int* warp_sums = first + MAX_REQUESTS + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
+  scan_tiles(p, first, warp_sums);
+  const int H = p.Hkv * p.chunks;
+  const int total = first[p.B] * H, per = (total + p.ctas - 1) / p.ctas;
+  const int t0 = blockIdx.x * per, t1 = min(t0 + per, total);
+  if (t0 >= t1) return;
+
+  const uint32_t ring = smem_u32(smem) + warp * (STAGES * 2 * F::STRIP_BYTES);
+  const int64_t page = (int64_t)p.BS * p.D;                                // values of a page of one head
+  // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  `ld` is the row of the next strip to fetch.
+  const int s_end = t1 * 4;
+  Row ld;
+  row_at(first, p.B, H, t0, ld);
+  int ld_n = rows_of(p, ld.b), ld_s = t0 * 4 + warp;
+  const int c0 = lane % CH, r0l = lane / CH;                                // CH = 8, 16, 32: a lane's piece of a key and its first key
+  constexpr int RSTEP = CH >= 32 ? 1 : 32 / CH;
+  auto fetch = [&](int stage) {
+    while (ld_s < s_end && ld_s >= ld.end * 4) {
+      next_row(first, H, ld);
+      ld_n = rows_of(p, ld.b);
+    }
+    if (ld_s < s_end) {
+      const int tok = (ld_s - ld.begin * 4) * STRIP;
+      if (tok < ld_n) {
+        int64_t blk = p.block_table[ld.b * p.bt_stride + tok / p.BS];
+        if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;              // (a table may not say that; nothing is read outside the cache)
+        const int off = tok % p.BS, h = ld.hc / p.chunks;
+        const T* k = reinterpret_cast<const T*>(p.cache) + (blk * 2 * p.Hkv + h) * page;
+        const T* v = k + p.Hkv * page;
+        const uint32_t to = ring + stage * (2 * F::STRIP_BYTES);
+        const bool real = c0 * 8 < p.D;
+        const T* src = k + (int64_t)off * p.D + (real ? c0 * 8 : 0);
+#pragma unroll
+        for (int i = 0; i < STRIP / RSTEP; ++i) {
+          const int r = r0l + i * RSTEP;
+          cp_async16(to + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), src + (int64_t)r * p.D, real);
+        }
+        if constexpr (VT) {                                                // values stored [dim][token of the page]
+          const int half = lane & 1, d0 = lane >> 1;
+          const T* sv = v + off + half * 8;
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {
+            const int d = d0 + i * 16;
+            cp_async16(to + F::STRIP_BYTES + d * 32 + ((half ^ ((d >> 2) & 1)) << 4), sv + (int64_t)d * p.BS, true);
+          }
+        } else {
+          const T* sv = v + (int64_t)off * p.D + (real ? c0 * 8 : 0);
+#pragma unroll
+          for (int i = 0; i < STRIP / RSTEP; ++i) {
+            const int r = r0l + i * RSTEP;
+            cp_async16(to + F::STRIP_BYTES + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), sv + (int64_t)r * p.D, real);
+          }
+        }
+      }
+      ld_s += WARPS;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+
+  const int r0 = lane >> 2, q0 = (lane & 3) * 2;
+  const int mi = lane >> 3, l7 = lane & 7;
+  Row row;
+  row_at(first, p.B, H, t0, row);
+  int s = t0 * 4 + warp, turn = 0;
+  while (true) {
+    const int seg_end = min(row.end, t1) * 4;
+    const int h = row.hc / p.chunks, g0 = row.hc % p.chunks * 16, G = min(p.G - g0, 16);
+    const int n = rows_of(p, row.b);
+    uint32_t q[KD][NT][2];
+    {
+      const T* qp = reinterpret_cast<const T*>(p.q) + row.b * p.q_stride + (int64_t)(h * p.G + g0) * p.D;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = k * 16 + j * 8 + q0;
+            q[k][nt][j] = nt * 8 + r0 < G && d < p.D ? *reinterpret_cast<const uint32_t*>(qp + (nt * 8 + r0) * p.D + d) : 0u;
+          }
+    }
+    float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < KD; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) { m_run[nt][u] = -INFINITY; l_run[nt][u] = 0.f; }
+    }
+    for (; s < seg_end; s += WARPS) {
+      const int stage = turn;
+      turn = turn + 1 == STAGES ? 0 : turn + 1;
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);                          // into the stage of the strip before, which the whole warp has read
+      const int tok = (s - row.begin * 4) * STRIP;
+      if (tok < n) {
+        const uint32_t ks = ring + stage * (2 * F::STRIP_BYTES), vs = ks + F::STRIP_BYTES;
+        float sc[NT][4], sd[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[nt][i] = sd[nt][i] = 0.f;
+        const uint32_t k_row = ks + ((mi & 1) * 8 + l7) * (DP * 2);
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {
+          uint32_t a[4];
+          ldsm4(a, k_row + (((k * 2 + (mi >> 1)) ^ l7) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<T>(k & 1 ? sd[nt] : sc[nt], a, q[k][nt][0], q[k][nt][1]);
+        }
+        const bool cut = tok + STRIP > n;
+        const bool in[2] = {!cut || tok + r0 < n, !cut || tok + 8 + r0 < n};
+        float* raw = p.raw + ((int64_t)(row.begin - row.hc % p.chunks * (row.end - row.begin)) * TILE + tok) * p.G + g0;
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float mx[2], alpha[2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = sc[nt][i] + sd[nt][i];
+            sc[nt][i] = in[i >> 1] ? (CAP ? prompt::cap_any(x * p.ku, p.c2) : x * p.scale_log2) : -INFINITY;
+            const int g = nt * 8 + q0 + (i & 1);
+            if (g < G) raw[(int64_t)(r0 + (i >> 1) * 8) * p.G + g] = sc[nt][i];
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) mx[u] = fmaxf(sc[nt][u], sc[nt][2 + u]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], x));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float was = m_run[nt][u];
+            const float at = mx[u] - SHIFT;
+            const bool up = at > was + 8.f || (was == -INFINITY && at > -INFINITY);            // else the old reference stays
+            alpha[u] = up && was != -INFINITY ? ex2(was - at) : 1.f;
+            m_run[nt][u] = up ? at : was;
+          }
+          if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < KD; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[i][nt][j] *= alpha[j & 1];
+            l_run[nt][0] *= alpha[0]; l_run[nt][1] *= alpha[1];
+          }
+          const float ref[2] = {m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float x = ex2(sc[nt][2 * t] - ref[0]), y = ex2(sc[nt][2 * t + 1] - ref[1]);
+            l_run[nt][0] += x; l_run[nt][1] += y;
+            const uint32_t hi = pack2<T>(x, y);
+            ph[nt][t] = turn8(hi);
+            const float2 back = unpack2<T>(hi);
+            pl[nt][t] = turn8(pack2<T>(x - back.x, y - back.y));
+          }
+        }
+        uint32_t keepm[2] = {0xffffffffu, 0xffffffffu};                     // of tokens q0, q0 + 1 of either group of eight
+        if (cut) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = tok + j * 8 + q0;
+            keepm[j] = (t < n ? 0xffffu : 0u) | (t + 1 < n ? 0xffff0000u : 0u);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < KD; ++i) {
+          uint32_t a[4];
+          if constexpr (VT) {
+            const int d = i * 16 + (mi & 1) * 8 + l7;
+            ldsm4(a, vs + d * 32 + (((mi >> 1) ^ ((d >> 2) & 1)) << 4));
+          } else {
+            // stored [token][dim], turned by the load: matrices (dims 0-7, tokens 0-7), (dims 8-15, tokens 0-7), (dims 0-7, tokens 8-15), ...
+            const int t = (mi >> 1) * 8 + l7;
+            ldsm4_t(a, vs + t * (DP * 2) + (((i * 2 + (mi & 1)) ^ (t & 7)) << 4));
+          }
+          if (cut) {           // slots behind the sequence may hold what a weight of 0 does not cancel
+            a[0] &= keepm[0]; a[1] &= keepm[0]; a[2] &= keepm[1]; a[3] &= keepm[1];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<T>(o[i][nt], a, ph[nt][0], ph[nt][1]);
+            mma16816<T>(o[i][nt], a, pl[nt][0], pl[nt][1]);
+          }
+        }
+      }
+    }
+    // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
+    float* part = p.part + (int64_t)(row.index + blockIdx.x) * 16 * (p.D + 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
+#pragma unroll
+      for (int half = WARPS / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) {
+          float* to = exch + (warp - half) * F::REGS * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < KD; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[(i * 4 + j) * 32] = o[i][nt][j];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) { to[(KD * 4 + u) * 32] = m_run[nt][u]; to[(KD * 4 + 2 + u) * 32] = l_run[nt][u]; }
+        }
+        __syncthreads();
+        if (warp < half) {
+          const float* from = exch + warp * F::REGS * 32 + lane;
+          float fa[2], fb[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float mb = from[(KD * 4 + u) * 32], top = fmaxf(m_run[nt][u], mb);
+            fa[u] = m_run[nt][u] == -INFINITY ? 0.f : ex2(m_run[nt][u] - top);
+            fb[u] = mb == -INFINITY ? 0.f : ex2(mb - top);
+            m_run[nt][u] = top;
+            l_run[nt][u] = l_run[nt][u] * fa[u] + from[(KD * 4 + 2 + u) * 32] * fb[u];
+          }
+#pragma unroll
+          for (int i = 0; i < KD; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][nt][j] = o[i][nt][j] * fa[j & 1] + from[(i * 4 + j) * 32] * fb[j & 1];
+        }
+      }
+      if (warp == 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int g = nt * 8 + q0 + u;
+          if (g < G) {
+            float* to = part + g * (p.D + 2);
+#pragma unroll
+            for (int i = 0; i < KD; ++i) {
+              if (i * 16 + r0 < p.D) to[i * 16 + r0] = o[i][nt][u];
+              if (i * 16 + 8 + r0 < p.D) to[i * 16 + 8 + r0] = o[i][nt][2 + u];
+            }
+            if (r0 == 0) { to[p.D] = m_run[nt][u]; to[p.D + 1] = l_run[nt][u]; }
+          }
+        }
+      }
+    }
+    if (row.end >= t1) break;
+    next_row(first, H, row);
+  }
+  cp_async_wait<0>();
+}
+
+// Grid (blocks of KEYS keys, kv heads, requests): the first block of a row joins its outputs; every block adds the weights of its keys.
+constexpr int KEYS = 512, JOIN = 256;
+template <typename T>
+__global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
+  extern __shared__ float join_smem[];                // lse of the G heads, in powers of two
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, h = blockIdx.y, H = p.Hkv * p.chunks;
+  const int n = rows_of(p, b);
+  const int key0 = blockIdx.x * KEYS;
+  if (key0 >= n && blockIdx.x > 0) return;
+  // tiles in front of the request, and all
+  int mine = 0, all = 0;
+  for (int i = threadIdx.x; i < p.B; i += JOIN) {
+    const int t = (rows_of(p, i) + TILE - 1) / TILE;
+    all += t;
+    if (i < b) mine += t;
+  }
+  __shared__ int sums[2][JOIN / 32];
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = mine; sums[1][threadIdx.x >> 5] = all; }
+  __syncthreads();
+  mine = all = 0;
+#pragma unroll
+  for (int i = 0; i < JOIN / 32; ++i) { mine += sums[0][i]; all += sums[1][i]; }
+  const int per = (all * H + p.ctas - 1) / p.ctas, tiles = (n + TILE - 1) / TILE;
+  const int PD = p.D + 2;
+  for (int g = threadIdx.x; g < p.G; g += JOIN) {      // log-sum-exp of a head: its parts and the sink
+    const int hc = h * p.chunks + g / 16;
+    const float sink = p.sinks ? p.sinks[h * p.G + g] * LOG2E : -INFINITY;
+    float m = sink;
+    const int begin = mine * H + hc * tiles;
+    float lse = INFINITY;                              // no key and no sink: weights of 0
+    if (tiles > 0) {
+      const int a = begin / per, z = (begin + tiles - 1) / per;
+      for (int c = a; c <= z; ++c) m = fmaxf(m, p.part[((int64_t)(b * H + hc + c) * 16 + g % 16) * PD + p.D]);
+      const float top = m == -INFINITY ? 0.f : m;
+      float l = p.sinks ? ex2(sink - top) : 0.f;
+      for (int c = a; c <= z; ++c) {
+        const float* x = p.part + ((int64_t)(b * H + hc + c) * 16 + g % 16) * PD + p.D;
+        l += x[1] * ex2(x[0] - top);
+      }
+      if (l > 0.f) lse = top + log2f(l);
+    }
+    join_smem[g] = lse;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < p.G * p.D; i += JOIN) {
+      const int g = i / p.D, d = i % p.D, hc = h * p.chunks + g / 16;
+      const int begin = mine * H + hc * tiles;
+      float acc = 0.f;
+      if (tiles > 0) {
+        const int a = begin / per, z = (begin + tiles - 1) / per;
+        const float lse = join_smem[g];
+        for (int c = a; c <= z; ++c) {
+          const float* x = p.part + ((int64_t)(b * H + hc + c) * 16 + g % 16) * PD;
+          acc += x[d] * ex2(x[p.D] - lse);
+        }
+      }
+      reinterpret_cast<T*>(p.out)[b * p.out_stride + (int64_t)(h * p.G + g) * p.D + d] = from_f32<T>(acc);
+    }
+  }
+  const float* raw = p.raw + ((int64_t)mine * H + (int64_t)h * p.chunks * tiles) * TILE * p.G;
+  float* sc = p.scores + b * p.sc_req + h * p.sc_head;
+  for (int k = key0 + threadIdx.x; k < min(key0 + KEYS, n); k += JOIN) {
+    const float* x = raw + (int64_t)k * p.G;
+    float w = 0.f;
+    for (int g = 0; g < p.G; ++g) w += ex2(x[g] - join_smem[g]);
+    sc[k] += w;
+  }
+}
+
+template <typename T, int DP, int NT, bool VT, bool CAP>
+static int launch(const Params& p, cudaStream_t st) {
+  using F = Form<DP>;
+  auto k = decode_kernel<T, DP, NT, VT, CAP>;
+  static bool set = false;
+  if (!set) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM) != cudaSuccess) return (int)cudaGetLastError();
+    set = true;
+  }
+  vb_launch(k, dim3(p.ctas), dim3(F::THREADS), (size_t)F::SMEM, st, p);
+  vb_launch(join_kernel<T>, dim3((p.max_rows + KEYS - 1) / KEYS, p.Hkv, p.B), dim3(JOIN), (size_t)p.G * 4, st, p);
+  return (int)cudaGetLastError();
+}
+template <typename T, int DP, bool VT>
+static int pick(const Params& p, bool cap, cudaStream_t st) {
+  if (p.G > 8) return cap ? launch<T, DP, 2, VT, true>(p, st) : launch<T, DP, 2, VT, false>(p, st);
+  return cap ? launch<T, DP, 1, VT, true>(p, st) : launch<T, DP, 1, VT, false>(p, st);
+}
+template <typename T>
+static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
+  if (vt) return p.D == 128 ? pick<T, 128, true>(p, cap, st) : -2;
+  if (p.D <= 64) return pick<T, 64, false>(p, cap, st);
+  if (p.D <= 128) return pick<T, 128, false>(p, cap, st);
+  return pick<T, 256, false>(p, cap, st);
+}
+
+}  // namespace sdec
+
+
+// `ws`: for rows = min(B, 1024) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + rows ceil(max_rows / 64) 64 G floats.  max_rows: rows of a request that the block
+// table and the scores have room for.
+EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, void* out, float* scores,
+                            const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int64_t q_stride, int64_t out_stride,
+                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
+  using namespace sdec;
+  if (B <= 0) return 0;
+  if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1) return -1;
+  Params p;
+  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16;
+  p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head;
+  p.num_blocks = num_blocks; p.cache = cache; p.sinks = sinks;
+  p.scale_log2 = scale * LOG2E;
+  p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E;
+  for (int b0 = 0; b0 < B; b0 += MAX_REQUESTS) {
+    p.B = B - b0 < MAX_REQUESTS ? B - b0 : MAX_REQUESTS;
+    p.q = reinterpret_cast<const char*>(q) + b0 * q_stride * 2;
+    p.out = reinterpret_cast<char*>(out) + b0 * out_stride * 2;
+    p.block_table = block_table + b0 * bt_stride;
+    p.seq_lens = seq_lens + b0;
+    p.scores = scores + b0 * sc_req;
+    const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE);
+    if (tiles >= (1 << 29)) return -3;                 // flat strip numbers are 32 bits
+    p.ctas = ctas < tiles ? ctas : (int)tiles;
+    p.part = ws;
+    p.raw = ws + (rows + p.ctas) * 16 * (D + 2);
+    const int rc = dtype == DT_BF16 ? go<__nv_bfloat16>(p, vt != 0, soft_cap > 0.f, st) : go<__half>(p, vt != 0, soft_cap > 0.f, st);
+    if (rc) return rc;
+  }
+  return 0;
+}

@@ -550,6 +550,52 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
     return out
 
 
+_scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _f, _f,
+                      _i, _i, _vp)
+
+
+def _key_pages(kv_cache, md, scores):
+    """(block table, lengths, rows that both the table and ``scores`` have room for) of kernels over paged keys; they read no row behind that."""
+    bt, sl = md.block_table, md.seq_lens
+    if bt.dtype != torch.int32 or bt.stride(1) != 1 or sl.dtype != torch.int32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
+        raise ValueError("paged keys: a 16-byte aligned cache, int32 block tables with a request's pages next to each other, int32 lengths")
+    return bt, sl, min(bt.shape[1] * kv_cache.shape[3], scores.shape[2])
+
+
+def _q_heads(q):
+    """Queries with the heads of a token next to each other and rows at 16-byte addresses."""
+    if q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        return q.clone(memory_format=torch.contiguous_format)
+    return _heads(q)
+
+
+def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=None):
+    """Attention of one token per request that adds the keys' weights to ``scores`` (csrc/scored_decode.cu)."""
+    if batch_invariant():                    # that kernel deals the keys of all requests to the SMs
+        from vllm_b200 import ops
+        o, lse = paged_attention(q, kv_cache, md, scale, None, soft_cap, out=out, sinks=sinks, return_lse=True)
+        ops.key_weights(q, kv_cache, md, scale, lse, scores, soft_cap)
+        return o
+    B, Hq, D = md.num_reqs, q.shape[1], q.shape[2]
+    Hkv, BS = kv_cache.shape[2], kv_cache.shape[3]
+    q = _q_heads(q)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.stride(2) != 1 or out.stride(1) != D:
+        raise ValueError("scored_attention: the heads of an output row are next to each other")
+    if sinks is not None:
+        sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+    bt, sl, rows = _key_pages(kv_cache, md, scores)
+    G, ctas = Hq // Hkv, num_sms()
+    n = min(B, 1024) * Hkv * -(-G // 16)
+    # (of this call: two calls at once, or two captured graphs, share nothing)
+    ws = torch.empty((n + ctas) * 16 * (D + 2) + n * -(-rows // 64) * 64 * G, dtype=torch.float32, device=q.device)
+    _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks),
+                          ws.data_ptr(), B, Hq, Hkv, D, BS, rows, q.stride(0), out.stride(0), bt.stride(0), scores.stride(0), scores.stride(1), ctas, scale,
+                          soft_cap, int(md.kv_vt), _DT[q.dtype], _st()), f"scored_decode(D={D}, G={G})", 2 * -(-B // 1024))
+    return out
+
+
 def merge_attn_states(o1, lse1, o2, lse2):
     T, H, D = o1.shape
     out = torch.empty_like(o1)

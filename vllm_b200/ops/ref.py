@@ -153,8 +153,8 @@ def gather_kv(kv_cache: torch.Tensor, block_table_row: torch.Tensor, seq_len: in
     bs = kv_cache.shape[3]
     nb = (seq_len + bs - 1) // bs
     blocks = kv_cache[block_table_row[:nb].long()]  # [nb, 2, H, bs, D]
-    k = blocks[:, 0].permute(1, 0, 2, 3).reshape(kv_cache.shape[2], nb * bs, -1)[:, :seq_len]
-    v = blocks[:, 1].permute(1, 0, 2, 3).reshape(kv_cache.shape[2], nb * bs, -1)[:, :seq_len]
+    k = blocks[:, 0].permute(1, 0, 2, 3).reshape(kv_cache.shape[2], nb * bs, kv_cache.shape[-1])[:, :seq_len]
+    v = blocks[:, 1].permute(1, 0, 2, 3).reshape(kv_cache.shape[2], nb * bs, kv_cache.shape[-1])[:, :seq_len]
     return k, v
 
 
@@ -587,6 +587,60 @@ def fused_moe(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_w: torc
 def identity_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, experts: int) -> torch.Tensor:
     """What expert numbers from ``experts`` on contribute: their weights times the input."""
     return (x.float() * (topk_w.float() * (topk_ids >= experts)).sum(-1, keepdim=True)).to(x.dtype)
+
+
+def key_weights(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor, scale: float,
+                lse: torch.Tensor, scores: torch.Tensor, logits_soft_cap: float = 0.0, last: int = 0) -> torch.Tensor:
+    """In place: scores[i, kv head, key] += the weights e^(score - lse) that request i's query rows (its ``last`` ones, 0: all) give to a cached
+    key, over the query heads of the kv head.  A row whose ``lse`` is -inf or NaN gives none."""
+    Hkv = kv_cache.shape[2]
+    qsl, sls = query_start_loc.tolist(), seq_lens.tolist()
+    for i, n in enumerate(sls):
+        s, e = qsl[i], qsl[i + 1]
+        t = min(last or e - s, e - s)
+        if t <= 0 or n <= 0:
+            continue
+        k = gather_kv(kv_cache, block_table[i], n)[0].float()
+        x = torch.einsum("thgd,hnd->hgtn", q[e - t:e].float().unflatten(1, (Hkv, -1)), k) * scale
+        if logits_soft_cap > 0:
+            x = logits_soft_cap * torch.tanh(x / logits_soft_cap)
+        norm = lse[e - t:e].float().unflatten(1, (Hkv, -1)).permute(1, 2, 0)[..., None]
+        seen = torch.arange(n, device=q.device) <= torch.arange(n - t, n, device=q.device)[:, None]
+        w = torch.where(seen & (norm > float("-inf")), torch.exp(x - norm), 0.0)
+        scores[i, :, :n] += w.sum((1, 2))
+    return scores
+
+
+def evict_keys(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scores: torch.Tensor, keep: int, first: int = 0, recent: int = 0,
+               positions: Optional[torch.Tensor] = None, vt: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """See ``ops.evict_keys``."""
+    _, _, Hkv, BS, D = kv_cache.shape
+    L, dev = scores.shape[2], scores.device
+    rows = torch.arange(L, device=dev)
+    new = torch.zeros_like(scores, memory_format=torch.contiguous_format)
+    places = torch.empty(scores.shape, dtype=torch.int32, device=dev)
+    left = seq_lens.clamp(max=keep)
+    keys, values = kv_cache[:, 0], kv_cache[:, 1]
+    if vt:
+        values = values.view(kv_cache.shape[0], Hkv, D, BS).transpose(2, 3)
+    for i, (n, m) in enumerate(zip(seq_lens.tolist(), left.tolist())):
+        for h in range(Hkv):
+            place = rows[:n].int() if positions is None else positions[i, h, :n]
+            total = int(place.max()) + 1 if n else 0
+            stays = (place < first) | (place >= total - recent)
+            value = scores[i, h, :n].double().clamp(max=1e300)           # (what stays is above an infinite score, too)
+            value = torch.where(value.isnan(), float("-inf"), value).masked_fill(stays, float("inf"))
+            kept = torch.zeros(n, dtype=torch.bool, device=dev)
+            kept[value.sort(descending=True, stable=True)[1][:m]] = True
+            to, source = (~kept[:m]).nonzero()[:, 0], kept[m:].nonzero()[:, 0] + m
+            at = rows[:m].clone()
+            at[to] = source
+            new[i, h, :m], places[i, h, :m] = scores[i, h, at], place[at].int()
+            places[i, h, m:] = torch.arange(total, total + L - m, device=dev)
+            b = block_table[i].long()
+            for x in (keys, values):
+                x[b[to // BS], h, to % BS] = x[b[source // BS], h, source % BS]
+    return left, new, places
 
 
 # ---------------------------------------------------------- cache maintenance
