@@ -1,8 +1,10 @@
 """A key-value cache with a budget on the device: scored attention, key weights and eviction against 64 bits."""
+import dataclasses
+
 import pytest
 import torch
 
-from tests.key_budget_oracle import attend, step, unit, weight_error
+from tests.key_budget_oracle import attend, evict, step, unit, weight_error
 from vllm_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +50,47 @@ def test_decode_lengths(lens, vt):
     Hq, Hkv = (32, 8) if len(lens) < 300 else (2, 1)
     q, cache, md, scores = step(lens, [1] * len(lens), Hq, Hkv, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=len(lens))
     _check_decode(q, cache, md, scores)
+
+
+def _check_evict(cache, md, scores, keep, first=0, recent=0, positions=None):
+    want = evict(cache.cpu(), _on_cpu(md), scores.cpu(), keep, first, recent, None if positions is None else positions.cpu())
+    got = ops.evict_keys(cache, md, scores, keep, first, recent, positions)
+    assert torch.equal(got[0].cpu(), want[1]) and torch.equal(got[2].cpu(), want[3])
+    assert torch.equal(got[1].cpu().view(torch.int32), want[2].view(torch.int32))
+    assert torch.equal(cache.cpu().view(torch.int16), want[0].view(torch.int16))
+    return got
+
+
+def _on_cpu(md):
+    return dataclasses.replace(md, block_table=md.block_table.cpu(), seq_lens=md.seq_lens.cpu())
+
+
+@pytest.mark.parametrize("D,BS,vt,dtype", [(128, 64, True, torch.bfloat16), (128, 64, False, torch.float16), (64, 16, False, torch.bfloat16), (80, 48, False, torch.bfloat16),
+                                           (256, 32, False, torch.float16), (8, 16, False, torch.bfloat16)])
+@pytest.mark.parametrize("lens,keep,first,recent", [([5, 33, 0, 16], 10, 0, 0), ([5, 33, 0, 16], 33, 2, 3), ([40, 90], 1, 1, 0), ([40, 900, 64], 64, 4, 60), ([128], 127, 0, 1),
+                                                    ([1500, 31, 777], 512, 4, 100), ([4500], 4000, 0, 0)])
+@pytest.mark.parametrize("kind", ["", "equal", "odd"])
+def test_evict(D, BS, vt, dtype, lens, keep, first, recent, kind):
+    Hkv = 3 if vt else 2
+    _, cache, md, scores = step(lens, [1] * len(lens), Hkv, Hkv, D, BS, dtype, "cuda", vt=vt, seed=keep)
+    if kind == "equal":
+        scores = scores.round()
+    if kind == "odd":
+        scores[:, :, ::3], scores[:, :, 1::7], scores[:, :, 2::9] = float("nan"), float("inf"), -0.0
+        scores[:, 1, 4::9], scores[:, 0] = float("-inf"), -scores[:, 0]
+    new, positions = None, None
+    for _ in range(2):
+        new, scores, positions = _check_evict(cache, md, scores, keep, first, recent, positions)
+        grown = torch.minimum(new + 4, md.seq_lens)
+        scores += torch.rand_like(scores) * (torch.arange(scores.shape[2], device="cuda") < grown[:, None, None])
+        md.seq_lens, keep = grown, max(1, keep - 2)
+        first, recent = min(first, keep), min(recent, keep - min(first, keep))
+
+
+@pytest.mark.parametrize("n,keep", [(4096, 1000), (4097, 4000), (9000, 100), (33000, 8000), (33000, 32990), (450000, 2000)])
+def test_evict_long(n, keep):
+    """A request of a cluster, and one that its shared memory does not hold."""
+    _, cache, md, scores = step([n, n // 3], [1, 1], 2, 2, 8, 64, torch.bfloat16, "cuda", seed=n)
+    _, scores, positions = _check_evict(cache, md, scores, keep, 3, 50)
+    md.seq_lens = torch.clamp(md.seq_lens, max=keep)
+    _check_evict(cache, md, scores, keep // 2, 1, 20, positions)

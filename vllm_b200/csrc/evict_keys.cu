@@ -1,0 +1,329 @@
+// Cutting a paged cache back: of a request's n rows a kv head keeps m = min(n, keep), those of the lowest and the newest positions and of the others those
+// of the highest scores (ties: the first row); kept rows behind row m move into the evicted rows in front of it, the i-th into the i-th.
+//
+// A row's place is a 32-bit key that orders like (protected, score); the m-th largest key is found digit by digit (11, 11 and 10 bits) from
+// counts in shared memory.  A row of up to 4096 rows is a CTA's, longer ones a cluster's, whose CTAs add their counts through distributed shared memory; the
+// keys are read from memory once and stay in shared memory.  Warps hold runs of neighbours, so ranks among equal keys, evicted and moving
+// rows are counts of bits in front.  A second kernel moves the rows: nothing is read that is written (sources lie behind m, targets in front), so the
+// order does not matter.  Filling the gaps moves as many rows as were evicted in front of m, where keeping the order would move nearly all.
+#include "cluster.cuh"
+
+namespace evict {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048;
+constexpr uint32_t LOWEST = 0x007fffffu, PROTECTED = 0xffffffffu;        // -inf; above +inf
+constexpr int CTA_ROWS = 4096;                                           // rows of a CTA, where eight are enough for them
+constexpr int SMEM_ROWS = 50 * 1024;                                     // of which the keys fit; beyond 8 times that they are made anew in every pass
+
+struct Params {
+  const float* scores;
+  const int* positions;      // null: a row's number
+  const int* seq_lens;
+  float* new_scores;         // [B, Hkv, L]
+  int* new_positions;
+  int* new_lens;
+  int* count;                // [B Hkv]: rows that move
+  int* target;               // [B Hkv][cap]
+  int* source;
+  int64_t sc_req, sc_head, po_req, po_head;
+  int Hkv, L, max_rows, keep, first, recent, parts, cap;
+};
+
+VB_DEVICE uint32_t ordered(float x) {
+  if (x != x) return LOWEST;
+  const uint32_t u = __float_as_uint(x + 0.f);                            // (-0 is 0)
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// sum over the CTA's threads in front and over all
+VB_DEVICE int scan_block(int mine, int* sums, int& all) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sums[w] = x;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < w) before += sums[i];
+    all += sums[i];
+  }
+  return before + x - mine;
+}
+
+// The same where each warp has one number (in all its lanes): over the warps in front, in front in the cluster too, and over the cluster.
+VB_DEVICE int scan_warps(int mine, int* sums, int* mailbox, int parts, int rank, int& all) {
+  const int w = threadIdx.x >> 5;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sums[w] = mine;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < w) before += sums[i];
+    all += sums[i];
+  }
+  if (parts > 1) {
+    if (threadIdx.x == 0) *mailbox = all;
+    cluster_sync();
+    const int cta = all;
+    all = 0;
+    for (int i = 0; i < parts; ++i) {
+      const int x = i == rank ? cta : __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(mailbox), i)));
+      if (i < rank) before += x;
+      all += x;
+    }
+  }
+  return before;
+}
+
+template <bool KEPT>                                     // the keys are kept in shared memory
+__global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
+  extern __shared__ uint32_t evict_smem[];
+  uint32_t* hist = evict_smem;                           // BINS
+  uint32_t* masks = hist + BINS;                         // a bit per row: kept (of rows of a CTA / 32 words, rounded up)
+  __shared__ int sums[WARPS], box[4];
+  __shared__ uint32_t found[2];
+  pdl_trigger();
+  pdl_wait();
+  const int rank = blockIdx.x % p.parts, row = blockIdx.x / p.parts, b = row / p.Hkv, h = row % p.Hkv;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = min(max(p.seq_lens[b], 0), p.max_rows), m = min(n, p.keep);
+  const int chunk = ((n + p.parts - 1) / p.parts + 31) & ~31;
+  const int lo = min(rank * chunk, n), hi = min(lo + chunk, n);
+  const int seg = ((hi - lo + WARPS - 1) / WARPS + 31) & ~31;
+  const int w0 = min(lo + w * seg, hi), w1 = min(w0 + seg, hi);           // the warp's run
+  uint32_t* keys = masks + (p.max_rows / p.parts + 63) / 32 + 1 - lo;     // keys[i] of row i
+  const float* scores = p.scores + b * p.sc_req + h * p.sc_head;
+  const int* positions = p.positions ? p.positions + b * p.po_req + h * p.po_head : nullptr;
+  float* new_scores = p.new_scores + (int64_t)row * p.L;
+  int* new_positions = p.new_positions + (int64_t)row * p.L;
+  if (rank == 0 && h == 0 && threadIdx.x == 0) p.new_lens[b] = m;
+
+  int total = n;                                         // the next position
+  if (positions) {
+    int top = -1;
+    for (int i = w0 + lane; i < w1; i += 32) top = max(top, positions[i]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) sums[w] = top;
+    __syncthreads();
+    top = -1;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) top = max(top, sums[i]);
+    if (p.parts > 1) {
+      if (threadIdx.x == 0) box[0] = top;
+      cluster_sync();
+      for (int i = 0; i < p.parts; ++i) top = max(top, __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&box[0]), i))));
+    }
+    total = top + 1;
+  }
+  auto make = [&](int i) {
+    const int place = positions ? positions[i] : i;
+    return place < p.first || place >= total - p.recent ? PROTECTED : ordered(scores[i]);
+  };
+  auto key = [&](int i) { return KEPT ? keys[i] : make(i); };
+  if (KEPT)
+    for (int i = w0 + lane; i < w1; i += 32) keys[i] = make(i);
+
+  // ---- the m-th largest key, and how many of its equals stay
+  uint32_t prefix = 0, above = 0;                        // digits found so far, and their mask
+  int need = m;
+  if (m < n) {
+#pragma unroll 1
+    for (int d = 0; d < 3; ++d) {
+      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
+      for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
+      __syncthreads();
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const uint32_t k = key(i);
+        if ((k & above) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
+      }
+      __syncthreads();
+      if (p.parts > 1) cluster_sync();
+      int c[BINS / THREADS], mine = 0;                   // from the highest bin down
+#pragma unroll
+      for (int j = 0; j < BINS / THREADS; ++j) {
+        const int bin = BINS - 1 - (threadIdx.x * (BINS / THREADS) + j);
+        c[j] = hist[bin];
+        for (int i = 1; i < p.parts; ++i) {
+          const int r = rank + i < p.parts ? rank + i : rank + i - p.parts;
+          c[j] += __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&hist[bin]), r)));
+        }
+        mine += c[j];
+      }
+      int all, before = scan_block(mine, sums, all);
+      if (before < need && before + mine >= need) {
+#pragma unroll
+        for (int j = 0; j < BINS / THREADS; ++j) {
+          if (before < need && before + c[j] >= need) {
+            found[0] = BINS - 1 - (threadIdx.x * (BINS / THREADS) + j);
+            found[1] = need - before;
+          }
+          before += c[j];
+        }
+      }
+      __syncthreads();
+      prefix |= found[0] << shift;
+      above |= ((1u << bits) - 1) << shift;
+      need = found[1];
+      if (p.parts > 1) cluster_sync();                   // the others have read this CTA's counts
+      __syncthreads();
+    }
+  }
+  // ---- which rows stay: a bit each
+  int equal = 0, all;
+  if (m < n) {
+    for (int i = w0; i < w1; i += 32) equal += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(i + lane) == prefix));
+    equal = scan_warps(equal, sums, &box[1], p.parts, rank, all);
+  }
+  int holes = 0, movers = 0;
+  for (int i = w0; i < w1; i += 32) {
+    const bool there = i + lane < w1;
+    uint32_t stay;
+    if (m < n) {
+      const uint32_t k = there ? key(i + lane) : 0u;
+      const uint32_t same = __ballot_sync(0xffffffffu, there && k == prefix);
+      const bool s = there && (k > prefix || (k == prefix && equal + __popc(same & ((1u << lane) - 1)) < need));
+      equal += __popc(same);
+      stay = __ballot_sync(0xffffffffu, s);
+    } else {
+      stay = __ballot_sync(0xffffffffu, there);
+    }
+    const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1, here = __ballot_sync(0xffffffffu, there);
+    holes += __popc(~stay & front & here);
+    movers += __popc(stay & ~front);
+    if (lane == 0) masks[(i - lo) >> 5] = stay;
+  }
+  __syncwarp();
+  int n_holes, n_movers;
+  holes = scan_warps(holes, sums, &box[2], p.parts, rank, n_holes);
+  movers = scan_warps(movers, sums, &box[3], p.parts, rank, n_movers);
+  if (rank == 0 && threadIdx.x == 0) p.count[row] = n_holes;
+  // ---- lists, and scores and positions of the rows that do not move
+  int* target = p.target + (int64_t)row * p.cap;
+  int* source = p.source + (int64_t)row * p.cap;
+  for (int i = w0; i < w1; i += 32) {
+    const uint32_t stay = masks[(i - lo) >> 5];
+    const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1;
+    const uint32_t here = w1 - i >= 32 ? 0xffffffffu : (1u << (w1 - i)) - 1, me = 1u << lane;
+    const uint32_t hole = ~stay & front & here, mover = stay & ~front;
+    if (hole & me) target[holes + __popc(hole & (me - 1))] = i + lane;
+    if (mover & me) source[movers + __popc(mover & (me - 1))] = i + lane;
+    if (stay & front & me) {
+      new_scores[i + lane] = scores[i + lane];
+      new_positions[i + lane] = positions ? positions[i + lane] : i + lane;
+    }
+    holes += __popc(hole);
+    movers += __popc(mover);
+  }
+  for (int i = m + rank * THREADS + threadIdx.x; i < p.L; i += p.parts * THREADS) {
+    new_scores[i] = 0.f;
+    new_positions[i] = total + i - m;
+  }
+  if (p.parts > 1) cluster_sync();                       // the others may still read this CTA's mailboxes
+}
+
+struct Move {
+  const float* scores;
+  const int* positions;
+  float* new_scores;
+  int* new_positions;
+  const int* count;
+  const int* target;
+  const int* source;
+  uint16_t* cache;
+  const int* block_table;
+  int64_t sc_req, sc_head, po_req, po_head, bt_stride, num_blocks;
+  int Hkv, L, cap, D, BS;
+};
+
+constexpr int PAIRS = 32, MOVERS = 256;
+// Grid (groups of 32 moves, kv heads, requests).  Transposed values (VT): a lane per move, a dimension at a time, as neighbours in the list are near each
+// other in source and target.
+template <bool VT>
+__global__ void __launch_bounds__(MOVERS) move_kernel(const Move p) {
+  __shared__ int64_t from[PAIRS], to[PAIRS];              // places of the keys in the cache (VT: of the first value, too)
+  __shared__ int64_t vfrom[PAIRS], vto[PAIRS];
+  pdl_trigger();
+  pdl_wait();
+  const int h = blockIdx.y, b = blockIdx.z, row = b * p.Hkv + h, j0 = blockIdx.x * PAIRS;
+  const int n = min(p.count[row] - j0, PAIRS);
+  if (n <= 0) return;
+  if (threadIdx.x < n) {
+    const int t = p.target[(int64_t)row * p.cap + j0 + threadIdx.x], s = p.source[(int64_t)row * p.cap + j0 + threadIdx.x];
+    p.new_scores[(int64_t)row * p.L + t] = p.scores[b * p.sc_req + h * p.sc_head + s];
+    p.new_positions[(int64_t)row * p.L + t] = p.positions ? p.positions[b * p.po_req + h * p.po_head + s] : s;
+    const int64_t page = (int64_t)p.BS * p.D;
+    int64_t bt = p.block_table[b * p.bt_stride + t / p.BS], bs = p.block_table[b * p.bt_stride + s / p.BS];
+    const bool ok = (uint64_t)bt < (uint64_t)p.num_blocks && (uint64_t)bs < (uint64_t)p.num_blocks;   // (a table may not say else; nothing outside the
+    if (!ok) bt = bs = 0;                                                                             // cache is touched)
+    const int64_t kt = (bt * 2 * p.Hkv + h) * page, ks = (bs * 2 * p.Hkv + h) * page, v = p.Hkv * page;
+    to[threadIdx.x] = ok ? kt + (int64_t)(t % p.BS) * p.D : -1;
+    from[threadIdx.x] = ks + (int64_t)(s % p.BS) * p.D;
+    vto[threadIdx.x] = VT ? kt + v + t % p.BS : kt + v + (int64_t)(t % p.BS) * p.D;
+    vfrom[threadIdx.x] = VT ? ks + v + s % p.BS : from[threadIdx.x] + v;
+  }
+  __syncthreads();
+  const int ch = p.D / 8, items = n * ch;
+  for (int i = threadIdx.x; i < items; i += MOVERS) {
+    const int j = i / ch, c = i % ch * 8;
+    if (to[j] < 0) continue;
+    const uint4 k = *reinterpret_cast<const uint4*>(p.cache + from[j] + c);
+    if (!VT) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p.cache + vfrom[j] + c);
+      *reinterpret_cast<uint4*>(p.cache + vto[j] + c) = v;
+    }
+    *reinterpret_cast<uint4*>(p.cache + to[j] + c) = k;
+  }
+  if (VT) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (lane < n && to[lane] >= 0) {
+      const uint16_t* src = p.cache + vfrom[lane];
+      uint16_t* dst = p.cache + vto[lane];
+      constexpr int U = 16;
+      uint16_t x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = src[(int64_t)(w * U + u) * p.BS];        // 128 dimensions, 8 warps
+#pragma unroll
+      for (int u = 0; u < U; ++u) dst[(int64_t)(w * U + u) * p.BS] = x[u];
+    }
+  }
+}
+
+}  // namespace evict
+
+// `ws`: B Hkv (1 + 2 cap) ints, cap = max(0, min(keep, max_rows - keep)) moves of a row.  max_rows: rows of a request that the block table and the scores
+// have room for.
+EXPORT int vb_evict_keys(void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const float* scores, const int* positions,
+                         float* new_scores, int* new_positions, int* new_lens, int* ws, int B, int Hkv, int D, int BS, int L, int max_rows, int keep, int first,
+                         int recent, int64_t bt_stride, int64_t sc_req, int64_t sc_head, int64_t po_req, int64_t po_head, int vt, cudaStream_t st) {
+  using namespace evict;
+  if (B <= 0 || Hkv <= 0) return 0;
+  if (D % 8 || (vt && (D != 128 || BS != 64)) || keep < 1 || max_rows > L || max_rows < 0) return -1;
+  const int spare = max_rows - keep, cap = spare <= 0 ? 0 : spare < keep ? spare : keep;
+  Params p{scores, positions, seq_lens, new_scores, new_positions, new_lens, ws, ws + (int64_t)B * Hkv, ws + (int64_t)B * Hkv * (1 + cap),
+           sc_req, sc_head, po_req, po_head, Hkv, L, max_rows, keep, first, recent, 1, cap};
+  while (p.parts < 8 && max_rows > CTA_ROWS * p.parts) p.parts *= 2;
+  const int rows = (max_rows + p.parts - 1) / p.parts + 32;
+  const bool kept = rows <= SMEM_ROWS;
+  const size_t smem = (size_t)(BINS + (max_rows / p.parts + 63) / 32 + 1 + (kept ? rows : 0)) * 4;
+  if (smem > 227 * 1024) return -3;
+  auto k = kept ? select_kernel<true> : select_kernel<false>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)cudaGetLastError();
+  if (vb_launch_parts(k, dim3((unsigned)(B * Hkv * p.parts)), dim3(THREADS), smem, st, (unsigned)p.parts, p) != cudaSuccess) return (int)cudaGetLastError();
+  if (cap > 0) {
+    Move mv{scores, positions, new_scores, new_positions, p.count, p.target, p.source, reinterpret_cast<uint16_t*>(cache), block_table,
+            sc_req, sc_head, po_req, po_head, bt_stride, num_blocks, Hkv, L, cap, D, BS};
+    const dim3 grid((cap + PAIRS - 1) / PAIRS, Hkv, B);
+    if ((vt ? vb_launch(move_kernel<true>, grid, dim3(MOVERS), 0, st, mv) : vb_launch(move_kernel<false>, grid, dim3(MOVERS), 0, st, mv)) != cudaSuccess)
+      return (int)cudaGetLastError();
+  }
+  return (int)cudaGetLastError();
+}

@@ -596,6 +596,26 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     return out
 
 
+_evict_keys = _sig("vb_evict_keys", _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64,
+                   _i, _vp)
+
+
+def evict_keys(kv_cache, md, scores, keep: int, first: int, recent: int, positions=None):
+    """Keeps ``keep`` rows of every request and kv head (csrc/evict_keys.cu); (lengths, scores, positions)."""
+    B, Hkv, L = scores.shape
+    bt, sl, rows = _key_pages(kv_cache, md, scores)
+    dev = scores.device
+    new, places = torch.empty((B, Hkv, L), dtype=torch.float32, device=dev), torch.empty((B, Hkv, L), dtype=torch.int32, device=dev)
+    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    cap = max(0, min(keep, rows - keep))
+    ws = torch.empty(B * Hkv * (1 + 2 * cap), dtype=torch.int32, device=dev)
+    po = (0, 0) if positions is None else positions.stride()
+    _check(_evict_keys(kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), scores.data_ptr(), _p(positions), new.data_ptr(), places.data_ptr(),
+                       lens.data_ptr(), ws.data_ptr(), B, Hkv, kv_cache.shape[4], kv_cache.shape[3], L, rows, keep, first, recent, bt.stride(0), scores.stride(0),
+                       scores.stride(1), po[0], po[1], int(md.kv_vt), _st()), "evict_keys", 2 if cap else 1)
+    return lens, new, places
+
+
 def merge_attn_states(o1, lse1, o2, lse2):
     T, H, D = o1.shape
     out = torch.empty_like(o1)
