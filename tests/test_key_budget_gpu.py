@@ -94,3 +94,50 @@ def test_evict_long(n, keep):
     _, scores, positions = _check_evict(cache, md, scores, keep, 3, 50)
     md.seq_lens = torch.clamp(md.seq_lens, max=keep)
     _check_evict(cache, md, scores, keep // 2, 1, 20, positions)
+
+
+def _check_weights(q, cache, md, scores, cap=0.0, last=0, scale=None, lse=None):
+    D = q.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    if lse is None:
+        lse = attend(q, cache, md, scale, cap)[1].float()
+    _, _, weights, _, terms = attend(q, cache, md, scale, cap, None, last, torch.where(lse > float("-inf"), lse, torch.inf))
+    before = scores.clone()
+    assert ops.key_weights(q, cache, md, scale, lse, scores, cap, last) is scores
+    n = weights.shape[2]
+    total = before.double()
+    total[:, :, :n] += weights
+    # each weight as exact as its exponential; 128 columns are added in chains of 34, their sums without loss; the last addition is rounded
+    bound = 2.0 ** -24 * total
+    bound[:, :, :n] += (weight_error(terms, D) + 38 * 2.0 ** -24) * weights + 2.0 ** -126
+    assert ((scores.double() - total).abs() <= bound).all(), ((scores.double() - total).abs() / bound.clamp(min=1e-300)).max()
+    seen = torch.arange(scores.shape[2], device="cuda") < md.seq_lens[:, None, None]
+    assert torch.equal(scores[~seen.expand_as(scores)], before[~seen.expand_as(scores)])
+
+
+SHAPES = [(8, 2, 128, 64, True), (16, 1, 128, 64, True), (3, 3, 128, 64, True), (10, 2, 64, 16, False), (24, 2, 64, 32, False), (6, 6, 80, 16, False), (8, 2, 96, 48, False),
+          (40, 1, 128, 128, False), (4, 2, 256, 64, False), (16, 1, 192, 256, False), (2, 1, 8, 16, False), (128, 1, 72, 16, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D,BS,vt", SHAPES)
+@pytest.mark.parametrize("cap,last", [(0.0, 0), (30.0, 5), (0.0, 64)])
+def test_weights(dtype, Hq, Hkv, D, BS, vt, cap, last):
+    lens, queries = [300, 1, 700, 0, 64, 130, 511, 513], [300, 1, 45, 0, 1, 129, 256, 3]
+    q, cache, md, scores = step(lens, queries, Hq, Hkv, D, BS, dtype, "cuda", vt=vt, seed=Hq + D, spread=2.0)
+    _check_weights(q, cache, md, scores, cap, last)
+
+
+@pytest.mark.parametrize("lens,queries,last", [([1], [1], 0), ([2500], [2500], 0), ([2500], [2500], 64), ([9000, 300], [20, 300], 0), ([40] * 130, [40] * 130, 7),
+                                               ([200, 300, 1000], [1, 1, 1], 0), ([257, 256, 255], [257, 256, 255], 1)])
+def test_weights_lengths(lens, queries, last):
+    q, cache, md, scores = step(lens, queries, 8, 2, 128, 64, torch.bfloat16, "cuda", vt=True, seed=len(lens))
+    _check_weights(q, cache, md, scores, last=last)
+
+
+def test_weights_of_rows_without():
+    """Rows whose log-sum-exp says that they have no key, or is NaN, give nothing."""
+    q, cache, md, scores = step([300, 200], [100, 200], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=1)
+    lse = attend(q, cache, md, 128 ** -0.5)[1].float()
+    lse[::3], lse[1::5] = float("-inf"), float("nan")
+    _check_weights(q, cache, md, scores, lse=lse)
