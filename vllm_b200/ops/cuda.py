@@ -596,7 +596,8 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     return out
 
 
-_key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _f, _f, _i, _vp)
+_key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64,
+                    _f, _f, _i, _vp)
 
 
 def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last: int = 0):
@@ -605,12 +606,17 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     Hkv = kv_cache.shape[2]
     if Hq // Hkv > 128:
         raise ValueError(f"key_weights: {Hq // Hkv} query heads for a kv head; up to 128")
+    if not scale:
+        raise ValueError("key_weights: a scale of 0")          # (the kernel divides by it)
     q, lse = _q_heads(q), lse.contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    qsl = None if md.decode_only else md.query_start_loc
+    qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
+    ctas = num_sms()
+    part = scores.new_empty(ctas * 512)
     _check(_key_weights(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), _p(qsl), lse.data_ptr(), scores.data_ptr(),
-                        _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, last, q.stride(0), bt.stride(0), scores.stride(0),
-                        scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()), f"key_weights(D={D}, G={Hq // Hkv})")
+                        part.data_ptr(), _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, min(last or most, most), last, ctas,
+                        int(batch_invariant()), q.stride(0), bt.stride(0), scores.stride(0), scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()),
+           f"key_weights(D={D}, G={Hq // Hkv})", 2)
     return scores
 
 
