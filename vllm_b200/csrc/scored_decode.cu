@@ -42,12 +42,13 @@ struct Params {
 VB_DEVICE int rows_of(const Params& p, int b) { return min(max(p.seq_lens[b], 0), p.max_rows); }
 
 // first[b]: tiles of all rows in front of request b, as if each request had one kv head; first[B]: of all
-VB_DEVICE void scan_tiles(const Params& p, int* first, int* warp_sums) {
+VB_DEVICE void scan_tiles(const Params& p, int* first, int* lens, int* warp_sums) {
   const int n_threads = blockDim.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = n_threads >> 5;
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += n_threads) {
     const int b = b0 + threadIdx.x;
-    const int mine = b < p.B ? (rows_of(p, b) + TILE - 1) / TILE : 0;
+    const int n = b < p.B ? rows_of(p, b) : 0, mine = (n + TILE - 1) / TILE;
+    if (b < p.B) lens[b] = n;
     int x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -127,7 +128,7 @@ template <int DP_> struct Form {
   static constexpr int STAGES = DP == 64 ? 6 : 3;
   static constexpr int RING = WARPS * STAGES * 2 * STRIP_BYTES;
   static constexpr int REGS = DP / 16 * 4 + 4;                             // of a group of heads: output, maxima, sums
-  static constexpr int SMEM = RING + WARPS / 2 * REGS * 128 + (MAX_REQUESTS + 1 + 32) * 4;
+  static constexpr int SMEM = RING + WARPS / 2 * REGS * 128 + (2 * MAX_REQUESTS + 1 + 32) * 4;
 };
 
 template <typename T, int DP, int NT, bool VT, bool CAP>
@@ -140,11 +141,12 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
   extern __shared__ __align__(128) unsigned char smem[];
   float* exch = reinterpret_cast<float*>(smem + F::RING);
   int* first = reinterpret_cast<int*>(smem + F::RING + WARPS / 2 * F::REGS * 128);
-  int* warp_sums = first + MAX_REQUESTS + 1;
+  int* lens = first + MAX_REQUESTS + 1;
+  int* warp_sums = lens + MAX_REQUESTS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_trigger();
   pdl_wait();
-  scan_tiles(p, first, warp_sums);
+  pdl_trigger();             // (here: the joining kernel may read the lengths as soon as it starts)
+  scan_tiles(p, first, lens, warp_sums);
   const int H = p.Hkv * p.chunks;
   const int total = first[p.B] * H, per = (total + p.ctas - 1) / p.ctas;
   const int t0 = blockIdx.x * per, t1 = min(t0 + per, total);
@@ -152,52 +154,59 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
 
   const uint32_t ring = smem_u32(smem) + warp * (STAGES * 2 * F::STRIP_BYTES);
   const int64_t page = (int64_t)p.BS * p.D;                                // values of a page of one head
-  // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  `ld` is the row of the next strip to fetch.
+  // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  Where they lie is looked up for 32 of them at once, a lane each: a block number comes
+  // out of memory before the copies can be issued, and one at a time that was most of a short run.
   const int s_end = t1 * 4;
-  Row ld;
-  row_at(first, p.B, H, t0, ld);
-  int ld_n = rows_of(p, ld.b), ld_s = t0 * 4 + warp;
+  int64_t my_page = 0;                                                      // of the lane's strip: place of the page, token in it (-1: nothing to fetch)
+  int my_off = -1, fetched = 0;
   const int c0 = lane % CH, r0l = lane / CH;                                // CH = 8, 16, 32: a lane's piece of a key and its first key
   constexpr int RSTEP = CH >= 32 ? 1 : 32 / CH;
+  const bool real = c0 * 8 < p.D;
   auto fetch = [&](int stage) {
-    while (ld_s < s_end && ld_s >= ld.end * 4) {
-      next_row(first, H, ld);
-      ld_n = rows_of(p, ld.b);
+    if ((fetched & 31) == 0) {
+      const int s = t0 * 4 + warp + (fetched + lane) * WARPS;
+      my_off = -1;
+      if (s < s_end) {
+        Row r;
+        row_at(first, p.B, H, s >> 2, r);
+        const int tok = (s - r.begin * 4) * STRIP;
+        if (tok < lens[r.b]) {
+          int64_t blk = p.block_table[r.b * p.bt_stride + tok / p.BS];
+          if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
+          my_page = (blk * 2 * p.Hkv + r.hc / p.chunks) * page;
+          my_off = tok % p.BS;
+        }
+      }
     }
-    if (ld_s < s_end) {
-      const int tok = (ld_s - ld.begin * 4) * STRIP;
-      if (tok < ld_n) {
-        int64_t blk = p.block_table[ld.b * p.bt_stride + tok / p.BS];
-        if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;              // (a table may not say that; nothing is read outside the cache)
-        const int off = tok % p.BS, h = ld.hc / p.chunks;
-        const T* k = reinterpret_cast<const T*>(p.cache) + (blk * 2 * p.Hkv + h) * page;
-        const T* v = k + p.Hkv * page;
-        const uint32_t to = ring + stage * (2 * F::STRIP_BYTES);
-        const bool real = c0 * 8 < p.D;
-        const T* src = k + (int64_t)off * p.D + (real ? c0 * 8 : 0);
+    const int off = __shfl_sync(0xffffffffu, my_off, fetched & 31);
+    const int64_t at = __shfl_sync(0xffffffffu, my_page, fetched & 31);
+    ++fetched;
+    if (off >= 0) {
+      const T* k = reinterpret_cast<const T*>(p.cache) + at;
+      const T* v = k + p.Hkv * page;
+      const uint32_t to = ring + stage * (2 * F::STRIP_BYTES);
+      const T* src = k + (int64_t)off * p.D + (real ? c0 * 8 : 0);
+#pragma unroll
+      for (int i = 0; i < STRIP / RSTEP; ++i) {
+        const int r = r0l + i * RSTEP;
+        cp_async16(to + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), src + (int64_t)r * p.D, real);
+      }
+      if constexpr (VT) {                                                  // values stored [dim][token of the page]
+        const int half = lane & 1, d0 = lane >> 1;
+        const T* sv = v + off + half * 8;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const int d = d0 + i * 16;
+          cp_async16(to + F::STRIP_BYTES + d * 32 + ((half ^ ((d >> 2) & 1)) << 4), sv + (int64_t)d * p.BS, true);
+        }
+      } else {
+        const T* sv = v + (int64_t)off * p.D + (real ? c0 * 8 : 0);
 #pragma unroll
         for (int i = 0; i < STRIP / RSTEP; ++i) {
           const int r = r0l + i * RSTEP;
-          cp_async16(to + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), src + (int64_t)r * p.D, real);
-        }
-        if constexpr (VT) {                                                // values stored [dim][token of the page]
-          const int half = lane & 1, d0 = lane >> 1;
-          const T* sv = v + off + half * 8;
-#pragma unroll
-          for (int i = 0; i < DP / 16; ++i) {
-            const int d = d0 + i * 16;
-            cp_async16(to + F::STRIP_BYTES + d * 32 + ((half ^ ((d >> 2) & 1)) << 4), sv + (int64_t)d * p.BS, true);
-          }
-        } else {
-          const T* sv = v + (int64_t)off * p.D + (real ? c0 * 8 : 0);
-#pragma unroll
-          for (int i = 0; i < STRIP / RSTEP; ++i) {
-            const int r = r0l + i * RSTEP;
-            cp_async16(to + F::STRIP_BYTES + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), sv + (int64_t)r * p.D, real);
-          }
+          cp_async16(to + F::STRIP_BYTES + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), sv + (int64_t)r * p.D, real);
         }
       }
-      ld_s += WARPS;
     }
     cp_async_commit();
   };
@@ -209,23 +218,25 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
   Row row;
   row_at(first, p.B, H, t0, row);
   int s = t0 * 4 + warp, turn = 0;
+  uint32_t q[KD][NT][2];
+  auto load_q = [&]() {
+    const int g0 = row.hc % p.chunks * 16, G = min(p.G - g0, 16);
+    const T* qp = reinterpret_cast<const T*>(p.q) + row.b * p.q_stride + (int64_t)(row.hc / p.chunks * p.G + g0) * p.D;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < KD; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = k * 16 + j * 8 + q0;
+          q[k][nt][j] = nt * 8 + r0 < G && d < p.D ? *reinterpret_cast<const uint32_t*>(qp + (nt * 8 + r0) * p.D + d) : 0u;
+        }
+  };
+  load_q();
   while (true) {
     const int seg_end = min(row.end, t1) * 4;
-    const int h = row.hc / p.chunks, g0 = row.hc % p.chunks * 16, G = min(p.G - g0, 16);
-    const int n = rows_of(p, row.b);
-    uint32_t q[KD][NT][2];
-    {
-      const T* qp = reinterpret_cast<const T*>(p.q) + row.b * p.q_stride + (int64_t)(h * p.G + g0) * p.D;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < KD; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int d = k * 16 + j * 8 + q0;
-            q[k][nt][j] = nt * 8 + r0 < G && d < p.D ? *reinterpret_cast<const uint32_t*>(qp + (nt * 8 + r0) * p.D + d) : 0u;
-          }
-    }
+    const int g0 = row.hc % p.chunks * 16, G = min(p.G - g0, 16);
+    const int n = lens[row.b];
     float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -336,6 +347,11 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
     }
     // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
     float* part = p.part + (int64_t)(row.index + blockIdx.x) * 16 * (p.D + 2);
+    const bool more = row.end < t1;
+    if (more) {                              // (the next row's queries are on their way meanwhile)
+      next_row(first, H, row);
+      load_q();
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -388,20 +404,19 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
         }
       }
     }
-    if (row.end >= t1) break;
-    next_row(first, H, row);
+    if (!more) break;
   }
   cp_async_wait<0>();
 }
 
 // Grid (blocks of KEYS keys, kv heads, requests): the first block of a row joins its outputs; every block adds the weights of its keys.
-constexpr int KEYS = 512, JOIN = 256;
+constexpr int KEYS = 1024, JOIN = 256, FACTORS = 32;
 template <typename T>
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
-  extern __shared__ float join_smem[];                // lse of the G heads, in powers of two
+  extern __shared__ float join_smem[];                // of the G heads: log-sum-exp in powers of two, then a factor for each of the first FACTORS parts
+  __shared__ int sums[2][JOIN / 32];
   pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.z, h = blockIdx.y, H = p.Hkv * p.chunks;
+  const int b = blockIdx.z, h = blockIdx.y, H = p.Hkv * p.chunks, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = rows_of(p, b);
   const int key0 = blockIdx.x * KEYS;
   if (key0 >= n && blockIdx.x > 0) return;
@@ -412,59 +427,88 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
     all += t;
     if (i < b) mine += t;
   }
-  __shared__ int sums[2][JOIN / 32];
   mine = __reduce_add_sync(0xffffffffu, mine);
   all = __reduce_add_sync(0xffffffffu, all);
-  if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = mine; sums[1][threadIdx.x >> 5] = all; }
+  if (lane == 0) { sums[0][w] = mine; sums[1][w] = all; }
   __syncthreads();
   mine = all = 0;
 #pragma unroll
   for (int i = 0; i < JOIN / 32; ++i) { mine += sums[0][i]; all += sums[1][i]; }
   const int per = (all * H + p.ctas - 1) / p.ctas, tiles = (n + TILE - 1) / TILE;
   const int PD = p.D + 2;
-  for (int g = threadIdx.x; g < p.G; g += JOIN) {      // log-sum-exp of a head: its parts and the sink
-    const int hc = h * p.chunks + g / 16;
+  float* factors = join_smem + ((p.G + 3) & ~3);
+  pdl_wait();
+  // parts of a head: segments of CTAs a .. z, at row + CTA
+  auto parts = [&](int g, int& a, int& z) -> const float* {
+    const int hc = h * p.chunks + g / 16, begin = mine * H + hc * tiles;
+    a = tiles > 0 ? begin / per : 0;
+    z = tiles > 0 ? (begin + tiles - 1) / per : -1;
+    return p.part + ((int64_t)(b * H + hc + a) * 16 + g % 16) * PD;
+  };
+  for (int g = w; g < p.G; g += JOIN / 32) {          // a warp: log-sum-exp of a head, its parts and the sink
+    int a, z;
+    const float* x = parts(g, a, z) + p.D;
     const float sink = p.sinks ? p.sinks[h * p.G + g] * LOG2E : -INFINITY;
     float m = sink;
-    const int begin = mine * H + hc * tiles;
-    float lse = INFINITY;                              // no key and no sink: weights of 0
-    if (tiles > 0) {
-      const int a = begin / per, z = (begin + tiles - 1) / per;
-      for (int c = a; c <= z; ++c) m = fmaxf(m, p.part[((int64_t)(b * H + hc + c) * 16 + g % 16) * PD + p.D]);
-      const float top = m == -INFINITY ? 0.f : m;
-      float l = p.sinks ? ex2(sink - top) : 0.f;
-      for (int c = a; c <= z; ++c) {
-        const float* x = p.part + ((int64_t)(b * H + hc + c) * 16 + g % 16) * PD + p.D;
-        l += x[1] * ex2(x[0] - top);
-      }
-      if (l > 0.f) lse = top + log2f(l);
-    }
-    join_smem[g] = lse;
+    for (int c = lane; c <= z - a; c += 32) m = fmaxf(m, x[(int64_t)c * 16 * PD]);
+    m = warp_max(m);
+    const float top = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int c = lane; c <= z - a; c += 32) l += x[(int64_t)c * 16 * PD + 1] * ex2(x[(int64_t)c * 16 * PD] - top);
+    l = warp_sum(l) + (p.sinks ? ex2(sink - top) : 0.f);
+    const float lse = l > 0.f ? top + log2f(l) : INFINITY;                  // no key and no sink: weights of 0
+    if (lane == 0) join_smem[g] = lse;
+    factors[g * FACTORS + lane] = lane <= z - a ? ex2(x[(int64_t)lane * 16 * PD] - lse) : 0.f;
   }
   __syncthreads();
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < p.G * p.D; i += JOIN) {
-      const int g = i / p.D, d = i % p.D, hc = h * p.chunks + g / 16;
-      const int begin = mine * H + hc * tiles;
+      const int g = i / p.D, d = i % p.D;
+      int a, z;
+      const float* x = parts(g, a, z);
       float acc = 0.f;
-      if (tiles > 0) {
-        const int a = begin / per, z = (begin + tiles - 1) / per;
-        const float lse = join_smem[g];
-        for (int c = a; c <= z; ++c) {
-          const float* x = p.part + ((int64_t)(b * H + hc + c) * 16 + g % 16) * PD;
-          acc += x[d] * ex2(x[p.D] - lse);
-        }
-      }
+#pragma unroll 4
+      for (int c = 0; c <= min(z - a, FACTORS - 1); ++c) acc += x[(int64_t)c * 16 * PD + d] * factors[g * FACTORS + c];
+      for (int c = FACTORS; c <= z - a; ++c) acc += x[(int64_t)c * 16 * PD + d] * ex2(x[(int64_t)c * 16 * PD + p.D] - join_smem[g]);
       reinterpret_cast<T*>(p.out)[b * p.out_stride + (int64_t)(h * p.G + g) * p.D + d] = from_f32<T>(acc);
     }
   }
   const float* raw = p.raw + ((int64_t)mine * H + (int64_t)h * p.chunks * tiles) * TILE * p.G;
   float* sc = p.scores + b * p.sc_req + h * p.sc_head;
-  for (int k = key0 + threadIdx.x; k < min(key0 + KEYS, n); k += JOIN) {
-    const float* x = raw + (int64_t)k * p.G;
-    float w = 0.f;
-    for (int g = 0; g < p.G; ++g) w += ex2(x[g] - join_smem[g]);
-    sc[k] += w;
+  const int end = min(key0 + KEYS, n);
+  constexpr int U = KEYS / JOIN;
+  float add[U] = {0.f, 0.f, 0.f, 0.f}, old[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = key0 + u * JOIN + threadIdx.x;
+    old[u] = k < end ? sc[k] : 0.f;
+  }
+  if (p.G % 4 == 0) {
+    for (int g = 0; g < p.G; g += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(join_smem + g);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = key0 + u * JOIN + threadIdx.x;
+        if (k < end) {
+          const float4 x = *reinterpret_cast<const float4*>(raw + (int64_t)k * p.G + g);
+          add[u] += (ex2(x.x - l.x) + ex2(x.y - l.y)) + (ex2(x.z - l.z) + ex2(x.w - l.w));
+        }
+      }
+    }
+  } else {
+    for (int g = 0; g < p.G; ++g) {
+      const float l = join_smem[g];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = key0 + u * JOIN + threadIdx.x;
+        if (k < end) add[u] += ex2(raw[(int64_t)k * p.G + g] - l);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = key0 + u * JOIN + threadIdx.x;
+    if (k < end) sc[k] = old[u] + add[u];
   }
 }
 
@@ -478,7 +522,7 @@ static int launch(const Params& p, cudaStream_t st) {
     set = true;
   }
   vb_launch(k, dim3(p.ctas), dim3(F::THREADS), (size_t)F::SMEM, st, p);
-  vb_launch(join_kernel<T>, dim3((p.max_rows + KEYS - 1) / KEYS, p.Hkv, p.B), dim3(JOIN), (size_t)p.G * 4, st, p);
+  vb_launch(join_kernel<T>, dim3((p.max_rows + KEYS - 1) / KEYS, p.Hkv, p.B), dim3(JOIN), (size_t)(((p.G + 3) & ~3) + p.G * FACTORS) * 4, st, p);
   return (int)cudaGetLastError();
 }
 template <typename T, int DP, bool VT>
