@@ -35,19 +35,22 @@ struct Params {
   float* part;             // [segment][G][D + 2]: output, maximum, sum
   int64_t q_stride, out_stride, bt_stride, sc_req, sc_head;
   int64_t num_blocks;
-  int B, Hkv, G, D, BS, max_rows, ctas, chunks;      // chunks: of at most 16 query heads of a kv head
+  int B, Hkv, G, D, BS, max_rows, ctas, chunks, extra;      // chunks: of at most 16 query heads of a kv head
   float scale_log2, ku, c2;
 };
 
 VB_DEVICE int rows_of(const Params& p, int b) { return min(max(p.seq_lens[b], 0), p.max_rows); }
 
-// first[b]: tiles of all rows in front of request b, as if each request had one kv head; first[B]: of all
+// A row's tiles, and what its end costs in tiles
+VB_DEVICE int slots_of(const Params& p, int n) { return n > 0 ? (n + TILE - 1) / TILE + p.extra : 0; }
+
+// first[b]: slots of all rows in front of request b, as if each request had one kv head; first[B]: of all
 VB_DEVICE void scan_tiles(const Params& p, int* first, int* lens, int* warp_sums) {
   const int n_threads = blockDim.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = n_threads >> 5;
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += n_threads) {
     const int b = b0 + threadIdx.x;
-    const int n = b < p.B ? rows_of(p, b) : 0, mine = (n + TILE - 1) / TILE;
+    const int n = b < p.B ? rows_of(p, b) : 0, mine = slots_of(p, n);
     if (b < p.B) lens[b] = n;
     int x = mine;
 #pragma unroll
@@ -69,7 +72,7 @@ VB_DEVICE void scan_tiles(const Params& p, int* first, int* lens, int* warp_sums
   __syncthreads();
 }
 
-// A row: request, kv head, chunk of query heads; its tiles are [begin, end) of the order of all
+// A row: request, kv head, chunk of query heads; its slots are [begin, end) of the order of all
 struct Row {
   int index, b, hc, begin, end;
 };
@@ -347,11 +350,13 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
     }
     // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
     float* part = p.part + (int64_t)(row.index + blockIdx.x) * 16 * (p.D + 2);
+    const bool empty = max(row.begin, t0) >= row.begin + (n + TILE - 1) / TILE;      // nothing but the row's further slots
     const bool more = row.end < t1;
     if (more) {                              // (the next row's queries are on their way meanwhile)
       next_row(first, H, row);
       load_q();
     }
+    if (!empty)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
   // tiles in front of the request, and all
   int mine = 0, all = 0;
   for (int i = threadIdx.x; i < p.B; i += JOIN) {
-    const int t = (rows_of(p, i) + TILE - 1) / TILE;
+    const int t = slots_of(p, rows_of(p, i));
     all += t;
     if (i < b) mine += t;
   }
@@ -434,13 +439,13 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
   mine = all = 0;
 #pragma unroll
   for (int i = 0; i < JOIN / 32; ++i) { mine += sums[0][i]; all += sums[1][i]; }
-  const int per = (all * H + p.ctas - 1) / p.ctas, tiles = (n + TILE - 1) / TILE;
+  const int per = (all * H + p.ctas - 1) / p.ctas, tiles = (n + TILE - 1) / TILE, slots = slots_of(p, n);
   const int PD = p.D + 2;
   float* factors = join_smem + ((p.G + 3) & ~3);
   pdl_wait();
   // parts of a head: segments of CTAs a .. z, at row + CTA
   auto parts = [&](int g, int& a, int& z) -> const float* {
-    const int hc = h * p.chunks + g / 16, begin = mine * H + hc * tiles;
+    const int hc = h * p.chunks + g / 16, begin = mine * H + hc * slots;
     a = tiles > 0 ? begin / per : 0;
     z = tiles > 0 ? (begin + tiles - 1) / per : -1;
     return p.part + ((int64_t)(b * H + hc + a) * 16 + g % 16) * PD;
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
       reinterpret_cast<T*>(p.out)[b * p.out_stride + (int64_t)(h * p.G + g) * p.D + d] = from_f32<T>(acc);
     }
   }
-  const float* raw = p.raw + ((int64_t)mine * H + (int64_t)h * p.chunks * tiles) * TILE * p.G;
+  const float* raw = p.raw + ((int64_t)mine * H + (int64_t)h * p.chunks * slots) * TILE * p.G;
   float* sc = p.scores + b * p.sc_req + h * p.sc_head;
   const int end = min(key0 + KEYS, n);
   constexpr int U = KEYS / JOIN;
@@ -541,16 +546,17 @@ static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
 }  // namespace sdec
 
 
-// `ws`: for rows = min(B, 1024) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + rows ceil(max_rows / 64) 64 G floats.  max_rows: rows of a request that the block
+// `ws`: for rows = min(B, 1024) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + rows (ceil(max_rows / 64) + extra) 64 G floats.  extra: tiles
+// that a row counts for beside its own.  max_rows: rows of a request that the block
 // table and the scores have room for.
 EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, void* out, float* scores,
                             const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int64_t q_stride, int64_t out_stride,
-                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
+                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int extra, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
   using namespace sdec;
   if (B <= 0) return 0;
   if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1) return -1;
   Params p;
-  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16;
+  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16; p.extra = extra;
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head;
   p.num_blocks = num_blocks; p.cache = cache; p.sinks = sinks;
   p.scale_log2 = scale * LOG2E;
@@ -562,7 +568,7 @@ EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks
     p.block_table = block_table + b0 * bt_stride;
     p.seq_lens = seq_lens + b0;
     p.scores = scores + b0 * sc_req;
-    const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE);
+    const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE + p.extra);
     if (tiles >= (1 << 29)) return -3;                 // flat strip numbers are 32 bits
     p.ctas = ctas < tiles ? ctas : (int)tiles;
     p.part = ws;

@@ -217,34 +217,34 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
     return o.to(q.dtype) if out is None else out.copy_(o)
 
 
-def _check_scores(scores, kv_cache, md, op: str) -> None:
-    if scores.dtype != torch.float32 or scores.dim() != 3 or scores.stride(2) != 1:
+_F32 = torch.float32
+
+
+def _check_scores(scores, kv_cache, md, op: str, cuda: bool) -> tuple[int, int, int]:
+    """Scores beside a paged cache, and what the kernels over both take; (kv heads, page, head size)."""
+    if scores.dtype is not _F32 or scores.dim() != 3 or scores.stride(2) != 1:
         raise ValueError(f"{op}: scores are fp32 [requests, kv heads, rows] with rows next to each other")
-    if scores.shape[0] < md.num_reqs or scores.shape[1] != kv_cache.shape[2] or scores.shape[2] < md.max_seq_len:
-        raise ValueError(f"{op}: scores of {tuple(scores.shape)} for {md.num_reqs} requests of up to {md.max_seq_len} rows and {kv_cache.shape[2]} kv heads")
-    if scores.device != kv_cache.device or kv_cache.dim() != 5:
+    if kv_cache.dim() != 5 or scores.device != kv_cache.device:
         raise ValueError(f"{op}: a cache [blocks, 2, kv heads, page, head size] and scores on its device")
+    _, _, H, BS, D = kv_cache.shape
+    R, Hs, L = scores.shape
+    if R < md.num_reqs or Hs != H or L < md.max_seq_len:
+        raise ValueError(f"{op}: scores of {tuple(scores.shape)} for {md.num_reqs} requests of up to {md.max_seq_len} rows and {H} kv heads")
+    if cuda:
+        if kv_cache.dtype not in _HALF or D % 8 or D > 256 or BS % 16 or not kv_cache.is_contiguous():
+            raise ValueError(f"{op}: 16-bit caches, heads of up to 256 in steps of 8, pages in steps of 16; got {kv_cache.dtype}, {D}, {BS}")
+        if md.kv_vt and (D != 128 or BS != 64):
+            raise ValueError(f"{op}: transposed values are of heads of 128 and pages of 64")
+    return H, BS, D
 
 
-def _check_keys(q, kv_cache, md, scores, op: str) -> None:
-    """Queries over a cache with scores: the head shapes and types that scored_attention and key_weights take."""
-    _check_scores(scores, kv_cache, md, op)
-    if q.dim() != 3 or q.shape[2] != kv_cache.shape[4] or q.shape[1] % kv_cache.shape[2] or q.dtype != kv_cache.dtype or q.device != kv_cache.device:
-        raise ValueError(f"{op}: queries {tuple(q.shape)} of {q.dtype} for a cache of {kv_cache.shape[2]} heads of {kv_cache.shape[4]}, {kv_cache.dtype}")
+def _check_queries(q, kv_cache, md, H: int, D: int, op: str) -> None:
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H or q.dtype != kv_cache.dtype or q.device != kv_cache.device:
+        raise ValueError(f"{op}: queries {tuple(q.shape)} of {q.dtype} for a cache of {H} heads of {D}, {kv_cache.dtype}")
     if not md.causal:
         raise ValueError(f"{op}: causal attention only")
     if md.decode_only and q.shape[0] < md.num_reqs:
         raise ValueError(f"{op}: {q.shape[0]} queries for {md.num_reqs} requests")
-    if _use_cuda(q):
-        _check_paged_heads(kv_cache, md, op)
-
-
-def _check_paged_heads(kv_cache, md, op: str) -> None:
-    D, BS = kv_cache.shape[4], kv_cache.shape[3]
-    if kv_cache.dtype not in _HALF or D % 8 or D > 256 or BS % 16 or not kv_cache.is_contiguous():
-        raise ValueError(f"{op}: 16-bit caches, heads of up to 256 in steps of 8, pages in steps of 16; got {kv_cache.dtype}, {D}, {BS}")
-    if md.kv_vt and (D, BS) != (128, 64):
-        raise ValueError(f"{op}: transposed values are of heads of 128 and pages of 64")
 
 
 def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.0, sinks: Optional[torch.Tensor] = None, last: int = 0,
@@ -253,16 +253,18 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
     over the query heads of its kv head and the request's query rows (its ``last`` ones, 0: all): what ``evict_keys`` chooses by.  Returns the
     output.  Rows of ``scores`` behind a request's last key stay as they are; rows that are not in the cache yet have to be 0 when they come.
     No two requests may share a row of ``scores``."""
-    _check_keys(q, kv_cache, md, scores, "scored_attention")
+    cuda = _use_cuda(q)
+    H, _, D = _check_scores(scores, kv_cache, md, "scored_attention", cuda)
+    _check_queries(q, kv_cache, md, H, D, "scored_attention")
     if last < 0:
         raise ValueError(f"scored_attention: last {last}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"scored_attention: out {tuple(out.shape)} of {out.dtype}")
     if sinks is not None and sinks.numel() != q.shape[1]:
         raise ValueError(f"scored_attention: {sinks.numel()} sinks for {q.shape[1]} heads")
-    if not _use_cuda(q) and md.kv_vt:
+    if not cuda and md.kv_vt:
         raise ValueError("scored_attention: the tensor-core cache layout is CUDA only")
-    if _use_cuda(q) and md.decode_only:
+    if cuda and md.decode_only:
         return cuda_ops().scored_decode(q, kv_cache, md, scale, scores, logits_soft_cap, sinks, out)
     o, lse = paged_attention(q, kv_cache, md, scale, None, logits_soft_cap, out=out, sinks=sinks, return_lse=True)
     key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap, last)
@@ -273,10 +275,12 @@ def key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap: float = 0.
     """In place: scores[request, kv head, key] += sum of e^(score - lse) over the request's query rows (its ``last`` ones, 0: all) that see the
     key and the query heads of the kv head.  ``lse`` [T, query heads]: what ``paged_attention(..., return_lse=True)`` returns; a row where it is
     -inf (no key) or NaN gives nothing.  Returns ``scores``."""
-    _check_keys(q, kv_cache, md, scores, "key_weights")
+    cuda = _use_cuda(q)
+    H, _, D = _check_scores(scores, kv_cache, md, "key_weights", cuda)
+    _check_queries(q, kv_cache, md, H, D, "key_weights")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device or last < 0:
         raise ValueError(f"key_weights: lse {tuple(lse.shape)} of {lse.dtype} for queries {tuple(q.shape)}, last {last}")
-    if _use_cuda(q):
+    if cuda:
         return cuda_ops().key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap, last)
     sl = md.seq_lens_cpu if md.seq_lens_cpu is not None else md.seq_lens.cpu()
     if md.decode_only:
@@ -296,15 +300,15 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int = 0, recent: int = 0,
     ``positions`` [requests, kv heads, rows] int32: the place in the text of each row, as the eviction before returned it; None: the row's
     number.  Returns (seq_lens, scores, positions), new tensors: lengths; scores of the rows, 0 behind them; positions of the rows, behind
     them those that the next tokens will have."""
-    _check_scores(scores, kv_cache, md, "evict_keys")
+    cuda = _use_cuda(kv_cache)
+    _check_scores(scores, kv_cache, md, "evict_keys", cuda)
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
         raise ValueError(f"evict_keys: first {first} and recent {recent} of keep {keep}")
     if positions is not None and (positions.shape != scores.shape or positions.dtype != torch.int32 or positions.stride(2) != 1 or positions.device != scores.device):
         raise ValueError(f"evict_keys: positions {tuple(positions.shape)} of {positions.dtype} for scores {tuple(scores.shape)}")
     if scores.shape[0] != md.num_reqs:
         raise ValueError(f"evict_keys: scores of {scores.shape[0]} requests, {md.num_reqs} in the step")
-    if _use_cuda(kv_cache):
-        _check_paged_heads(kv_cache, md, "evict_keys")
+    if cuda:
         return cuda_ops().evict_keys(kv_cache, md, scores, keep, first, recent, positions)
     return ref.evict_keys(kv_cache, md.block_table, md.seq_lens[:md.num_reqs], scores, keep, first, recent, positions, md.kv_vt)
 

@@ -550,8 +550,8 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
     return out
 
 
-_scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _f, _f,
-                      _i, _i, _vp)
+_scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _f,
+                      _f, _i, _i, _vp)
 
 
 def _key_pages(kv_cache, md, scores):
@@ -569,6 +569,11 @@ def _q_heads(q):
     return _heads(q)
 
 
+# tiles that a row counts for beside its own, as its end costs about as much: us for 24 x 60 to 924 of 16 / 8 heads of 64, 0 to 4 and 6 of them,
+# 24.5, 18.4, 16.7, 16.0, 16.0, 16.2; 64 x 1000 of 32 / 8 heads of 128 65.0, 64.3, 64.0, 64.9, 65.3, 65.3
+SCORED_EXTRA = 3
+
+
 def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=None):
     """Attention of one token per request that adds the keys' weights to ``scores`` (csrc/scored_decode.cu)."""
     if batch_invariant():                    # that kernel deals the keys of all requests to the SMs
@@ -576,23 +581,25 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
         o, lse = paged_attention(q, kv_cache, md, scale, None, soft_cap, out=out, sinks=sinks, return_lse=True)
         ops.key_weights(q, kv_cache, md, scale, lse, scores, soft_cap)
         return o
-    B, Hq, D = md.num_reqs, q.shape[1], q.shape[2]
-    Hkv, BS = kv_cache.shape[2], kv_cache.shape[3]
-    q = _q_heads(q)
+    B, (_, Hq, D), (blocks, _, Hkv, BS, _) = md.num_reqs, q.shape, kv_cache.shape
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = _q_heads(q)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.stride(2) != 1 or out.stride(1) != D:
-        raise ValueError("scored_attention: the heads of an output row are next to each other")
+        out, out_row = torch.empty_like(q, memory_format=torch.contiguous_format), Hq * D
+    else:
+        out_row, head, one = out.stride()
+        if one != 1 or head != D:
+            raise ValueError("scored_attention: the heads of an output row are next to each other")
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    G, ctas = Hq // Hkv, num_sms()
+    G, ctas, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
     n = min(B, 1024) * Hkv * -(-G // 16)
     # (of this call: two calls at once, or two captured graphs, share nothing)
-    ws = torch.empty((n + ctas) * 16 * (D + 2) + n * -(-rows // 64) * 64 * G, dtype=torch.float32, device=q.device)
-    _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks),
-                          ws.data_ptr(), B, Hq, Hkv, D, BS, rows, q.stride(0), out.stride(0), bt.stride(0), scores.stride(0), scores.stride(1), ctas, scale,
-                          soft_cap, int(md.kv_vt), _DT[q.dtype], _st()), f"scored_decode(D={D}, G={G})", 2 * -(-B // 1024))
+    ws = scores.new_empty((n + ctas) * 16 * (D + 2) + n * (-(-rows // 64) + SCORED_EXTRA) * 64 * G)
+    _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), ws.data_ptr(), B,
+                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
+                          _DT[q.dtype], _st()), "scored_decode", 2 * -(-B // 1024))
     return out
 
 
@@ -608,7 +615,9 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
         raise ValueError(f"key_weights: {Hq // Hkv} query heads for a kv head; up to 128")
     if not scale:
         raise ValueError("key_weights: a scale of 0")          # (the kernel divides by it)
-    q, lse = _q_heads(q), lse.contiguous()
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = _q_heads(q)
+    lse = lse.contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
     qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
     ctas = num_sms()
@@ -616,7 +625,7 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     _check(_key_weights(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), _p(qsl), lse.data_ptr(), scores.data_ptr(),
                         part.data_ptr(), _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, min(last or most, most), last, ctas,
                         int(batch_invariant()), q.stride(0), bt.stride(0), scores.stride(0), scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()),
-           f"key_weights(D={D}, G={Hq // Hkv})", 2)
+           "key_weights", 2)
     return scores
 
 
@@ -628,11 +637,9 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int, recent: int, positio
     """Keeps ``keep`` rows of every request and kv head (csrc/evict_keys.cu); (lengths, scores, positions)."""
     B, Hkv, L = scores.shape
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    dev = scores.device
-    new, places = torch.empty((B, Hkv, L), dtype=torch.float32, device=dev), torch.empty((B, Hkv, L), dtype=torch.int32, device=dev)
-    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    new, places, lens = scores.new_empty((B, Hkv, L)), sl.new_empty((B, Hkv, L)), sl.new_empty(B)
     cap = max(0, min(keep, rows - keep))
-    ws = torch.empty(B * Hkv * (1 + 2 * cap), dtype=torch.int32, device=dev)
+    ws = sl.new_empty(B * Hkv * (1 + 2 * cap))
     po = (0, 0) if positions is None else positions.stride()
     _check(_evict_keys(kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), scores.data_ptr(), _p(positions), new.data_ptr(), places.data_ptr(),
                        lens.data_ptr(), ws.data_ptr(), B, Hkv, kv_cache.shape[4], kv_cache.shape[3], L, rows, keep, first, recent, bt.stride(0), scores.stride(0),
