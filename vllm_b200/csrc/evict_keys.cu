@@ -1,18 +1,21 @@
 // Cutting a paged cache back: of a request's n rows a kv head keeps m = min(n, keep), those of the lowest and the newest positions and of the others those
 // of the highest scores (ties: the first row); kept rows behind row m move into the evicted rows in front of it, the i-th into the i-th.
 //
-// A row's place is a 32-bit key that orders like (protected, score); the m-th largest key is found digit by digit (11, 11 and 10 bits) from
-// counts in shared memory.  A row of up to 4096 rows is a CTA's, longer ones a cluster's, whose CTAs add their counts through distributed shared memory; the
-// keys are read from memory once and stay in shared memory.  Warps hold runs of neighbours, so ranks among equal keys, evicted and moving
-// rows are counts of bits in front.  A second kernel moves the rows: nothing is read that is written (sources lie behind m, targets in front), so the
-// order does not matter.  Filling the gaps moves as many rows as were evicted in front of m, where keeping the order would move nearly all.
+// A row's place is a 32-bit key that orders like (protected, score); the m-th largest key is found digit by digit (8 bits) from counts in shared
+// memory.  A request of up to 4096 rows is a CTA's for each kv head, longer ones a cluster's, whose CTAs add their counts through distributed
+// shared memory; the keys are made once and stay in shared memory.  Warps hold runs of neighbours, so ranks among equal keys, evicted and moving rows
+// are counts of bits in front.  What bounds it is the chain of passes and exchanges: digits of 11 bits, whose bins take longer to add up than a pass over
+// the rows, took 29 us for 64 x 1200 rows of 8 heads and 86 us for 4 x 30000.
+// A second kernel moves the rows: nothing is read that is written (sources lie behind m, targets in front), so the order does not matter.  Filling the
+// gaps moves as many rows as were evicted in front of m, where keeping the order would move nearly all.
 #include "cluster.cuh"
 
 namespace evict {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048;
+constexpr int BINS = 256, DIGITS = 4;
 constexpr uint32_t LOWEST = 0x007fffffu, PROTECTED = 0xffffffffu;        // -inf; above +inf
 constexpr int CTA_ROWS = 4096;                                           // rows of a CTA, where eight are enough for them
+constexpr int MANY = 296;                                                // CTAs from which they have 8 warps instead of 16: two for each SM
 constexpr int SMEM_ROWS = 50 * 1024;                                     // of which the keys fit; beyond 8 times that they are made anew in every pass
 
 struct Params {
@@ -35,64 +38,16 @@ VB_DEVICE uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// sum over the CTA's threads in front and over all
-VB_DEVICE int scan_block(int mine, int* sums, int& all) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) sums[w] = x;
-  __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    if (i < w) before += sums[i];
-    all += sums[i];
-  }
-  return before + x - mine;
-}
-
-// The same where each warp has one number (in all its lanes): over the warps in front, in front in the cluster too, and over the cluster.
-VB_DEVICE int scan_warps(int mine, int* sums, int* mailbox, int parts, int rank, int& all) {
-  const int w = threadIdx.x >> 5;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sums[w] = mine;
-  __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    if (i < w) before += sums[i];
-    all += sums[i];
-  }
-  if (parts > 1) {
-    if (threadIdx.x == 0) *mailbox = all;
-    cluster_sync();
-    const int cta = all;
-    all = 0;
-    for (int i = 0; i < parts; ++i) {
-      const int x = i == rank ? cta : __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(mailbox), i)));
-      if (i < rank) before += x;
-      all += x;
-    }
-  }
-  return before;
-}
-
-template <bool KEPT>                                     // the keys are kept in shared memory
+template <bool KEPT, int THREADS>                        // KEPT: the keys are kept in shared memory
 __global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
+  constexpr int WARPS = THREADS / 32;
   extern __shared__ uint32_t evict_smem[];
-  uint32_t* hist = evict_smem;                           // BINS
-  uint32_t* masks = hist + BINS;                         // a bit per row: kept (of rows of a CTA / 32 words, rounded up)
-  __shared__ int sums[WARPS], box[4];
-  __shared__ uint32_t found[2];
-  pdl_trigger();
+  uint32_t* hist = evict_smem;                           // [DIGITS][BINS]
+  uint32_t* masks = hist + DIGITS * BINS;                // a bit per row: kept (of rows of a CTA / 32 words, rounded up)
+  __shared__ int sums[2][WARPS], box[4];
+  __shared__ int all_bins[BINS], found[3];
   pdl_wait();
+  pdl_trigger();                                         // (here: the moving kernel is waiting when this one ends)
   const int rank = blockIdx.x % p.parts, row = blockIdx.x / p.parts, b = row / p.Hkv, h = row % p.Hkv;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = min(max(p.seq_lens[b], 0), p.max_rows), m = min(n, p.keep);
@@ -106,17 +61,19 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
   float* new_scores = p.new_scores + (int64_t)row * p.L;
   int* new_positions = p.new_positions + (int64_t)row * p.L;
   if (rank == 0 && h == 0 && threadIdx.x == 0) p.new_lens[b] = m;
+  for (int i = threadIdx.x; i < DIGITS * BINS; i += THREADS) hist[i] = 0;
 
   int total = n;                                         // the next position
   if (positions) {
     int top = -1;
+#pragma unroll 8
     for (int i = w0 + lane; i < w1; i += 32) top = max(top, positions[i]);
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) sums[w] = top;
+    if (lane == 0) sums[0][w] = top;
     __syncthreads();
     top = -1;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) top = max(top, sums[i]);
+    for (int i = 0; i < WARPS; ++i) top = max(top, sums[0][i]);
     if (p.parts > 1) {
       if (threadIdx.x == 0) box[0] = top;
       cluster_sync();
@@ -129,105 +86,172 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
     return place < p.first || place >= total - p.recent ? PROTECTED : ordered(scores[i]);
   };
   auto key = [&](int i) { return KEPT ? keys[i] : make(i); };
-  if (KEPT)
-    for (int i = w0 + lane; i < w1; i += 32) keys[i] = make(i);
-
-  // ---- the m-th largest key, and how many of its equals stay
-  uint32_t prefix = 0, above = 0;                        // digits found so far, and their mask
-  int need = m;
-  if (m < n) {
-#pragma unroll 1
-    for (int d = 0; d < 3; ++d) {
-      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-      for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t k = key(i);
-        if ((k & above) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
-      }
-      __syncthreads();
-      if (p.parts > 1) cluster_sync();
-      int c[BINS / THREADS], mine = 0;                   // from the highest bin down
+  constexpr int U = 4;                                   // loads on their way at a time
+  if (KEPT) {
+    for (int i0 = w0 + lane; i0 < w1; i0 += 32 * U) {
+      float x[U];
+      int place[U];
 #pragma unroll
-      for (int j = 0; j < BINS / THREADS; ++j) {
-        const int bin = BINS - 1 - (threadIdx.x * (BINS / THREADS) + j);
-        c[j] = hist[bin];
-        for (int i = 1; i < p.parts; ++i) {
-          const int r = rank + i < p.parts ? rank + i : rank + i - p.parts;
-          c[j] += __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&hist[bin]), r)));
-        }
-        mine += c[j];
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * 32, w1 - 1);
+        x[u] = scores[i];
+        place[u] = positions ? positions[i] : i;
       }
-      int all, before = scan_block(mine, sums, all);
-      if (before < need && before + mine >= need) {
 #pragma unroll
-        for (int j = 0; j < BINS / THREADS; ++j) {
-          if (before < need && before + c[j] >= need) {
-            found[0] = BINS - 1 - (threadIdx.x * (BINS / THREADS) + j);
-            found[1] = need - before;
-          }
-          before += c[j];
-        }
-      }
-      __syncthreads();
-      prefix |= found[0] << shift;
-      above |= ((1u << bits) - 1) << shift;
-      need = found[1];
-      if (p.parts > 1) cluster_sync();                   // the others have read this CTA's counts
-      __syncthreads();
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * 32 < w1) keys[i0 + u * 32] = place[u] < p.first || place[u] >= total - p.recent ? PROTECTED : ordered(x[u]);
     }
   }
-  // ---- which rows stay: a bit each
-  int equal = 0, all;
+
+  // ---- the m-th largest key, and how many of its equals stay
+  uint32_t prefix = 0;
+  int need = m;
+  bool ties = false;                                     // not all of them
   if (m < n) {
+    __syncthreads();
+#pragma unroll 1
+    for (int d = 0; d < DIGITS; ++d) {
+      const int shift = 24 - 8 * d;
+      const uint32_t above = d == 0 ? 0u : 0xffffffffu << (shift + 8);
+      uint32_t* bins = hist + d * BINS;
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const uint32_t k = key(i);
+        if ((k & above) == prefix) atomicAdd(&bins[k >> shift & 255], 1u);
+      }
+      if (p.parts > 1) {
+        cluster_sync();
+        for (int bin = threadIdx.x; bin < BINS; bin += THREADS) {
+          int c = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < p.parts) c += __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&bins[bin]), i)));
+          all_bins[bin] = c;
+        }
+      }
+      __syncthreads();
+      if (w == 0) {                                      // eight bins a lane, from the highest down
+        const int* from = p.parts > 1 ? all_bins : reinterpret_cast<const int*>(bins);
+        int c[8], mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mine += c[j] = from[BINS - 1 - (lane * 8 + j)];
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        int before = x - mine;
+        if (before < need && before + mine >= need) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (before < need && before + c[j] >= need) {
+              found[0] = BINS - 1 - (lane * 8 + j);
+              found[1] = need - before;
+              found[2] = c[j];
+            }
+            before += c[j];
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= (uint32_t)found[0] << shift;
+      need = found[1];
+      ties = need < found[2];
+    }
+  }
+  // The same number of a warp in all its lanes: sums over the warps in front, in front in the cluster too, and over the cluster, for two of them.
+  auto scan_two = [&](int& x, int& y, int& all_x, int slot) {
+    __syncthreads();
+    if (lane == 0) { sums[0][w] = x; sums[1][w] = y; }
+    __syncthreads();
+    int bx = 0, by = 0, ax = 0, ay = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      if (i < w) { bx += sums[0][i]; by += sums[1][i]; }
+      ax += sums[0][i]; ay += sums[1][i];
+    }
+    if (p.parts > 1) {
+      if (threadIdx.x == 0) { box[slot] = ax; box[slot + 1] = ay; }
+      cluster_sync();
+      const int own = ax;
+      ax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < p.parts) {
+          const int vx = i == rank ? own : __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&box[slot]), i)));
+          const int vy = i < rank ? __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(&box[slot + 1]), i))) : 0;
+          if (i < rank) { bx += vx; by += vy; }
+          ax += vx;
+        }
+      }
+    }
+    x = bx; y = by; all_x = ax;
+  };
+  // ---- which rows stay: a bit each
+  int equal = 0, none = 0, all;
+  if (ties) {
     for (int i = w0; i < w1; i += 32) equal += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(i + lane) == prefix));
-    equal = scan_warps(equal, sums, &box[1], p.parts, rank, all);
+    scan_two(equal, none, all, 0);
   }
   int holes = 0, movers = 0;
   for (int i = w0; i < w1; i += 32) {
     const bool there = i + lane < w1;
-    uint32_t stay;
+    const uint32_t here = w1 - i >= 32 ? 0xffffffffu : (1u << (w1 - i)) - 1;
+    uint32_t stay = here;
     if (m < n) {
       const uint32_t k = there ? key(i + lane) : 0u;
-      const uint32_t same = __ballot_sync(0xffffffffu, there && k == prefix);
-      const bool s = there && (k > prefix || (k == prefix && equal + __popc(same & ((1u << lane) - 1)) < need));
-      equal += __popc(same);
-      stay = __ballot_sync(0xffffffffu, s);
-    } else {
-      stay = __ballot_sync(0xffffffffu, there);
+      if (ties) {
+        const uint32_t same = __ballot_sync(0xffffffffu, there && k == prefix);
+        stay = __ballot_sync(0xffffffffu, there && (k > prefix || (k == prefix && equal + __popc(same & ((1u << lane) - 1)) < need)));
+        equal += __popc(same);
+      } else {
+        stay = __ballot_sync(0xffffffffu, there && k >= prefix);
+      }
     }
-    const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1, here = __ballot_sync(0xffffffffu, there);
+    const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1;
     holes += __popc(~stay & front & here);
     movers += __popc(stay & ~front);
     if (lane == 0) masks[(i - lo) >> 5] = stay;
   }
   __syncwarp();
-  int n_holes, n_movers;
-  holes = scan_warps(holes, sums, &box[2], p.parts, rank, n_holes);
-  movers = scan_warps(movers, sums, &box[3], p.parts, rank, n_movers);
+  int n_holes;
+  scan_two(holes, movers, n_holes, 2);
   if (rank == 0 && threadIdx.x == 0) p.count[row] = n_holes;
   // ---- lists, and scores and positions of the rows that do not move
   int* target = p.target + (int64_t)row * p.cap;
   int* source = p.source + (int64_t)row * p.cap;
-  for (int i = w0; i < w1; i += 32) {
-    const uint32_t stay = masks[(i - lo) >> 5];
-    const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1;
-    const uint32_t here = w1 - i >= 32 ? 0xffffffffu : (1u << (w1 - i)) - 1, me = 1u << lane;
-    const uint32_t hole = ~stay & front & here, mover = stay & ~front;
-    if (hole & me) target[holes + __popc(hole & (me - 1))] = i + lane;
-    if (mover & me) source[movers + __popc(mover & (me - 1))] = i + lane;
-    if (stay & front & me) {
-      new_scores[i + lane] = scores[i + lane];
-      new_positions[i + lane] = positions ? positions[i + lane] : i + lane;
+  for (int i0 = w0; i0 < w1; i0 += 32 * U) {
+    float x[U];
+    int place[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 32 + lane;
+      x[u] = i < min(w1, m) ? scores[i] : 0.f;
+      place[u] = positions && i < min(w1, m) ? positions[i] : i;
     }
-    holes += __popc(hole);
-    movers += __popc(mover);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 32;
+      if (i >= w1) break;
+      const uint32_t stay = masks[(i - lo) >> 5];
+      const uint32_t front = i >= m ? 0u : m - i >= 32 ? 0xffffffffu : (1u << (m - i)) - 1;
+      const uint32_t here = w1 - i >= 32 ? 0xffffffffu : (1u << (w1 - i)) - 1, me = 1u << lane;
+      const uint32_t hole = ~stay & front & here, mover = stay & ~front;
+      if (hole & me) target[holes + __popc(hole & (me - 1))] = i + lane;
+      if (mover & me) source[movers + __popc(mover & (me - 1))] = i + lane;
+      if (stay & front & me) {
+        new_scores[i + lane] = x[u];
+        new_positions[i + lane] = place[u];
+      }
+      holes += __popc(hole);
+      movers += __popc(mover);
+    }
   }
   for (int i = m + rank * THREADS + threadIdx.x; i < p.L; i += p.parts * THREADS) {
     new_scores[i] = 0.f;
     new_positions[i] = total + i - m;
   }
-  if (p.parts > 1) cluster_sync();                       // the others may still read this CTA's mailboxes
+  if (p.parts > 1) cluster_sync();                       // the others may still read this CTA's counts and mailboxes
 }
 
 struct Move {
@@ -313,11 +337,15 @@ EXPORT int vb_evict_keys(void* cache, int64_t num_blocks, const int* block_table
   while (p.parts < 8 && max_rows > CTA_ROWS * p.parts) p.parts *= 2;
   const int rows = (max_rows + p.parts - 1) / p.parts + 32;
   const bool kept = rows <= SMEM_ROWS;
-  const size_t smem = (size_t)(BINS + (max_rows / p.parts + 63) / 32 + 1 + (kept ? rows : 0)) * 4;
+  const size_t smem = (size_t)(DIGITS * BINS + (max_rows / p.parts + 63) / 32 + 1 + (kept ? rows : 0)) * 4;
   if (smem > 227 * 1024) return -3;
-  auto k = kept ? select_kernel<true> : select_kernel<false>;
+  // Few CTAs wait for their chains, many for instructions that every warp has of its own.  us of both kernels with 8 and 16 warps: 1 request of 700 rows
+  // (8 CTAs) 10.8 and 10.2, 16 of 2000 (64) 22.4 and 14.0, 64 of 1200 (512) 74.3 and 77.4, 4 of 30000 (256 in clusters) 97.5 and 82.9
+  const bool many = p.parts == 1 && (int64_t)B * Hkv > MANY;
+  auto k = !kept ? select_kernel<false, 512> : many ? select_kernel<true, 256> : select_kernel<true, 512>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)cudaGetLastError();
-  if (vb_launch_parts(k, dim3((unsigned)(B * Hkv * p.parts)), dim3(THREADS), smem, st, (unsigned)p.parts, p) != cudaSuccess) return (int)cudaGetLastError();
+  if (vb_launch_parts(k, dim3((unsigned)(B * Hkv * p.parts)), dim3(many ? 256 : 512), smem, st, (unsigned)p.parts, p) != cudaSuccess)
+    return (int)cudaGetLastError();
   if (cap > 0) {
     Move mv{scores, positions, new_scores, new_positions, p.count, p.target, p.source, reinterpret_cast<uint16_t*>(cache), block_table,
             sc_req, sc_head, po_req, po_head, bt_stride, num_blocks, Hkv, L, cap, D, BS};
