@@ -20,7 +20,7 @@
 namespace sdec {
 
 constexpr int TILE = 64, STRIP = 16;
-constexpr int MAX_REQUESTS = 1024;          // of a launch: their first tiles lie in shared memory
+constexpr int MAX_REQUESTS = 512;           // of a launch: their first tiles lie in shared memory
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
@@ -31,11 +31,12 @@ struct Params {
   void* out;
   float* scores;
   const float* sinks;
-  float* raw;              // [tile of a row][64][G]: scores in powers of two
-  float* part;             // [segment][G][D + 2]: output, maximum, sum
+  float* raw;              // [request][kv head][raw_rows][G]: scores in powers of two
+  float* part;             // [segment][16][D + 2]: output, maximum, sum
+  int2* info;              // [row]: its first CTA, and how many
   int64_t q_stride, out_stride, bt_stride, sc_req, sc_head;
   int64_t num_blocks;
-  int B, Hkv, G, D, BS, max_rows, ctas, chunks, extra;      // chunks: of at most 16 query heads of a kv head
+  int B, Hkv, G, D, BS, max_rows, raw_rows, ctas, chunks, extra, block;      // chunks: of at most 16 query heads of a kv head
   float scale_log2, ku, c2;
 };
 
@@ -126,7 +127,7 @@ VB_DEVICE uint32_t turn8(uint32_t x) { uint32_t r; asm("movmatrix.sync.aligned.m
 
 // DP: head size, rounded up to 64, 128 or 256 (what is behind it is zeros in shared memory); NT: groups of eight query heads
 template <int DP_> struct Form {
-  static constexpr int DP = DP_, WARPS = DP == 256 ? 4 : 8, THREADS = WARPS * 32;
+  static constexpr int DP = DP_, WARPS = 4, THREADS = WARPS * 32, CTAS = DP == 256 ? 1 : 2;      // CTAS: of an SM
   static constexpr int STRIP_BYTES = STRIP * DP * 2;                       // of keys; values behind them
   static constexpr int STAGES = DP == 64 ? 6 : 3;
   static constexpr int RING = WARPS * STAGES * 2 * STRIP_BYTES;
@@ -135,7 +136,7 @@ template <int DP_> struct Form {
 };
 
 template <typename T, int DP, int NT, bool VT, bool CAP>
-__global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kernel(const Params p) {
   using F = Form<DP>;
   // The reference of a head's weights is its largest score less SHIFT, or up to 8 below that.  fp16 has no values under 2^-24: as multiples of 2^-32 of the
   // largest weight the tail of a long request is not lost.
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
         }
         const bool cut = tok + STRIP > n;
         const bool in[2] = {!cut || tok + r0 < n, !cut || tok + 8 + r0 < n};
-        float* raw = p.raw + ((int64_t)(row.begin - row.hc % p.chunks * (row.end - row.begin)) * TILE + tok) * p.G + g0;
+        float* raw = p.raw + ((int64_t)(row.b * p.Hkv + row.hc / p.chunks) * p.raw_rows + tok) * p.G + g0;
         uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -351,6 +352,8 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
     // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
     float* part = p.part + (int64_t)(row.index + blockIdx.x) * 16 * (p.D + 2);
     const bool empty = max(row.begin, t0) >= row.begin + (n + TILE - 1) / TILE;      // nothing but the row's further slots
+    if (!empty && row.begin >= t0 && threadIdx.x == 0)
+      p.info[row.index] = make_int2(blockIdx.x, (row.begin + (n + TILE - 1) / TILE - 1) / per - blockIdx.x + 1);
     const bool more = row.end < t1;
     if (more) {                              // (the next row's queries are on their way meanwhile)
       next_row(first, H, row);
@@ -414,106 +417,118 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, 1) decode_kernel(const Para
   cp_async_wait<0>();
 }
 
-// Grid (blocks of KEYS keys, kv heads, requests): the first block of a row joins its outputs; every block adds the weights of its keys.
-constexpr int KEYS = 1024, JOIN = 256, FACTORS = 32;
+// Grid (blocks of p.block keys, kv heads, requests): joins a row's outputs and adds the weights of its keys.  It is a chain of reads from memory (the row's
+// parts, then what they say), so what does not wait for another read is read first, and there are as many blocks as the SMs hold at a time.
+constexpr int JOIN = 256, JOINERS = 4, U = 4, KEYS = U * JOIN, FACTORS = 32;      // JOINERS: blocks of an SM
 template <typename T>
-__global__ void __launch_bounds__(JOIN) join_kernel(const Params p) {
+__global__ void __launch_bounds__(JOIN, JOINERS) join_kernel(const Params p) {
   extern __shared__ float join_smem[];                // of the G heads: log-sum-exp in powers of two, then a factor for each of the first FACTORS parts
-  __shared__ int sums[2][JOIN / 32];
   pdl_trigger();
-  const int b = blockIdx.z, h = blockIdx.y, H = p.Hkv * p.chunks, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = rows_of(p, b);
-  const int key0 = blockIdx.x * KEYS;
-  if (key0 >= n && blockIdx.x > 0) return;
-  // tiles in front of the request, and all
-  int mine = 0, all = 0;
-  for (int i = threadIdx.x; i < p.B; i += JOIN) {
-    const int t = slots_of(p, rows_of(p, i));
-    all += t;
-    if (i < b) mine += t;
-  }
-  mine = __reduce_add_sync(0xffffffffu, mine);
-  all = __reduce_add_sync(0xffffffffu, all);
-  if (lane == 0) { sums[0][w] = mine; sums[1][w] = all; }
-  __syncthreads();
-  mine = all = 0;
-#pragma unroll
-  for (int i = 0; i < JOIN / 32; ++i) { mine += sums[0][i]; all += sums[1][i]; }
-  const int per = (all * H + p.ctas - 1) / p.ctas, tiles = (n + TILE - 1) / TILE, slots = slots_of(p, n);
-  const int PD = p.D + 2;
-  float* factors = join_smem + ((p.G + 3) & ~3);
   pdl_wait();
-  // parts of a head: segments of CTAs a .. z, at row + CTA
-  auto parts = [&](int g, int& a, int& z) -> const float* {
-    const int hc = h * p.chunks + g / 16, begin = mine * H + hc * slots;
-    a = tiles > 0 ? begin / per : 0;
-    z = tiles > 0 ? (begin + tiles - 1) / per : -1;
-    return p.part + ((int64_t)(b * H + hc + a) * 16 + g % 16) * PD;
+  const int b = blockIdx.z, h = blockIdx.y, H = p.Hkv * p.chunks, lane = threadIdx.x & 31, w = threadIdx.x >> 5, PD = p.D + 2;
+  const int n = rows_of(p, b), end = min(((int)blockIdx.x + 1) * p.block, n);
+  int key0 = blockIdx.x * p.block;
+  // the keys' scores so far, and what the first four heads say of them
+  const float* raw = p.raw + (int64_t)(b * p.Hkv + h) * p.raw_rows * p.G;
+  float* sc = p.scores + b * p.sc_req + h * p.sc_head;
+  const bool four = p.G % 4 == 0;
+  float old[U];
+  float4 x4[U];
+  auto read_keys = [&]() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = key0 + u * JOIN + threadIdx.x;
+      old[u] = k < end ? sc[k] : 0.f;
+      x4[u] = four && k < end ? *reinterpret_cast<const float4*>(raw + (int64_t)k * p.G) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   };
+  read_keys();
+  // parts of a head: segments of CTAs, at row + CTA
+  const int64_t step = (int64_t)16 * PD;
+  auto parts = [&](int g, int& count) -> const float* {
+    const int row = b * H + h * p.chunks + g / 16;
+    const int2 at = n > 0 ? p.info[row] : make_int2(0, 0);
+    count = at.y;
+    return p.part + ((int64_t)(row + at.x) * 16 + g % 16) * PD;
+  };
+  float* factors = join_smem + ((p.G + 3) & ~3);
   for (int g = w; g < p.G; g += JOIN / 32) {          // a warp: log-sum-exp of a head, its parts and the sink
-    int a, z;
-    const float* x = parts(g, a, z) + p.D;
+    int count;
+    const float* x = parts(g, count) + p.D;
     const float sink = p.sinks ? p.sinks[h * p.G + g] * LOG2E : -INFINITY;
-    float m = sink;
-    for (int c = lane; c <= z - a; c += 32) m = fmaxf(m, x[(int64_t)c * 16 * PD]);
+    const float m0 = lane < count ? x[lane * step] : -INFINITY, l0 = lane < count ? x[lane * step + 1] : 0.f;
+    float m = fmaxf(m0, sink);
+    for (int c = 32 + lane; c < count; c += 32) m = fmaxf(m, x[c * step]);
     m = warp_max(m);
     const float top = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int c = lane; c <= z - a; c += 32) l += x[(int64_t)c * 16 * PD + 1] * ex2(x[(int64_t)c * 16 * PD] - top);
+    float l = l0 * ex2(m0 - top);
+    for (int c = 32 + lane; c < count; c += 32) l += x[c * step + 1] * ex2(x[c * step] - top);
     l = warp_sum(l) + (p.sinks ? ex2(sink - top) : 0.f);
     const float lse = l > 0.f ? top + log2f(l) : INFINITY;                  // no key and no sink: weights of 0
     if (lane == 0) join_smem[g] = lse;
-    factors[g * FACTORS + lane] = lane <= z - a ? ex2(x[(int64_t)lane * 16 * PD] - lse) : 0.f;
+    factors[g * FACTORS + lane] = ex2(m0 - lse);
+  }
+  // the thread's first output: its first parts
+  constexpr int AHEAD = 8;
+  float o[AHEAD];
+  auto read_parts = [&](const float* x, int from, int count) {
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) o[c] = from + c < count ? x[(from + c) * step] : 0.f;
+  };
+  const int first = blockIdx.x * JOIN + threadIdx.x;
+  if (first < p.G * p.D) {
+    int count;
+    const float* x = parts(first / p.D, count);
+    read_parts(x + first % p.D, 0, count);
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < p.G * p.D; i += JOIN) {
-      const int g = i / p.D, d = i % p.D;
-      int a, z;
-      const float* x = parts(g, a, z);
-      float acc = 0.f;
-#pragma unroll 4
-      for (int c = 0; c <= min(z - a, FACTORS - 1); ++c) acc += x[(int64_t)c * 16 * PD + d] * factors[g * FACTORS + c];
-      for (int c = FACTORS; c <= z - a; ++c) acc += x[(int64_t)c * 16 * PD + d] * ex2(x[(int64_t)c * 16 * PD + p.D] - join_smem[g]);
-      reinterpret_cast<T*>(p.out)[b * p.out_stride + (int64_t)(h * p.G + g) * p.D + d] = from_f32<T>(acc);
+  for (int i = first; i < p.G * p.D; i += gridDim.x * JOIN) {
+    const int g = i / p.D;
+    int count;
+    const float* x = parts(g, count) + i % p.D;
+    float acc = 0.f;
+    for (int from = 0; from < count; from += AHEAD) {
+      if (from > 0 || i != first) read_parts(x, from, count);
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) {
+        const int at = from + c;
+        if (at < count) acc += o[c] * (at < FACTORS ? factors[g * FACTORS + at] : ex2(x[at * step + p.D - i % p.D] - join_smem[g]));
+      }
     }
+    reinterpret_cast<T*>(p.out)[b * p.out_stride + (int64_t)h * p.G * p.D + i] = from_f32<T>(acc);
   }
-  const float* raw = p.raw + ((int64_t)mine * H + (int64_t)h * p.chunks * slots) * TILE * p.G;
-  float* sc = p.scores + b * p.sc_req + h * p.sc_head;
-  const int end = min(key0 + KEYS, n);
-  constexpr int U = KEYS / JOIN;
-  float add[U] = {0.f, 0.f, 0.f, 0.f}, old[U];
+  while (key0 < end) {
+    float sum[U] = {0.f, 0.f, 0.f, 0.f};
+    if (four) {
+      for (int g = 0; g < p.G; g += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(join_smem + g);
+        if (g > 0) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int k = key0 + u * JOIN + threadIdx.x;
-    old[u] = k < end ? sc[k] : 0.f;
-  }
-  if (p.G % 4 == 0) {
-    for (int g = 0; g < p.G; g += 4) {
-      const float4 l = *reinterpret_cast<const float4*>(join_smem + g);
+          for (int u = 0; u < U; ++u) {
+            const int k = key0 + u * JOIN + threadIdx.x;
+            if (k < end) x4[u] = *reinterpret_cast<const float4*>(raw + (int64_t)k * p.G + g);
+          }
+        }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = key0 + u * JOIN + threadIdx.x;
-        if (k < end) {
-          const float4 x = *reinterpret_cast<const float4*>(raw + (int64_t)k * p.G + g);
-          add[u] += (ex2(x.x - l.x) + ex2(x.y - l.y)) + (ex2(x.z - l.z) + ex2(x.w - l.w));
+        for (int u = 0; u < U; ++u) sum[u] += (ex2(x4[u].x - l.x) + ex2(x4[u].y - l.y)) + (ex2(x4[u].z - l.z) + ex2(x4[u].w - l.w));
+      }
+    } else {
+      for (int g = 0; g < p.G; ++g) {
+        const float l = join_smem[g];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = key0 + u * JOIN + threadIdx.x;
+          if (k < end) sum[u] += ex2(raw[(int64_t)k * p.G + g] - l);
         }
       }
     }
-  } else {
-    for (int g = 0; g < p.G; ++g) {
-      const float l = join_smem[g];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = key0 + u * JOIN + threadIdx.x;
-        if (k < end) add[u] += ex2(raw[(int64_t)k * p.G + g] - l);
-      }
+    for (int u = 0; u < U; ++u) {
+      const int k = key0 + u * JOIN + threadIdx.x;
+      if (k < end) sc[k] = old[u] + sum[u];
     }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int k = key0 + u * JOIN + threadIdx.x;
-    if (k < end) sc[k] = old[u] + add[u];
+    key0 += KEYS;
+    if (key0 < end) read_keys();
   }
 }
 
@@ -527,7 +542,7 @@ static int launch(const Params& p, cudaStream_t st) {
     set = true;
   }
   vb_launch(k, dim3(p.ctas), dim3(F::THREADS), (size_t)F::SMEM, st, p);
-  vb_launch(join_kernel<T>, dim3((p.max_rows + KEYS - 1) / KEYS, p.Hkv, p.B), dim3(JOIN), (size_t)(((p.G + 3) & ~3) + p.G * FACTORS) * 4, st, p);
+  vb_launch(join_kernel<T>, dim3((p.max_rows + p.block - 1) / p.block, p.Hkv, p.B), dim3(JOIN), (size_t)(((p.G + 3) & ~3) + p.G * FACTORS) * 4, st, p);
   return (int)cudaGetLastError();
 }
 template <typename T, int DP, bool VT>
@@ -546,12 +561,12 @@ static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
 }  // namespace sdec
 
 
-// `ws`: for rows = min(B, 1024) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + rows (ceil(max_rows / 64) + extra) 64 G floats.  extra: tiles
+// `ws`: for rows = min(B, 512) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + min(B, 512) Hq ceil(max_rows / 64) 64 + 2 rows floats.  extra: tiles
 // that a row counts for beside its own.  max_rows: rows of a request that the block
 // table and the scores have room for.
 EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, void* out, float* scores,
                             const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int64_t q_stride, int64_t out_stride,
-                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int extra, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
+                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int sms, int extra, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
   using namespace sdec;
   if (B <= 0) return 0;
   if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1) return -1;
@@ -559,6 +574,7 @@ EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks
   p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16; p.extra = extra;
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head;
   p.num_blocks = num_blocks; p.cache = cache; p.sinks = sinks;
+  p.raw_rows = (max_rows + TILE - 1) / TILE * TILE;
   p.scale_log2 = scale * LOG2E;
   p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E;
   for (int b0 = 0; b0 < B; b0 += MAX_REQUESTS) {
@@ -571,8 +587,11 @@ EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks
     const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE + p.extra);
     if (tiles >= (1 << 29)) return -3;                 // flat strip numbers are 32 bits
     p.ctas = ctas < tiles ? ctas : (int)tiles;
+    const int64_t blocks = JOINERS * (int64_t)sms / ((int64_t)p.B * Hkv), most = (max_rows + JOIN - 1) / JOIN;
+    p.block = (int)((most + (blocks < 1 ? 1 : blocks) - 1) / (blocks < 1 ? 1 : blocks)) * JOIN;
     p.part = ws;
     p.raw = ws + (rows + p.ctas) * 16 * (D + 2);
+    p.info = reinterpret_cast<int2*>(p.raw + (int64_t)p.B * Hq * p.raw_rows);
     const int rc = dtype == DT_BF16 ? go<__nv_bfloat16>(p, vt != 0, soft_cap > 0.f, st) : go<__half>(p, vt != 0, soft_cap > 0.f, st);
     if (rc) return rc;
   }

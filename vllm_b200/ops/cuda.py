@@ -550,8 +550,8 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
     return out
 
 
-_scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _f,
-                      _f, _i, _i, _vp)
+_scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i,
+                      _f, _f, _i, _i, _vp)
 
 
 def _key_pages(kv_cache, md, scores):
@@ -593,13 +593,14 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    G, ctas, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
-    n = min(B, 1024) * Hkv * -(-G // 16)
+    G, ctas, (sc_req, sc_head, _) = Hq // Hkv, num_sms() * (2 if D <= 128 else 1), scores.stride()
+    n = min(B, 512) * Hkv
     # (of this call: two calls at once, or two captured graphs, share nothing)
-    ws = scores.new_empty((n + ctas) * 16 * (D + 2) + n * (-(-rows // 64) + SCORED_EXTRA) * 64 * G)
+    heads = n * -(-G // 16)
+    ws = scores.new_empty((heads + ctas) * 16 * (D + 2) + n * G * -(-rows // 64) * 64 + 2 * heads)
     _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), ws.data_ptr(), B,
-                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
-                          _DT[q.dtype], _st()), "scored_decode", 2 * -(-B // 1024))
+                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, num_sms(), SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
+                          _DT[q.dtype], _st()), "scored_decode", 2 * -(-B // 512))
     return out
 
 
