@@ -220,31 +220,32 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
 _F32 = torch.float32
 
 
-def _check_scores(scores, kv_cache, md, op: str, cuda: bool) -> tuple[int, int, int]:
-    """Scores beside a paged cache, and what the kernels over both take; (kv heads, page, head size)."""
-    if scores.dtype is not _F32 or scores.dim() != 3 or scores.stride(2) != 1:
+def _check_scores(scores, kv_cache, md, op: str, cuda: bool) -> tuple[int, int]:
+    """Scores beside a paged cache, and what the kernels over both take; (kv heads, head size)."""
+    shape, rows = kv_cache.shape, scores.shape
+    if scores.dtype is not _F32 or len(rows) != 3 or scores.stride(2) != 1:
         raise ValueError(f"{op}: scores are fp32 [requests, kv heads, rows] with rows next to each other")
-    if kv_cache.dim() != 5 or scores.device != kv_cache.device:
+    if len(shape) != 5 or scores.get_device() != kv_cache.get_device():
         raise ValueError(f"{op}: a cache [blocks, 2, kv heads, page, head size] and scores on its device")
-    _, _, H, BS, D = kv_cache.shape
-    R, Hs, L = scores.shape
-    if R < md.num_reqs or Hs != H or L < md.max_seq_len:
-        raise ValueError(f"{op}: scores of {tuple(scores.shape)} for {md.num_reqs} requests of up to {md.max_seq_len} rows and {H} kv heads")
+    _, _, H, BS, D = shape
+    if rows[0] < md.num_reqs or rows[1] != H or rows[2] < md.max_seq_len:
+        raise ValueError(f"{op}: scores of {tuple(rows)} for {md.num_reqs} requests of up to {md.max_seq_len} rows and {H} kv heads")
     if cuda:
         if kv_cache.dtype not in _HALF or D % 8 or D > 256 or BS % 16 or not kv_cache.is_contiguous():
             raise ValueError(f"{op}: 16-bit caches, heads of up to 256 in steps of 8, pages in steps of 16; got {kv_cache.dtype}, {D}, {BS}")
         if md.kv_vt and (D != 128 or BS != 64):
             raise ValueError(f"{op}: transposed values are of heads of 128 and pages of 64")
-    return H, BS, D
+    return H, D
 
 
 def _check_queries(q, kv_cache, md, H: int, D: int, op: str) -> None:
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H or q.dtype != kv_cache.dtype or q.device != kv_cache.device:
-        raise ValueError(f"{op}: queries {tuple(q.shape)} of {q.dtype} for a cache of {H} heads of {D}, {kv_cache.dtype}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] % H or q.dtype is not kv_cache.dtype or q.get_device() != kv_cache.get_device():
+        raise ValueError(f"{op}: queries {tuple(shape)} of {q.dtype} for a cache of {H} heads of {D}, {kv_cache.dtype}")
     if not md.causal:
         raise ValueError(f"{op}: causal attention only")
-    if md.decode_only and q.shape[0] < md.num_reqs:
-        raise ValueError(f"{op}: {q.shape[0]} queries for {md.num_reqs} requests")
+    if md.decode_only and shape[0] < md.num_reqs:
+        raise ValueError(f"{op}: {shape[0]} queries for {md.num_reqs} requests")
 
 
 def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.0, sinks: Optional[torch.Tensor] = None, last: int = 0,
@@ -254,7 +255,7 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
     output.  Rows of ``scores`` behind a request's last key stay as they are; rows that are not in the cache yet have to be 0 when they come.
     No two requests may share a row of ``scores``."""
     cuda = _use_cuda(q)
-    H, _, D = _check_scores(scores, kv_cache, md, "scored_attention", cuda)
+    H, D = _check_scores(scores, kv_cache, md, "scored_attention", cuda)
     _check_queries(q, kv_cache, md, H, D, "scored_attention")
     if last < 0:
         raise ValueError(f"scored_attention: last {last}")
@@ -276,7 +277,7 @@ def key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap: float = 0.
     key and the query heads of the kv head.  ``lse`` [T, query heads]: what ``paged_attention(..., return_lse=True)`` returns; a row where it is
     -inf (no key) or NaN gives nothing.  Returns ``scores``."""
     cuda = _use_cuda(q)
-    H, _, D = _check_scores(scores, kv_cache, md, "key_weights", cuda)
+    H, D = _check_scores(scores, kv_cache, md, "key_weights", cuda)
     _check_queries(q, kv_cache, md, H, D, "key_weights")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device or last < 0:
         raise ValueError(f"key_weights: lse {tuple(lse.shape)} of {lse.dtype} for queries {tuple(q.shape)}, last {last}")

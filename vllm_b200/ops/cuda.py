@@ -554,11 +554,16 @@ _scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _v
                       _f, _f, _i, _i, _vp)
 
 
+_I32 = torch.int32
+
+
 def _key_pages(kv_cache, md, scores):
     """(block table, lengths, rows that both the table and ``scores`` have room for) of kernels over paged keys; they read no row behind that."""
     bt, sl = md.block_table, md.seq_lens
-    if bt.dtype != torch.int32 or bt.stride(1) != 1 or sl.dtype != torch.int32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
+    if bt.dtype is not _I32 or bt.stride(1) != 1 or sl.dtype is not _I32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
         raise ValueError("paged keys: a 16-byte aligned cache, int32 block tables with a request's pages next to each other, int32 lengths")
+    if scores.get_device() != _device():
+        raise ValueError(f"paged keys: tensors of device {scores.get_device()} while {_device()} is the current one")
     return bt, sl, min(bt.shape[1] * kv_cache.shape[3], scores.shape[2])
 
 
@@ -586,6 +591,8 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
         q = _q_heads(q)
     if out is None:
         out, out_row = torch.empty_like(q, memory_format=torch.contiguous_format), Hq * D
+        if q.shape[0] > B:                   # (padding rows are written by no CTA: keep them finite)
+            out[B:].zero_()
     else:
         out_row, head, one = out.stride()
         if one != 1 or head != D:
@@ -593,13 +600,14 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    G, ctas, (sc_req, sc_head, _) = Hq // Hkv, num_sms() * (2 if D <= 128 else 1), scores.stride()
+    G, sms, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
+    ctas = sms * (2 if D <= 128 else 1)
     n = min(B, 512) * Hkv
     # (of this call: two calls at once, or two captured graphs, share nothing)
     heads = n * -(-G // 16)
     ws = scores.new_empty((heads + ctas) * 16 * (D + 2) + n * G * -(-rows // 64) * 64 + 2 * heads)
     _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), ws.data_ptr(), B,
-                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, num_sms(), SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
+                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, sms, SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
                           _DT[q.dtype], _st()), "scored_decode", 2 * -(-B // 512))
     return out
 
@@ -621,6 +629,8 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     lse = lse.contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
     qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
+    if qsl is not None and (qsl.dtype is not _I32 or not qsl.is_contiguous()):
+        raise ValueError("key_weights: int32 query offsets")
     ctas = num_sms()
     part = scores.new_empty(ctas * 512)
     _check(_key_weights(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), _p(qsl), lse.data_ptr(), scores.data_ptr(),
@@ -638,7 +648,8 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int, recent: int, positio
     """Keeps ``keep`` rows of every request and kv head (csrc/evict_keys.cu); (lengths, scores, positions)."""
     B, Hkv, L = scores.shape
     bt, sl, rows = _key_pages(kv_cache, md, scores)
-    new, places, lens = scores.new_empty((B, Hkv, L)), sl.new_empty((B, Hkv, L)), sl.new_empty(B)
+    new = torch.empty_like(scores, memory_format=torch.contiguous_format)
+    places, lens = torch.empty_like(new, dtype=torch.int32), torch.empty_like(sl) if sl.shape[0] == B else sl.new_empty(B)
     cap = max(0, min(keep, rows - keep))
     ws = sl.new_empty(B * Hkv * (1 + 2 * cap))
     po = (0, 0) if positions is None else positions.stride()
