@@ -6,6 +6,7 @@ import torch
 
 from tests.key_budget_oracle import attend, evict, step, unit, weight_error
 from vllm_b200 import ops
+from vllm_b200.ops import cuda_ops
 
 pytestmark = pytest.mark.gpu
 LENS = [1, 15, 16, 17, 63, 64, 65, 300, 1030]
@@ -38,17 +39,24 @@ def _check_decode(q, cache, md, scores, cap=0.0, sinks=None, scale=None, out=Non
                                             (6, 6, 80, 16, False), (8, 2, 96, 48, False), (20, 1, 128, 32, False), (40, 1, 128, 64, True), (4, 2, 256, 64, False),
                                             (16, 1, 256, 16, False), (2, 1, 8, 16, False), (5, 1, 72, 128, False)])
 @pytest.mark.parametrize("cap,sink", [(0.0, False), (30.0, True)])
-def test_decode(dtype, Hq, Hkv, D, BS, vt, cap, sink):
+@pytest.mark.parametrize("runs", [False, True])
+def test_decode(dtype, Hq, Hkv, D, BS, vt, cap, sink, runs, monkeypatch):
+    """In clusters where the sizes allow it, and in runs of equal length."""
+    if runs:
+        monkeypatch.setattr(cuda_ops(), "scored_parts", lambda *a: 0)
     q, cache, md, scores = step(LENS, [1] * len(LENS), Hq, Hkv, D, BS, dtype, "cuda", vt=vt, seed=Hq + D, spread=2.0)
     sinks = torch.randn(Hq, device="cuda") if sink else None
     _check_decode(q, cache, md, scores, cap, sinks)
 
 
-@pytest.mark.parametrize("lens", [[1], [0], [0, 40, 0, 0, 7, 0], [5000], [64] * 200, [1] * 700, [17000, 3, 9001], [2000] * 40, [700] * 3 + [0] * 1100 + [33] * 2])
+@pytest.mark.parametrize("lens", [[1], [0], [0, 40, 0, 0, 7, 0], [5000], [2048], [2047, 130], [64, 0, 65], [64] * 200, [1] * 700, [17000, 3, 9001], [2000] * 40, [700] * 3 + [0] * 1100 + [33] * 2])
 @pytest.mark.parametrize("vt", [True, False])
-def test_decode_lengths(lens, vt):
+@pytest.mark.parametrize("room", [0, 2048])
+def test_decode_lengths(lens, vt, room):
     Hq, Hkv = (32, 8) if len(lens) < 300 else (2, 1)
-    q, cache, md, scores = step(lens, [1] * len(lens), Hq, Hkv, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=len(lens))
+    q, cache, md, scores = step(lens, [1] * len(lens), Hq, Hkv, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=len(lens), room=max(room, max(lens) + 5))
+    if room:                                  # a table for as many rows
+        md.block_table = torch.nn.functional.pad(md.block_table, (0, max(0, 32 - md.block_table.shape[1])))
     _check_decode(q, cache, md, scores)
 
 

@@ -9,13 +9,19 @@
 // the weights.
 //
 // First kernel: rows are pairs (request, kv head); all their tiles of 64 keys, in order, are dealt to the CTAs in equal runs, so that ragged and
-// few long requests keep all SMs as busy as many equal ones.  In a run a warp takes every eighth strip of 16 keys through
+// few long requests keep all SMs as busy as many equal ones.  In a run a warp takes every fourth strip of 16 keys through
 // S^T = K Q^T (m16n8k16: keys are rows, the at most 16 query heads columns), an own running maximum and O^T += V^T P^T; its strips
 // come by asynchronous copies of its own, STAGES of them on their way across the borders of rows, so warps meet only where a row
 // ends.  Weights enter the second product as two 16-bit parts, P = hi + lo: the output is then as exact as its own rounding.
+// Few short requests (ops/cuda.py: scored_parts) are one kernel's instead: a cluster has a row, its scores stay in shared memory, and the parts meet there.
+//
 // Decode is bound by the bytes of the cache; a tcgen05 product (128 keys x 16) would take the scores through tensor memory and
-// barriers between roles for products that are a few percent of the time.
+// barriers between roles for products that are a few percent of the time.  us for 64 requests of 1000 with 32 / 8 heads of 128 (bytes 40.9):
+// 61.7, of which the first kernel takes 52 and its copies alone 47.6 (43.8 for values stored in rows; transposed ones come in pieces of 32 bytes); two of
+// 95000 (121) 146; one of 700 (0.45) 6.8 in clusters and 8.6 without; 24 of 60 to 924 with 16 / 8 heads of 64, capped, fp16 (3.8) 15.6.
+// The other way to the weights, a second pass over the keys, would read half the cache again.
 #include "attention_prompt.cuh"
+#include "cluster.cuh"
 
 namespace sdec {
 
@@ -36,7 +42,7 @@ struct Params {
   int2* info;              // [row]: its first CTA, and how many
   int64_t q_stride, out_stride, bt_stride, sc_req, sc_head;
   int64_t num_blocks;
-  int B, Hkv, G, D, BS, max_rows, raw_rows, ctas, chunks, extra, block;      // chunks: of at most 16 query heads of a kv head
+  int B, Hkv, G, D, BS, max_rows, raw_rows, ctas, chunks, extra, block, parts;      // chunks: of at most 16 query heads of a kv head
   float scale_log2, ku, c2;
 };
 
@@ -135,7 +141,8 @@ template <int DP_> struct Form {
   static constexpr int SMEM = RING + WARPS / 2 * REGS * 128 + (2 * MAX_REQUESTS + 1 + 32) * 4;
 };
 
-template <typename T, int DP, int NT, bool VT, bool CAP>
+// FUSED: a row's tiles are the p.parts CTAs' of a cluster, and everything is done here: the scores stay in shared memory until the parts have met.
+template <typename T, int DP, int NT, bool VT, bool CAP, bool FUSED>
 __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kernel(const Params p) {
   using F = Form<DP>;
   // The reference of a head's weights is its largest score less SHIFT, or up to 8 below that.  fp16 has no values under 2^-24: as multiples of 2^-32 of the
@@ -150,11 +157,33 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_trigger();             // (here: the joining kernel may read the lengths as soon as it starts)
-  scan_tiles(p, first, lens, warp_sums);
-  const int H = p.Hkv * p.chunks;
-  const int total = first[p.B] * H, per = (total + p.ctas - 1) / p.ctas;
-  const int t0 = blockIdx.x * per, t1 = min(t0 + per, total);
-  if (t0 >= t1) return;
+  const int H = p.Hkv * p.chunks, PD = p.D + 2;
+  int t0, t1, per;
+  Row row;
+  float *raw_s = nullptr, *part_s = nullptr, *factor_s = nullptr;          // FUSED: scores of the CTA's keys, its part, log-sum-exps and factors of the parts
+  const int rank = FUSED ? blockIdx.x % p.parts : 0;
+  if constexpr (FUSED) {
+    row.index = blockIdx.x / p.parts;
+    row.b = row.index / p.Hkv;
+    row.hc = row.index % p.Hkv;
+    row.begin = 0;
+    row.end = (rows_of(p, row.b) + TILE - 1) / TILE;
+    per = (row.end + p.parts - 1) / p.parts;
+    t0 = min(rank * per, row.end);
+    t1 = min(t0 + per, row.end);
+    part_s = reinterpret_cast<float*>(first);
+    factor_s = part_s + p.G * PD;
+    raw_s = factor_s + p.G * 9 + (-(p.G * (PD + 9)) & 3);
+  } else {
+    scan_tiles(p, first, lens, warp_sums);
+    const int total = first[p.B] * H;
+    per = (total + p.ctas - 1) / p.ctas;
+    t0 = blockIdx.x * per;
+    t1 = min(t0 + per, total);
+    if (t0 >= t1) return;
+    row_at(first, p.B, H, t0, row);
+  }
+  int n = FUSED ? rows_of(p, row.b) : lens[row.b];
 
   const uint32_t ring = smem_u32(smem) + warp * (STAGES * 2 * F::STRIP_BYTES);
   const int64_t page = (int64_t)p.BS * p.D;                                // values of a page of one head
@@ -171,10 +200,10 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
       const int s = t0 * 4 + warp + (fetched + lane) * WARPS;
       my_off = -1;
       if (s < s_end) {
-        Row r;
-        row_at(first, p.B, H, s >> 2, r);
+        Row r = row;
+        if (!FUSED) row_at(first, p.B, H, s >> 2, r);
         const int tok = (s - r.begin * 4) * STRIP;
-        if (tok < lens[r.b]) {
+        if (tok < (FUSED ? n : lens[r.b])) {
           int64_t blk = p.block_table[r.b * p.bt_stride + tok / p.BS];
           if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
           my_page = (blk * 2 * p.Hkv + r.hc / p.chunks) * page;
@@ -219,8 +248,6 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
 
   const int r0 = lane >> 2, q0 = (lane & 3) * 2;
   const int mi = lane >> 3, l7 = lane & 7;
-  Row row;
-  row_at(first, p.B, H, t0, row);
   int s = t0 * 4 + warp, turn = 0;
   uint32_t q[KD][NT][2];
   auto load_q = [&]() {
@@ -240,7 +267,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
   while (true) {
     const int seg_end = min(row.end, t1) * 4;
     const int g0 = row.hc % p.chunks * 16, G = min(p.G - g0, 16);
-    const int n = lens[row.b];
+    if (!FUSED) n = lens[row.b];
     float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -275,7 +302,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
         }
         const bool cut = tok + STRIP > n;
         const bool in[2] = {!cut || tok + r0 < n, !cut || tok + 8 + r0 < n};
-        float* raw = p.raw + ((int64_t)(row.b * p.Hkv + row.hc / p.chunks) * p.raw_rows + tok) * p.G + g0;
+        float* raw = FUSED ? raw_s + (tok - t0 * TILE) * p.G : p.raw + ((int64_t)(row.b * p.Hkv + row.hc / p.chunks) * p.raw_rows + tok) * p.G + g0;
         uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -350,11 +377,11 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
       }
     }
     // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
-    float* part = p.part + (int64_t)(row.index + blockIdx.x) * 16 * (p.D + 2);
-    const bool empty = max(row.begin, t0) >= row.begin + (n + TILE - 1) / TILE;      // nothing but the row's further slots
-    if (!empty && row.begin >= t0 && threadIdx.x == 0)
+    float* part = FUSED ? part_s : p.part + (int64_t)(row.index + blockIdx.x) * 16 * PD;
+    const bool empty = !FUSED && max(row.begin, t0) >= row.begin + (n + TILE - 1) / TILE;      // nothing but the row's further slots
+    if (!FUSED && !empty && row.begin >= t0 && threadIdx.x == 0)
       p.info[row.index] = make_int2(blockIdx.x, (row.begin + (n + TILE - 1) / TILE - 1) / per - blockIdx.x + 1);
-    const bool more = row.end < t1;
+    const bool more = !FUSED && row.end < t1;
     if (more) {                              // (the next row's queries are on their way meanwhile)
       next_row(first, H, row);
       load_q();
@@ -401,7 +428,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
         for (int u = 0; u < 2; ++u) {
           const int g = nt * 8 + q0 + u;
           if (g < G) {
-            float* to = part + g * (p.D + 2);
+            float* to = part + g * PD;
 #pragma unroll
             for (int i = 0; i < KD; ++i) {
               if (i * 16 + r0 < p.D) to[i * 16 + r0] = o[i][nt][u];
@@ -415,6 +442,38 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
     if (!more) break;
   }
   cp_async_wait<0>();
+  if constexpr (FUSED) {
+    cluster_sync();
+    const uint32_t parts_at = smem_u32(part_s);
+    const int h = row.hc;
+    for (int g = warp; g < p.G; g += WARPS) {            // a warp: log-sum-exp of a head, its parts and the sink
+      const uint32_t at = parts_at + (g * PD + p.D) * 4;
+      const float m0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at, lane)) : -INFINITY, l0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at + 4, lane)) : 0.f;
+      const float sink = p.sinks ? p.sinks[h * p.G + g] * LOG2E : -INFINITY;
+      const float m = warp_max(fmaxf(m0, sink)), top = m == -INFINITY ? 0.f : m;
+      const float l = warp_sum(l0 * ex2(m0 - top)) + (p.sinks ? ex2(sink - top) : 0.f);
+      const float lse = l > 0.f ? top + log2f(l) : INFINITY;                // no key and no sink: weights of 0
+      if (lane < 8) factor_s[g * 9 + lane] = ex2(m0 - lse);
+      if (lane == 8) factor_s[g * 9 + 8] = lse;
+    }
+    __syncthreads();
+    for (int i = rank * F::THREADS + threadIdx.x; i < p.G * p.D; i += p.parts * F::THREADS) {
+      const int g = i / p.D, d = i % p.D;
+      float x[8], acc = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] = c < p.parts ? ld_dsmem_f32(dsmem_addr(parts_at + (g * PD + d) * 4, c)) : 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc += x[c] * factor_s[g * 9 + c];
+      reinterpret_cast<T*>(p.out)[row.b * p.out_stride + (int64_t)h * p.G * p.D + i] = from_f32<T>(acc);
+    }
+    float* sc = p.scores + row.b * p.sc_req + h * p.sc_head;
+    for (int k = t0 * TILE + threadIdx.x; k < min(t1 * TILE, n); k += F::THREADS) {
+      float w = 0.f;
+      for (int g = 0; g < p.G; ++g) w += ex2(raw_s[(k - t0 * TILE) * p.G + g] - factor_s[g * 9 + 8]);
+      sc[k] += w;
+    }
+    cluster_sync();                                      // the others may still read this CTA's part
+  }
 }
 
 // Grid (blocks of p.block keys, kv heads, requests): joins a row's outputs and adds the weights of its keys.  It is a chain of reads from memory (the row's
@@ -532,10 +591,26 @@ __global__ void __launch_bounds__(JOIN, JOINERS) join_kernel(const Params p) {
   }
 }
 
+constexpr int FUSED_TILES = 4;                           // of a CTA, at most, where a cluster has a row
+template <typename F> constexpr int EXCH_BYTES = F::WARPS / 2 * F::REGS * 128;
+
 template <typename T, int DP, int NT, bool VT, bool CAP>
 static int launch(const Params& p, cudaStream_t st) {
   using F = Form<DP>;
-  auto k = decode_kernel<T, DP, NT, VT, CAP>;
+  if constexpr (DP <= 128) if (p.parts > 0) {
+    auto k = decode_kernel<T, DP, NT, VT, CAP, true>;
+    constexpr int MOST = F::RING + EXCH_BYTES<F> + (16 * (DP + 2 + 9) + 4 + FUSED_TILES * TILE * 16) * 4;
+    static bool set = false;
+    if (!set) {
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess) return (int)cudaGetLastError();
+      set = true;
+    }
+    const int tiles = (p.max_rows + TILE - 1) / TILE, per = (tiles + p.parts - 1) / p.parts;
+    const size_t smem = F::RING + EXCH_BYTES<F> + (size_t)(p.G * (p.D + 2 + 9) + 4 + per * TILE * p.G) * 4;
+    vb_launch_parts(k, dim3(p.B * p.Hkv * p.parts), dim3(F::THREADS), smem, st, (unsigned)p.parts, p);
+    return (int)cudaGetLastError();
+  }
+  auto k = decode_kernel<T, DP, NT, VT, CAP, false>;
   static bool set = false;
   if (!set) {
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM) != cudaSuccess) return (int)cudaGetLastError();
@@ -562,16 +637,17 @@ static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
 
 
 // `ws`: for rows = min(B, 512) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + min(B, 512) Hq ceil(max_rows / 64) 64 + 2 rows floats.  extra: tiles
-// that a row counts for beside its own.  max_rows: rows of a request that the block
+// that a row counts for beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request that the block
 // table and the scores have room for.
 EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, void* out, float* scores,
                             const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int64_t q_stride, int64_t out_stride,
-                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int sms, int extra, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
+                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int sms, int extra, int parts, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
   using namespace sdec;
   if (B <= 0) return 0;
-  if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1) return -1;
+  if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1 || parts < 0 || parts > 8) return -1;
+  if (parts > 0 && (parts < 2 || D > 128 || Hq / Hkv > 16 || B > MAX_REQUESTS || (max_rows + TILE - 1) / TILE > FUSED_TILES * parts)) return -1;
   Params p;
-  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16; p.extra = extra;
+  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16; p.extra = extra; p.parts = parts;
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head;
   p.num_blocks = num_blocks; p.cache = cache; p.sinks = sinks;
   p.raw_rows = (max_rows + TILE - 1) / TILE * TILE;

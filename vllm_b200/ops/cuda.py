@@ -551,7 +551,7 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
 
 
 _scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i,
-                      _f, _f, _i, _i, _vp)
+                      _i, _f, _f, _i, _i, _vp)
 
 
 _I32 = torch.int32
@@ -579,6 +579,14 @@ def _q_heads(q):
 SCORED_EXTRA = 3
 
 
+def scored_parts(pairs: int, tiles: int, G: int, D: int, ctas: int) -> int:
+    """CTAs of a cluster that has a request's kv head, where all of them run at a time and have few tiles; 0: equal runs and a second kernel."""
+    if tiles > 32 or G > 16 or D > 128:
+        return 0
+    parts = 8 if tiles > 4 else 4 if tiles > 2 else 2
+    return parts if pairs * parts <= ctas else 0
+
+
 def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=None):
     """Attention of one token per request that adds the keys' weights to ``scores`` (csrc/scored_decode.cu)."""
     if batch_invariant():                    # that kernel deals the keys of all requests to the SMs
@@ -601,14 +609,14 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
     G, sms, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
-    ctas = sms * (2 if D <= 128 else 1)
-    n = min(B, 512) * Hkv
-    # (of this call: two calls at once, or two captured graphs, share nothing)
-    heads = n * -(-G // 16)
-    ws = scores.new_empty((heads + ctas) * 16 * (D + 2) + n * G * -(-rows // 64) * 64 + 2 * heads)
-    _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), ws.data_ptr(), B,
-                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, sms, SCORED_EXTRA, scale, soft_cap, int(md.kv_vt),
-                          _DT[q.dtype], _st()), "scored_decode", 2 * -(-B // 512))
+    ctas, n, tiles = sms * (2 if D <= 128 else 1), min(B, 512) * Hkv, -(-rows // 64)
+    parts, ws = scored_parts(B * Hkv, tiles, G, D, ctas), None
+    if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
+        heads = n * -(-G // 16)
+        ws = scores.new_empty((heads + ctas) * 16 * (D + 2) + n * G * tiles * 64 + 2 * heads)
+    _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), _p(ws), B,
+                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, sms, SCORED_EXTRA, parts, scale, soft_cap, int(md.kv_vt),
+                          _DT[q.dtype], _st()), "scored_decode", 1 if parts else 2 * -(-B // 512))
     return out
 
 
