@@ -143,6 +143,14 @@ def test_weights_lengths(lens, queries, last):
     _check_weights(q, cache, md, scores, last=last)
 
 
+@pytest.mark.parametrize("told", [1, 4000])
+def test_weights_with_another_maximum(told):
+    """The longest query of the metadata only chooses how the work is dealt out."""
+    q, cache, md, scores = step([1500, 700], [1500, 300], 8, 2, 128, 64, torch.bfloat16, "cuda", vt=True)
+    md.max_query_len = told
+    _check_weights(q, cache, md, scores)
+
+
 def test_weights_of_rows_without():
     """Rows whose log-sum-exp says that they have no key, or is NaN, give nothing."""
     q, cache, md, scores = step([300, 200], [100, 200], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=1)

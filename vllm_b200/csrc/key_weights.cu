@@ -487,7 +487,7 @@ static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const Params& p,
     set = true;
   }
   vb_launch(k, dim3(ctas), dim3(NUM_THREADS), (size_t)Form<KB>::SMEM, st, tq, tk, p);
-  if (!p.whole && ctas > 1) vb_launch(join_kernel, dim3(ctas - 1), dim3(KEYS), 0, st, p, ctas);
+  if (p.part && ctas > 1) vb_launch(join_kernel, dim3(ctas - 1), dim3(KEYS), 0, st, p, ctas);
   return (int)cudaGetLastError();
 }
 template <typename T, bool CAP>
@@ -503,11 +503,11 @@ static int pick(const CUtensorMap& tq, const CUtensorMap& tk, const Params& p, i
 }  // namespace kweights
 
 // `error` (device or pinned int, may be null) becomes 1 when a wait inside the kernel ran into its limit.  max_rows: rows of a request that the
-// block table and the scores have room for; max_query: of its query rows that count.  part: ctas x 512 floats.  whole: a key's sum does not depend on
-// other requests (batch-invariant mode).
+// block table and the scores have room for; max_query: of its query rows that count.  part: ctas x 512 floats, or null: no block is split between CTAs (a
+// key's sum then does not depend on other requests).
 EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, const float* lse,
                           float* scores, float* part, int* error, int B, int T, int Hq, int Hkv, int D, int BS, int max_rows, int max_query, int last, int ctas,
-                          int whole, int64_t q_stride, int64_t bt_stride, int64_t sc_req, int64_t sc_head, float scale, float soft_cap, int dtype,
+                          int64_t q_stride, int64_t bt_stride, int64_t sc_req, int64_t sc_head, float scale, float soft_cap, int dtype,
                           cudaStream_t st) {
   using namespace kweights;
   if (B <= 0 || T <= 0 || max_rows <= 0) return 0;
@@ -519,7 +519,7 @@ EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, 
   Params p;
   p.block_table = block_table; p.seq_lens = seq_lens; p.qsl = qsl; p.lse = lse; p.scores = scores; p.part = part; p.error = error;
   p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head; p.num_blocks = num_blocks;
-  p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.last = last; p.whole = whole;
+  p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.last = last; p.whole = part == nullptr;
   p.box_rows = BS & -BS;                                         // a page is whole boxes
   if (p.box_rows > TILE) p.box_rows = TILE;
   const int columns = D <= 192 ? COLS : COLS / 2;

@@ -620,7 +620,7 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     return out
 
 
-_key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64,
+_key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64,
                     _f, _f, _i, _vp)
 
 
@@ -639,12 +639,14 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
     if qsl is not None and (qsl.dtype is not _I32 or not qsl.is_contiguous()):
         raise ValueError("key_weights: int32 query offsets")
-    ctas = num_sms()
-    part = scores.new_empty(ctas * 512)
+    ctas, most = num_sms(), min(last or most, most)
+    # a tile of queries is 256 columns (128 for heads above 192), a power of two of tokens; where that is all of them, no sum is split
+    one = most <= 1 << (((256 if D <= 192 else 128) // (Hq // Hkv)).bit_length() - 1)
+    part = None if one or batch_invariant() else scores.new_empty(ctas * 512)
     _check(_key_weights(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), _p(qsl), lse.data_ptr(), scores.data_ptr(),
-                        part.data_ptr(), _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, min(last or most, most), last, ctas,
-                        int(batch_invariant()), q.stride(0), bt.stride(0), scores.stride(0), scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()),
-           "key_weights", 2)
+                        _p(part), _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, most, last, ctas, q.stride(0), bt.stride(0),
+                        scores.stride(0), scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()), "key_weights",
+           1 if part is None else 2)
     return scores
 
 
