@@ -30,6 +30,7 @@ struct Params {
   const float* lse;          // [T, Hq]
   float* scores;
   float* part;               // [CTA][2][KEYS]: sums of a block that began in an earlier CTA; of one that goes on in the next
+  int4* info;                // [CTA]: where that begins which it continues as the first: request, kv head, block (-1: nothing), its CTAs from here on
   int* error;                // raised when a wait ran into its limit
   int64_t bt_stride, sc_req, sc_head, num_blocks;
   int B, row0, T, Hq, Hkv, G, TQ, D, BS, max_rows, last, box_rows, whole;      // TQ: tokens of a tile, a power of 2; whole: blocks are not split
@@ -243,51 +244,58 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
     if (s1 < total) { g.start(p, first, s1, 1); if (g.j > 0) s1 += g.count - g.j; }
   }
 
+  if (p.part && s0 >= s1 && threadIdx.x == 0) p.info[blockIdx.x] = make_int4(0, 0, -1, 0);
   if (s0 < s1) {
     Segment g;
     g.start(p, first, s0, s1 - s0);
+    if (p.part && threadIdx.x == 2 * 32)
+      p.info[blockIdx.x] = make_int4(g.b, g.h, g.j > 0 && g.j <= per ? g.i : -1, (s0 - g.j + g.count + per - 1) / per - blockIdx.x);
     if (warp == 0) {
-      if (lane == 0) {
-        int tile = 0, seg = 0;
-        for (int s = s0; budget >= 0;) {
-          const int n = min(g.len, p.max_rows);
-          const int* bt = p.block_table + g.b * p.bt_stride;
-          auto load_q = [&](int j) {
-            const int qs = tile % QS;
+      int tile = 0, seg = 0;
+      for (int s = s0;;) {
+        const int n = min(g.len, p.max_rows), k0 = g.i * KEYS;
+        // page numbers of the block's at most 16 boxes, a lane each
+        int64_t blk = 0;
+        if (lane * p.box_rows < KEYS && k0 + lane * p.box_rows < n) blk = p.block_table[g.b * p.bt_stride + (k0 + lane * p.box_rows) / p.BS];
+        if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;                // (a table may not say that)
+        auto load_q = [&](int j) {
+          const int qs = tile % QS;
+          if (lane == 0) {
             mbar_wait_lim(&q_empty[qs], ((tile / QS) & 1) ^ 1, budget);
-            if (budget < 0) return;
-            mbar_expect_tx(&q_full[qs], KB * used * 128);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-              prompt::tma_load_3d(q_smem + qs * F::Q_BYTES + kb * (F::COLUMNS * 128), &tmap_q, kb * 64, g.h * p.G, g.q_end - (g.count - j) * p.TQ, &q_full[qs]);
-            ++tile;
-          };
-          for (int t = 0; t < 2 && budget >= 0; ++t) {
-            const int k0 = g.i * KEYS + t * TILE;
-            int boxes = 0;
-            for (int r = 0; r < TILE && k0 + r < n; r += p.box_rows) ++boxes;
-            mbar_wait_lim(&k_empty[t], (seg & 1) ^ 1, budget);
-            if (budget < 0) break;
-            mbar_expect_tx(&k_full[t], boxes * KB * p.box_rows * 128);       // (none of a tile behind the last row: the barrier falls by itself)
-            for (int i = 0; i < boxes; ++i) {
-              const int r = i * p.box_rows, key = k0 + r;
-              int64_t blk = bt[key / p.BS];
-              if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;          // (a table may not say that)
+            if (budget >= 0) {
+              mbar_expect_tx(&q_full[qs], KB * used * 128);
 #pragma unroll
               for (int kb = 0; kb < KB; ++kb)
-                prompt::tma_load_3d(k_smem + (t * KB + kb) * BLK + r * 128, &tmap_k, kb * 64, key % p.BS, (int)(blk * 2 * p.Hkv + g.h), &k_full[t]);
+                prompt::tma_load_3d(q_smem + qs * F::Q_BYTES + kb * (F::COLUMNS * 128), &tmap_q, kb * 64, g.h * p.G, g.q_end - (g.count - j) * p.TQ, &q_full[qs]);
             }
-            if (t == 0) load_q(g.j);
           }
-          for (int j = g.j + 1; j < g.j + g.n && budget >= 0; ++j) load_q(j);
-          if (budget < 0) break;
-          s += g.n;
-          ++seg;
-          if (s >= s1) break;
-          g.next(p, first, s1 - s);
+          ++tile;
+        };
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          const int boxes = max(0, min(TILE, n - k0 - t * TILE) + p.box_rows - 1) / p.box_rows;
+          if (lane == 0) {
+            mbar_wait_lim(&k_empty[t], (seg & 1) ^ 1, budget);
+            if (budget >= 0) mbar_expect_tx(&k_full[t], boxes * KB * p.box_rows * 128);      // (none of a tile behind the last row: the barrier falls by itself)
+          }
+          for (int i = 0; i < boxes; ++i) {
+            const int r = i * p.box_rows;
+            const int at = __shfl_sync(0xffffffffu, (int)blk, (t * TILE + r) / p.box_rows);
+            if (lane == 0 && budget >= 0) {
+#pragma unroll
+              for (int kb = 0; kb < KB; ++kb)
+                prompt::tma_load_3d(k_smem + (t * KB + kb) * BLK + r * 128, &tmap_k, kb * 64, (k0 + t * TILE + r) % p.BS, at * 2 * p.Hkv + g.h, &k_full[t]);
+            }
+          }
+          if (t == 0) load_q(g.j);
         }
-        if (budget < 0) { mbar_let_land(k_full, 2); mbar_let_land(q_full, QS); }
+        for (int j = g.j + 1; j < g.j + g.n; ++j) load_q(j);
+        s += g.n;
+        ++seg;
+        if (s >= s1 || __shfl_sync(0xffffffffu, budget, 0) < 0) break;
+        g.next(p, first, s1 - s);
       }
+      if (lane == 0 && budget < 0) { mbar_let_land(k_full, 2); mbar_let_land(q_full, QS); }
     } else if (warp == 1) {
       const uint32_t idesc = umma_idesc_f16(TILE, pieces * 32, DTypeOf<T>::v == DT_BF16);
       const uint64_t da = umma_desc_sw128(k_smem), d_one = umma_desc_sw32(one_smem), d_aug = umma_desc_sw32(aug_smem);
@@ -461,21 +469,19 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
 }
 
 // Blocks that several CTAs have summed: one CTA for each border between runs, at work where the border is the first within a block.
-__global__ void __launch_bounds__(KEYS) join_kernel(const Params p, int ctas) {
-  __shared__ int first[MAX_REQUESTS + 1], warp_sums[32];
+__global__ void __launch_bounds__(KEYS) join_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();
-  scan_requests(p, first, warp_sums);
-  const int total = first[p.B], per = (total + ctas - 1) / ctas;
   const int c = blockIdx.x + 1;
-  if ((int64_t)c * per >= total) return;
-  Segment g;
-  g.start(p, first, c * per, 1);
-  if (g.j == 0 || g.j > per) return;
-  const int end = c * per - g.j + g.count, key = g.i * KEYS + threadIdx.x;
+  const int4 at = p.info[c];
+  if (at.z < 0) return;
+  const int key = at.z * KEYS + threadIdx.x, n = min(max(p.seq_lens[at.x], 0), p.max_rows);
+  float* score = p.scores + at.x * p.sc_req + at.y * p.sc_head + key;
+  const float old = key < n ? *score : 0.f;
   float sum = p.part[((int64_t)(c - 1) * 2 + 1) * KEYS + threadIdx.x];
-  for (int i = c; (int64_t)i * per < end; ++i) sum += p.part[(int64_t)i * 2 * KEYS + threadIdx.x];
-  if (key < min(g.len, p.max_rows)) p.scores[g.b * p.sc_req + g.h * p.sc_head + key] += sum;
+#pragma unroll 4
+  for (int i = c; i < c + at.w; ++i) sum += p.part[(int64_t)i * 2 * KEYS + threadIdx.x];
+  if (key < n) *score = old + sum;
 }
 
 template <typename T, int KB, bool CAP>
@@ -487,7 +493,7 @@ static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const Params& p,
     set = true;
   }
   vb_launch(k, dim3(ctas), dim3(NUM_THREADS), (size_t)Form<KB>::SMEM, st, tq, tk, p);
-  if (p.part && ctas > 1) vb_launch(join_kernel, dim3(ctas - 1), dim3(KEYS), 0, st, p, ctas);
+  if (p.part && ctas > 1) vb_launch(join_kernel, dim3(ctas - 1), dim3(KEYS), 0, st, p);
   return (int)cudaGetLastError();
 }
 template <typename T, bool CAP>
@@ -503,7 +509,7 @@ static int pick(const CUtensorMap& tq, const CUtensorMap& tk, const Params& p, i
 }  // namespace kweights
 
 // `error` (device or pinned int, may be null) becomes 1 when a wait inside the kernel ran into its limit.  max_rows: rows of a request that the
-// block table and the scores have room for; max_query: of its query rows that count.  part: ctas x 512 floats, or null: no block is split between CTAs (a
+// block table and the scores have room for; max_query: of its query rows that count.  part: ctas x 516 floats, or null: no block is split between CTAs (a
 // key's sum then does not depend on other requests).
 EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, const float* lse,
                           float* scores, float* part, int* error, int B, int T, int Hq, int Hkv, int D, int BS, int max_rows, int max_query, int last, int ctas,
@@ -517,7 +523,7 @@ EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, 
   const bool bf16 = dtype == DT_BF16;
   const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   Params p;
-  p.block_table = block_table; p.seq_lens = seq_lens; p.qsl = qsl; p.lse = lse; p.scores = scores; p.part = part; p.error = error;
+  p.block_table = block_table; p.seq_lens = seq_lens; p.qsl = qsl; p.lse = lse; p.scores = scores; p.part = part; p.error = error; p.info = reinterpret_cast<int4*>(part + (int64_t)ctas * 2 * KEYS);
   p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head; p.num_blocks = num_blocks;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.last = last; p.whole = part == nullptr;
   p.box_rows = BS & -BS;                                         // a page is whole boxes

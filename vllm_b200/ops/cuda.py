@@ -642,7 +642,7 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     ctas, most = num_sms(), min(last or most, most)
     # a tile of queries is 256 columns (128 for heads above 192), a power of two of tokens; where that is all of them, no sum is split
     one = most <= 1 << (((256 if D <= 192 else 128) // (Hq // Hkv)).bit_length() - 1)
-    part = None if one or batch_invariant() else scores.new_empty(ctas * 512)
+    part = None if one or batch_invariant() else scores.new_empty(ctas * 516)
     _check(_key_weights(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), sl.data_ptr(), _p(qsl), lse.data_ptr(), scores.data_ptr(),
                         _p(part), _error_flag(q.device), md.num_reqs, T, Hq, Hkv, D, kv_cache.shape[3], rows, most, last, ctas, q.stride(0), bt.stride(0),
                         scores.stride(0), scores.stride(1), scale, soft_cap, _DT[q.dtype], _st()), "key_weights",
