@@ -16,6 +16,7 @@ constexpr int BINS = 256, DIGITS = 4;
 constexpr uint32_t LOWEST = 0x007fffffu, PROTECTED = 0xffffffffu;        // -inf; above +inf
 constexpr int CTA_ROWS = 4096;                                           // rows of a CTA, where eight are enough for them
 constexpr int MANY = 296;                                                // CTAs from which they have 8 warps instead of 16: two for each SM
+constexpr int FUSED_CTAS = 148, FUSED_MOVES = 1024;                      // up to which there is one kernel
 constexpr int SMEM_ROWS = 50 * 1024;                                     // of which the keys fit; beyond 8 times that they are made anew in every pass
 
 struct Params {
@@ -38,8 +39,106 @@ VB_DEVICE uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <bool KEPT, int THREADS>                        // KEPT: the keys are kept in shared memory
-__global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
+struct Move {
+  const float* scores;
+  const int* positions;
+  float* new_scores;
+  int* new_positions;
+  const int* count;
+  const int* target;
+  const int* source;
+  uint16_t* cache;
+  const int* block_table;
+  int64_t sc_req, sc_head, po_req, po_head, bt_stride, num_blocks;
+  int Hkv, L, cap, D, BS;
+};
+
+// Of up to N moves: places of the keys in the cache (to: -1, none), and of the values
+template <int N> struct Places { int64_t from[N], to[N], vfrom[N], vto[N]; };
+
+// A CTA moves the rows j0 .. j0 + n - 1 of a list, n <= N <= THREADS.  Transposed values: a lane per move, a dimension at a time, as neighbours in the list
+// are near each other in source and target.  Nearly all of the 32-byte pieces of a page's values hold a row that moves or one that makes room,
+// so those pages are read and written almost whole: 317 MB at 5.5 TB/s for 4 x 30000 rows down to 4096, 57 us.
+template <int THREADS, int N> VB_DEVICE void move_rows(const Move& p, Places<N>& at, bool vt, int b, int h, int j0, int n) {
+  const int row = b * p.Hkv + h;
+  if ((int)threadIdx.x < n) {
+    const int t = p.target[(int64_t)row * p.cap + j0 + threadIdx.x], s = p.source[(int64_t)row * p.cap + j0 + threadIdx.x];
+    p.new_scores[(int64_t)row * p.L + t] = p.scores[b * p.sc_req + h * p.sc_head + s];
+    p.new_positions[(int64_t)row * p.L + t] = p.positions ? p.positions[b * p.po_req + h * p.po_head + s] : s;
+    const int64_t page = (int64_t)p.BS * p.D;
+    int64_t bt = p.block_table[b * p.bt_stride + t / p.BS], bs = p.block_table[b * p.bt_stride + s / p.BS];
+    const bool ok = (uint64_t)bt < (uint64_t)p.num_blocks && (uint64_t)bs < (uint64_t)p.num_blocks;   // (a table may not say else; nothing outside the
+    if (!ok) bt = bs = 0;                                                                             // cache is touched)
+    const int64_t kt = (bt * 2 * p.Hkv + h) * page, ks = (bs * 2 * p.Hkv + h) * page, v = p.Hkv * page;
+    const int64_t to = kt + (int64_t)(t % p.BS) * p.D, from = ks + (int64_t)(s % p.BS) * p.D;
+    at.to[threadIdx.x] = ok ? to : -1;
+    at.from[threadIdx.x] = from;
+    at.vto[threadIdx.x] = vt ? kt + v + t % p.BS : to + v;
+    at.vfrom[threadIdx.x] = vt ? ks + v + s % p.BS : from + v;
+  }
+  __syncthreads();
+  // transposed values, a warp: 32 moves, DIMS dimensions; the warp's first ones are on their way while the keys move
+  constexpr int DIMS = N == 32 ? 16 : 32, UNITS = 128 / DIMS;
+  const int lane = threadIdx.x & 31, units = vt ? (n + 31) / 32 * UNITS : 0;
+  int unit = threadIdx.x >> 5;
+  uint16_t x[DIMS];
+  auto read = [&]() -> uint16_t* {                       // where they go, or null
+    const int j = unit / UNITS * 32 + lane, d = unit % UNITS * DIMS;
+    if (unit >= units || j >= n || at.to[j] < 0) return nullptr;
+    const uint16_t* src = p.cache + at.vfrom[j] + d * p.BS;
+#pragma unroll
+    for (int u = 0; u < DIMS; ++u) x[u] = src[u * p.BS];
+    return p.cache + at.vto[j] + d * p.BS;
+  };
+  uint16_t* to_x = read();
+  const int ch = p.D / 8, items = n * ch;
+  constexpr int U = 2;                                   // pieces on their way at a time
+  for (int i0 = threadIdx.x; i0 < items; i0 += U * THREADS) {
+    uint4 k[U], v[U];
+    int64_t to[U], vto[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * THREADS, j = i / ch, c = i % ch * 8;
+      to[u] = i < items ? at.to[j] : -1;
+      if (to[u] >= 0) {
+        k[u] = *reinterpret_cast<const uint4*>(p.cache + at.from[j] + c);
+        if (!vt) v[u] = *reinterpret_cast<const uint4*>(p.cache + at.vfrom[j] + c);
+        to[u] += c;
+        vto[u] = at.vto[j] + c;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (to[u] >= 0) {
+        if (!vt) *reinterpret_cast<uint4*>(p.cache + vto[u]) = v[u];
+        *reinterpret_cast<uint4*>(p.cache + to[u]) = k[u];
+      }
+    }
+  }
+  while (unit < units) {
+    if (to_x) {
+#pragma unroll
+      for (int u = 0; u < DIMS; ++u) to_x[u * p.BS] = x[u];
+    }
+    unit += THREADS / 32;
+    to_x = read();
+  }
+}
+
+constexpr int PAIRS = 32, MOVERS = 256;
+// Grid (groups of 32 moves, kv heads, requests)
+template <bool VT>
+__global__ void __launch_bounds__(MOVERS) move_kernel(const Move p) {
+  __shared__ Places<PAIRS> at;
+  pdl_trigger();
+  pdl_wait();
+  const int h = blockIdx.y, b = blockIdx.z, j0 = blockIdx.x * PAIRS, n = min(p.count[b * p.Hkv + h] - j0, PAIRS);
+  if (n > 0) move_rows<MOVERS, PAIRS>(p, at, VT, b, h, j0, n);
+}
+
+// KEPT: the keys are kept in shared memory.  FUSED (1: values in rows, 2: transposed): the CTA or the cluster moves its rows, too
+template <bool KEPT, int THREADS, int FUSED>
+__global__ void __launch_bounds__(THREADS) select_kernel(const Params p, const Move mv) {
   constexpr int WARPS = THREADS / 32;
   extern __shared__ uint32_t evict_smem[];
   uint32_t* hist = evict_smem;                           // [DIGITS][BINS]
@@ -251,72 +350,13 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
     new_scores[i] = 0.f;
     new_positions[i] = total + i - m;
   }
-  if (p.parts > 1) cluster_sync();                       // the others may still read this CTA's counts and mailboxes
-}
-
-struct Move {
-  const float* scores;
-  const int* positions;
-  float* new_scores;
-  int* new_positions;
-  const int* count;
-  const int* target;
-  const int* source;
-  uint16_t* cache;
-  const int* block_table;
-  int64_t sc_req, sc_head, po_req, po_head, bt_stride, num_blocks;
-  int Hkv, L, cap, D, BS;
-};
-
-constexpr int PAIRS = 32, MOVERS = 256;
-// Grid (groups of 32 moves, kv heads, requests).  Transposed values (VT): a lane per move, a dimension at a time, as neighbours in the list are near each
-// other in source and target.
-template <bool VT>
-__global__ void __launch_bounds__(MOVERS) move_kernel(const Move p) {
-  __shared__ int64_t from[PAIRS], to[PAIRS];              // places of the keys in the cache (VT: of the first value, too)
-  __shared__ int64_t vfrom[PAIRS], vto[PAIRS];
-  pdl_trigger();
-  pdl_wait();
-  const int h = blockIdx.y, b = blockIdx.z, row = b * p.Hkv + h, j0 = blockIdx.x * PAIRS;
-  const int n = min(p.count[row] - j0, PAIRS);
-  if (n <= 0) return;
-  if (threadIdx.x < n) {
-    const int t = p.target[(int64_t)row * p.cap + j0 + threadIdx.x], s = p.source[(int64_t)row * p.cap + j0 + threadIdx.x];
-    p.new_scores[(int64_t)row * p.L + t] = p.scores[b * p.sc_req + h * p.sc_head + s];
-    p.new_positions[(int64_t)row * p.L + t] = p.positions ? p.positions[b * p.po_req + h * p.po_head + s] : s;
-    const int64_t page = (int64_t)p.BS * p.D;
-    int64_t bt = p.block_table[b * p.bt_stride + t / p.BS], bs = p.block_table[b * p.bt_stride + s / p.BS];
-    const bool ok = (uint64_t)bt < (uint64_t)p.num_blocks && (uint64_t)bs < (uint64_t)p.num_blocks;   // (a table may not say else; nothing outside the
-    if (!ok) bt = bs = 0;                                                                             // cache is touched)
-    const int64_t kt = (bt * 2 * p.Hkv + h) * page, ks = (bs * 2 * p.Hkv + h) * page, v = p.Hkv * page;
-    to[threadIdx.x] = ok ? kt + (int64_t)(t % p.BS) * p.D : -1;
-    from[threadIdx.x] = ks + (int64_t)(s % p.BS) * p.D;
-    vto[threadIdx.x] = VT ? kt + v + t % p.BS : kt + v + (int64_t)(t % p.BS) * p.D;
-    vfrom[threadIdx.x] = VT ? ks + v + s % p.BS : from[threadIdx.x] + v;
-  }
-  __syncthreads();
-  const int ch = p.D / 8, items = n * ch;
-  for (int i = threadIdx.x; i < items; i += MOVERS) {
-    const int j = i / ch, c = i % ch * 8;
-    if (to[j] < 0) continue;
-    const uint4 k = *reinterpret_cast<const uint4*>(p.cache + from[j] + c);
-    if (!VT) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p.cache + vfrom[j] + c);
-      *reinterpret_cast<uint4*>(p.cache + vto[j] + c) = v;
-    }
-    *reinterpret_cast<uint4*>(p.cache + to[j] + c) = k;
-  }
-  if (VT) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (lane < n && to[lane] >= 0) {
-      const uint16_t* src = p.cache + vfrom[lane];
-      uint16_t* dst = p.cache + vto[lane];
-      constexpr int U = 16;
-      uint16_t x[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = src[(int64_t)(w * U + u) * p.BS];        // 128 dimensions, 8 warps
-#pragma unroll
-      for (int u = 0; u < U; ++u) dst[(int64_t)(w * U + u) * p.BS] = x[u];
+  if (p.parts > 1) cluster_sync();                       // the others may still read this CTA's counts and mailboxes (and have written their lists)
+  if constexpr (FUSED != 0) {
+    __shared__ Places<THREADS> at;
+    const int share = (n_holes + p.parts - 1) / p.parts, last = min((rank + 1) * share, n_holes);
+    for (int j0 = rank * share; j0 < last; j0 += THREADS) {
+      __syncthreads();
+      move_rows<THREADS, THREADS>(mv, at, FUSED == 2, b, h, j0, min(last - j0, THREADS));
     }
   }
 }
@@ -342,13 +382,19 @@ EXPORT int vb_evict_keys(void* cache, int64_t num_blocks, const int* block_table
   // Few CTAs wait for their chains, many for instructions that every warp has of its own.  us of both kernels with 8 and 16 warps: 1 request of 700 rows
   // (8 CTAs) 10.8 and 10.2, 16 of 2000 (64) 22.4 and 14.0, 64 of 1200 (512) 74.3 and 77.4, 4 of 30000 (256 in clusters) 97.5 and 82.9
   const bool many = p.parts == 1 && (int64_t)B * Hkv > MANY;
-  auto k = !kept ? select_kernel<false, 512> : many ? select_kernel<true, 256> : select_kernel<true, 512>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)cudaGetLastError();
-  if (vb_launch_parts(k, dim3((unsigned)(B * Hkv * p.parts)), dim3(many ? 256 : 512), smem, st, (unsigned)p.parts, p) != cudaSuccess)
+  const Move mv{scores, positions, new_scores, new_positions, p.count, p.target, p.source, reinterpret_cast<uint16_t*>(cache), block_table,
+                sc_req, sc_head, po_req, po_head, bt_stride, num_blocks, Hkv, L, cap, D, BS};
+  // One kernel where that leaves a CTA for every SM at most and few moves to each: a cut is called now and then, and a launch costs the host 3 us.  A call and
+  // its kernels, us, in two and in one: 700 rows to 512, 8 heads 23.1 and 20.0 (10.1 and 12.4), 16 x 2000 to 1500, 4 heads of 64 24.2 and 21.0 (14.0 and 13.2)
+  const bool fused = kept && !many && (int64_t)B * Hkv * p.parts <= FUSED_CTAS && cap <= FUSED_MOVES && rows <= CTA_ROWS + 32;
+  auto k = !kept ? select_kernel<false, 512, 0>
+           : many ? select_kernel<true, 256, 0>
+           : !fused ? select_kernel<true, 512, 0>
+           : vt ? select_kernel<true, 512, 2> : select_kernel<true, 512, 1>;
+  if (smem > 24 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)cudaGetLastError();
+  if (vb_launch_parts(k, dim3((unsigned)(B * Hkv * p.parts)), dim3(many ? 256 : 512), smem, st, (unsigned)p.parts, p, mv) != cudaSuccess)
     return (int)cudaGetLastError();
-  if (cap > 0) {
-    Move mv{scores, positions, new_scores, new_positions, p.count, p.target, p.source, reinterpret_cast<uint16_t*>(cache), block_table,
-            sc_req, sc_head, po_req, po_head, bt_stride, num_blocks, Hkv, L, cap, D, BS};
+  if (cap > 0 && !fused) {
     const dim3 grid((cap + PAIRS - 1) / PAIRS, Hkv, B);
     if ((vt ? vb_launch(move_kernel<true>, grid, dim3(MOVERS), 0, st, mv) : vb_launch(move_kernel<false>, grid, dim3(MOVERS), 0, st, mv)) != cudaSuccess)
       return (int)cudaGetLastError();
