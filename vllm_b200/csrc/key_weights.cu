@@ -169,6 +169,12 @@ VB_DEVICE float ex2_poly(float x) {
 }
 
 // tmem_ld_wait for these registers: no use of them moves in front of it
+VB_DEVICE void wait_for(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
 VB_DEVICE void wait_for(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
@@ -382,8 +388,8 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
         g.next(p, first, s1 - s);
       }
     } else {
-      // A warp has 32 keys of one key tile and every second piece of 32 columns.  The eight warps of a key tile go through its products by themselves, so
-      // one tile's are issued and read while the other's are summed.
+      // A warp has 32 keys of one key tile and every second piece of 32 columns, half of which is on its way out of tensor memory while the other half is
+      // summed.  The eight warps of a key tile go through its products by themselves, so one tile's are issued while the other's are summed.
       const int qd = warp & 3, half = ((warp - 4) >> 2) & 1, t = (warp - 4) >> 3, mine = t * TILE + qd * 32 + lane;
       const int groups = (pieces - half + 1) / 2;                // 2 to 4
       const uint32_t from = tmem + t * COLS + half * 32 + ((uint32_t)(qd * 32) << 16);
@@ -409,33 +415,46 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
           const bool full = pos >= key0 + TILE - 1 && !odd[slot];                      // every row sees every key
           const int c_lo = min(max(key - pos, 0), COLS) * p.G - half * 32;             // columns that see the key begin here
-          if (key0 < n) {
+          auto release = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[t]);
+          };
+          if (key0 < n && full) {
+            auto weigh = [&](const uint32_t (&v)[16], const float* lc) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const float4 l = CAP ? *reinterpret_cast<const float4*>(lc + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                acc[0] += weight(v[i], l.x, false);
+                acc[1] += weight(v[i + 1], l.y, false);
+                acc[2] += weight(v[i + 2], l.z, i % 8 == 4);
+                acc[3] += weight(v[i + 3], l.w, false);
+              }
+            };
+            uint32_t va[16], vb[16];
+            tmem_ld_32x16(from, va);
+#pragma unroll 1
+            for (int c = 0; c < groups; ++c) {
+              wait_for(va);
+              tmem_ld_32x16(from + c * 64 + 16, vb);
+              weigh(va, ls + c * 64);
+              wait_for(vb);
+              if (c + 1 < groups) tmem_ld_32x16(from + c * 64 + 64, va);
+              else release();
+              weigh(vb, ls + c * 64 + 16);
+            }
+          } else if (key0 < n) {
 #pragma unroll 1
             for (int c = 0; c < groups; ++c) {
               uint32_t v[32];
               tmem_ld_32x32(from + c * 64, v);
               wait_for(v);
-              if (c == groups - 1) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_empty[t]);
-              }
+              if (c == groups - 1) release();
               const float* lc = ls + c * 64;
-              if (full) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                  const float4 l = CAP ? *reinterpret_cast<const float4*>(lc + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                  acc[0] += weight(v[i], l.x, false);
-                  acc[1] += weight(v[i + 1], l.y, false);
-                  acc[2] += weight(v[i + 2], l.z, i % 8 == 4);
-                  acc[3] += weight(v[i + 3], l.w, false);
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float l = lc[i], x = weight(v[i], l, false);
-                  acc[i & 3] += c * 64 + i < c_lo || l == -INFINITY ? 0.f : x;
-                }
+              for (int i = 0; i < 32; ++i) {
+                const float l = lc[i], x = weight(v[i], l, false);
+                acc[i & 3] += c * 64 + i < c_lo || l == -INFINITY ? 0.f : x;
               }
             }
           } else if (lane == 0) {
