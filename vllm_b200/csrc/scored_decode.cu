@@ -185,7 +185,11 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
   }
   int n = FUSED ? rows_of(p, row.b) : lens[row.b];
 
-  const uint32_t ring = smem_u32(smem) + warp * (STAGES * 2 * F::STRIP_BYTES);
+  // A warp's stages of keys, with its values behind each; transposed values (VT) come as whole pages of 64 keys, a warp's strip being a quarter of them:
+  // each warp fetches 32 of their 128 rows, and the warps meet once a page.
+  constexpr int STAGE = (VT ? 1 : 2) * F::STRIP_BYTES;
+  static_assert(!VT || (DP == 128 && WARPS * STRIP == TILE), "a page of transposed values is a tile");
+  const uint32_t ring = smem_u32(smem) + warp * (STAGES * STAGE), v_ring = smem_u32(smem) + WARPS * STAGES * F::STRIP_BYTES;
   const int64_t page = (int64_t)p.BS * p.D;                                // values of a page of one head
   // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  Where they lie is looked up for 32 of them at once, a lane each: a block number comes
   // out of memory before the copies can be issued, and one at a time that was most of a short run.
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
       if (s < s_end) {
         Row r = row;
         if (!FUSED) row_at(first, p.B, H, s >> 2, r);
-        const int tok = (s - r.begin * 4) * STRIP;
+        const int tok = VT ? ((s >> 2) - r.begin) * TILE : (s - r.begin * 4) * STRIP;      // VT: of the page
         if (tok < (FUSED ? n : lens[r.b])) {
           int64_t blk = p.block_table[r.b * p.bt_stride + tok / p.BS];
           if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
@@ -217,20 +221,20 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
     if (off >= 0) {
       const T* k = reinterpret_cast<const T*>(p.cache) + at;
       const T* v = k + p.Hkv * page;
-      const uint32_t to = ring + stage * (2 * F::STRIP_BYTES);
-      const T* src = k + (int64_t)off * p.D + (real ? c0 * 8 : 0);
+      const uint32_t to = ring + stage * STAGE;
+      const T* src = k + (int64_t)(VT ? warp * STRIP : off) * p.D + (real ? c0 * 8 : 0);
 #pragma unroll
       for (int i = 0; i < STRIP / RSTEP; ++i) {
         const int r = r0l + i * RSTEP;
         cp_async16(to + r * (DP * 2) + ((c0 ^ (r & 7)) << 4), src + (int64_t)r * p.D, real);
       }
       if constexpr (VT) {                                                  // values stored [dim][token of the page]
-        const int half = lane & 1, d0 = lane >> 1;
-        const T* sv = v + off + half * 8;
+        const int c = lane & 7, d0 = warp * 32 + (lane >> 3);
+        const uint32_t vt = v_ring + stage * (TILE * DP * 2);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const int d = d0 + i * 16;
-          cp_async16(to + F::STRIP_BYTES + d * 32 + ((half ^ ((d >> 2) & 1)) << 4), sv + (int64_t)d * p.BS, true);
+        for (int i = 0; i < 8; ++i) {
+          const int d = d0 + i * 4;
+          cp_async16(vt + d * 128 + ((c ^ (d & 7)) << 4), v + d * TILE + c * 8, true);
         }
       } else {
         const T* sv = v + (int64_t)off * p.D + (real ? c0 * 8 : 0);
@@ -282,11 +286,12 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
       const int stage = turn;
       turn = turn + 1 == STAGES ? 0 : turn + 1;
       cp_async_wait<STAGES - 2>();
-      __syncwarp();
-      fetch(stage == 0 ? STAGES - 1 : stage - 1);                          // into the stage of the strip before, which the whole warp has read
+      if constexpr (VT) __syncthreads();
+      else __syncwarp();
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);                          // into the stage of the strip before, which the whole warp (VT: all warps) has read
       const int tok = (s - row.begin * 4) * STRIP;
       if (tok < n) {
-        const uint32_t ks = ring + stage * (2 * F::STRIP_BYTES), vs = ks + F::STRIP_BYTES;
+        const uint32_t ks = ring + stage * STAGE, vs = VT ? v_ring + stage * (TILE * DP * 2) : ks + F::STRIP_BYTES;
         float sc[NT][4], sd[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(Form<DP>::THREADS, Form<DP>::CTAS) decode_kern
           uint32_t a[4];
           if constexpr (VT) {
             const int d = i * 16 + (mi & 1) * 8 + l7;
-            ldsm4(a, vs + d * 32 + (((mi >> 1) ^ ((d >> 2) & 1)) << 4));
+            ldsm4(a, vs + d * 128 + (((warp * 2 + (mi >> 1)) ^ (d & 7)) << 4));
           } else {
             // stored [token][dim], turned by the load: matrices (dims 0-7, tokens 0-7), (dims 8-15, tokens 0-7), (dims 0-7, tokens 8-15), ...
             const int t = (mi >> 1) * 8 + l7;
