@@ -17,8 +17,8 @@
 //
 // Decode is bound by the bytes of the cache; a tcgen05 product (128 keys x 16) would take the scores through tensor memory and
 // barriers between roles for products that are a few percent of the time.  us for 64 requests of 1000 with 32 / 8 heads of 128 (bytes 40.9):
-// 61.7, of which the first kernel takes 52 and its copies alone 47.6 (43.8 for values stored in rows; transposed ones come in pieces of 32 bytes); two of
-// 95000 (121) 146; one of 700 (0.45) 6.8 in clusters and 8.6 without; 24 of 60 to 924 with 16 / 8 heads of 64, capped, fp16 (3.8) 15.6.
+// 54, of which the first kernel takes 46 and the join 8; two of 95000 (121) 136; one of 700 (0.45) 6.3 in clusters and 8.6 without; 24 of 60 to 924 with
+// 16 / 8 heads of 64, capped, fp16 (3.8) 15.7.
 // The other way to the weights, a second pass over the keys, would read half the cache again.
 #include "attention_prompt.cuh"
 #include "cluster.cuh"
@@ -106,9 +106,10 @@ VB_DEVICE void next_row(const int* first, int H, Row& r) {                     /
   r.end = r.begin + first[r.b + 1] - first[r.b];
 }
 
+// (the cache is read once and leaves L2 first, so that the scores that are read again stay in it: 64 x 1000 58 to 54 us, 2 x 95000 141 to 136)
 VB_DEVICE void cp_async16(uint32_t dst, const void* src, bool real) {
   const int n = real ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(n), "l"(L2_EVICT_FIRST) : "memory");
 }
 VB_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> VB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
