@@ -147,7 +147,9 @@ VB_DEVICE float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(
 
 // Other scores: a column gets sixteen more dimensions, three of which hold -lse / scale in parts of 16 bits, the keys' are constant.  The product is
 // then what the exponential takes but for a factor: no log-sum-exps out of shared memory, where 128-bit reads by all threads and the operands of the
-// products want the same bandwidth.  fp16: parts of 1 / 64, as lse / scale may be large.
+// products want the same bandwidth.  fp16: parts of 1 / 64, as lse / scale may be large.  They are added a little behind the middle of a product: its sums are
+// cut towards 0, and half of them are then above 0 and half below for the keys with much weight.  Relative error of the weights of 300 tokens 4.4e-7 with them
+// last, 8.6e-7 first, 1.3e-7 so (heads of 128); of 900 with heads of 256 1.1e-6, 2.5e-6 and 1.8e-7; 32-bit multiplications and additions have 1.2e-7.
 template <typename T> constexpr float ONE = DTypeOf<T>::v == DT_F16 ? 64.f : 1.f;
 // rows of 32 bytes, 8-row groups 256 bytes apart, SWIZZLE_32B
 VB_DEVICE uint64_t umma_desc_sw32(const void* smem_tile) {
@@ -321,10 +323,11 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
             __syncwarp();
             if (t == 0 || second) {
 #pragma unroll
-              for (int k = 0; k < KB * 4; ++k)
+              for (int k = 0; k < KB * 4; ++k) {
                 warp_umma_f16(tmem + t * COLS, da + (uint64_t)((t * KB + (k >> 2)) * (BLK / 16) + (k & 3) * 2),
                               db + (uint64_t)((k >> 2) * (F::COLUMNS * 128 / 16) + (k & 3) * 2), idesc, k != 0);
-              if (!CAP) warp_umma_f16(tmem + t * COLS, d_one, d_aug + (uint64_t)((tile & 1) * (COLS * 32 / 16)), idesc, 1);
+                if (!CAP && k == KB * 2 + KB / 2) warp_umma_f16(tmem + t * COLS, d_one, d_aug + (uint64_t)((tile & 1) * (COLS * 32 / 16)), idesc, 1);
+              }
             }
             warp_umma_commit(&s_full[t]);
             if (j == g.n - 1) warp_umma_commit(&k_empty[t]);
