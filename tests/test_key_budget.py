@@ -123,3 +123,17 @@ def test_refusals():
     md.causal = False
     with pytest.raises(ValueError):
         ops.scored_attention(q, cache, md, 1.0, scores)
+
+
+def test_numbers_above_32_bits():
+    """A budget, a protected part or a window larger than any request."""
+    q, cache, md, scores = step([5, 33], [5, 33], 4, 2, 24, 16, torch.float32, "cpu", vt=False)
+    lse = torch.zeros(38, 4)
+    want = ops.key_weights(q, cache, md, 1.0, lse, scores.clone())
+    for last in (2 ** 31, 2 ** 32 + 1):
+        assert torch.equal(ops.key_weights(q, cache, md, 1.0, lse, scores.clone(), last=last), want)
+    for numbers in ((2 ** 31, 0, 0), (2 ** 32 + 4, 0, 0), (2 ** 34, 2 ** 32 + 1, 2 ** 32 + 1)):
+        was = cache.clone()
+        lens, new, _ = ops.evict_keys(cache, md, scores, *numbers)
+        assert lens.tolist() == [5, 33] and lens.dtype is torch.int32 and torch.equal(cache.view(torch.int32), was.view(torch.int32))
+        assert torch.equal(new[1, :, :33], scores[1, :, :33])

@@ -25,9 +25,9 @@ def _check_decode(q, cache, md, scores, cap=0.0, sinks=None, scale=None, out=Non
     n = weights.shape[2]
     total = before.double()
     total[:md.num_reqs, :, :n] += weights
-    # each weight as exact as its exponential and the log-sum-exp; the sum is rounded once
+    # each weight as exact as its exponential and the log-sum-exp; an addition for every head of a kv head; the sum is rounded once
     bound = 2.0 ** -24 * total + 0.0
-    bound[:md.num_reqs, :, :n] += (2 * eps + 2.0 ** -20) * weights + 2.0 ** -126
+    bound[:md.num_reqs, :, :n] += (2 * eps + max(2.0 ** -20, q.shape[1] // cache.shape[2] * 2.0 ** -24)) * weights + 2.0 ** -126
     assert ((scores.double() - total).abs() <= bound).all(), ((scores.double() - total).abs() / bound.clamp(min=1e-300)).max()
     seen = torch.arange(scores.shape[2], device="cuda") < md.seq_lens[:md.num_reqs, None, None]
     assert torch.equal(scores[:md.num_reqs][~seen.expand_as(scores[:md.num_reqs])], before[:md.num_reqs][~seen.expand_as(scores[:md.num_reqs])])
@@ -334,6 +334,43 @@ def test_same_bits():
         got = ops.scored_attention(q, cache, md, 0.1, s), s, ops.key_weights(pq, pcache, pmd, 0.1, lse, t)
         assert want is None or all(torch.equal(a, b) for a, b in zip(got, want))
         want = got
+
+
+def test_numbers_above_32_bits():
+    q, cache, md, scores = step([5, 300], [5, 300], 8, 2, 128, 64, torch.bfloat16, "cuda")
+    lse = torch.full((305, 8), 3.0, device="cuda")
+    want = ops.key_weights(q, cache, md, 0.1, lse, scores.clone())
+    for last in (2 ** 31, 2 ** 32 + 1):
+        assert torch.equal(ops.key_weights(q, cache, md, 0.1, lse, scores.clone(), last=last), want)
+    for numbers in ((2 ** 31, 0, 0), (2 ** 32 + 4, 0, 0), (2 ** 34, 2 ** 32 + 1, 2 ** 32 + 1)):
+        was = cache.clone()
+        lens, new, _ = ops.evict_keys(cache, md, scores, *numbers)
+        assert lens.tolist() == [5, 300] and torch.equal(cache.view(torch.int16), was.view(torch.int16)) and torch.equal(new[1, :, :300], scores[1, :, :300])
+
+
+@pytest.mark.parametrize("Hq,D,BS", [(256, 64, 16), (255, 128, 64)])
+def test_decode_many_heads(Hq, D, BS):
+    q, cache, md, scores = step([1, 200, 70], [1] * 3, Hq, 1, D, BS, torch.bfloat16, "cuda", spread=2.0)
+    _check_decode(q, cache, md, scores)
+
+
+def test_step_refusals():
+    """What a step says of its requests: too few of them, or on the host."""
+    q, cache, md, scores = step([33, 5], [1, 1], 8, 2, 128, 64, torch.bfloat16, "cuda", vt=True)
+    lse = torch.zeros(2, 8, device="cuda")
+    replace = dataclasses.replace
+    for md_ in (replace(md, block_table=md.block_table.cpu()), replace(md, seq_lens=md.seq_lens.cpu()), replace(md, block_table=md.block_table[:1]),
+                replace(md, seq_lens=md.seq_lens[:1]), replace(md, block_table=md.block_table[0])):
+        for call in (lambda: ops.scored_attention(q, cache, md_, 0.1, scores), lambda: ops.key_weights(q, cache, md_, 0.1, lse, scores),
+                     lambda: ops.evict_keys(cache, md_, scores, 4)):
+            with pytest.raises(ValueError):
+                call()
+    for qsl in (md.query_start_loc[:2], md.query_start_loc.cpu()):
+        with pytest.raises(ValueError):
+            ops.key_weights(q, cache, replace(md, decode_only=False, query_start_loc=qsl), 0.1, lse, scores)
+    many = step([33, 5], [1, 1], 257, 1, 64, 16, torch.bfloat16, "cuda")
+    with pytest.raises(ValueError):
+        ops.scored_attention(many[0], many[1], many[2], 0.1, many[3])
 
 
 def test_refusals(monkeypatch):

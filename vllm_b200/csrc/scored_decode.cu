@@ -17,7 +17,7 @@
 //
 // Decode is bound by the bytes of the cache; a tcgen05 product (128 keys x 16) would take the scores through tensor memory and
 // barriers between roles for products that are a few percent of the time.  us for 64 requests of 1000 with 32 / 8 heads of 128 (bytes 40.9):
-// 54, of which the first kernel takes 46 and the join 8; two of 95000 (121) 136; one of 700 (0.45) 6.3 in clusters and 8.6 without; 24 of 60 to 924 with
+// 54, of which the first kernel takes 46 and the join 8; two of 95000 (121) 131; one of 700 (0.45) 6.3 in clusters and 8.6 without; 24 of 60 to 924 with
 // 16 / 8 heads of 64, capped, fp16 (3.8) 15.7.
 // The other way to the weights, a second pass over the keys, would read half the cache again.
 #include "attention_prompt.cuh"

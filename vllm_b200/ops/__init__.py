@@ -281,6 +281,7 @@ def key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap: float = 0.
     _check_queries(q, kv_cache, md, H, D, "key_weights")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device or last < 0:
         raise ValueError(f"key_weights: lse {tuple(lse.shape)} of {lse.dtype} for queries {tuple(q.shape)}, last {last}")
+    last = min(last, q.shape[0])                 # (kernels take 32 bits)
     if cuda:
         return cuda_ops().key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap, last)
     sl = md.seq_lens_cpu if md.seq_lens_cpu is not None else md.seq_lens.cpu()
@@ -309,6 +310,7 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int = 0, recent: int = 0,
         raise ValueError(f"evict_keys: positions {tuple(positions.shape)} of {positions.dtype} for scores {tuple(scores.shape)}")
     if scores.shape[0] != md.num_reqs:
         raise ValueError(f"evict_keys: scores of {scores.shape[0]} requests, {md.num_reqs} in the step")
+    keep, first, recent = (min(x, max(scores.shape[2], 1)) for x in (keep, first, recent))          # (the same, and in 32 bits)
     if cuda:
         return cuda_ops().evict_keys(kv_cache, md, scores, keep, first, recent, positions)
     return ref.evict_keys(kv_cache, md.block_table, md.seq_lens[:md.num_reqs], scores, keep, first, recent, positions, md.kv_vt)

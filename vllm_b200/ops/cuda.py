@@ -559,11 +559,13 @@ _I32 = torch.int32
 
 def _key_pages(kv_cache, md, scores):
     """(block table, lengths, rows that both the table and ``scores`` have room for) of kernels over paged keys; they read no row behind that."""
-    bt, sl = md.block_table, md.seq_lens
-    if bt.dtype is not _I32 or bt.stride(1) != 1 or sl.dtype is not _I32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
+    bt, sl, dev, B = md.block_table, md.seq_lens, _device(), md.num_reqs
+    if bt.dtype is not _I32 or len(bt.shape) != 2 or bt.stride(1) != 1 or sl.dtype is not _I32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
         raise ValueError("paged keys: a 16-byte aligned cache, int32 block tables with a request's pages next to each other, int32 lengths")
-    if scores.get_device() != _device():
-        raise ValueError(f"paged keys: tensors of device {scores.get_device()} while {_device()} is the current one")
+    if scores.get_device() != dev or bt.get_device() != dev or sl.get_device() != dev:
+        raise ValueError(f"paged keys: scores, pages and lengths on {scores.device}, {bt.device}, {sl.device} while device {dev} is the current one")
+    if bt.shape[0] < B or sl.shape[0] < B:
+        raise ValueError(f"paged keys: pages of {bt.shape[0]} and lengths of {sl.shape[0]} requests for {B}")
     return bt, sl, min(bt.shape[1] * kv_cache.shape[3], scores.shape[2])
 
 
@@ -609,6 +611,8 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
     G, sms, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
+    if G > 256:                              # (the second kernel has the factors of all of them in shared memory)
+        raise ValueError(f"scored_attention: {G} query heads for a kv head; up to 256")
     ctas, n, tiles = sms * (2 if D <= 128 else 1), min(B, 512) * Hkv, -(-rows // 64)
     parts, ws = scored_parts(B * Hkv, tiles, G, D, ctas), None
     if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
@@ -637,8 +641,8 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     lse = lse.contiguous()
     bt, sl, rows = _key_pages(kv_cache, md, scores)
     qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
-    if qsl is not None and (qsl.dtype is not _I32 or not qsl.is_contiguous()):
-        raise ValueError("key_weights: int32 query offsets")
+    if qsl is not None and (qsl.dtype is not _I32 or not qsl.is_contiguous() or qsl.get_device() != q.get_device() or qsl.numel() <= md.num_reqs):
+        raise ValueError("key_weights: int32 query offsets of all requests, on the device")
     ctas, most = num_sms(), min(last or most, most)
     # a tile of queries is 256 columns (128 for heads above 192), a power of two of tokens; where that is all of them, no sum is split
     one = most <= 1 << (((256 if D <= 192 else 128) // (Hq // Hkv)).bit_length() - 1)
