@@ -560,13 +560,14 @@ _I32 = torch.int32
 def _key_pages(kv_cache, md, scores):
     """(block table, lengths, rows that both the table and ``scores`` have room for) of kernels over paged keys; they read no row behind that."""
     bt, sl, dev, B = md.block_table, md.seq_lens, _device(), md.num_reqs
-    if bt.dtype is not _I32 or len(bt.shape) != 2 or bt.stride(1) != 1 or sl.dtype is not _I32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
+    if bt.dtype is not _I32 or bt.dim() != 2 or bt.stride(1) != 1 or sl.dtype is not _I32 or not sl.is_contiguous() or kv_cache.data_ptr() % 16:
         raise ValueError("paged keys: a 16-byte aligned cache, int32 block tables with a request's pages next to each other, int32 lengths")
     if scores.get_device() != dev or bt.get_device() != dev or sl.get_device() != dev:
         raise ValueError(f"paged keys: scores, pages and lengths on {scores.device}, {bt.device}, {sl.device} while device {dev} is the current one")
-    if bt.shape[0] < B or sl.shape[0] < B:
-        raise ValueError(f"paged keys: pages of {bt.shape[0]} and lengths of {sl.shape[0]} requests for {B}")
-    return bt, sl, min(bt.shape[1] * kv_cache.shape[3], scores.shape[2])
+    n, width = bt.shape
+    if n < B or sl.numel() < B:
+        raise ValueError(f"paged keys: pages of {n} and lengths of {sl.numel()} requests for {B}")
+    return bt, sl, min(width * kv_cache.shape[3], scores.shape[2])
 
 
 def _q_heads(q):
