@@ -377,11 +377,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
                   make_uint2(pack2<T>(to_f32(hi), to_f32(mid)), pack2<T>(rest - to_f32(mid), 0.f));
             }
           }
-          if (!CAP) {
-            fence_proxy_async();
-            __syncwarp();
-          }
+          if (!CAP) fence_proxy_async();
           none = __any_sync(0xffffffffu, none);
+          __syncwarp();                      // (a vote orders no memory: all lanes' values are there before lane 0 says so)
           if (lane == 0) {
             odd[slot] = none;
             mbar_arrive(&l_full[slot]);
