@@ -1,0 +1,105 @@
+"""Scored attention of prompts and of batch-invariant mode: what a call says is looked at before anything is launched.  Runs on the host: the launches
+are stand-ins that note that they were reached."""
+import dataclasses
+
+import pytest
+import torch
+
+from tests.key_budget_oracle import step
+from vllm_b200 import ops
+from vllm_b200.ops import cuda as cu
+from vllm_b200.ops import ref
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Names of what was launched, in order, with the queries and the output that each was given."""
+    seen = []
+
+    def attention(q, kv_cache, md, scale, window=None, cap=0.0, causal=True, out=None, return_lse=False, sinks=None, **_):
+        seen.append(("attention", q, out))
+        qsl = torch.arange(md.num_reqs + 1) if md.decode_only else md.query_start_loc
+        o, lse = ref.paged_attention(q[:int(qsl[-1])], kv_cache, md.block_table, md.seq_lens, qsl, scale, logits_soft_cap=cap, sinks=sinks, return_lse=True)
+        out = torch.full_like(q, float("nan"), memory_format=torch.contiguous_format) if out is None else out
+        out[:o.shape[0]] = o
+        return out, torch.cat([lse.float(), torch.full((q.shape[0] - o.shape[0], q.shape[1]), float("nan"))])
+
+    def weights(*a):
+        seen.append(("weights",))
+        return 0
+
+    def decode(*a):
+        seen.append(("decode",))
+        return 0
+    monkeypatch.setattr(ops, "_use_cuda", lambda x: True)
+    for name, f in (("paged_attention", attention), ("_key_weights", weights), ("_scored_decode", decode), ("_device", lambda: -1), ("_st", lambda: 0),
+                    ("num_sms", lambda: 148), ("_error_flag", lambda d: None)):
+        monkeypatch.setattr(cu, name, f)
+    return seen
+
+
+def _steps(invariant, monkeypatch, Hq=8, Hkv=2, D=24, BS=16, vt=False):
+    """A prompt, or a decode step in batch-invariant mode."""
+    if invariant:
+        monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
+    queries = [1, 1] if invariant else [20, 5]
+    q, cache, md, scores = step([33, 5], queries, Hq, Hkv, D, BS, torch.bfloat16, "cpu", vt=vt)
+    return q, cache.nan_to_num(0.0), md, scores
+
+
+@pytest.mark.parametrize("invariant", [False, True])
+def test_refusals(calls, monkeypatch, invariant):
+    q, cache, md, scores = _steps(invariant, monkeypatch)
+    replace = dataclasses.replace
+    odd = torch.zeros(cache.numel() + 4, dtype=cache.dtype)[4:].view(cache.shape)
+    assert odd.data_ptr() % 16 or cache.data_ptr() % 16
+    bad = [(q, odd if odd.data_ptr() % 16 else cache, md, {})]
+    for change in (dict(block_table=md.block_table.long()), dict(block_table=md.block_table[:1]), dict(block_table=md.block_table[0]), dict(block_table=md.block_table.t().contiguous().t()),
+                   dict(seq_lens=md.seq_lens.long()), dict(seq_lens=md.seq_lens[:1]), dict(query_start_loc=md.query_start_loc.long()),
+                   dict(query_start_loc=md.query_start_loc[:2]),
+                   dict(block_table=md.block_table[:, :2])):                      # (two pages of 16 for 33 rows)
+        bad.append((q, cache, replace(md, **change), {}))
+    if not invariant:
+        bad.append((q, cache, replace(md, query_start_loc=None), {}))
+    bad.append((q, cache, md, {"out": q.transpose(0, 1).contiguous().transpose(0, 1)}))
+    bad.append((q, cache, md, {"scale": 0.0}))
+    for q_, cache_, md_, more in bad:
+        more = {"scale": 0.1, **more}
+        with pytest.raises(ValueError):
+            ops.scored_attention(q_, cache_, md_, more.pop("scale"), scores, **more)
+        assert not calls, (calls, md_, more)
+    q, cache, md, scores = _steps(invariant, monkeypatch, Hq=129, Hkv=1)
+    with pytest.raises(ValueError):
+        ops.scored_attention(q, cache, md, 0.1, scores)
+    for heads in (5, 40):                                                       # transposed values: 128 is no multiple of the heads of a kv head
+        q, cache, md, scores = _steps(invariant, monkeypatch, Hq=heads, Hkv=1, D=128, BS=64, vt=True)
+        with pytest.raises(ValueError):
+            ops.scored_attention(q, cache, md, 0.1, scores)
+    assert not calls
+
+
+@pytest.mark.parametrize("invariant", [False, True])
+@pytest.mark.parametrize("where", ["", "given", "odd", "wide"])
+def test_padded_and_unaligned(calls, monkeypatch, invariant, where):
+    """Rows behind the last request are as they were in an output that was given; kernels get rows at 16-byte addresses."""
+    q, cache, md, scores = _steps(invariant, monkeypatch)
+    used = q.shape[0]
+    want = ref.paged_attention(q, cache, md.block_table, md.seq_lens, md.query_start_loc, 0.1)
+    q = torch.cat([q, torch.full_like(q[:1], float("nan")).expand(3, -1, -1)])
+    T = q.shape[0]
+    q = torch.cat([torch.zeros(T, 1, 24, dtype=q.dtype), q], 1).flatten(1)[:, 20:][:, 4:].unflatten(1, (8, 24))      # a slice of wider rows
+    out = {"": None, "given": torch.full((T, 8, 24), 7.0, dtype=q.dtype), "odd": torch.full((T * 192 + 4,), 7.0, dtype=q.dtype)[4:].view(T, 8, 24),
+           "wide": torch.full((T, 197), 7.0, dtype=q.dtype)[:, 5:].unflatten(1, (8, 24))}[where]
+    got = ops.scored_attention(q, cache, md, 0.1, scores, out=out)
+    assert [c[0] for c in calls] == ["attention", "weights"]
+    for x in calls[0][1:]:
+        assert x is not None and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) == 24 and x.stride(2) == 1
+    assert torch.equal(got[:used], want) and (out is None or (got[used:] == 7.0).all())
+    assert out is None or got is out
+
+
+def test_key_weights_without_offsets(calls, monkeypatch):
+    q, cache, md, scores = _steps(False, monkeypatch)
+    with pytest.raises(ValueError):
+        ops.key_weights(q, cache, dataclasses.replace(md, query_start_loc=None), 0.1, torch.zeros(25, 8), scores)
+    assert not calls

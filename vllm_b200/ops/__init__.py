@@ -253,7 +253,10 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
     """``paged_attention`` that also adds to ``scores`` [requests, kv heads, rows] (fp32, in place) the weights that each cached key gets, summed
     over the query heads of its kv head and the request's query rows (its ``last`` ones, 0: all): what ``evict_keys`` chooses by.  Returns the
     output.  Rows of ``scores`` behind a request's last key stay as they are; rows that are not in the cache yet have to be 0 when they come.
-    No two requests may share a row of ``scores``."""
+    No two requests may share a row of ``scores``.
+
+    On the device a kv head has up to 256 query heads in decode steps; up to 128, a power of two of them over transposed values, in prompts and in
+    batch-invariant mode, where ``scale`` is not 0.  As in ``paged_attention``, numbers of pages and lengths of prompts are taken as they are."""
     cuda = _use_cuda(q)
     H, D = _check_scores(scores, kv_cache, md, "scored_attention", cuda)
     _check_queries(q, kv_cache, md, H, D, "scored_attention")
@@ -265,8 +268,10 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
         raise ValueError(f"scored_attention: {sinks.numel()} sinks for {q.shape[1]} heads")
     if not cuda and md.kv_vt:
         raise ValueError("scored_attention: the tensor-core cache layout is CUDA only")
-    if cuda and md.decode_only:
-        return cuda_ops().scored_decode(q, kv_cache, md, scale, scores, logits_soft_cap, sinks, out)
+    if cuda:
+        if md.decode_only:
+            return cuda_ops().scored_decode(q, kv_cache, md, scale, scores, logits_soft_cap, sinks, out)
+        return cuda_ops().scored_rows(q, kv_cache, md, scale, scores, logits_soft_cap, sinks, last, out)
     o, lse = paged_attention(q, kv_cache, md, scale, None, logits_soft_cap, out=out, sinks=sinks, return_lse=True)
     key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap, last)
     return o

@@ -593,10 +593,7 @@ def scored_parts(pairs: int, tiles: int, G: int, D: int, ctas: int) -> int:
 def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=None):
     """Attention of one token per request that adds the keys' weights to ``scores`` (csrc/scored_decode.cu)."""
     if batch_invariant():                    # that kernel deals the keys of all requests to the SMs
-        from vllm_b200 import ops
-        o, lse = paged_attention(q, kv_cache, md, scale, None, soft_cap, out=out, sinks=sinks, return_lse=True)
-        ops.key_weights(q, kv_cache, md, scale, lse, scores, soft_cap)
-        return o
+        return scored_rows(q, kv_cache, md, scale, scores, soft_cap, sinks, 0, out)
     B, (_, Hq, D), (blocks, _, Hkv, BS, _) = md.num_reqs, q.shape, kv_cache.shape
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = _q_heads(q)
@@ -631,20 +628,59 @@ _key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _
 
 def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last: int = 0):
     """Adds the weights that query rows give to the cached keys to ``scores`` (csrc/key_weights.cu)."""
-    T, Hq, D = q.shape
-    Hkv = kv_cache.shape[2]
-    if Hq // Hkv > 128:
-        raise ValueError(f"key_weights: {Hq // Hkv} query heads for a kv head; up to 128")
-    if not scale:
-        raise ValueError("key_weights: a scale of 0")          # (the kernel divides by it)
+    pages = _weights_step(q, kv_cache, md, scale, scores)
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = _q_heads(q)
-    lse = lse.contiguous()
-    bt, sl, rows = _key_pages(kv_cache, md, scores)
-    qsl, most = (None, 1) if md.decode_only else (md.query_start_loc, md.max_query_len)
-    if qsl is not None and (qsl.dtype is not _I32 or not qsl.is_contiguous() or qsl.get_device() != q.get_device() or qsl.numel() <= md.num_reqs):
-        raise ValueError("key_weights: int32 query offsets of all requests, on the device")
-    ctas, most = num_sms(), min(last or most, most)
+    return _add_weights(q, kv_cache, md, scale, lse.contiguous(), scores, soft_cap, last, pages)
+
+
+def _query_offsets(md, device: int):
+    qsl = md.query_start_loc
+    if qsl is None or qsl.dtype is not _I32 or not qsl.is_contiguous() or qsl.get_device() != device or qsl.numel() <= md.num_reqs:
+        raise ValueError("key weights: int32 query offsets of all requests, on the device")
+    return qsl
+
+
+def _weights_step(q, kv_cache, md, scale, scores):
+    """(block table, lengths, rows, offsets) of a step, as the kernel takes them."""
+    G = q.shape[1] // kv_cache.shape[2]
+    if G > 128:
+        raise ValueError(f"key weights: {G} query heads for a kv head; up to 128")
+    if not scale:
+        raise ValueError("key weights: a scale of 0")          # (the kernel divides by it)
+    return (*_key_pages(kv_cache, md, scores), None if md.decode_only else _query_offsets(md, q.get_device()))
+
+
+def scored_rows(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, last=0, out=None):
+    """Attention, then the weights by its log-sum-exps: of prompts, and of decode steps in batch-invariant mode.  The attention kernels take a step's
+    addresses as they are, so everything is looked at before the first launch."""
+    (T, Hq, D), (_, _, Hkv, BS, _) = q.shape, kv_cache.shape
+    pages = _weights_step(q, kv_cache, md, scale, scores)
+    if md.query_start_loc is not None:
+        _query_offsets(md, q.get_device())
+    if pages[0].shape[1] * BS < md.max_seq_len:
+        raise ValueError(f"scored_attention: {pages[0].shape[1]} pages of {BS} for requests of up to {md.max_seq_len} rows")
+    if md.kv_vt and not tc_attention_ok(D, D, Hq // Hkv):
+        raise ValueError(f"scored_attention: {Hq // Hkv} query heads for a kv head over transposed values; a power of two up to 128 in prompts and batch-invariant mode")
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = _q_heads(q)
+    used, to = md.num_reqs if md.decode_only else md.num_actual_tokens, out
+    if out is not None and (out.stride(2) != 1 or out.stride(1) != D):
+        raise ValueError("scored_attention: the heads of an output row are next to each other")
+    if out is None or out.data_ptr() % 16 or out.stride(0) % 8:
+        to = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _, lse = paged_attention(q, kv_cache, md, scale, None, soft_cap, out=to, sinks=sinks, return_lse=True)
+    _add_weights(q, kv_cache, md, scale, lse, scores, soft_cap, min(last, T), pages)
+    if out is None or to is out:
+        return to
+    out[:used] = to[:used]
+    return out
+
+
+def _add_weights(q, kv_cache, md, scale, lse, scores, soft_cap, last, pages):
+    (T, Hq, D), Hkv, (bt, sl, rows, qsl) = q.shape, kv_cache.shape[2], pages
+    ctas, most = num_sms(), 1 if qsl is None else md.max_query_len
+    most = min(last or most, most)
     # a tile of queries is 256 columns (128 for heads above 192), a power of two of tokens; where that is all of them, no sum is split
     one = most <= 1 << (((256 if D <= 192 else 128) // (Hq // Hkv)).bit_length() - 1)
     part = None if one or batch_invariant() else scores.new_empty(ctas * 516)
