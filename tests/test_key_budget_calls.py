@@ -81,7 +81,7 @@ def test_refusals(calls, monkeypatch, invariant):
 @pytest.mark.parametrize("invariant", [False, True])
 @pytest.mark.parametrize("where", ["", "given", "odd", "wide"])
 def test_padded_and_unaligned(calls, monkeypatch, invariant, where):
-    """Rows behind the last request are as they were in an output that was given; kernels get rows at 16-byte addresses."""
+    """Rows behind the last request are zeros, or as they were in an output that was given; kernels get rows at 16-byte addresses."""
     q, cache, md, scores = _steps(invariant, monkeypatch)
     used = q.shape[0]
     want = ref.paged_attention(q, cache, md.block_table, md.seq_lens, md.query_start_loc, 0.1)
@@ -94,7 +94,7 @@ def test_padded_and_unaligned(calls, monkeypatch, invariant, where):
     assert [c[0] for c in calls] == ["attention", "weights"]
     for x in calls[0][1:]:
         assert x is not None and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) == 24 and x.stride(2) == 1
-    assert torch.equal(got[:used], want) and (out is None or (got[used:] == 7.0).all())
+    assert torch.equal(got[:used], want) and (got[used:] == (0.0 if out is None else 7.0)).all()
     assert out is None or got is out
 
 

@@ -49,7 +49,7 @@ def test_refusals_in_front_of_attention(invariant, monkeypatch):
 @pytest.mark.parametrize("where", ["", "given", "odd", "wide"])
 @pytest.mark.parametrize("D,BS,vt", [(128, 64, True), (64, 16, False), (80, 16, False)])
 def test_padded_and_unaligned(invariant, where, D, BS, vt, monkeypatch):
-    """Padding rows behind the last request, queries and outputs at odd addresses: the bits of a plain call, what was there behind them."""
+    """Padding rows behind the last request, queries and outputs at odd addresses: the bits of a plain call, zeros (or what was there) behind them."""
     if invariant:
         monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
     q, cache, md, scores = step([33, 70], [1, 1] if invariant else [20, 45], 8, 2, D, BS, torch.bfloat16, "cuda", vt=vt)
@@ -63,5 +63,5 @@ def test_padded_and_unaligned(invariant, where, D, BS, vt, monkeypatch):
     out = {"": None, "given": torch.full((T, 8, D), 7.0, dtype=q.dtype, device="cuda"), "odd": torch.full((T * 8 * D + 4,), 7.0, dtype=q.dtype, device="cuda")[4:].view(T, 8, D),
            "wide": torch.full((T, 8 * D + 5), 7.0, dtype=q.dtype, device="cuda")[:, 5:].unflatten(1, (8, D))}[where]
     got = ops.scored_attention(q, cache, md, 0.1, scores, out=out)
-    assert torch.equal(got[:used], want) and torch.equal(scores, other) and (out is None or (got[used:] == 7.0).all())
+    assert torch.equal(got[:used], want) and torch.equal(scores, other) and (got[used:] == (0.0 if out is None else 7.0)).all()
     assert out is None or got is out

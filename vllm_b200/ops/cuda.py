@@ -669,6 +669,8 @@ def scored_rows(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, last=0
         raise ValueError("scored_attention: the heads of an output row are next to each other")
     if out is None or out.data_ptr() % 16 or out.stride(0) % 8:
         to = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if T > used:                         # (padding rows are written by no CTA: keep them finite)
+            to[used:].zero_()
     _, lse = paged_attention(q, kv_cache, md, scale, None, soft_cap, out=to, sinks=sinks, return_lse=True)
     _add_weights(q, kv_cache, md, scale, lse, scores, soft_cap, min(last, T), pages)
     if out is None or to is out:
