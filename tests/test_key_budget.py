@@ -1,4 +1,6 @@
 """A key-value cache with a budget on the CPU: the plain forms against 64 bits, a run of the operators as a generation uses them, and what is refused."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -137,3 +139,13 @@ def test_numbers_above_32_bits():
         lens, new, _ = ops.evict_keys(cache, md, scores, *numbers)
         assert lens.tolist() == [5, 33] and lens.dtype is torch.int32 and torch.equal(cache.view(torch.int32), was.view(torch.int32))
         assert torch.equal(new[1, :, :33], scores[1, :, :33])
+
+
+def test_weights_infinite():
+    """Rows whose log-sum-exp is infinite or NaN give nothing, whatever their scores are."""
+    q, cache, md, scores = step([40], [9], 4, 2, 24, 16, torch.float32, "cpu")
+    lse = attend(q, cache, md, 0.3)[1].float()
+    want = ops.key_weights(q[5:], cache, dataclasses.replace(md, query_start_loc=torch.tensor([0, 4]), query_start_loc_cpu=torch.tensor([0, 4])), 0.3, lse[5:], scores.clone())
+    lse[0], lse[1], lse[2:5] = float("nan"), float("-inf"), float("inf")
+    q[3] = float("inf")
+    assert torch.equal(ops.key_weights(q, cache, md, 0.3, lse, scores.clone()), want)

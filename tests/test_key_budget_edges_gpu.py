@@ -4,7 +4,7 @@ import dataclasses
 import pytest
 import torch
 
-from tests.key_budget_oracle import step
+from tests.key_budget_oracle import attend, step, weight_error
 from tests.test_key_budget_gpu import _check_weights
 from vllm_b200 import ops
 
@@ -65,3 +65,55 @@ def test_padded_and_unaligned(invariant, where, D, BS, vt, monkeypatch):
     got = ops.scored_attention(q, cache, md, 0.1, scores, out=out)
     assert torch.equal(got[:used], want) and torch.equal(scores, other) and (got[used:] == (0.0 if out is None else 7.0)).all()
     assert out is None or got is out
+
+
+def _check_sums(q, cache, md, scores, scale, lse, cap=0.0, last=0):
+    """``_check_weights`` for scales of either sign, with log-sum-exps that may be larger than the scores: the factor, the product, the parts and the
+    sums that they join (at most D / 16 + 4 additions, cut or rounded) are off by 2^-23 of them each."""
+    D, turn = q.shape[2], -1 if scale < 0 else 1
+    given = torch.where(lse.isfinite(), lse, torch.inf)
+    _, _, weights, _, terms = attend(q * turn, cache, md, scale * turn, cap, None, last, given)
+    size = float(lse[lse.isfinite()].abs().max())
+    before = scores.clone()
+    ops.key_weights(q, cache, md, scale, lse, scores, cap, last)
+    n = weights.shape[2]
+    total = before.double()
+    total[:, :, :n] += weights
+    bound = 2.0 ** -24 * total
+    bound[:, :, :n] += (weight_error(terms, D) + (D / 16 + 4) * 2.0 ** -23 * size + 38 * 2.0 ** -24) * weights + 2.0 ** -126
+    assert ((scores.double() - total).abs() <= bound).all(), ((scores.double() - total).abs() / bound.clamp(min=1e-300)).max()
+    seen = torch.arange(scores.shape[2], device="cuda") < md.seq_lens[:, None, None]
+    assert torch.equal(scores[~seen.expand_as(scores)], before[~seen.expand_as(scores)])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D,BS,vt", [(8, 2, 128, 64, True), (9, 1, 64, 16, False), (6, 2, 256, 32, False)])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_weights_infinite(dtype, Hq, Hkv, D, BS, vt, cap):
+    """Rows whose log-sum-exp is infinite or NaN give nothing, in tiles that all rows see and in those on the diagonal."""
+    q, cache, md, scores = step([900, 400], [300, 400], Hq, Hkv, D, BS, dtype, "cuda", vt=vt, seed=1)
+    lse = attend(q, cache, md, D ** -0.5, cap)[1].float()
+    lse[::3], lse[1::5], lse[2::7] = float("inf"), float("-inf"), float("nan")
+    _check_sums(q, cache, md, scores, D ** -0.5, lse, cap)
+    lse[:, 1:] = float("inf")
+    _check_sums(q, cache, md, scores, D ** -0.5, lse, cap)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,BS,vt", [(8, 2, 128, 64, True), (9, 1, 64, 16, False), (33, 1, 128, 32, False), (10, 2, 256, 16, False)])
+@pytest.mark.parametrize("scale,cap", [(-0.1, 0.0), (-0.1, 30.0), (0.1, 0.0), (0.1, 30.0)])
+def test_weights_of_either_sign(Hq, Hkv, D, BS, vt, scale, cap):
+    """Scales below 0, also where heads x tokens of a tile leave columns that nothing uses."""
+    q, cache, md, scores = step([900, 200], [300, 200], Hq, Hkv, D, BS, torch.bfloat16, "cuda", vt=vt, seed=2)
+    turn = -1 if scale < 0 else 1
+    lse = attend(q * turn, cache, md, scale * turn, cap)[1].float()
+    _check_sums(q, cache, md, scores, scale, lse, cap)
+
+
+@pytest.mark.parametrize("dtype,scale,spread", [(torch.float16, 1e-7, 1.0), (torch.float16, 1e-10, 1.0), (torch.float16, 64.0, 2.0 ** -7), (torch.float16, -64.0, 2.0 ** -7),
+                                                (torch.bfloat16, 1e-10, 1.0), (torch.bfloat16, 3e-38, 1.0), (torch.bfloat16, 1e-40, 1.0), (torch.bfloat16, 64.0, 2.0 ** -7)])
+@pytest.mark.parametrize("D,BS", [(8, 16), (128, 32)])
+def test_weights_of_small_and_large_scales(dtype, scale, spread, D, BS):
+    """Scales whose quotients with the log-sum-exps do not fit into the cache's type, or are small in it."""
+    q, cache, md, scores = step([700, 90], [200, 90], 4, 2, D, BS, dtype, "cuda", seed=3, spread=spread)
+    turn = -1 if scale < 0 else 1
+    _check_sums(q, cache, md, scores, scale, attend(q * turn, cache, md, scale * turn)[1].float())

@@ -35,7 +35,7 @@ struct Params {
   int* error;                // raised when a wait ran into its limit
   int64_t bt_stride, sc_req, sc_head, num_blocks;
   int B, row0, T, Hq, Hkv, G, TQ, D, BS, max_rows, last, box_rows, whole;      // TQ: tokens of a tile, a power of 2; whole: blocks are not split
-  float lse_in;            // -1 / (scale ONE)
+  float one, lse_in;       // what the parts of a log-sum-exp are multiples of; -1 / (scale one)
   float scale_log2, cap_in, cap_out;      // capped: 2 log2(e) scale / cap, cap log2(e)
 };
 
@@ -148,10 +148,12 @@ VB_DEVICE float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(
 
 // Other scores: a column gets sixteen more dimensions, three of which hold -lse / scale in parts of 16 bits, the keys' are constant.  The product is
 // then what the exponential takes but for a factor: no log-sum-exps out of shared memory, where 128-bit reads by all threads and the operands of the
-// products want the same bandwidth.  fp16: parts of 1 / 64, as lse / scale may be large.  They are added a little behind the middle of a product: its sums are
-// cut towards 0, and half of them are then above 0 and half below for the keys with much weight.  Relative error of the weights of 300 tokens 4.4e-7 with them
-// last, 8.6e-7 first, 1.3e-7 so (heads of 128); of 900 with heads of 256 1.1e-6, 2.5e-6 and 1.8e-7; 32-bit multiplications and additions have 1.2e-7.
-template <typename T> constexpr float ONE = DTypeOf<T>::v == DT_F16 ? 64.f : 1.f;
+// products want the same bandwidth.  fp16: they are multiples of a power of two that makes them lse / 4 to lse / 8, far from either end of the type.  Where they do
+// not fit all the same (scales next to 0) the product gets zeros and the sum the log-sum-exp, as where scores are capped.  They are added a little behind the middle
+// of a product: its sums are cut towards 0, and half of them are then above 0 and half below for the keys with much weight.  Relative error of the weights of 300
+// tokens 4.4e-7 with them last, 8.6e-7 first, 1.3e-7 so (heads of 128); of 900 with heads of 256 1.1e-6, 2.5e-6 and 1.8e-7; 32-bit multiplications and additions
+// have 1.2e-7.
+template <typename T> constexpr float MOST = DTypeOf<T>::v == DT_F16 ? 60000.f : 1e38f;          // of a part
 // rows of 32 bytes, 8-row groups 256 bytes apart, SWIZZLE_32B
 VB_DEVICE uint64_t umma_desc_sw32(const void* smem_tile) {
   return (uint64_t)((smem_u32(smem_tile) & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)6 << 61;
@@ -198,7 +200,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   unsigned char* q_smem = k_smem + F::K_BYTES;                   // [stage][KB]
   unsigned char* one_smem = q_smem + QS * F::Q_BYTES;            // [TILE][16]: what a column's sixteen further dimensions are multiplied with
   unsigned char* aug_smem = one_smem + TILE * 32;                // [slot][COLS][16]: those: less the log-sum-exp, in three parts
-  float* lse_smem = reinterpret_cast<float*>(aug_smem + 2 * COLS * 32);          // [slot][COLS]: less the log-sum-exp, in powers of two
+  float* lse_smem = reinterpret_cast<float*>(aug_smem + 2 * COLS * 32);          // [slot][COLS]: less what the product has not of the log-sum-exp, in powers of two
   float* exch = lse_smem + 2 * COLS;                             // [KEYS]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(exch + KEYS);   // [key tile]
   uint64_t* k_empty = k_full + 2;
@@ -211,7 +213,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + QS);
   int* first = reinterpret_cast<int*>(tmem_slot + 4);
   int* warp_sums = first + MAX_REQUESTS + 1;
-  __shared__ int odd[2];                     // of a tile: some column gives no weights
+  __shared__ int odd[2];                     // of a tile: some column gives no weights, or has its log-sum-exp outside the product
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int budget = MBAR_BUDGET;
@@ -235,7 +237,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
     for (int i = threadIdx.x; i < TILE * 2; i += NUM_THREADS) {
       const int row = i >> 1;                                    // (pieces of 16 bytes; those of rows 4 to 7 of eight change places)
       const bool front = ((i ^ (row >> 2)) & 1) == 0;
-      reinterpret_cast<uint4*>(one_smem)[i] = front ? make_uint4(pack2<T>(ONE<T>, ONE<T>), pack2<T>(ONE<T>, 0.f), 0, 0) : make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(one_smem)[i] = front ? make_uint4(pack2<T>(p.one, p.one), pack2<T>(p.one, 0.f), 0, 0) : make_uint4(0, 0, 0, 0);
     }
   }
   fence_proxy_async();
@@ -344,6 +346,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
       }
     } else if (warp < 4) {                   // one for each slot: a load takes as long as a tile
       constexpr int PER = COLS / 32;
+      const float never = copysignf(INFINITY, p.lse_in);         // in the place of less the log-sum-exp: a weight of 0, with a scale of either sign
       int at[PER], head[PER];                // of the lane's columns: token of the tile (-1: none), query head of the kv head
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
@@ -365,13 +368,15 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
           bool none = false;
 #pragma unroll
           for (int k = 0; k < PER; ++k) {
-            lse_smem[slot * COLS + lane + k * 32] = x[k] > -INFINITY ? x[k] * -LOG2E : -INFINITY;      // no row, or one without keys: 0
-            none |= at[k] >= 0 && !(x[k] > -INFINITY);
+            const bool row = fabsf(x[k]) < INFINITY;             // else none, or one without keys: 0
+            const float y = row ? x[k] * p.lse_in : never;
+            const bool fits = !CAP && fabsf(y) <= MOST<T>;
+            lse_smem[slot * COLS + lane + k * 32] = !row ? -INFINITY : fits ? 0.f : x[k] * -LOG2E;
+            none |= at[k] >= 0 && !(row && (CAP || fits));
             if (!CAP && k < pieces) {
               const int c = lane + k * 32;
-              const float y = x[k] > -INFINITY ? x[k] * p.lse_in : -INFINITY;
-              const T hi = from_f32<T>(y);
-              const float rest = x[k] > -INFINITY ? y - to_f32(hi) : 0.f;
+              const T hi = from_f32<T>(row && !fits ? 0.f : y);
+              const float rest = fits ? y - to_f32(hi) : 0.f;
               const T mid = from_f32<T>(rest);
               *reinterpret_cast<uint2*>(aug_smem + slot * (COLS * 32) + c * 32 + (((c >> 2) & 1) << 4)) =
                   make_uint2(pack2<T>(to_f32(hi), to_f32(mid)), pack2<T>(rest - to_f32(mid), 0.f));
@@ -395,9 +400,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
       const int qd = warp & 3, half = ((warp - 4) >> 2) & 1, t = (warp - 4) >> 3, mine = t * TILE + qd * 32 + lane;
       const int groups = (pieces - half + 1) / 2;                // 2 to 4
       const uint32_t from = tmem + t * COLS + half * 32 + ((uint32_t)(qd * 32) << 16);
-      auto weight = [&](uint32_t s, float l, bool poly) {
+      auto weight = [&](uint32_t s, float l, bool poly, bool add = CAP) {
         const float x = __uint_as_float(s);
-        const float y = CAP ? fmaf(rcp(1.f + ex2(x * p.cap_in)), -2.f * p.cap_out, p.cap_out) + l : x * p.scale_log2;
+        const float y = CAP ? fmaf(rcp(1.f + ex2(x * p.cap_in)), -2.f * p.cap_out, p.cap_out) + l : add ? fmaf(x, p.scale_log2, l) : x * p.scale_log2;
         return poly ? ex2_poly(y) : ex2(y);
       };
       int tile = 0;
@@ -455,7 +460,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
               const float* lc = ls + c * 64;
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float l = lc[i], x = weight(v[i], l, false);
+                const float l = lc[i], x = weight(v[i], l, false, true);
                 acc[i & 3] += c * 64 + i < c_lo || l == -INFINITY ? 0.f : x;
               }
             }
@@ -553,7 +558,12 @@ EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, 
   p.TQ = columns;
   while (p.TQ * p.G > columns) p.TQ /= 2;
   p.scale_log2 = scale * LOG2E;
-  p.lse_in = -1.f / (scale * (bf16 ? ONE<__nv_bfloat16> : ONE<__half>));
+  p.one = 1.f;
+  if (!bf16) {                                                   // (a power of two that fp16 has)
+    const int e = ilogbf(scale);
+    p.one = ldexpf(1.f, e > 16 ? -14 : e < -13 ? 15 : 2 - e);
+  }
+  p.lse_in = -1.f / (scale * p.one);
   p.cap_in = soft_cap > 0.f ? 2.f * LOG2E * scale / soft_cap : 0.f; p.cap_out = soft_cap * LOG2E;
   CUtensorMap tq, tk;
   cuuint32_t es[3] = {1, 1, 1};

@@ -280,7 +280,7 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
 def key_weights(q, kv_cache, md, scale, lse, scores, logits_soft_cap: float = 0.0, last: int = 0):
     """In place: scores[request, kv head, key] += sum of e^(score - lse) over the request's query rows (its ``last`` ones, 0: all) that see the
     key and the query heads of the kv head.  ``lse`` [T, query heads]: what ``paged_attention(..., return_lse=True)`` returns; a row where it is
-    -inf (no key) or NaN gives nothing.  Returns ``scores``."""
+    infinite (-inf: no key) or NaN gives nothing.  Returns ``scores``."""
     cuda = _use_cuda(q)
     H, D = _check_scores(scores, kv_cache, md, "key_weights", cuda)
     _check_queries(q, kv_cache, md, H, D, "key_weights")

@@ -592,7 +592,7 @@ def identity_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tens
 def key_weights(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor, scale: float,
                 lse: torch.Tensor, scores: torch.Tensor, logits_soft_cap: float = 0.0, last: int = 0) -> torch.Tensor:
     """In place: scores[i, kv head, key] += the weights e^(score - lse) that request i's query rows (its ``last`` ones, 0: all) give to a cached
-    key, over the query heads of the kv head.  A row whose ``lse`` is -inf or NaN gives none."""
+    key, over the query heads of the kv head.  A row whose ``lse`` is infinite or NaN gives none."""
     Hkv = kv_cache.shape[2]
     qsl, sls = query_start_loc.tolist(), seq_lens.tolist()
     for i, n in enumerate(sls):
@@ -606,7 +606,7 @@ def key_weights(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tens
             x = logits_soft_cap * torch.tanh(x / logits_soft_cap)
         norm = lse[e - t:e].float().unflatten(1, (Hkv, -1)).permute(1, 2, 0)[..., None]
         seen = torch.arange(n, device=q.device) <= torch.arange(n - t, n, device=q.device)[:, None]
-        w = torch.where(seen & (norm > float("-inf")), torch.exp(x - norm), 0.0)
+        w = torch.where(seen & norm.isfinite(), torch.exp(x - norm), 0.0)
         scores[i, :, :n] += w.sum((1, 2))
     return scores
 
