@@ -117,3 +117,32 @@ def test_weights_of_small_and_large_scales(dtype, scale, spread, D, BS):
     q, cache, md, scores = step([700, 90], [200, 90], 4, 2, D, BS, dtype, "cuda", seed=3, spread=spread)
     turn = -1 if scale < 0 else 1
     _check_sums(q, cache, md, scores, scale, attend(q * turn, cache, md, scale * turn)[1].float())
+
+
+def _small_numbers(q, cache):
+    """Queries and keys of -1, 0 and 1 (in place): their products are exact in any order."""
+    q.copy_(q.round().clamp(-1, 1))
+    keys = cache[:, 0]
+    keys.copy_(keys.nan_to_num(0.0).round().clamp(-1, 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,D,BS,vt", [(4, 128, 64, True), (5, 64, 16, False), (2, 256, 32, False)])
+@pytest.mark.parametrize("cap", [5.0, 30.0, 50.0])
+@pytest.mark.parametrize("scale", [1 / 64, 1 / 4, 4.0])
+def test_weights_capped_exactly(dtype, H, D, BS, vt, cap, scale):
+    """Weights of one query row and head each, its products exact: what is left is the error of the cap and of the exponential."""
+    q, cache, md, scores = step([2000, 300], [300, 300], H, H, D, BS, dtype, "cuda", vt=vt, seed=6)
+    _small_numbers(q, cache)
+    scores.zero_()
+    lse = torch.zeros(600, H, device="cuda") if scale < 0.1 else attend(q, cache, md, scale, cap)[1].float()
+    ops.key_weights(q, cache, md, scale, lse, scores, cap, last=1)
+    want = attend(q, cache, md, scale, cap, None, 1, lse)[2]
+    for b, n in enumerate([2000, 300]):
+        last = lse[300 * b + 299].double()[:, None]
+        size = (want[b, :, :n].log() + last).abs()                             # of the capped scores
+        # the cap: its factors, two products and a polynomial of 1.6e-7 (or an exponential of 2^-22 below 1 / 4 of it, a reciprocal and a
+        # difference); the log-sum-exp: a factor and a product; the difference of both; an exponential of 2^-22; two sums
+        error = size * (5 * 2.0 ** -24 + 1.6e-7) + last.abs() * 2.0 ** -23 + (size + last.abs()) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23
+        off = (scores[b, :, :n].double() - want[b, :, :n]).abs() / want[b, :, :n]
+        assert (off <= error + 2.0 ** -126 / want[b, :, :n]).all(), (off / error).max()

@@ -36,7 +36,7 @@ struct Params {
   int64_t bt_stride, sc_req, sc_head, num_blocks;
   int B, row0, T, Hq, Hkv, G, TQ, D, BS, max_rows, last, box_rows, whole;      // TQ: tokens of a tile, a power of 2; whole: blocks are not split
   float one, lse_in;       // what the parts of a log-sum-exp are multiples of; -1 / (scale one)
-  float scale_log2, cap_in, cap_out;      // capped: 2 log2(e) scale / cap, cap log2(e)
+  float scale_log2, ku, c2;               // capped: scale / cap, cap log2(e)
 };
 
 // What a request needs: the tiles of tokens lie side by side up to its last token.  Key block i has the last tiles(i) of them.
@@ -143,8 +143,11 @@ template <int KB> struct Form {              // KB: blocks of 64 dimensions
 };
 
 VB_DEVICE float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// Capped scores: c tanh(x) = c (1 - 2 / (1 + e^(2 x))), for all x.  Next to 0 that is off by 2^-23 c instead of a part of x, but it is an exponent:
-// its absolute error counts, as for larger x.
+// Capped scores, c2 tanh(x): up to |x| = 1 by the polynomial of the attention kernels, off by a part of x where 1 - 2 / (1 + e^(2 x)) is off by a part of the cap
+// (2e-6 of a weight for a cap of 50); the log-sum-exps are sums of the same values then.  8000 tokens of 32 / 8 heads, 512 behind 25000 twice of 16 / 4: 721 and
+// 286 us where no score of a piece is above the cap, 1442 and 565 where some are everywhere (1 - 2 / (1 + e^(2 x)) for all: 779 and 316).
+VB_DEVICE float cap_far(float x, float c2) { return copysignf(fmaf(-2.f, rcp(1.f + ex2(fabsf(x) * 2.8853900817779268f)), 1.f), x) * c2; }
+VB_DEVICE float cap_near_or_far(float x, float c2) { return fabsf(x) <= 1.f ? prompt::cap_small(x, c2) : cap_far(x, c2); }
 
 // Other scores: a column gets sixteen more dimensions, three of which hold -lse / scale in parts of 16 bits, the keys' are constant.  The product is
 // then what the exponential takes but for a factor: no log-sum-exps out of shared memory, where 128-bit reads by all threads and the operands of the
@@ -400,9 +403,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
       const int qd = warp & 3, half = ((warp - 4) >> 2) & 1, t = (warp - 4) >> 3, mine = t * TILE + qd * 32 + lane;
       const int groups = (pieces - half + 1) / 2;                // 2 to 4
       const uint32_t from = tmem + t * COLS + half * 32 + ((uint32_t)(qd * 32) << 16);
-      auto weight = [&](uint32_t s, float l, bool poly, bool add = CAP) {
+      auto weight = [&](uint32_t s, float l, bool poly, bool add, bool near) {
         const float x = __uint_as_float(s);
-        const float y = CAP ? fmaf(rcp(1.f + ex2(x * p.cap_in)), -2.f * p.cap_out, p.cap_out) + l : add ? fmaf(x, p.scale_log2, l) : x * p.scale_log2;
+        const float y = CAP ? (near ? prompt::cap_small(x * p.ku, p.c2) : cap_near_or_far(x * p.ku, p.c2)) + l : add ? fmaf(x, p.scale_log2, l) : x * p.scale_log2;
         return poly ? ex2_poly(y) : ex2(y);
       };
       int tile = 0;
@@ -428,14 +431,25 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
             if (lane == 0) mbar_arrive(&s_empty[t]);
           };
           if (key0 < n && full) {
-            auto weigh = [&](const uint32_t (&v)[16], const float* lc) {
+            auto weigh_as = [&](const uint32_t (&v)[16], const float* lc, bool near) {
 #pragma unroll
               for (int i = 0; i < 16; i += 4) {
                 const float4 l = CAP ? *reinterpret_cast<const float4*>(lc + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                acc[0] += weight(v[i], l.x, false);
-                acc[1] += weight(v[i + 1], l.y, false);
-                acc[2] += weight(v[i + 2], l.z, i % 8 == 4);
-                acc[3] += weight(v[i + 3], l.w, false);
+                acc[0] += weight(v[i], l.x, false, false, near);
+                acc[1] += weight(v[i + 1], l.y, false, false, near);
+                acc[2] += weight(v[i + 2], l.z, i % 8 == 4, false, near);
+                acc[3] += weight(v[i + 3], l.w, false, false, near);
+              }
+            };
+            auto weigh = [&](const uint32_t (&v)[16], const float* lc) {
+              if constexpr (CAP) {                               // (the whole warp takes one way)
+                float far = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) far = fmaxf(far, fabsf(__uint_as_float(v[i])));
+                if (__all_sync(0xffffffffu, far * fabsf(p.ku) <= 1.f)) weigh_as(v, lc, true);
+                else weigh_as(v, lc, false);
+              } else {
+                weigh_as(v, lc, false);
               }
             };
             uint32_t va[16], vb[16];
@@ -460,7 +474,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
               const float* lc = ls + c * 64;
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float l = lc[i], x = weight(v[i], l, false, true);
+                const float l = lc[i], x = weight(v[i], l, false, true, false);
                 acc[i & 3] += c * 64 + i < c_lo || l == -INFINITY ? 0.f : x;
               }
             }
@@ -564,7 +578,7 @@ EXPORT int vb_key_weights(const void* q, const void* cache, int64_t num_blocks, 
     p.one = ldexpf(1.f, e > 16 ? -14 : e < -13 ? 15 : 2 - e);
   }
   p.lse_in = -1.f / (scale * p.one);
-  p.cap_in = soft_cap > 0.f ? 2.f * LOG2E * scale / soft_cap : 0.f; p.cap_out = soft_cap * LOG2E;
+  p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E;
   CUtensorMap tq, tk;
   cuuint32_t es[3] = {1, 1, 1};
   {
