@@ -4,7 +4,7 @@ import dataclasses
 import pytest
 import torch
 
-from tests.key_budget_oracle import attend, step, weight_error
+from tests.key_budget_oracle import attend, step, unit, weight_error
 from tests.test_key_budget_gpu import _check_weights
 from vllm_b200 import ops
 
@@ -146,3 +146,61 @@ def test_weights_capped_exactly(dtype, H, D, BS, vt, cap, scale):
         error = size * (5 * 2.0 ** -24 + 1.6e-7) + last.abs() * 2.0 ** -23 + (size + last.abs()) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23
         off = (scores[b, :, :n].double() - want[b, :, :n]).abs() / want[b, :, :n]
         assert (off <= error + 2.0 ** -126 / want[b, :, :n]).all(), (off / error).max()
+
+
+def _check_prompt(q, cache, md, scores, scale, cap=0.0, sinks=None, last=0, out=None):
+    """Output and scores of a prompt whose queries and keys are small whole numbers (``_small_numbers``), against 64 bits."""
+    D, n_max = q.shape[2], max(md.seq_lens.tolist())
+    want, norm, weights, mass, terms = attend(q, cache, md, scale, cap, sinks, last)
+    before = scores.clone()
+    got = ops.scored_attention(q, cache, md, scale, scores, logits_soft_cap=cap, sinks=sinks, last=last, out=out)
+    assert out is None or got is out
+    lse = float(norm[norm.isfinite()].abs().max())
+    size = min(terms, cap or terms)                                            # of the scores, whose products are exact
+    # a weight of the attention: factors and differences of its exponent, the cap (5 roundings and 1.6e-7), an exponential; the log-sum-exp: chains of 64
+    # weights in a tile, of the tiles and of warps (up to 130 additions), a logarithm, its factors
+    weight = 6 * 2.0 ** -24 * (size + lse) + (5 * 2.0 ** -24 + 1.6e-7) * size * (cap > 0) + 2.0 ** -22
+    of_lse = weight + 130 * 2.0 ** -24 + 2.0 ** -22 * (lse + 1)
+    # of a key: the same exponent, or the log-sum-exp in the middle of a product whose sums are cut (D / 32 + 3 of them left); chains of additions
+    of_key = weight + of_lse + (D / 32 + 3) * 2.0 ** -23 * (terms + lse) * (cap == 0) + 38 * 2.0 ** -24
+    u, n = unit(q.dtype), weights.shape[2]
+    bound = u * want.abs() + (u + weight + of_lse + 2.0 ** -13) * mass + (2.0 ** -25 * (1 + 6 * n_max) if q.dtype is torch.float16 else 0.0)
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / bound).max()
+    total = before.double()
+    total[:, :, :n] += weights
+    bound = 2.0 ** -24 * total
+    bound[:, :, :n] += of_key * weights + 2.0 ** -126
+    assert ((scores.double() - total).abs() <= bound).all(), ((scores.double() - total).abs() / bound.clamp(min=1e-300)).max()
+    seen = torch.arange(scores.shape[2], device="cuda") < md.seq_lens[:, None, None]
+    assert torch.equal(scores[~seen.expand_as(scores)], before[~seen.expand_as(scores)])
+
+
+PROMPTS = [(8, 2, 128, 64, True), (16, 1, 128, 64, True), (3, 3, 128, 64, True), (8, 2, 64, 16, False), (24, 3, 64, 32, False), (10, 2, 64, 16, False), (8, 2, 96, 48, False),
+           (6, 6, 80, 16, False), (8, 4, 128, 32, False), (4, 2, 256, 32, False), (33, 1, 128, 16, False), (2, 1, 8, 16, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D,BS,vt", PROMPTS)
+@pytest.mark.parametrize("cap,sink,last", [(0.0, False, 0), (0.0, True, 7), (30.0, False, 7), (4.0, True, 0)])
+@pytest.mark.parametrize("where", ["", "strided"])
+def test_prompts(dtype, Hq, Hkv, D, BS, vt, cap, sink, last, where):
+    """Prompts through every kind of attention kernel: the log-sum-exps that they hand on hold the cap and the sinks."""
+    lens, queries = [300, 1, 700, 0, 64, 130, 513], [300, 1, 45, 0, 1, 129, 3]
+    q, cache, md, scores = step(lens, queries, Hq, Hkv, D, BS, dtype, "cuda", vt=vt, seed=Hq + D)
+    _small_numbers(q, cache)
+    out = None
+    if where:
+        T = q.shape[0]
+        wide = torch.zeros(T, Hq * D + 24, dtype=dtype, device="cuda")
+        wide[:, 16:-8] = q.flatten(1)
+        q, out = wide[:, 16:-8].unflatten(1, (Hq, D)), torch.zeros(T, Hq + 3, D, dtype=dtype, device="cuda")[:, 2:-1]
+    sinks = torch.randn(Hq, generator=torch.Generator().manual_seed(1)).cuda() if sink else None
+    _check_prompt(q, cache, md, scores, D ** -0.5, cap, sinks, last, out)
+
+
+@pytest.mark.parametrize("lens,queries,last", [([3000], [3000], 0), ([2500, 700], [2500, 700], 64), ([9000, 300], [20, 300], 0), ([40] * 130, [40] * 130, 0)])
+@pytest.mark.parametrize("D,BS,vt", [(128, 64, True), (64, 16, False)])
+def test_prompts_lengths(lens, queries, last, D, BS, vt):
+    q, cache, md, scores = step(lens, queries, 8, 2, D, BS, torch.bfloat16, "cuda", vt=vt, seed=len(lens))
+    _small_numbers(q, cache)
+    _check_prompt(q, cache, md, scores, D ** -0.5, last=last)
