@@ -103,3 +103,15 @@ def test_key_weights_without_offsets(calls, monkeypatch):
     with pytest.raises(ValueError):
         ops.key_weights(q, cache, dataclasses.replace(md, query_start_loc=None), 0.1, torch.zeros(25, 8), scores)
     assert not calls
+
+
+def test_groups_of_a_decode_step():
+    """Requests of a launch: all of them where their workspace is small, else as many as have room, in groups of about the same size."""
+    for B, Hq, rows in ((1, 32, 700), (64, 32, 1344), (512, 32, 1000), (513, 8, 100), (64, 32, 131072), (512, 32, 131072), (3, 256, 10 ** 6), (1100, 8, 2000)):
+        tiles = -(-rows // 64)
+        n = cu.scored_group(B, Hq, tiles)
+        assert 1 <= n <= min(B, 512) and (n == 1 or n * Hq * tiles * 256 <= cu.SCORED_BYTES)
+        groups = -(-B // n)
+        assert n == 1 or groups * n < B + groups
+        assert groups == max(-(-B // 512), 1) or groups == 1 or (n + 1) * Hq * tiles * 256 > cu.SCORED_BYTES or -(-B // (groups - 1)) * Hq * tiles * 256 > cu.SCORED_BYTES
+    assert cu.scored_group(64, 32, 21) == 64 and cu.scored_group(512, 32, 16) == 512

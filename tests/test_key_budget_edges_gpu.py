@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from tests.key_budget_oracle import attend, step, unit, weight_error
-from tests.test_key_budget_gpu import _check_weights
+from tests.test_key_budget_gpu import _check_decode, _check_weights
 from vllm_b200 import ops
+from vllm_b200.ops import cuda_ops
 
 pytestmark = pytest.mark.gpu
 
@@ -204,3 +205,39 @@ def test_prompts_lengths(lens, queries, last, D, BS, vt):
     q, cache, md, scores = step(lens, queries, 8, 2, D, BS, torch.bfloat16, "cuda", vt=vt, seed=len(lens))
     _small_numbers(q, cache)
     _check_prompt(q, cache, md, scores, D ** -0.5, last=last)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,rows", [(64, 32, 8, 131072), (300, 8, 1, 131072), (2, 256, 1, 600000)])
+def test_decode_memory(B, Hq, Hkv, rows):
+    """Buffers for far longer texts than there are: what a call allocates has a bound."""
+    lens = [5 + 11 * i % 900 for i in range(B)]
+    q, cache, md, scores = step(lens, [1] * B, Hq, Hkv, 128, 64, torch.bfloat16, "cuda", vt=True, seed=7)
+    n = scores.shape[2]
+    scores = torch.nn.functional.pad(scores, (0, rows - n))
+    md.block_table = torch.nn.functional.pad(md.block_table, (0, rows // 64 - md.block_table.shape[1]))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before, was = scores[:, :, :n].clone(), torch.cuda.memory_allocated()
+    out = ops.scored_attention(q, cache, md, 0.1, scores)
+    torch.cuda.synchronize()
+    peak = torch.cuda.max_memory_allocated() - was
+    assert peak <= max(cuda_ops().SCORED_BYTES, rows * Hq * 4) + (64 << 20), peak
+    want, _, weights, mass, terms = attend(q, cache, md, 0.1)
+    eps, u = weight_error(terms, 128), unit(q.dtype)
+    assert ((out.double() - want).abs() <= u * want.abs() + (u * u + 2 * eps + 2.0 ** -13) * mass).all()
+    total = before.double()
+    total[:, :, :weights.shape[2]] += weights
+    bound = 2.0 ** -24 * total
+    bound[:, :, :weights.shape[2]] += (2 * eps + max(2.0 ** -20, Hq // Hkv * 2.0 ** -24)) * weights + 2.0 ** -126
+    assert ((scores[:, :, :n].double() - total).abs() <= bound).all() and not scores[:, :, n:].any()
+
+
+@pytest.mark.parametrize("vt", [True, False])
+def test_decode_in_groups(vt, monkeypatch):
+    """Requests of several launches, one workspace: as in one, to the bound of 64 bits; lengths of 0 among them."""
+    lens = [300, 0, 17, 1000, 64, 5, 0, 130, 700, 33, 1]
+    monkeypatch.setattr(cuda_ops(), "scored_parts", lambda *a: 0)
+    for most in (1, 3, 4, 8):
+        q, cache, md, scores = step(lens, [1] * len(lens), 8, 2, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=8)
+        monkeypatch.setattr(cuda_ops(), "SCORED_BYTES", most * 8 * 17 * 256)
+        _check_decode(q, cache, md, scores, sinks=torch.randn(8, device="cuda"))

@@ -642,16 +642,17 @@ static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
 }  // namespace sdec
 
 
-// `ws`: for rows = min(B, 512) Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + min(B, 512) Hq ceil(max_rows / 64) 64 + 2 rows floats.  extra: tiles
-// that a row counts for beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request that the block
-// table and the scores have room for.
+// `ws`: for rows = group Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + group Hq ceil(max_rows / 64) 64 + 2 rows floats.  group: requests of a launch, up to 512.
+// extra: tiles that a row counts for beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request
+// that the block table and the scores have room for.
 EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, void* out, float* scores,
                             const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int64_t q_stride, int64_t out_stride,
-                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int sms, int extra, int parts, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
+                            int64_t bt_stride, int64_t sc_req, int64_t sc_head, int ctas, int sms, int extra, int parts, int group, float scale, float soft_cap, int vt, int dtype, cudaStream_t st) {
   using namespace sdec;
   if (B <= 0) return 0;
+  if (group < 1 || group > MAX_REQUESTS) return -1;
   if (dtype == DT_F32 || D % 8 || D > 256 || BS % 16 || Hq % Hkv || ctas < 1 || max_rows < 1 || parts < 0 || parts > 8) return -1;
-  if (parts > 0 && (parts < 2 || D > 128 || Hq / Hkv > 16 || B > MAX_REQUESTS || (max_rows + TILE - 1) / TILE > FUSED_TILES * parts)) return -1;
+  if (parts > 0 && (parts < 2 || D > 128 || Hq / Hkv > 16 || B > group || (max_rows + TILE - 1) / TILE > FUSED_TILES * parts)) return -1;
   Params p;
   p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D; p.BS = BS; p.max_rows = max_rows; p.chunks = (p.G + 15) / 16; p.extra = extra; p.parts = parts;
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.sc_req = sc_req; p.sc_head = sc_head;
@@ -659,8 +660,8 @@ EXPORT int vb_scored_decode(const void* q, const void* cache, int64_t num_blocks
   p.raw_rows = (max_rows + TILE - 1) / TILE * TILE;
   p.scale_log2 = scale * LOG2E;
   p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E;
-  for (int b0 = 0; b0 < B; b0 += MAX_REQUESTS) {
-    p.B = B - b0 < MAX_REQUESTS ? B - b0 : MAX_REQUESTS;
+  for (int b0 = 0; b0 < B; b0 += group) {
+    p.B = B - b0 < group ? B - b0 : group;
     p.q = reinterpret_cast<const char*>(q) + b0 * q_stride * 2;
     p.out = reinterpret_cast<char*>(out) + b0 * out_stride * 2;
     p.block_table = block_table + b0 * bt_stride;

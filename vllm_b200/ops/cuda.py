@@ -551,7 +551,7 @@ def talking_attention(q, kv_cache, md, scale, sliding_window, soft_cap, talk, si
 
 
 _scored_decode = _sig("vb_scored_decode", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i,
-                      _i, _f, _f, _i, _i, _vp)
+                      _i, _i, _f, _f, _i, _i, _vp)
 
 
 _I32 = torch.int32
@@ -580,6 +580,17 @@ def _q_heads(q):
 # tiles that a row counts for beside its own, as its end costs about as much: us for 24 x 60 to 924 of 16 / 8 heads of 64, 0 to 4 and 6 of them,
 # 24.5, 18.4, 16.7, 16.0, 16.0, 16.2; 64 x 1000 of 32 / 8 heads of 128 65.0, 64.3, 64.0, 64.9, 65.3, 65.3
 SCORED_EXTRA = 3
+
+
+# of scores between the two kernels: 4 bytes for each query head and row that the table and the scores of a request have room for, however long it is.  Requests
+# that want more of it are taken in several launches, one after the other.
+SCORED_BYTES = 1 << 29
+
+
+def scored_group(B: int, Hq: int, tiles: int) -> int:
+    """Requests of a launch: up to 512 (their lengths lie in shared memory), in groups of about the same size."""
+    most = max(1, min(512, SCORED_BYTES // max(1, Hq * tiles * 256)))
+    return -(-B // max(1, -(-B // most)))
 
 
 def scored_parts(pairs: int, tiles: int, G: int, D: int, ctas: int) -> int:
@@ -611,14 +622,16 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     G, sms, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
     if G > 256:                              # (the second kernel has the factors of all of them in shared memory)
         raise ValueError(f"scored_attention: {G} query heads for a kv head; up to 256")
-    ctas, n, tiles = sms * (2 if D <= 128 else 1), min(B, 512) * Hkv, -(-rows // 64)
-    parts, ws = scored_parts(B * Hkv, tiles, G, D, ctas), None
+    ctas, tiles = sms * (2 if D <= 128 else 1), -(-rows // 64)
+    parts, ws, group = scored_parts(B * Hkv, tiles, G, D, ctas), None, B
     if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
+        group = scored_group(B, Hq, tiles)
+        n = group * Hkv
         heads = n * -(-G // 16)
         ws = scores.new_empty((heads + ctas) * 16 * (D + 2) + n * G * tiles * 64 + 2 * heads)
     _check(_scored_decode(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), sl.data_ptr(), out.data_ptr(), scores.data_ptr(), _p(sinks), _p(ws), B,
-                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, sms, SCORED_EXTRA, parts, scale, soft_cap, int(md.kv_vt),
-                          _DT[q.dtype], _st()), "scored_decode", 1 if parts else 2 * -(-B // 512))
+                          Hq, Hkv, D, BS, rows, q.stride(0), out_row, bt.stride(0), sc_req, sc_head, ctas, sms, SCORED_EXTRA, parts, group, scale, soft_cap,
+                          int(md.kv_vt), _DT[q.dtype], _st()), "scored_decode", 1 if parts else 2 * -(-B // group))
     return out
 
 
