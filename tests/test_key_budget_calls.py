@@ -115,3 +115,13 @@ def test_groups_of_a_decode_step():
         assert n == 1 or groups * n < B + groups
         assert groups == max(-(-B // 512), 1) or groups == 1 or (n + 1) * Hq * tiles * 256 > cu.SCORED_BYTES or -(-B // (groups - 1)) * Hq * tiles * 256 > cu.SCORED_BYTES
     assert cu.scored_group(64, 32, 21) == 64 and cu.scored_group(512, 32, 16) == 512
+
+
+def test_decode_without_rows(calls, monkeypatch):
+    """Tables or scores with room for no row: outputs of zeros, nothing is launched."""
+    q, cache, md, scores = step([0, 0], [1, 1], 4, 2, 24, 16, torch.bfloat16, "cpu")
+    for s, t in ((scores[..., :0], md.block_table), (scores, md.block_table[:, :0])):
+        out = torch.full_like(q, 7.0)
+        assert not ops.scored_attention(q, cache, dataclasses.replace(md, block_table=t), 0.1, s).any()
+        assert ops.scored_attention(q, cache, dataclasses.replace(md, block_table=t), 0.1, s, out=out) is out and not out.any()
+    assert not calls

@@ -622,6 +622,9 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     G, sms, (sc_req, sc_head, _) = Hq // Hkv, num_sms(), scores.stride()
     if G > 256:                              # (the second kernel has the factors of all of them in shared memory)
         raise ValueError(f"scored_attention: {G} query heads for a kv head; up to 256")
+    if not rows:
+        out[:B].zero_()
+        return out
     ctas, tiles = sms * (2 if D <= 128 else 1), -(-rows // 64)
     parts, ws, group = scored_parts(B * Hkv, tiles, G, D, ctas), None, B
     if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
