@@ -8,7 +8,6 @@ import torch
 from tests.key_budget_oracle import step
 from vllm_b200 import ops
 from vllm_b200.ops import cuda as cu
-from vllm_b200.ops import ref
 
 
 @pytest.fixture
@@ -18,11 +17,10 @@ def calls(monkeypatch):
 
     def attention(q, kv_cache, md, scale, window=None, cap=0.0, causal=True, out=None, return_lse=False, sinks=None, **_):
         seen.append(("attention", q, out))
-        qsl = torch.arange(md.num_reqs + 1) if md.decode_only else md.query_start_loc
-        o, lse = ref.paged_attention(q[:int(qsl[-1])], kv_cache, md.block_table, md.seq_lens, qsl, scale, logits_soft_cap=cap, sinks=sinks, return_lse=True)
+        used = md.num_reqs if md.decode_only else int(md.query_start_loc[-1])
         out = torch.full_like(q, float("nan"), memory_format=torch.contiguous_format) if out is None else out
-        out[:o.shape[0]] = o
-        return out, torch.cat([lse.float(), torch.full((q.shape[0] - o.shape[0], q.shape[1]), float("nan"))])
+        out[:used] = 2 * q[:used]                                               # (something that is exact)
+        return out, torch.zeros(q.shape[:2])
 
     def weights(*a):
         seen.append(("weights",))
@@ -84,7 +82,7 @@ def test_padded_and_unaligned(calls, monkeypatch, invariant, where):
     """Rows behind the last request are zeros, or as they were in an output that was given; kernels get rows at 16-byte addresses."""
     q, cache, md, scores = _steps(invariant, monkeypatch)
     used = q.shape[0]
-    want = ref.paged_attention(q, cache, md.block_table, md.seq_lens, md.query_start_loc, 0.1)
+    want = 2 * q
     q = torch.cat([q, torch.full_like(q[:1], float("nan")).expand(3, -1, -1)])
     T = q.shape[0]
     q = torch.cat([torch.zeros(T, 1, 24, dtype=q.dtype), q], 1).flatten(1)[:, 20:][:, 4:].unflatten(1, (8, 24))      # a slice of wider rows
