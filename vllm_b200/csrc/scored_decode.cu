@@ -13,7 +13,7 @@
 // S^T = K Q^T (m16n8k16: keys are rows, the at most 16 query heads columns), an own running maximum and O^T += V^T P^T; its strips
 // come by asynchronous copies of its own, STAGES of them on their way across the borders of rows, so warps meet only where a row
 // ends.  Weights enter the second product as two 16-bit parts, P = hi + lo: the output is then as exact as its own rounding.
-// Few short requests (ops/cuda.py: scored_parts) are one kernel's instead: a cluster has a row, its scores stay in shared memory, and the parts meet there.
+// Few short requests (scored_parts in ops/cuda.py) are one kernel's instead: a cluster has a row, its scores stay in shared memory, and the parts meet there.
 //
 // Decode is bound by the bytes of the cache; a tcgen05 product (128 keys x 16) would take the scores through tensor memory and
 // barriers between roles for products that are a few percent of the time.  us for 64 requests of 1000 with 32 / 8 heads of 128 (bytes 40.9):
@@ -600,8 +600,9 @@ __global__ void __launch_bounds__(JOIN, JOINERS) join_kernel(const Params p) {
 constexpr int FUSED_TILES = 4;                           // of a CTA, at most, where a cluster has a row
 template <typename F> constexpr int EXCH_BYTES = F::WARPS / 2 * F::REGS * 128;
 
+// `clusters`: nothing is launched, the clusters of a row that the device runs at a time are counted.
 template <typename T, int DP, int NT, bool VT, bool CAP>
-static int launch(const Params& p, cudaStream_t st) {
+static int launch(const Params& p, cudaStream_t st, int* clusters) {
   using F = Form<DP>;
   if constexpr (DP <= 128) if (p.parts > 0) {
     auto k = decode_kernel<T, DP, NT, VT, CAP, true>;
@@ -613,9 +614,18 @@ static int launch(const Params& p, cudaStream_t st) {
     }
     const int tiles = (p.max_rows + TILE - 1) / TILE, per = (tiles + p.parts - 1) / p.parts;
     const size_t smem = F::RING + EXCH_BYTES<F> + (size_t)(p.G * (p.D + 2 + 9) + 4 + per * TILE * p.G) * 4;
+    if (clusters) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr = {};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = p.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+      cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(F::THREADS); cfg.dynamicSmemBytes = smem; cfg.attrs = &attr; cfg.numAttrs = 1;
+      return (int)cudaOccupancyMaxActiveClusters(clusters, k, &cfg);
+    }
     vb_launch_parts(k, dim3(p.B * p.Hkv * p.parts), dim3(F::THREADS), smem, st, (unsigned)p.parts, p);
     return (int)cudaGetLastError();
   }
+  if (clusters) return -1;
   auto k = decode_kernel<T, DP, NT, VT, CAP, false>;
   static bool set = false;
   if (!set) {
@@ -627,20 +637,28 @@ static int launch(const Params& p, cudaStream_t st) {
   return (int)cudaGetLastError();
 }
 template <typename T, int DP, bool VT>
-static int pick(const Params& p, bool cap, cudaStream_t st) {
-  if (p.G > 8) return cap ? launch<T, DP, 2, VT, true>(p, st) : launch<T, DP, 2, VT, false>(p, st);
-  return cap ? launch<T, DP, 1, VT, true>(p, st) : launch<T, DP, 1, VT, false>(p, st);
+static int pick(const Params& p, bool cap, cudaStream_t st, int* clusters) {
+  if (p.G > 8) return cap ? launch<T, DP, 2, VT, true>(p, st, clusters) : launch<T, DP, 2, VT, false>(p, st, clusters);
+  return cap ? launch<T, DP, 1, VT, true>(p, st, clusters) : launch<T, DP, 1, VT, false>(p, st, clusters);
 }
 template <typename T>
-static int go(const Params& p, bool vt, bool cap, cudaStream_t st) {
-  if (vt) return p.D == 128 ? pick<T, 128, true>(p, cap, st) : -2;
-  if (p.D <= 64) return pick<T, 64, false>(p, cap, st);
-  if (p.D <= 128) return pick<T, 128, false>(p, cap, st);
-  return pick<T, 256, false>(p, cap, st);
+static int go(const Params& p, bool vt, bool cap, cudaStream_t st, int* clusters = nullptr) {
+  if (vt) return p.D == 128 ? pick<T, 128, true>(p, cap, st, clusters) : -2;
+  if (p.D <= 64) return pick<T, 64, false>(p, cap, st, clusters);
+  if (p.D <= 128) return pick<T, 128, false>(p, cap, st, clusters);
+  return pick<T, 256, false>(p, cap, st, clusters);
 }
 
 }  // namespace sdec
 
+// Into `clusters`: how many clusters of `parts` CTAs, each with a row of up to `tiles` tiles of a kv head with G query heads, the device runs at a time.
+EXPORT int vb_scored_clusters(int G, int D, int tiles, int parts, int vt, int cap, int dtype, int* clusters) {
+  using namespace sdec;
+  if (dtype == DT_F32 || D % 8 || D > 128 || G < 1 || G > 16 || parts < 2 || parts > 8 || tiles < 1 || tiles > FUSED_TILES * parts) return -1;
+  Params p{};
+  p.G = G; p.D = D; p.max_rows = tiles * TILE; p.parts = parts;
+  return dtype == DT_BF16 ? go<__nv_bfloat16>(p, vt != 0, cap != 0, nullptr, clusters) : go<__half>(p, vt != 0, cap != 0, nullptr, clusters);
+}
 
 // `ws`: for rows = group Hkv ceil(G / 16), (rows + ctas) 16 (D + 2) + group Hq ceil(max_rows / 64) 64 + 2 rows floats.  group: requests of a launch, up to 512.
 // extra: tiles that a row counts for beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request
