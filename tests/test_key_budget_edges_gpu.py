@@ -241,3 +241,15 @@ def test_decode_in_groups(vt, monkeypatch):
         q, cache, md, scores = step(lens, [1] * len(lens), 8, 2, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=8)
         monkeypatch.setattr(cuda_ops(), "SCORED_BYTES", most * 8 * 17 * 256)
         _check_decode(q, cache, md, scores, sinks=torch.randn(8, device="cuda"))
+
+
+def test_weights_between_products():
+    """Products on either side in the stream, whose tensor memory and that of the weights take turns: the same bits as by itself."""
+    q, cache, md, scores = step([300, 64], [1, 1], 8, 2, 128, 64, torch.bfloat16, "cuda", vt=True)
+    lse = torch.full((2, 8), 5.0, device="cuda")
+    x, w = torch.randn(64, 1024, device="cuda").bfloat16(), torch.randn(1024, 1024, device="cuda").bfloat16()
+    want = ops.key_weights(q, cache, md, 0.09, lse, scores.clone()), ops.linear(x, w), ops.paged_attention(q, cache, md, 0.09)
+    for _ in range(200):
+        got = [ops.linear(x, w), ops.key_weights(q, cache, md, 0.09, lse, scores.clone())]
+        got += [ops.linear(x, w), ops.paged_attention(q, cache, md, 0.09), ops.key_weights(q, cache, md, 0.09, lse, scores.clone())]
+        assert all(torch.equal(x, want[i]) for x, i in zip(got, (1, 0, 1, 2, 0)))

@@ -220,7 +220,6 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int budget = MBAR_BUDGET;
-  pdl_trigger();
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_q); tma_prefetch_desc(&tmap_k);
     for (int s = 0; s < QS; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
@@ -231,7 +230,6 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
     }
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
   const int used = p.TQ * p.G, pieces = (used + 31) / 32;        // columns, and groups of 32 of them
   if (used < pieces * 32)                                        // columns that no head has: zeros
     for (int i = threadIdx.x; i < QS * F::Q_BYTES / 16; i += NUM_THREADS) reinterpret_cast<uint4*>(q_smem)[i] = make_uint4(0, 0, 0, 0);
@@ -245,6 +243,11 @@ weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   }
   fence_proxy_async();
   pdl_wait();
+  // All of tensor memory: behind the kernel in front, which may allocate its own only after a wait of its own on the same SM, and before the next may begin.
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    pdl_trigger();
+  }
   scan_requests(p, first, warp_sums);
   tc_fence_before();
   __syncthreads();
