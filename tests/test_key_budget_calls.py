@@ -138,3 +138,19 @@ def test_clusters_of_a_decode_step(monkeypatch):
         assert cu.scored_parts(pairs, 20, 4, 128, 1, False, 0) == want
     for G, D in ((17, 128), (4, 256)):
         assert cu.scored_parts(1, 4, G, D, 0, False, 0) == 0
+
+
+@pytest.mark.parametrize("invariant", [False, True])
+def test_one_row_of_a_wider_one(calls, monkeypatch, invariant):
+    """A single row's distance to the next means nothing, but kernels are told one that is a multiple of 16 bytes."""
+    monkeypatch.setattr(cu, "_key_weights", lambda *a: calls.append(("weights", a[20])) or 0)
+    if invariant:
+        monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
+    q, cache, md, scores = step([33], [1], 8, 2, 24, 16, torch.bfloat16, "cpu")
+    md.decode_only = invariant
+    q = torch.cat([q.flatten(1), torch.zeros(1, 5, dtype=q.dtype)], 1).expand(3, -1).contiguous()[:, :192].unflatten(1, (8, 24))[:1]
+    assert q.is_contiguous() and q.stride(0) == 197
+    ops.scored_attention(q, cache, md, 0.1, scores)
+    ops.key_weights(q, cache, md, 0.1, torch.zeros(1, 8), scores)
+    assert [c[0] for c in calls] == ["attention", "weights", "weights"]
+    assert calls[0][1].stride(0) % 8 == 0 and calls[0][2].stride(0) % 8 == 0 and calls[1][1] % 8 == 0 and calls[2][1] % 8 == 0, calls

@@ -253,3 +253,17 @@ def test_weights_between_products():
         got = [ops.linear(x, w), ops.key_weights(q, cache, md, 0.09, lse, scores.clone())]
         got += [ops.linear(x, w), ops.paged_attention(q, cache, md, 0.09), ops.key_weights(q, cache, md, 0.09, lse, scores.clone())]
         assert all(torch.equal(x, want[i]) for x, i in zip(got, (1, 0, 1, 2, 0)))
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("D,BS,vt", [(128, 64, True), (64, 16, False)])
+def test_one_row_of_a_wider_one(prompt, D, BS, vt):
+    """A single query row out of rows of an odd width."""
+    q, cache, md, scores = step([300], [1], 8, 2, D, BS, torch.bfloat16, "cuda", vt=vt)
+    md.decode_only = not prompt
+    lse, other = torch.full((1, 8), 5.0, device="cuda"), scores.clone()
+    want = ops.scored_attention(q, cache, md, 0.1, other), ops.key_weights(q, cache, md, 0.1, lse, scores.clone())
+    q = torch.nn.functional.pad(q.flatten(1), (0, 5)).expand(3, -1).contiguous()[:, :8 * D].unflatten(1, (8, D))[:1]
+    assert q.is_contiguous() and q.stride(0) % 8
+    assert torch.equal(ops.key_weights(q, cache, md, 0.1, lse, scores.clone()), want[1])
+    assert torch.equal(ops.scored_attention(q, cache, md, 0.1, scores), want[0]) and torch.equal(scores, other)

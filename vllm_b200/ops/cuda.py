@@ -574,7 +574,7 @@ def _q_heads(q):
     """Queries with the heads of a token next to each other and rows at 16-byte addresses."""
     if q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         return q.clone(memory_format=torch.contiguous_format)
-    return _heads(q)
+    return _heads(q)                         # (a single row's distance to the next counts, too)
 
 
 # tiles that a row counts for beside its own, as its end costs about as much: us for 24 x 60 to 924 of 16 / 8 heads of 64, 0 to 4 and 6 of them,
@@ -622,7 +622,7 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
     if batch_invariant():                    # that kernel deals the keys of all requests to the SMs
         return scored_rows(q, kv_cache, md, scale, scores, soft_cap, sinks, 0, out)
     B, (_, Hq, D), (blocks, _, Hkv, BS, _) = md.num_reqs, q.shape, kv_cache.shape
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
         q = _q_heads(q)
     if out is None:
         out, out_row = torch.empty_like(q, memory_format=torch.contiguous_format), Hq * D
@@ -661,7 +661,7 @@ _key_weights = _sig("vb_key_weights", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _
 def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last: int = 0):
     """Adds the weights that query rows give to the cached keys to ``scores`` (csrc/key_weights.cu)."""
     pages = _weights_step(q, kv_cache, md, scale, scores)
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
         q = _q_heads(q)
     return _add_weights(q, kv_cache, md, scale, lse.contiguous(), scores, soft_cap, last, pages)
 
@@ -694,7 +694,7 @@ def scored_rows(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, last=0
         raise ValueError(f"scored_attention: {pages[0].shape[1]} pages of {BS} for requests of up to {md.max_seq_len} rows")
     if md.kv_vt and not tc_attention_ok(D, D, Hq // Hkv):
         raise ValueError(f"scored_attention: {Hq // Hkv} query heads for a kv head over transposed values; a power of two up to 128 in prompts and batch-invariant mode")
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
         q = _q_heads(q)
     used, to = md.num_reqs if md.decode_only else md.num_actual_tokens, out
     if out is not None and (out.stride(2) != 1 or out.stride(1) != D):
