@@ -191,3 +191,35 @@ if which in ("prompts", "all"):
     pool, A, b = torch.zeros(n + 1, nh * dk * dv, device="cuda"), torch.zeros(nh, device="cuda"), torch.zeros(nh, device="cuda")
     rep(lambda: cu.gated_delta(qkv, ba, A, b, pool, 0, prompts(n, q, (torch.arange(n, **i32) + 1).view(-1, 1)), nh, nh, dk, dv, 1.0, 1e-6))
     cu.check_kernel_error(torch.device("cuda", 0))
+if which in ("budget", "all"):
+    # a cache with a budget: key weights of a prompt, of its last rows and of a capped prompt; decode steps; a cut of long requests.  Three times each
+    from vllm_b200 import ops
+    from vllm_b200.forward_context import AttentionMetadata
+    H, D, BS = 8, 128, 64
+
+    def budget(lens, queries, room=0):
+        B, pages = len(lens), [-(-n // BS) for n in lens]
+        table = torch.zeros(B, max(pages), dtype=torch.int32)
+        order, at = torch.randperm(sum(pages)).int(), 0
+        for b, n in enumerate(pages):
+            table[b, :n], at = order[at:at + n], at + n
+        start = [0]
+        for n in queries:
+            start.append(start[-1] + n)
+        md = AttentionMetadata(num_reqs=B, num_actual_tokens=start[-1], max_query_len=max(queries), max_seq_len=max(lens),
+                               query_start_loc=torch.tensor(start, dtype=torch.int32, device="cuda"), seq_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                               block_table=table.cuda(), slot_mapping=torch.empty(0), decode_only=max(queries) == 1, kv_vt=True)
+        cache = torch.randn(sum(pages), 2, H, BS, D, device="cuda", dtype=dt)
+        q = torch.randn(start[-1], 4 * H, D, device="cuda", dtype=dt)
+        return q, cache, md, torch.rand(B, H, max(lens) + 64, device="cuda")
+    q, cache, md, scores = budget([8000], [8000])
+    lse = torch.full(q.shape[:2], 9.0, device="cuda")
+    for cap in (0.0, 50.0):
+        rep(lambda: ops.key_weights(q, cache, md, D ** -0.5, lse, scores, cap), 3)
+    q, cache, md, scores = budget([1500 + 86 * i for i in range(8)], [64] * 8)
+    lse = torch.full(q.shape[:2], 9.0, device="cuda")
+    rep(lambda: ops.key_weights(q, cache, md, D ** -0.5, lse, scores), 3)
+    q, cache, md, scores = budget([700 + 601 * i // 63 for i in range(64)], [1] * 64)
+    rep(lambda: ops.scored_attention(q, cache, md, D ** -0.5, scores), 3)
+    q, cache, md, scores = budget([28001, 29334, 30667, 32000], [1] * 4)
+    rep(lambda: ops.evict_keys(cache, md, scores, 4096, 4, 64), 3)

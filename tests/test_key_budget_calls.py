@@ -128,16 +128,15 @@ def test_decode_without_rows(calls, monkeypatch):
 def test_clusters_of_a_decode_step(monkeypatch):
     """A cluster per row where the device runs all of them at a time; of four or two CTAs also in two turns."""
     at_a_time = {8: 15, 4: 36, 2: 74}
-    monkeypatch.setattr(cu, "num_sms", lambda: 148)
     monkeypatch.setattr(cu, "_device", lambda: 0)
     monkeypatch.setattr(cu, "scored_clusters", lambda device, G, D, tiles, parts, *a: at_a_time[parts])
     for pairs, tiles, want in ((1, 11, 8), (15, 11, 8), (16, 11, 0), (32, 11, 0), (15, 32, 8), (15, 33, 0), (36, 4, 4), (72, 4, 4), (73, 4, 0), (74, 2, 2), (148, 1, 2), (149, 1, 0)):
-        assert cu.scored_parts(pairs, tiles, 8, 128, 1, False, 0) == want, (pairs, tiles)
+        assert cu.scored_parts(pairs, tiles, 8, 128, 148, 1, False, 0) == want, (pairs, tiles)
     at_a_time[8] = 33
     for pairs, want in ((33, 8), (34, 0)):
-        assert cu.scored_parts(pairs, 20, 4, 128, 1, False, 0) == want
+        assert cu.scored_parts(pairs, 20, 4, 128, 148, 1, False, 0) == want
     for G, D in ((17, 128), (4, 256)):
-        assert cu.scored_parts(1, 4, G, D, 0, False, 0) == 0
+        assert cu.scored_parts(1, 4, G, D, 148, 0, False, 0) == 0
 
 
 @pytest.mark.parametrize("invariant", [False, True])

@@ -604,7 +604,7 @@ def scored_clusters(device: int, G: int, D: int, tiles: int, parts: int, vt: int
     return n.value
 
 
-def scored_parts(pairs: int, tiles: int, G: int, D: int, vt: int, cap: bool, dtype: int) -> int:
+def scored_parts(pairs: int, tiles: int, G: int, D: int, sms: int, vt: int, cap: bool, dtype: int) -> int:
     """CTAs of a cluster that has a request's kv head, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel.  Clusters of four
     or two CTAs may take two turns.  us in clusters and in runs, heads of 128, 8 of a kv head: 15 rows of 700 (of the 15 clusters of eight that have one CTA on an
     SM) 7.2 and 11.9, 16 rows 12.9 and 12.5, 32 19.5 and 12.6; 4 of a kv head (two CTAs on an SM: 33 clusters) 33 rows of 2000 10.0 and 13.1, 34 15.8 and 13.3;
@@ -612,7 +612,7 @@ def scored_parts(pairs: int, tiles: int, G: int, D: int, vt: int, cap: bool, dty
     if tiles > 32 or G > 16 or D > 128 or pairs > 512:
         return 0
     parts = 8 if tiles > 4 else 4 if tiles > 2 else 2
-    if pairs > 2 * num_sms() // parts:       # (two CTAs of an SM at most)
+    if pairs > 2 * sms // parts:             # (two CTAs of an SM at most)
         return 0
     return parts if pairs <= scored_clusters(_device(), G, D, tiles, parts, vt, cap, dtype) * (1 if parts == 8 else 2) else 0
 
@@ -642,7 +642,7 @@ def scored_decode(q, kv_cache, md, scale, scores, soft_cap=0.0, sinks=None, out=
         out[:B].zero_()
         return out
     ctas, tiles = sms * (2 if D <= 128 else 1), -(-rows // 64)
-    parts, ws, group = scored_parts(B * Hkv, tiles, G, D, int(md.kv_vt), soft_cap > 0, _DT[q.dtype]), None, B
+    parts, ws, group = scored_parts(B * Hkv, tiles, G, D, sms, int(md.kv_vt), soft_cap > 0, _DT[q.dtype]), None, B
     if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
         group = scored_group(B, Hq, tiles)
         n = group * Hkv
