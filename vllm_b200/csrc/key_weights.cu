@@ -13,7 +13,7 @@
 // twice of 16 / 4 (of 64): a CTA per block with 8 warps for both key tiles 410 and 196; runs of equal length and 16 warps 442 and 170, where
 // packed polynomials cost more instructions than exponentials time; tiles of 256 columns, each key tile with its own warps 354 and 144; the
 // log-sum-exps in the products 341 and 138; one in eight exponentials a polynomial 328 and 132 (one in four 337 and 138);
-// half of a piece summed while the other half comes out of tensor memory 312 and 127.
+// half of a piece summed while the other half comes out of tensor memory 312 and 127 (at 1965 MHz; under the power cap, after some tenths of a second, 345).
 #include "attention_prompt.cuh"
 
 namespace kweights {
