@@ -15,6 +15,7 @@
 // log-sum-exps in the products 341 and 138; one in eight exponentials a polynomial 328 and 132 (one in four 337 and 138);
 // half of a piece summed while the other half comes out of tensor memory 312 and 127 (at 1965 MHz; under the power cap, after some tenths of a second, 345).
 #include "attention_prompt.cuh"
+#include "device_once.h"
 
 namespace kweights {
 
@@ -530,11 +531,8 @@ __global__ void __launch_bounds__(KEYS) join_kernel(const Params p) {
 template <typename T, int KB, bool CAP>
 static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const Params& p, int ctas, cudaStream_t st) {
   auto k = weights_kernel<T, KB, CAP>;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<KB>::SMEM) != cudaSuccess) return (int)cudaGetLastError();
-    set = true;
-  }
+  static std::atomic<uint64_t> devices{0};
+  if (vb_allow_smem(reinterpret_cast<const void*>(k), Form<KB>::SMEM, devices) != cudaSuccess) return (int)cudaGetLastError();
   vb_launch(k, dim3(ctas), dim3(NUM_THREADS), (size_t)Form<KB>::SMEM, st, tq, tk, p);
   if (p.part && ctas > 1) vb_launch(join_kernel, dim3(ctas - 1), dim3(KEYS), 0, st, p);
   return (int)cudaGetLastError();

@@ -22,6 +22,7 @@
 // The other way to the weights, a second pass over the keys, would read half the cache again.
 #include "attention_prompt.cuh"
 #include "cluster.cuh"
+#include "device_once.h"
 
 namespace sdec {
 
@@ -607,11 +608,8 @@ static int launch(const Params& p, cudaStream_t st, int* clusters) {
   if constexpr (DP <= 128) if (p.parts > 0) {
     auto k = decode_kernel<T, DP, NT, VT, CAP, true>;
     constexpr int MOST = F::RING + EXCH_BYTES<F> + (16 * (DP + 2 + 9) + 4 + FUSED_TILES * TILE * 16) * 4;
-    static bool set = false;
-    if (!set) {
-      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess) return (int)cudaGetLastError();
-      set = true;
-    }
+    static std::atomic<uint64_t> devices{0};
+    if (vb_allow_smem(reinterpret_cast<const void*>(k), MOST, devices) != cudaSuccess) return (int)cudaGetLastError();
     const int tiles = (p.max_rows + TILE - 1) / TILE, per = (tiles + p.parts - 1) / p.parts;
     const size_t smem = F::RING + EXCH_BYTES<F> + (size_t)(p.G * (p.D + 2 + 9) + 4 + per * TILE * p.G) * 4;
     if (clusters) {
@@ -627,11 +625,8 @@ static int launch(const Params& p, cudaStream_t st, int* clusters) {
   }
   if (clusters) return -1;
   auto k = decode_kernel<T, DP, NT, VT, CAP, false>;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM) != cudaSuccess) return (int)cudaGetLastError();
-    set = true;
-  }
+  static std::atomic<uint64_t> devices{0};
+  if (vb_allow_smem(reinterpret_cast<const void*>(k), F::SMEM, devices) != cudaSuccess) return (int)cudaGetLastError();
   vb_launch(k, dim3(p.ctas), dim3(F::THREADS), (size_t)F::SMEM, st, p);
   vb_launch(join_kernel<T>, dim3((p.max_rows + p.block - 1) / p.block, p.Hkv, p.B), dim3(JOIN), (size_t)(((p.G + 3) & ~3) + p.G * FACTORS) * 4, st, p);
   return (int)cudaGetLastError();
