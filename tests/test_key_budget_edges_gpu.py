@@ -1,5 +1,8 @@
 """A key-value cache with a budget on the device: values, shapes and calls at the edge of what the operators take."""
 import dataclasses
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -267,3 +270,54 @@ def test_one_row_of_a_wider_one(prompt, D, BS, vt):
     assert q.is_contiguous() and q.stride(0) % 8
     assert torch.equal(ops.key_weights(q, cache, md, 0.1, lse, scores.clone()), want[1])
     assert torch.equal(ops.scored_attention(q, cache, md, 0.1, scores), want[0]) and torch.equal(scores, other)
+
+
+FIRST = """
+import torch
+from tests.key_budget_oracle import step
+from vllm_b200 import ops
+lens = [300, 20, 1000]
+q, cache, md, scores = step(lens, [1, 1, 1], 8, 2, 128, 64, torch.bfloat16, "cuda", vt=True, room=1030)
+pq, _, pmd, _ = step([300], [40], 8, 2, 128, 64, torch.bfloat16, "cuda", room=1030)
+pmd.block_table, pmd.seq_lens, pmd.kv_vt = md.block_table[:1], md.seq_lens[:1], True
+lse, before, was = torch.full((40, 8), 6.0, device="cuda"), scores.clone(), cache.clone()
+def call():
+    out = ops.scored_attention(q, cache, md, 0.09, scores)
+    ops.key_weights(pq, cache, pmd, 0.09, lse, scores, 30.0)
+    return out, scores, cache, *ops.evict_keys(cache, md, scores, 200, 1, 9)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = call()
+graph.replay()
+got = [x.clone() for x in got]
+scores.copy_(before), cache.copy_(was)
+for x, y in zip(got, call()):
+    assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+torch.cuda.synchronize()
+print("same")
+"""
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first calls are captured: what is asked of the device once may be asked then."""
+    got = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=600, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert got.returncode == 0 and got.stdout.strip().endswith("same"), got.stderr[-2000:]
+
+
+@pytest.mark.parametrize("vt", [True, False])
+def test_pages_far_behind(vt):
+    """Pages whose values lie more than 2^32 values into the cache."""
+    q, cache, md, scores = step([300, 70, 700], [1, 1, 1], 8, 8, 128, 64, torch.bfloat16, "cuda", vt=vt, seed=9)
+    far = 34000
+    big = torch.empty(far + cache.shape[0], *cache.shape[1:], dtype=cache.dtype, device="cuda")
+    big[far:] = cache
+    shifted = dataclasses.replace(md, block_table=md.block_table + far)
+    lse, keep = torch.full((3, 8), 5.0, device="cuda"), scores.clone()
+    for call in (lambda c, m, s: ops.scored_attention(q, c, m, 0.1, s), lambda c, m, s: ops.key_weights(q, c, m, 0.1, lse, s),
+                 lambda c, m, s: ops.scored_attention(q, c, dataclasses.replace(m, decode_only=False), 0.1, s), lambda c, m, s: ops.evict_keys(c, m, s, 100, 2, 9)):
+        a, b = keep.clone(), keep.clone()
+        want, got = call(cache, md, a), call(big, shifted, b)
+        assert torch.equal(a, b)
+        for x, y in zip(want if isinstance(want, tuple) else (want,), got if isinstance(got, tuple) else (got,)):
+            assert torch.equal(x, y)
+        assert torch.equal(cache.view(torch.int16), big[far:].view(torch.int16))

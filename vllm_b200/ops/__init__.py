@@ -256,7 +256,8 @@ def scored_attention(q, kv_cache, md, scale, scores, logits_soft_cap: float = 0.
     No two requests may share a row of ``scores``.
 
     On the device a kv head has up to 256 query heads in decode steps; up to 128, a power of two of them over transposed values, in prompts and in
-    batch-invariant mode, where ``scale`` is not 0.  As in ``paged_attention``, numbers of pages and lengths of prompts are taken as they are."""
+    batch-invariant mode, where ``scale`` is not 0 and block tables have room for ``md.max_seq_len`` rows.  As in ``paged_attention``, numbers of pages and lengths
+    are taken as they are there."""
     cuda = _use_cuda(q)
     H, D = _check_scores(scores, kv_cache, md, "scored_attention", cuda)
     _check_queries(q, kv_cache, md, H, D, "scored_attention")
