@@ -322,6 +322,134 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int = 0, recent: int = 0,
     return ref.evict_keys(kv_cache, md.block_table, md.seq_lens[:md.num_reqs], scores, keep, first, recent, positions, md.kv_vt)
 
 
+# -- a key-value cache in 4 bits: csrc/cache_fp4.cu, csrc/attention_fp4.cu
+def fp4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int, head_size: int) -> tuple[int, ...]:
+    """Shape of a uint8 tensor that is a cache in 4 bits: [blocks, 2, kv heads, page, bytes of a row].
+
+    A row (a token's keys or values of one head) is its values y = x / factor in groups of 16: a scale e = e4m3(max |y| / 6) and codes e2m1(y / e), rounded
+    to nearest, ties to even; it stands for code * e * factor, 9 / 16 of a byte a value.  ``factor`` is the call's ``k_scale`` or ``v_scale``.  The bytes of a page
+    of one head are the codes of its rows (the even value in the low half of a byte), then their scales.  A group whose largest value is below
+    6 * 2^-10 of the factor is zeros, values above 2688 of it are cut off, a group with a NaN is NaNs."""
+    if head_size < 16 or head_size % 16 or block_size < 16 or block_size % 16:
+        raise ValueError(f"a cache in 4 bits has heads and pages in steps of 16; got {head_size} and {block_size}")
+    return num_blocks, 2, num_kv_heads, block_size, ref.fp4_row_bytes(head_size)
+
+
+def _check_fp4(kv_cache, op: str, k_scale: float = 1.0, v_scale: float = 1.0) -> tuple[int, int]:
+    """(kv heads, head size) of a cache in 4 bits."""
+    shape = kv_cache.shape
+    if kv_cache.dtype is not torch.uint8 or len(shape) != 5 or shape[1] != 2 or shape[3] < 16 or shape[3] % 16 or shape[4] < 9 or shape[4] % 9 \
+            or not kv_cache.is_contiguous():
+        raise ValueError(f"{op}: a contiguous uint8 cache of fp4_cache_shape; got {tuple(shape)} of {kv_cache.dtype}")
+    if not (0.0 < k_scale < float("inf") and 0.0 < v_scale < float("inf")):
+        raise ValueError(f"{op}: factors of keys and values above 0; got {k_scale} and {v_scale}")
+    return shape[2], shape[4] * 16 // 9
+
+
+def _check_slots(slot_mapping, T: int, kv_cache, op: str) -> None:
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] < T or not slot_mapping.is_contiguous() \
+            or slot_mapping.device != kv_cache.device:
+        raise ValueError(f"{op}: int64 slots of {T} tokens on the cache's device; got {tuple(slot_mapping.shape)} of {slot_mapping.dtype} on {slot_mapping.device}")
+
+
+def reshape_and_cache_fp4(key, value, kv_cache, slot_mapping, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    """``reshape_and_cache`` into a cache in 4 bits (``fp4_cache_shape``): key, value [T, kv heads, head size] to slots [T] (page * rows of a page + row; below 0 or
+    behind the cache: nowhere).  No two tokens of a call may have the same slot."""
+    op = "reshape_and_cache_fp4"
+    H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
+    if key.dim() != 3 or key.shape[1:] != (H, D) or value.shape != key.shape or value.dtype is not key.dtype or key.device != kv_cache.device \
+            or value.device != kv_cache.device:
+        raise ValueError(f"{op}: keys {tuple(key.shape)} and values {tuple(value.shape)} for {H} heads of {D}")
+    _check_slots(slot_mapping, key.shape[0], kv_cache, op)
+    if _use_cuda(key):
+        return cuda_ops().write_fp4(None, None, None, key, value, None, D, True, kv_cache, slot_mapping, k_scale, v_scale)
+    return ref.reshape_and_cache_fp4(key, value, kv_cache, slot_mapping[:key.shape[0]], k_scale, v_scale)
+
+
+def rope_and_cache_fp4(positions, q, k, v, cos_sin_cache, head_dim: int, is_neox: bool, kv_cache, slot_mapping, k_scale: float = 1.0, v_scale: float = 1.0,
+                       axes: Optional[torch.Tensor] = None):
+    """``rope_and_cache`` into a cache in 4 bits: q [T, heads * head_dim] is rotated in place (and returned), k rotated on its way into the cache and left as it is.
+
+    ``positions`` [T], or [n, T] with ``axes`` [rot / 2] int32: a token has a position on each of n axes (time, height, width), and pair j of a head turns by that on
+    axis axes[j].  Rotated values are rounded to the type of q before they are quantised, as a cache of that type would hold them."""
+    op = "rope_and_cache_fp4"
+    H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
+    T, rot = q.shape[0], cos_sin_cache.shape[-1]
+    if D != head_dim or q.dim() != 2 or q.shape[1] % D or k.shape != (T, H * D) or v.shape != k.shape or not q.dtype is k.dtype is v.dtype \
+            or not q.device == k.device == v.device == kv_cache.device:
+        raise ValueError(f"{op}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} for {H} kv heads of {D} and a rotation of heads of {head_dim}")
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype is not _F32 or not cos_sin_cache.is_contiguous() or not 0 < rot <= D or rot % 2 or cos_sin_cache.device != q.device:
+        raise ValueError(f"{op}: a contiguous fp32 table [positions, rot], rot up to {D}; got {tuple(cos_sin_cache.shape)} of {cos_sin_cache.dtype}")
+    if positions.dtype is not torch.int64 or positions.device != q.device or positions.shape[-1] < T or positions.dim() != (1 if axes is None else 2):
+        raise ValueError(f"{op}: int64 positions [T], or [axes, T] with axes; got {tuple(positions.shape)} of {positions.dtype}")
+    if axes is not None and (axes.dtype is not torch.int32 or axes.shape != (rot // 2,) or not axes.is_contiguous() or axes.device != q.device or not positions.shape[0]):
+        raise ValueError(f"{op}: axes int32 [{rot // 2}]; got {tuple(axes.shape)} of {axes.dtype}")
+    _check_slots(slot_mapping, T, kv_cache, op)
+    if _use_cuda(q) and rot % 16 == 0 and q.dtype in _HALF:
+        return cuda_ops().write_fp4(positions, axes, q, k, v, cos_sin_cache, D, is_neox, kv_cache, slot_mapping, k_scale, v_scale)
+    at, table = (positions[:T], cos_sin_cache) if axes is None else (torch.arange(T, device=q.device), ref.axes_table(positions[:, :T], cos_sin_cache, axes))
+    q2, k2 = ref.rotary_embedding(at, q, k, table, D, is_neox)
+    q.copy_(q2)
+    reshape_and_cache_fp4(k2.reshape(T, H, D), v.unflatten(1, (H, D)), kv_cache, slot_mapping, k_scale, v_scale)
+    return q
+
+
+def gather_cache_fp4(kv_cache, block_table, cu_seq_lens, k, v, max_tokens: int, seq_starts: Optional[torch.Tensor] = None, k_scale: float = 1.0,
+                     v_scale: float = 1.0) -> None:
+    """Reads a cache in 4 bits back: rows seq_starts[b] (None: 0) on of request b, cu_seq_lens[b + 1] - cu_seq_lens[b] of them (at most ``max_tokens``), to rows
+    cu_seq_lens[b] on of k and v [rows, kv heads, head size], in their type.  Rows that the block table [B, pages] has no page for are zeros."""
+    op = "gather_cache_fp4"
+    H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
+    B, dev = cu_seq_lens.numel() - 1, kv_cache.device
+    for t in (k, v):
+        if t.dim() != 3 or t.shape != (k.shape[0], H, D) or t.dtype is not k.dtype or t.device != dev:
+            raise ValueError(f"{op}: k {tuple(k.shape)} of {k.dtype} and v {tuple(v.shape)} of {v.dtype} for {H} heads of {D}")
+    if cu_seq_lens.dtype is not torch.int32 or cu_seq_lens.dim() != 1 or B < 0 or not cu_seq_lens.is_contiguous() or cu_seq_lens.device != dev:
+        raise ValueError(f"{op}: int32 offsets [requests + 1] on the cache's device; got {tuple(cu_seq_lens.shape)} of {cu_seq_lens.dtype}")
+    if seq_starts is not None and (seq_starts.dtype is not torch.int32 or seq_starts.shape[0] < B or not seq_starts.is_contiguous() or seq_starts.device != dev):
+        raise ValueError(f"{op}: int32 first rows of {B} requests; got {tuple(seq_starts.shape)} of {seq_starts.dtype}")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < B or block_table.device != dev:
+        raise ValueError(f"{op}: an int32 block table of {B} requests; got {tuple(block_table.shape)} of {block_table.dtype}")
+    if _use_cuda(kv_cache):
+        return cuda_ops().gather_fp4(kv_cache, block_table, cu_seq_lens, k, v, max_tokens, seq_starts, k_scale, v_scale)
+    return ref.gather_cache_fp4(kv_cache, block_table, cu_seq_lens, k, v, seq_starts, k_scale, v_scale)
+
+
+def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft_cap=0.0, causal=True, out: Optional[torch.Tensor] = None,
+                        alibi_slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, chunk_size: int = 0, return_lse: bool = False,
+                        out_scale: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0):
+    """``paged_attention`` over a cache in 4 bits; q [T, heads, head size] in 16 bits on the device, ``md.kv_vt`` False.  The output is that of the values
+    which the cache stands for."""
+    op = "paged_attention_fp4"
+    H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H or q.device != kv_cache.device:
+        raise ValueError(f"{op}: queries {tuple(q.shape)} of {q.dtype} for a cache of {H} heads of {D}")
+    if md.kv_vt:
+        raise ValueError(f"{op}: a cache in 4 bits has no transposed values")
+    if q.shape[0] < (md.num_reqs if md.decode_only else md.num_actual_tokens):
+        raise ValueError(f"{op}: {q.shape[0]} queries for a step of {md.num_reqs if md.decode_only else md.num_actual_tokens}")
+    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != D):
+        raise ValueError(f"{op}: out {tuple(out.shape)} of {out.dtype}, the heads of a row next to each other")
+    for name, t in (("sinks", sinks), ("alibi_slopes", alibi_slopes)):
+        if t is not None and t.numel() != q.shape[1]:
+            raise ValueError(f"{op}: {t.numel()} {name} for {q.shape[1]} heads")
+    if _use_cuda(q):
+        return cuda_ops().paged_attention_fp4(q, kv_cache, md, scale, sliding_window, logits_soft_cap, causal, out, alibi_slopes, sinks, chunk_size, return_lse,
+                                              out_scale, k_scale, v_scale)
+    sl = md.seq_lens_cpu if md.seq_lens_cpu is not None else md.seq_lens.cpu()
+    if md.decode_only and md.query_start_loc is None:
+        qsl = torch.arange(md.num_reqs + 1)
+    else:
+        qsl = md.query_start_loc_cpu if md.query_start_loc_cpu is not None else md.query_start_loc.cpu()
+    o, lse = ref.paged_attention(q, ref.fp4_cache_values(kv_cache, k_scale, v_scale), md.block_table, sl, qsl, scale, causal=causal, sliding_window=sliding_window,
+                                 logits_soft_cap=logits_soft_cap, alibi_slopes=alibi_slopes, sinks=sinks, chunk_size=chunk_size, return_lse=True)
+    if out_scale != 1.0:
+        o = o * out_scale
+    if out is not None:
+        o = out.copy_(o)
+    return (o, lse) if return_lse else o
+
+
 def mla_attention(q_nope_abs, q_pe, kv_cache, md, scale, kv_lora_rank, sliding_window: Optional[int] = None):
     """``q_pe`` None: no rope part."""
     if _use_cuda(q_nope_abs):

@@ -9,6 +9,7 @@ that defines it is compiled then, by itself: a process compiles the kernels its 
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import functools
 import os
@@ -742,6 +743,143 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int, recent: int, positio
                        lens.data_ptr(), ws.data_ptr(), B, Hkv, kv_cache.shape[4], kv_cache.shape[3], L, rows, keep, first, recent, bt.stride(0), scores.stride(0),
                        scores.stride(1), po[0], po[1], int(md.kv_vt), _st()), "evict_keys", 2 if cap else 1)
     return lens, new, places
+
+
+# ------------------------------------------------------------------ a cache in 4 bits (csrc/cache_fp4.cu, csrc/attention_fp4.cu)
+_write_fp4 = _sig("vb_write_fp4", _vp, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i, _f, _f, _i, _vp)
+_gather_fp4 = _sig("vb_gather_fp4", _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _i, _i, _f, _f, _i, _vp)
+_pages_fp4 = _sig("vb_pages_fp4", _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp)
+
+
+def _fp4_half(x, kv_cache, op: str) -> int:
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{op}: values of 16 bits on the device; got {x.dtype}")
+    if kv_cache.get_device() != _device() or kv_cache.data_ptr() % 16:
+        raise ValueError(f"{op}: a 16-byte aligned cache on the current device; got {kv_cache.device} while device {_device()} is the current one")
+    return _DT[x.dtype]
+
+
+def _fp4_rows(x, width: int):
+    """Rows of ``width`` values next to each other, at 16-byte addresses."""
+    if x.dim() == 3:
+        x = x.flatten(1) if x.stride(2) == 1 and x.stride(1) == x.shape[2] else x.reshape(x.shape[0], width)
+    return _heads(x if x.stride(1) == 1 else x.contiguous())
+
+
+def write_fp4(positions, axes, q, k, v, table, D: int, neox: bool, kv_cache, slots, k_scale: float, v_scale: float):
+    """Rotation (positions None: none) and quantisation of new tokens; q in place."""
+    T, H = k.shape[0], kv_cache.shape[2]
+    dtype = _fp4_half(k, kv_cache, "write_fp4")
+    if not T:
+        return q
+    k, v = _fp4_rows(k, H * D), _fp4_rows(v, H * D)
+    rot, Hq, turned = (0, 0, None) if positions is None else (table.shape[1], q.shape[1] // D, _fp4_rows(q, q.shape[1]))
+    if rot and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    _check(_write_fp4(_p(positions), 0 if axes is None else positions.stride(0), 1 if axes is None else positions.shape[0], _p(axes), _p(table),
+                      table.shape[0] if rot else 0, rot, int(neox), _p(turned), k.data_ptr(), v.data_ptr(), T, Hq, H, D, turned.stride(0) if rot else 0, k.stride(0),
+                      v.stride(0), kv_cache.data_ptr(), kv_cache.shape[0], slots.data_ptr(), kv_cache.shape[3], k_scale, v_scale, dtype, _st()), "write_fp4")
+    if turned is not None and turned.data_ptr() != q.data_ptr():
+        q.copy_(turned)
+    return q
+
+
+def gather_fp4(kv_cache, block_table, cu, k, v, max_tokens: int, starts, k_scale: float, v_scale: float) -> None:
+    _, _, H, BS, row = kv_cache.shape
+    D, dtype = row * 16 // 9, _fp4_half(k, kv_cache, "gather_cache_fp4")
+    for t in (k, v):
+        if t.stride(2) != 1 or t.stride(1) != D or t.data_ptr() % 16 or t.stride(0) % 8:
+            raise ValueError("gather_cache_fp4: rows of k and v at 16-byte addresses, their heads next to each other")
+    if block_table.stride(1) != 1:
+        raise ValueError("gather_cache_fp4: a request's pages are next to each other in the block table")
+    _check(_gather_fp4(kv_cache.data_ptr(), kv_cache.shape[0], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu.data_ptr(), _p(starts), k.data_ptr(),
+                       v.data_ptr(), k.stride(0), v.stride(0), k.shape[0], cu.numel() - 1, max_tokens, H, D, BS, k_scale, v_scale, dtype, _st()), "gather_cache_fp4")
+
+
+# of 16-bit pages that a prompt's cache is read back to at a time: requests that want more are taken in several goes
+FP4_PAGES_BYTES = 1 << 30
+
+
+def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[int, int, int, int]]:
+    """Runs of requests whose 16-bit pages fit into the workspace: (first, behind the last, pages of all, pages of the longest).  Lengths are those that the step
+    has on the host; without them every request counts with ``most`` pages."""
+    B = md.num_reqs
+    need = [most] * B
+    lens = getattr(md, "host_lens", None)
+    if lens is not None:
+        cu, sl = lens
+        need = [0 if not md.decode_only and cu[b + 1] - cu[b] <= few else min(-(-int(sl[b]) // PS), most) for b in range(B)]
+    elif md.seq_lens_cpu is not None:
+        need = [min(-(-n // PS), most) for n in md.seq_lens_cpu[:B].tolist()]
+    runs, first, total = [], 0, 0
+    for b, n in enumerate(need):
+        if total and (total + n) * page_bytes > FP4_PAGES_BYTES:
+            runs.append((first, b, total, max(need[first:b])))
+            first, total = b, 0
+        total += n
+    runs.append((first, B, total, max(need[first:], default=0)))
+    return runs
+
+
+def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, lse, alibi, sinks, chunk, out_scale, few: int) -> None:
+    """Attention of the requests with more than ``few`` new tokens: their cache is read back to 16-bit pages, which the attention kernels over those take.  Rows of
+    the other requests hold anything afterwards."""
+    (_, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
+    bt, sl = md.block_table, md.seq_lens
+    vt = tc_attention_ok(D, D, Hq // H) and alibi is None
+    PS = 32 if D == 256 else 64
+    qsl = None if md.decode_only else md.query_start_loc
+    most = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS)
+    for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * D):
+        n = b1 - b0
+        if n == 0 or (total == 0 and few >= 0):
+            continue
+        pages = torch.empty((max(total, 1), 2, H, PS, D), dtype=q.dtype, device=q.device)
+        table, lens = sl.new_empty((n, max(longest, 1))), sl.new_empty(n)
+        _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt[b0:].data_ptr(), bt.stride(0), bt.shape[1], sl[b0:].data_ptr(), None if qsl is None else qsl[b0:].data_ptr(), few,
+                          pages.data_ptr(), pages.shape[0], PS, int(vt), table.data_ptr(), table.shape[1], lens.data_ptr(), n, H, D, BS, _DT[q.dtype], _st()), "pages_fp4")
+        part = copy.copy(md)
+        part.num_reqs, part.block_table, part.seq_lens, part.max_seq_len, part.kv_vt, part.flat, part.cascade = n, table, lens, max(longest, 1) * PS, vt, False, None
+        if md.decode_only:
+            rows = slice(b0, b1)
+            part.query_start_loc = None if md.query_start_loc is None else md.query_start_loc[:n + 1]
+        else:
+            rows = slice(0, q.shape[0])
+            part.query_start_loc = qsl[b0:b1 + 1]
+        got = paged_attention(q[rows], pages, part, scale, window, soft_cap, causal, out[rows], return_lse=lse is not None, alibi_slopes=alibi, sinks=sinks, chunk_size=chunk,
+                              out_scale=out_scale)
+        if lse is not None:
+            if md.decode_only or n == md.num_reqs:
+                lse[rows] = got[1]
+            else:
+                t = torch.arange(q.shape[0], device=q.device)
+                lse.copy_(torch.where(((t >= qsl[b0]) & (t < qsl[b1]))[:, None], got[1], lse))
+
+
+def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causal=True, out=None, alibi=None, sinks=None, chunk=0, return_lse: bool = False,
+                        out_scale: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0):
+    T, Hq, D = q.shape
+    _fp4_half(q, kv_cache, "paged_attention_fp4")
+    bt, sl, B, dev = md.block_table, md.seq_lens, md.num_reqs, _device()
+    if bt.dtype is not _I32 or bt.dim() != 2 or bt.stride(1) != 1 or bt.shape[0] < B or sl.dtype is not _I32 or not sl.is_contiguous() or sl.numel() < B \
+            or bt.get_device() != dev or sl.get_device() != dev:
+        raise ValueError("paged_attention_fp4: int32 block tables with a request's pages next to each other and int32 lengths of all requests, on the current device")
+    if not md.decode_only:
+        _query_offsets(md, dev)
+    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
+        q = _q_heads(q)
+    used, to = B if md.decode_only else md.num_actual_tokens, out
+    if out is None or out.data_ptr() % 16 or out.stride(0) % 8:
+        to = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if T > used and out is None:             # (padding rows are written by no CTA: keep them finite)
+        to[used:].zero_()
+    if B:
+        _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, -1)
+    if out is not None and to is not out:
+        out[:used] = to[:used]
+        to = out
+    return (to, lse) if return_lse else to
 
 
 def merge_attn_states(o1, lse1, o2, lse2):

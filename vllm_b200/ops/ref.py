@@ -138,6 +138,82 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Te
     kv_cache[blk, 1, :, off, :] = value[valid].to(kv_cache.dtype)
 
 
+# ------------------------------------------------- KV cache in 4 bits
+def fp4_row_bytes(head_size: int) -> int:
+    """Bytes of a row of ``head_size`` values: two codes to a byte, a scale for every 16."""
+    return head_size // 2 + head_size // 16
+
+
+def fp4_parts(kv_cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes [blocks, 2, kv heads, page, D / 2] and scales [..., D / 16] as views of a contiguous cache."""
+    nb, _, H, bs, row = kv_cache.shape
+    D = row * 16 // 9
+    flat = kv_cache.view(nb, 2, H, bs * row)
+    return flat[..., :bs * D // 2].unflatten(-1, (bs, D // 2)), flat[..., bs * D // 2:].unflatten(-1, (bs, D // 16))
+
+
+def fp4_quant_rows(x: torch.Tensor, factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scale bytes of rows [..., D]: y = x / factor in groups of 16, e = e4m3(max |y| / 6) (at most 448), e2m1(y / e), to nearest, ties to
+    even.  A group with a NaN has the scale NaN."""
+    one = lambda v: torch.full((), v, dtype=torch.float32, device=x.device)               # noqa: E731  (a tensor: a number's reciprocal would be multiplied)
+    y = (x.float() / one(factor)).unflatten(-1, (-1, 16))
+    top = y.abs().amax(-1)
+    e = (top / one(6.0)).clamp(max=FP8_MAX).to(torch.float8_e4m3fn)
+    m = (y.abs() / e.float()[..., None]).masked_fill_((e.float() == 0)[..., None], 0.0).nan_to_num_(0.0, posinf=6.0)
+    code = torch.zeros_like(m, dtype=torch.uint8)
+    for border, up in ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)):
+        code += m >= border if up else m > border
+    code = (code + 8 * (y < 0).to(torch.uint8)).flatten(-2)
+    return code[..., 0::2] | (code[..., 1::2] << 4), e.view(torch.uint8)
+
+
+def fp4_rows(codes: torch.Tensor, scales: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
+    """The fp32 values that codes and scale bytes stand for."""
+    lut = torch.tensor(E2M1_VALUES + tuple(-v for v in E2M1_VALUES), dtype=torch.float32, device=codes.device)
+    y = lut[torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).long()].unflatten(-1, (-1, 16))
+    y = y * scales.contiguous().view(torch.float8_e4m3fn).float()[..., None]
+    return (y * torch.full((), factor, dtype=torch.float32, device=codes.device)).flatten(-2)
+
+
+def fp4_cache_values(kv_cache: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+    """The whole cache in 32 bits, [blocks, 2, kv heads, page, D]."""
+    codes, scales = fp4_parts(kv_cache)
+    return torch.stack([fp4_rows(codes[:, i], scales[:, i], f) for i, f in enumerate((k_scale, v_scale))], dim=1)
+
+
+def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: float = 1.0,
+                          v_scale: float = 1.0) -> None:
+    bs = kv_cache.shape[3]
+    valid = (slot_mapping >= 0) & (slot_mapping < kv_cache.shape[0] * bs)
+    slots = slot_mapping[valid].long()
+    blk, off = slots // bs, slots % bs
+    codes, scales = fp4_parts(kv_cache)
+    for part, (x, factor) in enumerate(((key, k_scale), (value, v_scale))):
+        codes[blk, part, :, off], scales[blk, part, :, off] = fp4_quant_rows(x[valid], factor)
+
+
+def axes_table(positions: torch.Tensor, cos_sin_cache: torch.Tensor, axes: torch.Tensor) -> torch.Tensor:
+    """Cosines and sines [T, rot] of tokens with positions [n, T], pair j turned by the position on axis axes[j]."""
+    half = cos_sin_cache.shape[-1] // 2
+    cs, pair, a = cos_sin_cache[positions.long()], torch.arange(half, device=positions.device), axes.long()
+    return torch.cat((cs[a, :, pair].t(), cs[a, :, half + pair].t()), dim=-1).contiguous()
+
+
+def gather_cache_fp4(kv_cache: torch.Tensor, block_table: torch.Tensor, cu_seq_lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     seq_starts: Optional[torch.Tensor] = None, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    bs = kv_cache.shape[3]
+    codes, scales = fp4_parts(kv_cache)
+    cu = cu_seq_lens.tolist()
+    starts = [0] * (len(cu) - 1) if seq_starts is None else seq_starts.tolist()
+    for i, first in enumerate(starts):
+        tok = torch.arange(first, first + cu[i + 1] - cu[i], device=kv_cache.device)
+        there = (tok >= 0) & (tok < block_table.shape[1] * bs)
+        blk = block_table[i][(tok.clamp(min=0) // bs).clamp(max=block_table.shape[1] - 1)].long()
+        for part, (to, factor) in enumerate(((k, k_scale), (v, v_scale))):
+            rows = fp4_rows(codes[blk, part, :, tok % bs], scales[blk, part, :, tok % bs], factor)
+            to[cu[i]:cu[i + 1]] = rows.masked_fill_(~there[:, None, None], 0.0).to(to.dtype)
+
+
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
                          slot_mapping: torch.Tensor) -> None:
     """kv_c: [T, R], k_pe: [T, P]; kv_cache: [nb, bs, R+P]."""
