@@ -1,0 +1,764 @@
+// Attention of few query rows (one new token per request, or some drafts) over a paged key-value cache in 4 bits (fp4.cuh).
+//
+//   s[r, k] = c(scale q_r . K_k) for the keys k that row r sees,  lse_r = log(sum_k e^s[r, k] + e^sink),  out_r = sum_k e^(s[r, k] - lse_r) V_k
+//
+// Query rows are pairs (new token, query head of a kv head), 16 of them (or 8, where there are no more) at a time: with a request and a kv head they are a
+// "row" of the schedule.  All rows' tiles of 64 keys, in order, are dealt to the CTAs in equal runs, so that ragged and few long requests keep all SMs as
+// busy as many equal ones; a row that one CTA has is finished there, one that several have is joined by a second kernel.  Where rows are few and short a cluster
+// has a row, and the parts meet in shared memory.
+//
+// A warp takes every fourth strip of 16 keys; codes and scales of a strip come by asynchronous copies of the warp's own, STAGES of them on their way across the
+// borders of rows.  S^T = K Q^T (m16n8k16: keys are rows, query rows columns), an own running maximum, O^T += V^T P^T.
+//
+// Codes become fp16 in registers (one conversion for two of them, one multiplication by their scale: exact, fp4.cuh), in the order in which the matrix
+// instruction wants them: dimensions of K may go to the instruction's k in any order that Q follows, so a lane reads D / 4 neighbouring
+// values of a key at once; the products with V pair up keys, so the nibbles of two keys are brought together first (a shift and a bitwise select for eight values),
+// and a lane has D / 8 neighbouring dimensions.  Q is fp16, bf16 rows scaled by a power of two to [2^14, 2^15): exact but for values below 2^-28 of the largest,
+// whose error is below 2^-39 of it.  Weights are fp16 multiples of 2^-24 of up to 2^15: off by 2^-12 of themselves (a result in bf16 is rounded to 2^-9), in two
+// such parts where the result is fp16.  Sums are in 32 bits.
+#include "attention_prompt.cuh"
+#include "cluster.cuh"
+#include "device_once.h"
+#include "fp4.cuh"
+
+namespace afp4 {
+
+constexpr int TILE = 64, STRIP = 16, WARPS = 4, THREADS = WARPS * 32;
+constexpr int MAX_REQUESTS = 512;            // of a launch: their first tiles lie in shared memory
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float SHIFT = 7.f;                 // the reference of a row's weights is its largest score less SHIFT, or up to 8 below that
+
+struct Params {
+  const void* q;
+  const uint8_t* cache;
+  const int* block_table;
+  const int* seq_lens;
+  const int* qsl;            // null: a token each
+  void* out;
+  float* lse;
+  const float* sinks;
+  float* part;               // [segment][COLS][D + 2]: output, maximum, sum
+  int2* info;                // [row]: its first CTA, and how many
+  int64_t q_stride, out_stride, bt_stride, num_blocks;
+  int B, Hkv, G, BS, max_rows, few, ctas, chunks, extra, parts, window, bf16;
+  float scale_log2, ku, c2, out_scale;
+};
+
+struct Request {
+  int n, t;                  // rows in the cache, new tokens among them (0: none of this kernel's)
+  VB_DEVICE int first_key(const Params& p) const { return p.window > 0 ? max(n - t - p.window + 1, 0) : 0; }      // that any of its rows sees
+  VB_DEVICE int first_tile(const Params& p) const { return first_key(p) / TILE; }
+  VB_DEVICE int tiles(const Params& p) const { return n > 0 && t > 0 ? (n + TILE - 1) / TILE - first_tile(p) : 0; }
+  VB_DEVICE int chunks(const Params& p, int cols) const { return (t * p.G + cols - 1) / cols; }
+};
+VB_DEVICE Request request(const Params& p, int b) {
+  Request r;
+  r.n = min(max(p.seq_lens[b], 0), p.max_rows);
+  r.t = p.qsl ? p.qsl[b + 1] - p.qsl[b] : 1;
+  if (r.t > p.few || r.t < 0) r.t = 0;
+  return r;
+}
+VB_DEVICE int slots_of(const Params& p, const Request& r) {          // a row's tiles, and what its end costs in tiles
+  const int n = r.tiles(p);
+  return n > 0 ? n + p.extra : 0;
+}
+
+// first[b]: slots of all rows in front of request b, as if each request had one kv head; first[B]: of all
+VB_DEVICE void scan_tiles(const Params& p, int cols, int* first, int2* reqs, int* warp_sums) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    int mine = 0;
+    if (b < p.B) {
+      const Request r = request(p, b);
+      reqs[b] = make_int2(r.n, r.t);
+      mine = slots_of(p, r) * r.chunks(p, cols);
+    }
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[w] = x;
+    __syncthreads();
+    int before = base;
+    for (int i = 0; i < WARPS; ++i) {
+      if (i < w) before += warp_sums[i];
+      base += warp_sums[i];
+    }
+    if (b < p.B) first[b] = before + x - mine;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first[p.B] = base;
+  __syncthreads();
+}
+
+// A row: request, kv head, chunk of query rows; its slots are [begin, end) of the order of all
+struct Row {
+  int b, h, c, begin, end;
+};
+VB_DEVICE void row_at(const Params& p, int cols, const int* first, const int2* reqs, int tile, Row& r) {      // the row that has this tile
+  int lo = 0, hi = p.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] * p.Hkv <= tile) lo = mid; else hi = mid - 1;
+  }
+  const Request q{reqs[lo].x, reqs[lo].y};               // (it has slots: the last request that begins at or in front of the tile)
+  const int n = slots_of(p, q), chunks = q.chunks(p, cols), i = (tile - first[lo] * p.Hkv) / n;
+  r.b = lo;
+  r.h = i / chunks;
+  r.c = i - r.h * chunks;
+  r.begin = first[lo] * p.Hkv + i * n;
+  r.end = r.begin + n;
+}
+VB_DEVICE void next_row(const Params& p, int cols, const int* first, const int2* reqs, Row& r) {                     // behind it there is one more
+  Request q{reqs[r.b].x, reqs[r.b].y};
+  if (++r.c == q.chunks(p, cols)) {
+    r.c = 0;
+    if (++r.h == p.Hkv) {
+      r.h = 0;
+      do { ++r.b; } while (first[r.b + 1] == first[r.b]);
+      q = Request{reqs[r.b].x, reqs[r.b].y};
+    }
+  }
+  r.begin = r.end;
+  r.end = r.begin + slots_of(p, q);
+}
+
+VB_DEVICE void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+VB_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> VB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+VB_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of 16-bit values, two to a lane, with rows and columns exchanged
+VB_DEVICE uint32_t turn8(uint32_t x) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x)); return r; }
+
+// N neighbouring bytes of shared memory as words; `at` is a multiple of what N is one of: 16, 8, 4, 2 or 1.  What the last word has behind them are copies: conversions of
+// codes that the compiler (nvcc 12.9) knows to be 0 came out as others'.
+template <int N> struct Bytes {
+  static constexpr int WORDS = (N + 3) / 4;
+  uint32_t w[WORDS];
+  VB_DEVICE void load(const unsigned char* at) {
+    if constexpr (N % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 16; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at + 16 * i);
+        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+      }
+    } else if constexpr (N % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i) {
+        const uint2 x = *reinterpret_cast<const uint2*>(at + 8 * i);
+        w[2 * i] = x.x; w[2 * i + 1] = x.y;
+      }
+    } else if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(at + 4 * i);
+    } else {
+      constexpr int S = N % 2 == 0 ? 2 : 1;
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j += S)
+          if (4 * i + j < N) x |= (S == 2 ? (uint32_t)*reinterpret_cast<const uint16_t*>(at + 4 * i + j) : (uint32_t)at[4 * i + j]) << (8 * j);
+        w[i] = 4 * i + 4 <= N ? x : N % 4 == 2 ? x | x << 16 : N % 4 == 1 ? x * 0x01010101u : x | x << 24;
+      }
+    }
+  }
+};
+
+template <int D_> struct Form {
+  static constexpr int D = D_, KD = D / 16;
+  static constexpr int CODES = STRIP * D / 2, SIDE = CODES + STRIP * D / 16, STAGE = 2 * SIDE;       // bytes of a strip's keys, values behind them
+  static constexpr int STAGES = D <= 64 ? 6 : D <= 128 ? 4 : 3;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int REGS = KD * 4 + 4;                                  // of eight query rows: output, maxima, sums
+  static constexpr int EXCH = WARPS / 2 * REGS * 128;
+  static constexpr int LISTS = (MAX_REQUESTS + 1 + 2 * MAX_REQUESTS + 32 + 3) / 4 * 16;
+  static constexpr int PART = 16 * (D + 2 + 9) * 4;                        // of a CTA of a cluster, instead of the lists
+  static constexpr int SMEM = RING + EXCH + (LISTS > PART ? LISTS : PART);
+  // a lane's D / 4 values of a key lie in GK groups, its D / 8 values of a value row in GV
+  static constexpr int SK = D / 4, SV = D / 8;
+  static constexpr int GK = SK % 16 == 0 ? SK / 16 : 16 % SK == 0 ? 1 : 2, GV = SV % 16 == 0 ? SV / 16 : 16 % SV == 0 ? 1 : 2;
+  static constexpr bool STRAIGHT_K = SK % 16 == 0 || 16 % SK == 0, STRAIGHT_V = SV % 16 == 0 || 16 % SV == 0;
+};
+
+template <int D, int NT, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p) {
+  using F = Form<D>;
+  constexpr int KD = F::KD, STAGES = F::STAGES, COLS = 8 * NT, PD = D + 2;
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* exch = reinterpret_cast<float*>(smem + F::RING);
+  int* first = reinterpret_cast<int*>(smem + F::RING + F::EXCH);
+  int2* reqs = reinterpret_cast<int2*>(first + MAX_REQUESTS + 2);
+  int* warp_sums = reinterpret_cast<int*>(reqs + MAX_REQUESTS);
+  float* part_s = reinterpret_cast<float*>(first);         // cluster: the CTA's part
+  float* factor_s = part_s + COLS * PD;                    // ... and factors of the parts
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool fused = p.parts > 0;
+  pdl_wait();
+  pdl_trigger();             // (here: the joining kernel may read the lengths as soon as it starts)
+  int t0, t1, per;
+  Row row;
+  Request req;
+  const int rank = fused ? blockIdx.x % p.parts : 0;
+  if (fused) {
+    const int i = blockIdx.x / p.parts;
+    row.c = i % p.chunks;
+    row.h = i / p.chunks % p.Hkv;
+    row.b = i / p.chunks / p.Hkv;
+    req = request(p, row.b);
+    row.begin = 0;
+    row.end = row.c < req.chunks(p, COLS) ? req.tiles(p) : 0;
+    per = (row.end + p.parts - 1) / p.parts;
+    t0 = min(rank * per, row.end);
+    t1 = min(t0 + per, row.end);
+  } else {
+    scan_tiles(p, COLS, first, reqs, warp_sums);
+    const int total = first[p.B] * p.Hkv;
+    per = (total + p.ctas - 1) / p.ctas;
+    t0 = blockIdx.x * per;
+    t1 = min(t0 + per, total);
+    if (t0 >= t1) return;
+    row_at(p, COLS, first, reqs, t0, row);
+    req = Request{reqs[row.b].x, reqs[row.b].y};
+  }
+
+  unsigned char* ring = smem + warp * (STAGES * F::STAGE);
+  const int64_t page = fp4::page_bytes(p.BS, D);
+  // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  Where they lie is looked up for 32 of them at once, a lane each.
+  const int s_end = t1 * 4;
+  int64_t my_page = 0;                                                      // of the lane's strip: place of the page, token in it (-1: nothing to fetch)
+  int my_off = -1, fetched = 0;
+  auto fetch = [&](int stage) {
+    if ((fetched & 31) == 0) {
+      const int s = t0 * 4 + warp + (fetched + lane) * WARPS;
+      my_off = -1;
+      if (s < s_end) {
+        Row r = row;
+        Request q = req;
+        if (!fused) {
+          row_at(p, COLS, first, reqs, s >> 2, r);
+          q = Request{reqs[r.b].x, reqs[r.b].y};
+        }
+        const int tok = ((s >> 2) - r.begin + q.first_tile(p)) * TILE + (s & 3) * STRIP;
+        if (tok < q.n) {
+          int64_t blk = p.block_table[r.b * p.bt_stride + tok / p.BS];
+          if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
+          my_page = (blk * 2 * p.Hkv + r.h) * page;
+          my_off = tok % p.BS;
+        }
+      }
+    }
+    const int off = __shfl_sync(0xffffffffu, my_off, fetched & 31);
+    const int64_t at = __shfl_sync(0xffffffffu, my_page, fetched & 31);
+    ++fetched;
+    if (off >= 0) {
+      const uint8_t* k = p.cache + at + off * (D / 2);
+      const uint8_t* ks = p.cache + at + (int64_t)p.BS * (D / 2) + off * (D / 16);
+      const int64_t to_v = p.Hkv * page;
+      const uint32_t to = smem_u32(ring + stage * F::STAGE);
+#pragma unroll
+      for (int i = 0; i < (D / 2 + 31) / 32; ++i) {
+        const int j = i * 32 + lane;
+        if (D / 2 % 32 == 0 || j < D / 2) {
+          const int d = D == 128 ? (j & ~3) | ((j & 3) ^ (j >> 3 & 2)) : j;  // (D = 128: pieces of a row change places so that lanes of a load meet in no bank)
+          cp_async16(to + d * 16, k + j * 16);
+          cp_async16(to + F::SIDE + d * 16, k + to_v + j * 16);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < (D / 8 + 31) / 32; ++i) {
+        const int j = i * 32 + lane, side = j >= D / 16;
+        if (j < D / 8) cp_async16(to + side * F::SIDE + F::CODES + (j - side * (D / 16)) * 16, ks + (side ? to_v : 0) + (j - side * (D / 16)) * 16);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+
+  const int r0 = lane >> 2, t4 = lane & 3, q0 = t4 * 2;
+  // rows of a product in front of slots of the next: row r is key r ^ (r >> 1 & 1), so that the keys of neighbouring lanes lie in both halves of the banks
+  const int key0 = r0 ^ (r0 >> 1 & 1);
+  const int vkey[4] = {q0 + (t4 & 1), q0 + 1 - (t4 & 1), q0 + 8 + (t4 & 1), q0 + 9 - (t4 & 1)};
+  int s = t0 * 4 + warp, turn = 0;
+  uint32_t q[KD][NT][2];
+  float undo[NT][2];
+  int hi[NT][2];                                                            // last key that a column sees
+  auto load_q = [&]() {
+    const int first_q = p.qsl ? p.qsl[row.b] : row.b;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row.c * COLS + nt * 8 + r0, tok = r / p.G;
+      const bool there = tok < req.t;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(first_q + tok) * p.q_stride + (int64_t)(row.h * p.G + r - tok * p.G) * D + t4 * (D / 4);
+#pragma unroll
+      for (int k = 0; k < KD; ++k) {
+        const uint2 x = there ? *reinterpret_cast<const uint2*>(qp + k * 4) : make_uint2(0u, 0u);
+        q[k][nt][0] = x.x; q[k][nt][1] = x.y;
+      }
+      float mine = 1.f;
+      if (p.bf16) {
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 x = unpack2<__nv_bfloat16>(q[k][nt][j]);
+            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 27), 254);                  // of the exponent's field; [2^-100, 2^127]
+        const float f = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);               // 2^(14 - (e - 127)), at least 2^-113
+        mine = __uint_as_float((uint32_t)(e - 14) << 23);
+#pragma unroll
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 x = unpack2<__nv_bfloat16>(q[k][nt][j]);
+            q[k][nt][j] = pack2<__half>(x.x * f, x.y * f);
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        undo[nt][u] = __shfl_sync(0xffffffffu, mine, (q0 + u) * 4);
+        hi[nt][u] = req.n - req.t + (row.c * COLS + nt * 8 + q0 + u) / p.G;
+      }
+    }
+  };
+  load_q();
+  while (true) {
+    const int seg_end = min(row.end, t1) * 4, n = req.n, tile0 = req.first_tile(p), low = req.first_key(p);
+    float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < KD; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) { m_run[nt][u] = -INFINITY; l_run[nt][u] = 0.f; }
+    }
+    for (; s < seg_end; s += WARPS) {
+      const int stage = turn;
+      turn = turn + 1 == STAGES ? 0 : turn + 1;
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);                          // into the stage of the strip before, which the whole warp has read
+      const int tok = ((s >> 2) - row.begin + tile0) * TILE + (s & 3) * STRIP;
+      if (tok >= n) continue;
+      const unsigned char* ks = ring + stage * F::STAGE;
+      const unsigned char* vs = ks + F::SIDE;
+      // ---- S^T = K Q^T
+      float sc[NT][4], sd[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[nt][i] = sd[nt][i] = 0.f;
+      {
+        Bytes<D / 8> c0, c1;
+        const int piece = D == 128 ? (t4 ^ (key0 >> 1 & 2)) * 16 : t4 * (D / 8);
+        c0.load(ks + key0 * (D / 2) + piece);
+        c1.load(ks + (key0 + 8) * (D / 2) + piece);
+        uint32_t s0[F::GK], s1[F::GK];
+        const int g0 = t4 * F::SK / 16, cross = (16 - t4 * F::SK % 16) / 4;          // (not STRAIGHT_K: the lane's values from the cross-th four on are the next group's)
+#pragma unroll
+        for (int g = 0; g < F::GK; ++g) {
+          const unsigned char* at = ks + F::CODES + key0 * (D / 16) + min(g0 + g, D / 16 - 1);
+          const uint32_t two = fp4::scales2(at[0] | (uint32_t)at[8 * (D / 16)] << 8);
+          s0[g] = fp4::low2(two);
+          s1[g] = fp4::high2(two);
+        }
+#pragma unroll
+        for (int w = 0; w < (KD + 1) / 2; ++w) {                                     // a word: two steps of the product
+          uint32_t a[4], b[4];
+          fp4::unpack8(c0.w[w], a);
+          fp4::unpack8(c1.w[w], b);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int k = 2 * w + half;
+            if (k < KD) {
+              const uint32_t f0 = F::STRAIGHT_K ? s0[F::GK > 1 ? k / 4 : 0] : k < cross ? s0[0] : s0[F::GK - 1];
+              const uint32_t f1 = F::STRAIGHT_K ? s1[F::GK > 1 ? k / 4 : 0] : k < cross ? s1[0] : s1[F::GK - 1];
+              const uint32_t a0 = fp4::mul2(a[2 * half], f0), a2 = fp4::mul2(a[2 * half + 1], f0), a1 = fp4::mul2(b[2 * half], f1), a3 = fp4::mul2(b[2 * half + 1], f1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816(k & 1 ? sd[nt] : sc[nt], a0, a1, a2, a3, q[k][nt][0], q[k][nt][1]);
+            }
+          }
+        }
+      }
+      // ---- weights
+      const bool cut = tok + STRIP > n - req.t + 1 || (p.window > 0 && tok < n - p.window);
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx[2], alpha[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = (sc[nt][i] + sd[nt][i]) * undo[nt][i & 1];
+          float y = p.ku > 0.f || p.ku < 0.f ? prompt::cap_any(x * p.ku, p.c2) : x * p.scale_log2;
+          if (cut) {
+            const int key = tok + key0 + (i >> 1) * 8, last = hi[nt][i & 1];
+            if (key > last || (p.window > 0 && key <= last - p.window)) y = -INFINITY;
+          }
+          sc[nt][i] = y;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) mx[u] = fmaxf(sc[nt][u], sc[nt][2 + u]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], x));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float was = m_run[nt][u], at = mx[u] - SHIFT;
+          const bool up = at > was + 8.f || (was == -INFINITY && at > -INFINITY);            // else the old reference stays
+          alpha[u] = up && was != -INFINITY ? ex2(was - at) : 1.f;
+          m_run[nt][u] = up ? at : was;
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < KD; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][nt][j] *= alpha[j & 1];
+          l_run[nt][0] *= alpha[0]; l_run[nt][1] *= alpha[1];
+        }
+        const float ref[2] = {m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float x = ex2(sc[nt][2 * t] - ref[0]), y = ex2(sc[nt][2 * t + 1] - ref[1]);
+          l_run[nt][0] += x; l_run[nt][1] += y;
+          const uint32_t h = pack2<__half>(x, y);
+          ph[nt][t] = turn8(h);
+          if (!p.bf16) {
+            const float2 back = unpack2<__half>(h);
+            pl[nt][t] = turn8(pack2<__half>(x - back.x, y - back.y));
+          }
+        }
+      }
+      // ---- O^T += V^T P^T
+      {
+        Bytes<D / 16> c[4];
+        uint32_t sa[F::GV], sb[F::GV];                                               // scales of the keys of slots (0, 1) and (8, 9)
+        const int g0 = r0 * F::SV / 16, cross = (16 - r0 * F::SV % 16) / 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = r0 * (D / 16);
+          c[j].load(vs + vkey[j] * (D / 2) + (D == 128 ? (((at >> 4) ^ (vkey[j] >> 1 & 2)) << 4 | (at & 15)) : at));
+        }
+#pragma unroll
+        for (int g = 0; g < F::GV; ++g) {
+          const unsigned char* at = vs + F::CODES + min(g0 + g, D / 16 - 1);
+          uint32_t x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = at[vkey[j] * (D / 16)];
+          if (tok + STRIP > n || tok < low)      // rows of nobody, or that no query row sees, may hold what a weight of 0 does not cancel
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = tok + vkey[j] < n && tok + vkey[j] >= low ? x[j] : 0u;
+          sa[g] = fp4::scales2(x[0] | x[1] << 8);
+          sb[g] = fp4::scales2(x[2] | x[3] << 8);
+        }
+#pragma unroll
+        for (int w = 0; w < Bytes<D / 16>::WORDS; ++w) {
+          // the nibbles of two keys next to each other: bytes of even values, and of odd ones
+          constexpr uint32_t LOW = 0x0f0f0f0fu;
+          uint32_t e01[4], o01[4], e23[4], o23[4];
+          fp4::unpack8((c[0].w[w] & LOW) | ((c[1].w[w] << 4) & ~LOW), e01);
+          fp4::unpack8(((c[0].w[w] >> 4) & LOW) | (c[1].w[w] & ~LOW), o01);
+          fp4::unpack8((c[2].w[w] & LOW) | ((c[3].w[w] << 4) & ~LOW), e23);
+          fp4::unpack8(((c[2].w[w] >> 4) & LOW) | (c[3].w[w] & ~LOW), o23);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * w + j;
+            if (i < KD) {
+              const uint32_t f0 = F::STRAIGHT_V ? sa[F::GV > 1 ? i / 8 : 0] : i < cross ? sa[0] : sa[F::GV - 1];
+              const uint32_t f1 = F::STRAIGHT_V ? sb[F::GV > 1 ? i / 8 : 0] : i < cross ? sb[0] : sb[F::GV - 1];
+              const uint32_t a0 = fp4::mul2(e01[j], f0), a1 = fp4::mul2(o01[j], f0), a2 = fp4::mul2(e23[j], f1), a3 = fp4::mul2(o23[j], f1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816(o[i][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                if (!p.bf16) mma16816(o[i][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+    // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
+    const int index = (row.b * p.Hkv + row.h) * p.chunks + row.c, live = row.begin + req.tiles(p);       // (behind its tiles a row has further slots)
+    const bool empty = !fused && max(row.begin, t0) >= live;
+    const int n_ctas = fused ? 1 : (live - 1) / per - row.begin / per + 1;
+    const bool whole = !fused && n_ctas == 1;
+    if (!fused && !empty && row.begin >= t0 && threadIdx.x == 0) p.info[index] = make_int2(blockIdx.x, n_ctas);
+    const Row done = row;
+    const Request done_req = req;
+    const bool more = !fused && row.end < t1;
+    if (more) {                              // (the next row's queries are on their way meanwhile)
+      next_row(p, COLS, first, reqs, row);
+      req = Request{reqs[row.b].x, reqs[row.b].y};
+      load_q();
+    }
+    if (!empty)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
+#pragma unroll
+      for (int half = WARPS / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) {
+          float* to = exch + (warp - half) * F::REGS * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < KD; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[(i * 4 + j) * 32] = o[i][nt][j];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) { to[(KD * 4 + u) * 32] = m_run[nt][u]; to[(KD * 4 + 2 + u) * 32] = l_run[nt][u]; }
+        }
+        __syncthreads();
+        if (warp < half) {
+          const float* from = exch + warp * F::REGS * 32 + lane;
+          float fa[2], fb[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float mb = from[(KD * 4 + u) * 32], top = fmaxf(m_run[nt][u], mb);
+            fa[u] = m_run[nt][u] == -INFINITY ? 0.f : ex2(m_run[nt][u] - top);
+            fb[u] = mb == -INFINITY ? 0.f : ex2(mb - top);
+            m_run[nt][u] = top;
+            l_run[nt][u] = l_run[nt][u] * fa[u] + from[(KD * 4 + 2 + u) * 32] * fb[u];
+          }
+#pragma unroll
+          for (int i = 0; i < KD; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][nt][j] = o[i][nt][j] * fa[j & 1] + from[(i * 4 + j) * 32] * fb[j & 1];
+        }
+      }
+      if (warp == 0) {
+        const int first_q = whole && p.qsl ? p.qsl[done.b] : done.b;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int g = nt * 8 + q0 + u, r = done.c * COLS + g, tok = r / p.G;
+          if (tok >= done_req.t) continue;
+          if (whole) {                       // nobody else has keys of the row
+            const int head = done.h * p.G + r - tok * p.G;
+            const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = fmaxf(m_run[nt][u], sink), base = top == -INFINITY ? 0.f : top;
+            const float l = (m_run[nt][u] == -INFINITY ? 0.f : l_run[nt][u] * ex2(m_run[nt][u] - base)) + (p.sinks ? ex2(sink - base) : 0.f);
+            const float f = l > 0.f && m_run[nt][u] > -INFINITY ? ex2(m_run[nt][u] - base) / l * p.out_scale : 0.f;
+            uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)head * D + r0 * (D / 8));
+#pragma unroll
+            for (int i = 0; i < KD; ++i) {
+              const float x = o[i][nt][u] * f, y = o[i][nt][2 + u] * f;
+              to[i] = p.bf16 ? pack2<__nv_bfloat16>(x, y) : pack2<__half>(x, y);
+            }
+            if (p.lse && r0 == 0) p.lse[(int64_t)(first_q + tok) * p.Hkv * p.G + head] = l > 0.f ? (base + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+          } else {
+            float* to = (fused ? part_s : p.part + (int64_t)(index + blockIdx.x) * COLS * PD) + g * PD + r0 * (D / 8);
+#pragma unroll
+            for (int i = 0; i < KD; ++i) *reinterpret_cast<float2*>(to + 2 * i) = make_float2(o[i][nt][u], o[i][nt][2 + u]);
+            if (r0 == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m_run[nt][u], l_run[nt][u]);
+          }
+        }
+      }
+    }
+    if (!more) break;
+  }
+  cp_async_wait<0>();
+  if (fused) {
+    cluster_sync();
+    const uint32_t parts_at = smem_u32(part_s);
+    const int live = min(max(req.t * p.G - row.c * COLS, 0), COLS), first_q = p.qsl ? p.qsl[row.b] : row.b;
+    for (int g = warp; g < live; g += WARPS) {           // a warp: log-sum-exp of a column, its parts and the sink
+      const uint32_t at = parts_at + (g * PD + D) * 4;
+      const int r = row.c * COLS + g, tok = r / p.G, head = row.h * p.G + r - tok * p.G;
+      const float m0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at, lane)) : -INFINITY, l0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at + 4, lane)) : 0.f;
+      const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
+      const float m = warp_max(fmaxf(m0, sink)), top = m == -INFINITY ? 0.f : m;
+      const float l = warp_sum(m0 == -INFINITY ? 0.f : l0 * ex2(m0 - top)) + (p.sinks ? ex2(sink - top) : 0.f);
+      if (lane < 8) factor_s[g * 9 + lane] = m0 == -INFINITY ? 0.f : ex2(m0 - top) / l * p.out_scale;
+      if (lane == 0 && rank == 0 && p.lse) p.lse[(int64_t)(first_q + tok) * p.Hkv * p.G + head] = l > 0.f ? (top + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+    }
+    __syncthreads();
+    for (int i = rank * THREADS + threadIdx.x; i < live * (D / 2); i += p.parts * THREADS) {
+      const int g = i / (D / 2), d = i % (D / 2) * 2, r = row.c * COLS + g, tok = r / p.G;
+      float2 x[8], acc = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] = c < p.parts ? ld_dsmem_f32x2(dsmem_addr(parts_at + (g * PD + d) * 4, c)) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float f = factor_s[g * 9 + c];
+        if (c < p.parts) { acc.x += x[c].x * f; acc.y += x[c].y * f; }
+      }
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)(row.h * p.G + r - tok * p.G) * D + d) =
+          p.bf16 ? pack2<__nv_bfloat16>(acc.x, acc.y) : pack2<__half>(acc.x, acc.y);
+    }
+    cluster_sync();                                      // the others may still read this CTA's part
+  }
+}
+
+// Grid (columns of a row, rows): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
+constexpr int JOIN = 128, FACTORS = 1024;
+__global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, int D) {
+  __shared__ float factor_s[FACTORS];
+  __shared__ float red[32];
+  pdl_trigger();
+  pdl_wait();
+  const int index = blockIdx.y, c = index % p.chunks, h = index / p.chunks % p.Hkv, b = index / p.chunks / p.Hkv, PD = D + 2;
+  const Request req = request(p, b);
+  const int r = c * cols + blockIdx.x, tok = r / p.G;
+  if (tok >= req.t) return;
+  const int2 at = req.n > 0 ? p.info[index] : make_int2(0, 0);
+  const int count = at.y;
+  if (req.n > 0 && count == 1) return;                   // done where its keys were
+  const int head = h * p.G + r - tok * p.G, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t step = (int64_t)cols * PD;
+  const float* x = p.part + ((int64_t)(index + at.x) * cols + blockIdx.x) * PD;
+  const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
+  float m = sink;
+  for (int i = threadIdx.x; i < count; i += JOIN) m = fmaxf(m, x[i * step + D]);
+  m = warp_max(m);
+  if (lane == 0) red[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float top = m == -INFINITY ? 0.f : m;
+  __syncthreads();
+  float l = 0.f;
+  for (int i = threadIdx.x; i < count; i += JOIN) {
+    const float2 ml = make_float2(x[i * step + D], x[i * step + D + 1]);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+    if (i < FACTORS) factor_s[i] = f;
+    l += ml.y * f;
+  }
+  l = block_sum(l, red) + (p.sinks ? ex2(sink - top) : 0.f);          // (a block barrier: the factors are there)
+  const int64_t token = (p.qsl ? p.qsl[b] : b) + tok;
+  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = l > 0.f ? (top + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+  const float f = l == 0.f ? 0.f : p.out_scale / l;
+  for (int d = threadIdx.x; d < D; d += JOIN) {
+    float acc = 0.f;
+    int i = 0;
+    for (; i + 8 <= min(count, FACTORS); i += 8) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = x[(i + j) * step + d];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc += y[j] * factor_s[i + j];
+    }
+    for (; i < count; ++i) acc += x[i * step + d] * (i < FACTORS ? factor_s[i] : x[i * step + D] == -INFINITY ? 0.f : ex2(x[i * step + D] - top));
+    uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D + d;
+    if (p.bf16) *reinterpret_cast<__nv_bfloat16*>(to) = from_f32<__nv_bfloat16>(acc * f);
+    else *reinterpret_cast<__half*>(to) = from_f32<__half>(acc * f);
+  }
+}
+
+constexpr int ctas_of(int D, int NT) { return D <= 128 ? (NT == 1 ? 4 : 3) : 2; }            // of an SM
+
+// `clusters`: nothing is launched, the clusters of a row that the device runs at a time are counted.
+template <int D, int NT>
+static int launch(const Params& p, cudaStream_t st, int* clusters, int* ctas) {
+  using F = Form<D>;
+  auto k = attention_kernel<D, NT, ctas_of(D, NT)>;
+  static std::atomic<uint64_t> devices{0};
+  if (vb_allow_smem(reinterpret_cast<const void*>(k), F::SMEM, devices) != cudaSuccess) return (int)cudaGetLastError();
+  if (ctas) { *ctas = ctas_of(D, NT); return 0; }
+  if (clusters) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = F::SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return (int)cudaOccupancyMaxActiveClusters(clusters, k, &cfg);
+  }
+  const int rows = p.B * p.Hkv * p.chunks;
+  if (p.parts > 0) {
+    vb_launch_parts(k, dim3(rows * p.parts), dim3(THREADS), (size_t)F::SMEM, st, (unsigned)p.parts, p);
+    return (int)cudaGetLastError();
+  }
+  vb_launch(k, dim3(p.ctas), dim3(THREADS), (size_t)F::SMEM, st, p);
+  vb_launch(join_kernel, dim3(min(8 * NT, p.few * p.G), rows), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
+  return (int)cudaGetLastError();
+}
+template <int D>
+static int pick(const Params& p, int nt, cudaStream_t st, int* clusters, int* ctas) {
+  return nt == 2 ? launch<D, 2>(p, st, clusters, ctas) : launch<D, 1>(p, st, clusters, ctas);
+}
+static int go(const Params& p, int D, int nt, cudaStream_t st, int* clusters = nullptr, int* ctas = nullptr) {
+  switch (D) {
+    case 32: return pick<32>(p, nt, st, clusters, ctas);
+    case 64: return pick<64>(p, nt, st, clusters, ctas);
+    case 80: return pick<80>(p, nt, st, clusters, ctas);
+    case 96: return pick<96>(p, nt, st, clusters, ctas);
+    case 128: return pick<128>(p, nt, st, clusters, ctas);
+    case 192: return pick<192>(p, nt, st, clusters, ctas);
+    case 256: return pick<256>(p, nt, st, clusters, ctas);
+  }
+  return -2;
+}
+
+}  // namespace afp4
+
+// Of heads of D and `rows` query rows (new tokens x query heads of a kv head) at most: columns of a row, CTAs of an SM, and, where parts > 0, clusters of that
+// many CTAs that the device runs at a time.
+EXPORT int vb_attention_fp4_plan(int D, int rows, int parts, int* cols, int* ctas, int* clusters) {
+  using namespace afp4;
+  Params p{};
+  p.parts = parts;
+  const int nt = rows > 8 ? 2 : 1;
+  *cols = 8 * nt;
+  int rc = go(p, D, nt, nullptr, nullptr, ctas);
+  if (rc == 0 && parts > 0) rc = parts > 8 ? -1 : go(p, D, nt, nullptr, clusters);
+  return rc;
+}
+
+// Requests of at most `few` new tokens (qsl null: one each); rows of q and out of the others are not touched.  `ws`: for rows = group Hkv chunks,
+// (rows + ctas) cols (D + 2) + 2 rows floats, chunks = ceil(few Hq / Hkv / cols).  group: requests of a launch, up to 512.  extra: tiles that a row counts for
+// beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request that the block table has room for.
+// lse [T, Hq] or null.
+EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, void* out, float* lse,
+                            const float* sinks, float* ws, int B, int Hq, int Hkv, int D, int BS, int max_rows, int few, int64_t q_stride, int64_t out_stride,
+                            int64_t bt_stride, int ctas, int extra, int parts, int group, int window, float scale, float soft_cap, float out_scale, int dtype,
+                            cudaStream_t st) {
+  using namespace afp4;
+  if (B <= 0) return 0;
+  if (group < 1 || group > MAX_REQUESTS || few < 1 || max_rows < 1 || ctas < 1 || extra < 0 || parts < 0 || parts > 8) return -1;
+  if ((dtype != DT_BF16 && dtype != DT_F16) || BS < 16 || BS % 16 || Hkv < 1 || Hq % Hkv || q_stride % 8 || out_stride % 8) return -1;
+  if (parts > 0 && B > group) return -1;
+  Params p;
+  p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.extra = extra; p.parts = parts; p.window = window; p.bf16 = dtype == DT_BF16;
+  if ((int64_t)few * p.G > 4096) return -1;
+  const int nt = few * p.G > 8 ? 2 : 1;
+  p.chunks = (few * p.G + 8 * nt - 1) / (8 * nt);
+  p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.num_blocks = num_blocks; p.cache = (const uint8_t*)cache; p.sinks = sinks;
+  p.scale_log2 = scale * LOG2E;
+  p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E; p.out_scale = out_scale;
+  p.lse = lse;
+  for (int b0 = 0; b0 < B; b0 += group) {
+    p.B = B - b0 < group ? B - b0 : group;
+    // with offsets, rows are where they say; without, request b0 + i has row b0 + i
+    p.q = qsl ? q : reinterpret_cast<const char*>(q) + b0 * q_stride * 2;
+    p.out = qsl ? out : reinterpret_cast<char*>(out) + b0 * out_stride * 2;
+    p.lse = qsl || !lse ? lse : lse + (int64_t)b0 * Hq;
+    p.qsl = qsl ? qsl + b0 : nullptr;
+    p.block_table = block_table + b0 * bt_stride;
+    p.seq_lens = seq_lens + b0;
+    const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE + extra);
+    if (tiles >= (1 << 29)) return -3;                 // flat strip numbers are 32 bits
+    if (rows > 65535) return -3;
+    p.ctas = ctas < tiles ? ctas : (int)tiles;
+    p.part = ws;
+    p.info = reinterpret_cast<int2*>(ws + (rows + p.ctas) * 8 * nt * (D + 2));
+    const int rc = go(p, D, nt, st);
+    if (rc) return rc;
+  }
+  return 0;
+}

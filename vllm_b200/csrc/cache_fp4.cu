@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) write_kernel(T* __restrict__ q, const T* 
       const uint32_t e8 = nan ? 0x7fu : fp4::scale_of(top);
       const float e4 = fp4::scale_value(e8);
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = e8 == 0u || nan ? 0.f : __fdiv_rn(y[e], e4);
+      for (int e = 0; e < N; ++e) y[e] = e8 == 0u || nan ? 0.f : __fdiv_rn(y[e], e4) + 0.f;      // (no code of -0 for a -0)
       if (i < n) {
         uint8_t* page = cache + ((blk * 2 + part) * Hkv + h) * bytes;
         *reinterpret_cast<uint32_t*>(page + (int64_t)off * (D / 2) + c * (N / 2)) = fp4::pack8(y);

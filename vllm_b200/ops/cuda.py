@@ -796,6 +796,51 @@ def gather_fp4(kv_cache, block_table, cu, k, v, max_tokens: int, starts, k_scale
                        v.data_ptr(), k.stride(0), v.stride(0), k.shape[0], cu.numel() - 1, max_tokens, H, D, BS, k_scale, v_scale, dtype, _st()), "gather_cache_fp4")
 
 
+_attention_fp4 = _sig("vb_attention_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _f, _f, _f,
+                      _i, _vp)
+_attention_fp4_plan = _sig("vb_attention_fp4_plan", _i, _i, _i, ctypes.POINTER(_i), ctypes.POINTER(_i), ctypes.POINTER(_i))
+FP4_HEADS = (32, 64, 80, 96, 128, 192, 256)
+FP4_EXTRA = 6                                # tiles that a row counts for beside its own, as its end costs about as much
+
+
+@functools.lru_cache(maxsize=None)
+def fp4_plan(device: int, D: int, rows: int, parts: int) -> tuple[int, int, int]:
+    """(columns of a row of the schedule, CTAs of an SM, clusters of ``parts`` CTAs that the device runs at a time) of requests with up to ``rows`` query rows."""
+    cols, ctas, clusters = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    _check(_attention_fp4_plan(D, rows, parts, ctypes.byref(cols), ctypes.byref(ctas), ctypes.byref(clusters)), "attention_fp4_plan", 0)
+    return cols.value, ctas.value, clusters.value
+
+
+def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
+    """CTAs of a cluster that has a row of the schedule, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel."""
+    if tiles > 64 or rows > 512:
+        return 0
+    parts = 8 if tiles > 8 else 4 if tiles > 4 else 2
+    return parts if rows <= fp4_plan(_device(), D, min(query_rows, 9), parts)[2] else 0
+
+
+def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
+    """Attention of the requests with at most ``few`` new tokens, straight from the cache; rows of the others are not touched."""
+    (_, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
+    bt, B, sms = md.block_table, md.num_reqs, num_sms()
+    max_rows = max(1, min(bt.shape[1] * BS, md.max_seq_len))
+    query_rows, tiles = few * (Hq // H), -(-max_rows // 64)
+    cols, ctas, _ = fp4_plan(_device(), D, min(query_rows, 9), 0)
+    chunks = -(-query_rows // cols)
+    group = min(512, 65535 // (H * chunks))
+    group = -(-B // -(-B // group))
+    parts = fp4_parts(B * H * chunks, tiles, D, query_rows) if group >= B else 0
+    ctas, rows, ws = ctas * sms, group * H * chunks, None
+    if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
+        ws = torch.empty((rows + ctas) * cols * (D + 2) + 2 * rows, dtype=torch.float32, device=q.device)
+    _check(_attention_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), None if md.decode_only else md.query_start_loc.data_ptr(),
+                          out.data_ptr(), _p(lse), _p(sinks), _p(ws), B, Hq, H, D, BS, max_rows, few, q.stride(0), out.stride(0), bt.stride(0), ctas, FP4_EXTRA, parts, group,
+                          window or 0, scale, soft_cap, out_scale, _DT[q.dtype], _st()), "attention_fp4", 1 if parts else 2 * -(-B // group))
+
+
+FP4_FEW_ROWS = 64                            # query rows (new tokens x query heads of a kv head) of requests that are attended straight from the cache
+
+
 # of 16-bit pages that a prompt's cache is read back to at a time: requests that want more are taken in several goes
 FP4_PAGES_BYTES = 1 << 30
 
@@ -804,13 +849,13 @@ def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[i
     """Runs of requests whose 16-bit pages fit into the workspace: (first, behind the last, pages of all, pages of the longest).  Lengths are those that the step
     has on the host; without them every request counts with ``most`` pages."""
     B = md.num_reqs
-    need = [most] * B
+    need = [max(most, 1)] * B
     lens = getattr(md, "host_lens", None)
     if lens is not None:
         cu, sl = lens
-        need = [0 if not md.decode_only and cu[b + 1] - cu[b] <= few else min(-(-int(sl[b]) // PS), most) for b in range(B)]
+        need = [0 if not md.decode_only and cu[b + 1] - cu[b] <= few else max(min(-(-int(sl[b]) // PS), most), 1) for b in range(B)]
     elif md.seq_lens_cpu is not None:
-        need = [min(-(-n // PS), most) for n in md.seq_lens_cpu[:B].tolist()]
+        need = [max(min(-(-n // PS), most), 1) for n in md.seq_lens_cpu[:B].tolist()]
     runs, first, total = [], 0, 0
     for b, n in enumerate(need):
         if total and (total + n) * page_bytes > FP4_PAGES_BYTES:
@@ -832,14 +877,14 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
     most = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS)
     for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * D):
         n = b1 - b0
-        if n == 0 or (total == 0 and few >= 0):
+        if total == 0:                       # (none of them has more than `few`)
             continue
-        pages = torch.empty((max(total, 1), 2, H, PS, D), dtype=q.dtype, device=q.device)
-        table, lens = sl.new_empty((n, max(longest, 1))), sl.new_empty(n)
+        pages = torch.empty((total, 2, H, PS, D), dtype=q.dtype, device=q.device)
+        table, lens = sl.new_empty((n, longest)), sl.new_empty(n)
         _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt[b0:].data_ptr(), bt.stride(0), bt.shape[1], sl[b0:].data_ptr(), None if qsl is None else qsl[b0:].data_ptr(), few,
                           pages.data_ptr(), pages.shape[0], PS, int(vt), table.data_ptr(), table.shape[1], lens.data_ptr(), n, H, D, BS, _DT[q.dtype], _st()), "pages_fp4")
         part = copy.copy(md)
-        part.num_reqs, part.block_table, part.seq_lens, part.max_seq_len, part.kv_vt, part.flat, part.cascade = n, table, lens, max(longest, 1) * PS, vt, False, None
+        part.num_reqs, part.block_table, part.seq_lens, part.max_seq_len, part.kv_vt, part.flat, part.cascade = n, table, lens, longest * PS, vt, False, None
         if md.decode_only:
             rows = slice(b0, b1)
             part.query_start_loc = None if md.query_start_loc is None else md.query_start_loc[:n + 1]
@@ -874,8 +919,15 @@ def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causa
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if T > used and out is None:             # (padding rows are written by no CTA: keep them finite)
         to[used:].zero_()
-    if B:
-        _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, -1)
+    if sinks is not None:
+        sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+    few, longest, G = 0, 1 if md.decode_only else md.max_query_len, Hq // kv_cache.shape[2]
+    if D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant():
+        few = min(longest, max(1, FP4_FEW_ROWS // G))
+    if B and few < longest:
+        _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few)
+    if B and few:
+        _fp4_few(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
     if out is not None and to is not out:
         out[:used] = to[:used]
         to = out
