@@ -7,7 +7,7 @@
 // busy as many equal ones; a row that one CTA has is finished there, one that several have is joined by a second kernel.  Where rows are few and short a cluster
 // has a row, and the parts meet in shared memory.
 //
-// A warp takes every fourth strip of 16 keys; codes and scales of a strip come by asynchronous copies of the warp's own, STAGES of them on their way across the
+// A warp takes every fourth strip of 32 keys; codes and scales of a strip come by asynchronous copies of the warp's own, the next strips on their way across the
 // borders of rows.  S^T = K Q^T (m16n8k16: keys are rows, query rows columns), an own running maximum, O^T += V^T P^T.
 //
 // Codes become fp16 in registers (one conversion for two of them, one multiplication by their scale: exact, fp4.cuh), in the order in which the matrix
@@ -21,12 +21,15 @@
 #include "device_once.h"
 #include "fp4.cuh"
 
+#include <type_traits>
+
 namespace afp4 {
 
-constexpr int TILE = 64, STRIP = 16, WARPS = 4, THREADS = WARPS * 32;
-constexpr int MAX_REQUESTS = 512;            // of a launch: their first tiles lie in shared memory
+constexpr int TILE = 64, STRIP = 32, WARPS = 4, THREADS = WARPS * 32;
+constexpr int MAX_REQUESTS = 512;            // of a launch: their first tiles and lengths lie in shared memory
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float SHIFT = 7.f;                 // the reference of a row's weights is its largest score less SHIFT, or up to 8 below that
+constexpr float NONE = -3e38f;               // the reference of a row that has seen no key: any score is far above it
 
 struct Params {
   const void* q;
@@ -178,32 +181,33 @@ template <int N> struct Bytes {
 template <int D_> struct Form {
   static constexpr int D = D_, KD = D / 16;
   static constexpr int CODES = STRIP * D / 2, SIDE = CODES + STRIP * D / 16, STAGE = 2 * SIDE;       // bytes of a strip's keys, values behind them
-  static constexpr int STAGES = D <= 64 ? 6 : D <= 128 ? 4 : 3;
+  static constexpr int STAGES = D <= 64 ? 3 : 2;
   static constexpr int RING = WARPS * STAGES * STAGE;
-  static constexpr int REGS = KD * 4 + 4;                                  // of eight query rows: output, maxima, sums
-  static constexpr int EXCH = WARPS / 2 * REGS * 128;
-  static constexpr int LISTS = (MAX_REQUESTS + 1 + 2 * MAX_REQUESTS + 32 + 3) / 4 * 16;
+  static constexpr int EXCH = WARPS * KD * 4 * 128, MAXIMA = WARPS * 16 * 8;   // the warps' outputs of eight query rows; maxima and sums of 16
+  static constexpr int lists(int B) { return ((3 * B + 2 + WARPS) * 4 + 15) & ~15; }                 // first tiles, lengths and new tokens of B requests
   static constexpr int PART = 16 * (D + 2 + 9) * 4;                        // of a CTA of a cluster, instead of the lists
-  static constexpr int SMEM = RING + EXCH + (LISTS > PART ? LISTS : PART);
+  static constexpr int FIXED = RING + EXCH + MAXIMA;
   // a lane's D / 4 values of a key lie in GK groups, its D / 8 values of a value row in GV
   static constexpr int SK = D / 4, SV = D / 8;
   static constexpr int GK = SK % 16 == 0 ? SK / 16 : 16 % SK == 0 ? 1 : 2, GV = SV % 16 == 0 ? SV / 16 : 16 % SV == 0 ? 1 : 2;
   static constexpr bool STRAIGHT_K = SK % 16 == 0 || 16 % SK == 0, STRAIGHT_V = SV % 16 == 0 || 16 % SV == 0;
 };
 
-template <int D, int NT, int CTAS>
+// BF16: type of queries and outputs, or fp16
+template <int D, int NT, bool BF16, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p) {
   using F = Form<D>;
   constexpr int KD = F::KD, STAGES = F::STAGES, COLS = 8 * NT, PD = D + 2;
   extern __shared__ __align__(128) unsigned char smem[];
   float* exch = reinterpret_cast<float*>(smem + F::RING);
-  int* first = reinterpret_cast<int*>(smem + F::RING + F::EXCH);
-  int2* reqs = reinterpret_cast<int2*>(first + MAX_REQUESTS + 2);
-  int* warp_sums = reinterpret_cast<int*>(reqs + MAX_REQUESTS);
-  float* part_s = reinterpret_cast<float*>(first);         // cluster: the CTA's part
-  float* factor_s = part_s + COLS * PD;                    // ... and factors of the parts
+  float2* maxima = reinterpret_cast<float2*>(smem + F::RING + F::EXCH);    // [warp][column]
+  int2* reqs = reinterpret_cast<int2*>(smem + F::FIXED);
+  int* first = reinterpret_cast<int*>(reqs + p.B);
+  int* warp_sums = first + p.B + 1;
+  float* part_s = reinterpret_cast<float*>(smem + F::FIXED);               // cluster: the CTA's part
+  float* factor_s = part_s + COLS * PD;                                    // ... and factors of the parts
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool fused = p.parts > 0;
+  const bool fused = p.parts > 0, capped = p.ku != 0.f;
   pdl_wait();
   pdl_trigger();             // (here: the joining kernel may read the lengths as soon as it starts)
   int t0, t1, per;
@@ -234,53 +238,79 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
 
   unsigned char* ring = smem + warp * (STAGES * F::STAGE);
   const int64_t page = fp4::page_bytes(p.BS, D);
-  // The warp's strips: flat numbers 4 t0 + warp + i WARPS.  Where they lie is looked up for 32 of them at once, a lane each.
-  const int s_end = t1 * 4;
-  int64_t my_page = 0;                                                      // of the lane's strip: place of the page, token in it (-1: nothing to fetch)
-  int my_off = -1, fetched = 0;
+  // The warp's strips: flat numbers PER_TILE t0 + warp + i WARPS.  Where their halves lie is looked up for 32 strips at once, a lane each: number of the page of a head
+  // (below 2^31: pages have 144 bytes or more) and row in it (-1: nothing to fetch).  Where pages are multiples of a strip the halves lie together.
+  constexpr int PER_TILE = TILE / STRIP;
+  const int s_end = t1 * PER_TILE;
+  const bool together = p.BS % STRIP == 0;
+  uint32_t my_page[2] = {0u, 0u};
+  int my_off[2] = {-1, -1}, fetched = 0;
+  const int64_t to_v = p.Hkv * page, codes = (int64_t)p.BS * (D / 2);
+  auto copy_codes = [&](uint32_t to, const uint8_t* from, auto pieces) {   // pieces of 16 bytes
+    constexpr int N = decltype(pieces)::value;
+#pragma unroll
+    for (int i = 0; i < (N + 31) / 32; ++i) {
+      const int j = i * 32 + lane;
+      if (N % 32 == 0 || j < N) {
+        const int d = D == 128 ? (j & ~3) | ((j & 3) ^ (j >> 3 & 2)) : j;  // (D = 128: pieces of a row change places so that lanes of a load meet in no bank)
+        cp_async16(to + d * 16, from + j * 16);
+        cp_async16(to + F::SIDE + d * 16, from + to_v + j * 16);
+      }
+    }
+  };
+  auto copy_scales = [&](uint32_t to, const uint8_t* from, auto pieces) {  // of keys, then of values
+    constexpr int N = decltype(pieces)::value;
+#pragma unroll
+    for (int i = 0; i < (2 * N + 31) / 32; ++i) {
+      const int j = i * 32 + lane, side = j >= N, jj = j - side * N;
+      if (2 * N % 32 == 0 || j < 2 * N) cp_async16(to + F::CODES + side * F::SIDE + jj * 16, from + codes + (side ? to_v : 0) + jj * 16);
+    }
+  };
   auto fetch = [&](int stage) {
     if ((fetched & 31) == 0) {
-      const int s = t0 * 4 + warp + (fetched + lane) * WARPS;
-      my_off = -1;
+      const int s = t0 * PER_TILE + warp + (fetched + lane) * WARPS;
+      my_off[0] = my_off[1] = -1;
       if (s < s_end) {
         Row r = row;
         Request q = req;
         if (!fused) {
-          row_at(p, COLS, first, reqs, s >> 2, r);
+          row_at(p, COLS, first, reqs, s / PER_TILE, r);
           q = Request{reqs[r.b].x, reqs[r.b].y};
         }
-        const int tok = ((s >> 2) - r.begin + q.first_tile(p)) * TILE + (s & 3) * STRIP;
-        if (tok < q.n) {
-          int64_t blk = p.block_table[r.b * p.bt_stride + tok / p.BS];
-          if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
-          my_page = (blk * 2 * p.Hkv + r.h) * page;
-          my_off = tok % p.BS;
+        const int tok = (s / PER_TILE - r.begin + q.first_tile(p)) * TILE + s % PER_TILE * STRIP;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int at = tok + half * 16;
+          if (at < q.n) {
+            int64_t blk = p.block_table[r.b * p.bt_stride + at / p.BS];
+            if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;           // (a table may not say that; nothing is read outside the cache)
+            my_page[half] = (uint32_t)(blk * 2 * p.Hkv + r.h);
+            my_off[half] = at % p.BS;
+          }
         }
       }
     }
-    const int off = __shfl_sync(0xffffffffu, my_off, fetched & 31);
-    const int64_t at = __shfl_sync(0xffffffffu, my_page, fetched & 31);
+    const uint32_t to = smem_u32(ring + stage * F::STAGE);
+    const int off = __shfl_sync(0xffffffffu, my_off[0], fetched & 31);
+    const uint8_t* base = p.cache + __shfl_sync(0xffffffffu, my_page[0], fetched & 31) * (uint64_t)(uint32_t)page;
+    if (together) {                          // (rows of the page behind the last one come along)
+      if (off >= 0) {
+        copy_codes(to, base + off * (D / 2), std::integral_constant<int, D>{});
+        copy_scales(to, base + off * (D / 16), std::integral_constant<int, D / 8>{});
+      }
+    } else {
+      const int off2 = __shfl_sync(0xffffffffu, my_off[1], fetched & 31);
+      const uint8_t* base2 = p.cache + __shfl_sync(0xffffffffu, my_page[1], fetched & 31) * (uint64_t)(uint32_t)page;
+      if (off >= 0) {
+        copy_codes(to, base + off * (D / 2), std::integral_constant<int, D / 2>{});
+        copy_scales(to, base + off * (D / 16), std::integral_constant<int, D / 16>{});
+      }
+      if (off2 >= 0) {
+        copy_codes(to + 8 * D, base2 + off2 * (D / 2), std::integral_constant<int, D / 2>{});
+        copy_scales(to + D, base2 + off2 * (D / 16), std::integral_constant<int, D / 16>{});
+      }
+    }
     ++fetched;
-    if (off >= 0) {
-      const uint8_t* k = p.cache + at + off * (D / 2);
-      const uint8_t* ks = p.cache + at + (int64_t)p.BS * (D / 2) + off * (D / 16);
-      const int64_t to_v = p.Hkv * page;
-      const uint32_t to = smem_u32(ring + stage * F::STAGE);
-#pragma unroll
-      for (int i = 0; i < (D / 2 + 31) / 32; ++i) {
-        const int j = i * 32 + lane;
-        if (D / 2 % 32 == 0 || j < D / 2) {
-          const int d = D == 128 ? (j & ~3) | ((j & 3) ^ (j >> 3 & 2)) : j;  // (D = 128: pieces of a row change places so that lanes of a load meet in no bank)
-          cp_async16(to + d * 16, k + j * 16);
-          cp_async16(to + F::SIDE + d * 16, k + to_v + j * 16);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < (D / 8 + 31) / 32; ++i) {
-        const int j = i * 32 + lane, side = j >= D / 16;
-        if (j < D / 8) cp_async16(to + side * F::SIDE + F::CODES + (j - side * (D / 16)) * 16, ks + (side ? to_v : 0) + (j - side * (D / 16)) * 16);
-      }
-    }
     cp_async_commit();
   };
 #pragma unroll
@@ -290,9 +320,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
   // rows of a product in front of slots of the next: row r is key r ^ (r >> 1 & 1), so that the keys of neighbouring lanes lie in both halves of the banks
   const int key0 = r0 ^ (r0 >> 1 & 1);
   const int vkey[4] = {q0 + (t4 & 1), q0 + 1 - (t4 & 1), q0 + 8 + (t4 & 1), q0 + 9 - (t4 & 1)};
-  int s = t0 * 4 + warp, turn = 0;
+  int s = t0 * PER_TILE + warp, turn = 0;
   uint32_t q[KD][NT][2];
-  float undo[NT][2];
+  float mult[NT][2];                                                        // of a column's sums: to powers of two, or to the cap
   int hi[NT][2];                                                            // last key that a column sees
   auto load_q = [&]() {
     const int first_q = p.qsl ? p.qsl[row.b] : row.b;
@@ -301,13 +331,21 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       const int r = row.c * COLS + nt * 8 + r0, tok = r / p.G;
       const bool there = tok < req.t;
       const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(first_q + tok) * p.q_stride + (int64_t)(row.h * p.G + r - tok * p.G) * D + t4 * (D / 4);
+      if constexpr (D % 32 == 0) {
 #pragma unroll
-      for (int k = 0; k < KD; ++k) {
-        const uint2 x = there ? *reinterpret_cast<const uint2*>(qp + k * 4) : make_uint2(0u, 0u);
-        q[k][nt][0] = x.x; q[k][nt][1] = x.y;
+        for (int k = 0; k < KD; k += 2) {
+          const uint4 x = there ? *reinterpret_cast<const uint4*>(qp + k * 4) : make_uint4(0u, 0u, 0u, 0u);
+          q[k][nt][0] = x.x; q[k][nt][1] = x.y; q[k + 1][nt][0] = x.z; q[k + 1][nt][1] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {
+          const uint2 x = there ? *reinterpret_cast<const uint2*>(qp + k * 4) : make_uint2(0u, 0u);
+          q[k][nt][0] = x.x; q[k][nt][1] = x.y;
+        }
       }
       float mine = 1.f;
-      if (p.bf16) {
+      if (BF16) {
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < KD; ++k)
@@ -329,17 +367,19 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
             q[k][nt][j] = pack2<__half>(x.x * f, x.y * f);
           }
       }
+      mine *= capped ? p.ku : p.scale_log2;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        undo[nt][u] = __shfl_sync(0xffffffffu, mine, (q0 + u) * 4);
+        mult[nt][u] = __shfl_sync(0xffffffffu, mine, (q0 + u) * 4);
         hi[nt][u] = req.n - req.t + (row.c * COLS + nt * 8 + q0 + u) / p.G;
       }
     }
   };
   load_q();
   while (true) {
-    const int seg_end = min(row.end, t1) * 4, n = req.n, tile0 = req.first_tile(p), low = req.first_key(p);
+    const int seg_end = min(row.end, t1) * PER_TILE, n = req.n, tile0 = req.first_tile(p), low = req.first_key(p);
     float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
+    bool huge = false;                       // products of scores and their factor have to be rounded before a reference is taken off: its rounding is above 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -347,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) { m_run[nt][u] = -INFINITY; l_run[nt][u] = 0.f; }
+      for (int u = 0; u < 2; ++u) { m_run[nt][u] = NONE; l_run[nt][u] = 0.f; }
     }
     for (; s < seg_end; s += WARPS) {
       const int stage = turn;
@@ -355,29 +395,40 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       cp_async_wait<STAGES - 2>();
       __syncwarp();
       fetch(stage == 0 ? STAGES - 1 : stage - 1);                          // into the stage of the strip before, which the whole warp has read
-      const int tok = ((s >> 2) - row.begin + tile0) * TILE + (s & 3) * STRIP;
+      const int tok = (s / PER_TILE - row.begin + tile0) * TILE + s % PER_TILE * STRIP;
       if (tok >= n) continue;
       const unsigned char* ks = ring + stage * F::STAGE;
       const unsigned char* vs = ks + F::SIDE;
-      // ---- S^T = K Q^T
-      float sc[NT][4], sd[NT][4];
+      // ---- S^T = K Q^T, 16 keys at a time
+      float sc[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int m = 0; m < 2; ++m) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = sd[nt][i] = 0.f;
-      {
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[m][nt][i] = 0.f;
         Bytes<D / 8> c0, c1;
-        const int piece = D == 128 ? (t4 ^ (key0 >> 1 & 2)) * 16 : t4 * (D / 8);
-        c0.load(ks + key0 * (D / 2) + piece);
-        c1.load(ks + (key0 + 8) * (D / 2) + piece);
+        const int key = m * 16 + key0, piece = D == 128 ? (t4 ^ (key0 >> 1 & 2)) * 16 : t4 * (D / 8);
+        c0.load(ks + key * (D / 2) + piece);
+        c1.load(ks + (key + 8) * (D / 2) + piece);
         uint32_t s0[F::GK], s1[F::GK];
         const int g0 = t4 * F::SK / 16, cross = (16 - t4 * F::SK % 16) / 4;          // (not STRAIGHT_K: the lane's values from the cross-th four on are the next group's)
+        const unsigned char* sp = ks + F::CODES + key * (D / 16);
+        if constexpr (F::GK % 2 == 0 && F::STRAIGHT_K && D / 16 % 2 == 0) {           // two scales of a key at once
 #pragma unroll
-        for (int g = 0; g < F::GK; ++g) {
-          const unsigned char* at = ks + F::CODES + key0 * (D / 16) + min(g0 + g, D / 16 - 1);
-          const uint32_t two = fp4::scales2(at[0] | (uint32_t)at[8 * (D / 16)] << 8);
-          s0[g] = fp4::low2(two);
-          s1[g] = fp4::high2(two);
+          for (int g = 0; g < F::GK; g += 2) {
+            const uint32_t x = fp4::scales2(*reinterpret_cast<const uint16_t*>(sp + g0 + g)), y = fp4::scales2(*reinterpret_cast<const uint16_t*>(sp + 8 * (D / 16) + g0 + g));
+            s0[g] = fp4::low2(x); s0[g + 1] = fp4::high2(x);
+            s1[g] = fp4::low2(y); s1[g + 1] = fp4::high2(y);
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < F::GK; ++g) {
+            const unsigned char* at = sp + min(g0 + g, D / 16 - 1);
+            const uint32_t two = fp4::scales2(at[0] | (uint32_t)at[8 * (D / 16)] << 8);
+            s0[g] = fp4::low2(two);
+            s1[g] = fp4::high2(two);
+          }
         }
 #pragma unroll
         for (int w = 0; w < (KD + 1) / 2; ++w) {                                     // a word: two steps of the product
@@ -392,79 +443,92 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
               const uint32_t f1 = F::STRAIGHT_K ? s1[F::GK > 1 ? k / 4 : 0] : k < cross ? s1[0] : s1[F::GK - 1];
               const uint32_t a0 = fp4::mul2(a[2 * half], f0), a2 = fp4::mul2(a[2 * half + 1], f0), a1 = fp4::mul2(b[2 * half], f1), a3 = fp4::mul2(b[2 * half + 1], f1);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816(k & 1 ? sd[nt] : sc[nt], a0, a1, a2, a3, q[k][nt][0], q[k][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma16816(sc[m][nt], a0, a1, a2, a3, q[k][nt][0], q[k][nt][1]);
             }
           }
         }
       }
       // ---- weights
       const bool cut = tok + STRIP > n - req.t + 1 || (p.window > 0 && tok < n - p.window);
-      uint32_t ph[NT][2], pl[NT][2];
+      uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float mx[2], alpha[2];
+        float by[2] = {mult[nt][0], mult[nt][1]};
+        if (capped || cut || huge) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = (sc[nt][i] + sd[nt][i]) * undo[nt][i & 1];
-          float y = p.ku > 0.f || p.ku < 0.f ? prompt::cap_any(x * p.ku, p.c2) : x * p.scale_log2;
-          if (cut) {
-            const int key = tok + key0 + (i >> 1) * 8, last = hi[nt][i & 1];
-            if (key > last || (p.window > 0 && key <= last - p.window)) y = -INFINITY;
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = sc[m][nt][i] * mult[nt][i & 1];
+              if (capped) x = prompt::cap_any(x, p.c2);
+              const int key = tok + m * 16 + key0 + (i >> 1) * 8, last = hi[nt][i & 1];
+              sc[m][nt][i] = key > last || (p.window > 0 && key <= last - p.window) ? -INFINITY : x;
+            }
+          by[0] = by[1] = 1.f;
+        }
+        float y[2][4], most[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[m][i] = fmaf(sc[m][nt][i], by[i & 1], -m_run[nt][i & 1]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) most[u] = fmaxf(fmaxf(y[0][u], y[0][2 + u]), fmaxf(y[1][u], y[1][2 + u]));
+        // the old reference stays where no weight is above 2^(8 + SHIFT)
+        if (__any_sync(0xffffffffu, fmaxf(most[0], most[1]) > 8.f + SHIFT)) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float mx = fmaxf(fmaxf(sc[0][nt][u], sc[0][nt][2 + u]), fmaxf(sc[1][nt][u], sc[1][nt][2 + u])) * by[u];
+            if (by[u] < 0.f) mx = fminf(fminf(sc[0][nt][u], sc[0][nt][2 + u]), fminf(sc[1][nt][u], sc[1][nt][2 + u])) * by[u];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float was = m_run[nt][u], at = fmaxf(mx - SHIFT, NONE);
+            const bool up = at > was + 8.f;
+            const float alpha = up ? ex2(was - at) : 1.f;
+            m_run[nt][u] = up ? at : was;
+            l_run[nt][u] *= alpha;
+#pragma unroll
+            for (int i = 0; i < KD; ++i) { o[i][nt][u] *= alpha; o[i][nt][2 + u] *= alpha; }
           }
-          sc[nt][i] = y;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[m][i] = __fsub_rn(__fmul_rn(sc[m][nt][i], by[i & 1]), m_run[nt][i & 1]);
+          huge |= __any_sync(0xffffffffu, (m_run[nt][0] > NONE && fabsf(m_run[nt][0]) > 0x1p20f) || (m_run[nt][1] > NONE && fabsf(m_run[nt][1]) > 0x1p20f));
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) mx[u] = fmaxf(sc[nt][u], sc[nt][2 + u]);
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], x));
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float was = m_run[nt][u], at = mx[u] - SHIFT;
-          const bool up = at > was + 8.f || (was == -INFINITY && at > -INFINITY);            // else the old reference stays
-          alpha[u] = up && was != -INFINITY ? ex2(was - at) : 1.f;
-          m_run[nt][u] = up ? at : was;
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int i = 0; i < KD; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][nt][j] *= alpha[j & 1];
-          l_run[nt][0] *= alpha[0]; l_run[nt][1] *= alpha[1];
-        }
-        const float ref[2] = {m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float x = ex2(sc[nt][2 * t] - ref[0]), y = ex2(sc[nt][2 * t + 1] - ref[1]);
-          l_run[nt][0] += x; l_run[nt][1] += y;
-          const uint32_t h = pack2<__half>(x, y);
-          ph[nt][t] = turn8(h);
-          if (!p.bf16) {
-            const float2 back = unpack2<__half>(h);
-            pl[nt][t] = turn8(pack2<__half>(x - back.x, y - back.y));
+          for (int t = 0; t < 2; ++t) {
+            const float a = ex2(y[m][2 * t]), b = ex2(y[m][2 * t + 1]);
+            l_run[nt][0] += a; l_run[nt][1] += b;
+            const uint32_t h = pack2<__half>(a, b);
+            ph[m][nt][t] = turn8(h);
+            if (!BF16) {
+              const float2 back = unpack2<__half>(h);
+              pl[m][nt][t] = turn8(pack2<__half>(a - back.x, b - back.y));
+            }
           }
-        }
       }
-      // ---- O^T += V^T P^T
-      {
+      // ---- O^T += V^T P^T, 16 keys at a time
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
         Bytes<D / 16> c[4];
         uint32_t sa[F::GV], sb[F::GV];                                               // scales of the keys of slots (0, 1) and (8, 9)
         const int g0 = r0 * F::SV / 16, cross = (16 - r0 * F::SV % 16) / 2;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int at = r0 * (D / 16);
-          c[j].load(vs + vkey[j] * (D / 2) + (D == 128 ? (((at >> 4) ^ (vkey[j] >> 1 & 2)) << 4 | (at & 15)) : at));
+          c[j].load(vs + (m * 16 + vkey[j]) * (D / 2) + (D == 128 ? (((at >> 4) ^ (vkey[j] >> 1 & 2)) << 4 | (at & 15)) : at));
         }
 #pragma unroll
         for (int g = 0; g < F::GV; ++g) {
-          const unsigned char* at = vs + F::CODES + min(g0 + g, D / 16 - 1);
+          const unsigned char* at = vs + F::CODES + m * D + min(g0 + g, D / 16 - 1);
           uint32_t x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = at[vkey[j] * (D / 16)];
           if (tok + STRIP > n || tok < low)      // rows of nobody, or that no query row sees, may hold what a weight of 0 does not cancel
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = tok + vkey[j] < n && tok + vkey[j] >= low ? x[j] : 0u;
+            for (int j = 0; j < 4; ++j) x[j] = tok + m * 16 + vkey[j] < n && tok + m * 16 + vkey[j] >= low ? x[j] : 0u;
           sa[g] = fp4::scales2(x[0] | x[1] << 8);
           sb[g] = fp4::scales2(x[2] | x[3] << 8);
         }
@@ -486,15 +550,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
               const uint32_t a0 = fp4::mul2(e01[j], f0), a1 = fp4::mul2(o01[j], f0), a2 = fp4::mul2(e23[j], f1), a3 = fp4::mul2(o23[j], f1);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816(o[i][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                if (!p.bf16) mma16816(o[i][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                mma16816(o[i][nt], a0, a1, a2, a3, ph[m][nt][0], ph[m][nt][1]);
+                if (!BF16) mma16816(o[i][nt], a0, a1, a2, a3, pl[m][nt][0], pl[m][nt][1]);
               }
             }
           }
         }
       }
     }
-    // ---- the warps' results of the segment: lanes hold the same places in every warp, so the upper half of the warps hands its registers over
+    // ---- the warps' results of the segment meet in shared memory
     const int index = (row.b * p.Hkv + row.h) * p.chunks + row.c, live = row.begin + req.tiles(p);       // (behind its tiles a row has further slots)
     const bool empty = !fused && max(row.begin, t0) >= live;
     const int n_ctas = fused ? 1 : (live - 1) / per - row.begin / per + 1;
@@ -508,68 +572,83 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       req = Request{reqs[row.b].x, reqs[row.b].y};
       load_q();
     }
-    if (!empty)
+    if (!empty) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
-#pragma unroll
-      for (int half = WARPS / 2; half > 0; half >>= 1) {
-        __syncthreads();
-        if (warp >= half && warp < 2 * half) {
-          float* to = exch + (warp - half) * F::REGS * 32 + lane;
-#pragma unroll
-          for (int i = 0; i < KD; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to[(i * 4 + j) * 32] = o[i][nt][j];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) { to[(KD * 4 + u) * 32] = m_run[nt][u]; to[(KD * 4 + 2 + u) * 32] = l_run[nt][u]; }
-        }
-        __syncthreads();
-        if (warp < half) {
-          const float* from = exch + warp * F::REGS * 32 + lane;
-          float fa[2], fb[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float mb = from[(KD * 4 + u) * 32], top = fmaxf(m_run[nt][u], mb);
-            fa[u] = m_run[nt][u] == -INFINITY ? 0.f : ex2(m_run[nt][u] - top);
-            fb[u] = mb == -INFINITY ? 0.f : ex2(mb - top);
-            m_run[nt][u] = top;
-            l_run[nt][u] = l_run[nt][u] * fa[u] + from[(KD * 4 + 2 + u) * 32] * fb[u];
-          }
-#pragma unroll
-          for (int i = 0; i < KD; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][nt][j] = o[i][nt][j] * fa[j & 1] + from[(i * 4 + j) * 32] * fb[j & 1];
-        }
-      }
-      if (warp == 0) {
-        const int first_q = whole && p.qsl ? p.qsl[done.b] : done.b;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int g = nt * 8 + q0 + u, r = done.c * COLS + g, tok = r / p.G;
-          if (tok >= done_req.t) continue;
-          if (whole) {                       // nobody else has keys of the row
-            const int head = done.h * p.G + r - tok * p.G;
-            const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = fmaxf(m_run[nt][u], sink), base = top == -INFINITY ? 0.f : top;
-            const float l = (m_run[nt][u] == -INFINITY ? 0.f : l_run[nt][u] * ex2(m_run[nt][u] - base)) + (p.sinks ? ex2(sink - base) : 0.f);
-            const float f = l > 0.f && m_run[nt][u] > -INFINITY ? ex2(m_run[nt][u] - base) / l * p.out_scale : 0.f;
-            uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)head * D + r0 * (D / 8));
 #pragma unroll
-            for (int i = 0; i < KD; ++i) {
-              const float x = o[i][nt][u] * f, y = o[i][nt][2 + u] * f;
-              to[i] = p.bf16 ? pack2<__nv_bfloat16>(x, y) : pack2<__half>(x, y);
+          for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
+          if (m_run[nt][u] == NONE) m_run[nt][u] = -INFINITY;
+          if (r0 == 0) maxima[warp * 16 + nt * 8 + q0 + u] = make_float2(m_run[nt][u], l_run[nt][u]);
+        }
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top[2], total[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float2 ml[WARPS];
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) ml[w] = maxima[w * 16 + nt * 8 + q0 + u];
+          top[u] = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+          total[u] = 0.f;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) total[u] += ml[w].x == -INFINITY ? 0.f : ml[w].y * ex2(ml[w].x - top[u]);
+          const float f = m_run[nt][u] == -INFINITY ? 0.f : ex2(m_run[nt][u] - top[u]);
+#pragma unroll
+          for (int i = 0; i < KD; ++i) { o[i][nt][u] *= f; o[i][nt][2 + u] *= f; }
+        }
+        float* to = exch + warp * (KD * 128) + lane;
+#pragma unroll
+        for (int i = 0; i < KD; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[(i * 4 + j) * 32] = o[i][nt][j];
+        __syncthreads();
+        // a thread: a column's values of half of a lane's dimensions
+        constexpr int HALF = (KD + 1) / 2;
+        const int u = warp & 1, i0 = warp >> 1 ? HALF : 0, g = nt * 8 + q0 + u, r = done.c * COLS + g, tok = r / p.G, d0 = r0 * (D / 8) + 2 * i0;
+        const float m = u ? top[1] : top[0], l = u ? total[1] : total[0];
+        float2 x[HALF];
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+          x[i] = make_float2(0.f, 0.f);
+          if (KD % 2 == 0 || i0 + i < KD) {
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+              const float* from = exch + w * (KD * 128) + ((i0 + i) * 4 + u) * 32 + lane;
+              x[i].x += from[0];
+              x[i].y += from[64];
             }
-            if (p.lse && r0 == 0) p.lse[(int64_t)(first_q + tok) * p.Hkv * p.G + head] = l > 0.f ? (base + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
-          } else {
-            float* to = (fused ? part_s : p.part + (int64_t)(index + blockIdx.x) * COLS * PD) + g * PD + r0 * (D / 8);
-#pragma unroll
-            for (int i = 0; i < KD; ++i) *reinterpret_cast<float2*>(to + 2 * i) = make_float2(o[i][nt][u], o[i][nt][2 + u]);
-            if (r0 == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m_run[nt][u], l_run[nt][u]);
           }
         }
+        if (tok < done_req.t) {
+          if (whole) {                       // nobody else has keys of the row
+            const int head = done.h * p.G + r - tok * p.G, first_q = p.qsl ? p.qsl[done.b] : done.b;
+            const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, most = fmaxf(m, sink), base = most == -INFINITY ? 0.f : most;
+            const float sum = (m == -INFINITY ? 0.f : l * ex2(m - base)) + (p.sinks ? ex2(sink - base) : 0.f);
+            const float f = sum == 0.f || m == -INFINITY ? 0.f : ex2(m - base) / sum * p.out_scale;
+            uint32_t y[HALF];
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) y[i] = BF16 ? pack2<__nv_bfloat16>(x[i].x * f, x[i].y * f) : pack2<__half>(x[i].x * f, x[i].y * f);
+            uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)head * D + d0;
+            if constexpr (HALF == 4 && KD == 8) {
+              *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < HALF; ++i)
+                if (KD % 2 == 0 || i0 + i < KD) reinterpret_cast<uint32_t*>(out)[i] = y[i];
+            }
+            if (p.lse && r0 == 0 && i0 == 0) p.lse[(int64_t)(first_q + tok) * p.Hkv * p.G + head] = sum > 0.f ? (base + log2f(sum)) * LN2 : sum == 0.f ? -INFINITY : sum;
+          } else {
+            float* part = (fused ? part_s : p.part + (int64_t)(index + blockIdx.x) * COLS * PD) + g * PD;
+#pragma unroll
+            for (int i = 0; i < HALF; ++i)
+              if (KD % 2 == 0 || i0 + i < KD) *reinterpret_cast<float2*>(part + d0 + 2 * i) = x[i];
+            if (r0 == 0 && i0 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+          }
+        }
+        if (NT > 1 && nt == 0) __syncthreads();          // (in front of the next row: the barrier behind the maxima)
       }
     }
     if (!more) break;
@@ -601,16 +680,16 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
         if (c < p.parts) { acc.x += x[c].x * f; acc.y += x[c].y * f; }
       }
       *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)(row.h * p.G + r - tok * p.G) * D + d) =
-          p.bf16 ? pack2<__nv_bfloat16>(acc.x, acc.y) : pack2<__half>(acc.x, acc.y);
+          BF16 ? pack2<__nv_bfloat16>(acc.x, acc.y) : pack2<__half>(acc.x, acc.y);
     }
     cluster_sync();                                      // the others may still read this CTA's part
   }
 }
 
 // Grid (columns of a row, rows): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
-constexpr int JOIN = 128, FACTORS = 1024;
+constexpr int JOIN = 128, AHEAD = 16;
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, int D) {
-  __shared__ float factor_s[FACTORS];
+  __shared__ float factor_s[JOIN];
   __shared__ float red[32];
   pdl_trigger();
   pdl_wait();
@@ -624,73 +703,96 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, in
   const int head = h * p.G + r - tok * p.G, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t step = (int64_t)cols * PD;
   const float* x = p.part + ((int64_t)(index + at.x) * cols + blockIdx.x) * PD;
-  const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
-  float m = sink;
-  for (int i = threadIdx.x; i < count; i += JOIN) m = fmaxf(m, x[i * step + D]);
-  m = warp_max(m);
-  if (lane == 0) red[w] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float top = m == -INFINITY ? 0.f : m;
-  __syncthreads();
-  float l = 0.f;
-  for (int i = threadIdx.x; i < count; i += JOIN) {
-    const float2 ml = make_float2(x[i * step + D], x[i * step + D + 1]);
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-    if (i < FACTORS) factor_s[i] = f;
-    l += ml.y * f;
-  }
-  l = block_sum(l, red) + (p.sinks ? ex2(sink - top) : 0.f);          // (a block barrier: the factors are there)
   const int64_t token = (p.qsl ? p.qsl[b] : b) + tok;
-  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = l > 0.f ? (top + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
-  const float f = l == 0.f ? 0.f : p.out_scale / l;
-  for (int d = threadIdx.x; d < D; d += JOIN) {
-    float acc = 0.f;
-    int i = 0;
-    for (; i + 8 <= min(count, FACTORS); i += 8) {
-      float y[8];
+  const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
+  // a thread: two dimensions of every second part (heads above 128: of every part); the first parts' are read before their factors are known
+  const int pairs = D / 2, lanes = JOIN / pairs < 1 ? 1 : JOIN / pairs, mine = threadIdx.x / pairs;      // parts that a block takes at once
+  const float2* out = reinterpret_cast<const float2*>(x) + threadIdx.x % pairs;
+  const bool has = mine < lanes;
+  float2 ahead[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = x[(i + j) * step + d];
+  for (int i = 0; i < AHEAD; ++i) {
+    const int part = i * lanes + mine;
+    ahead[i] = has && part < count ? out[part * (step / 2)] : make_float2(0.f, 0.f);
+  }
+  float top = -INFINITY, total = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+  for (int from = 0; from == 0 || from < count; from += JOIN) {                      // (nearly always one round)
+    const int part = from + threadIdx.x;
+    const float2 ml = part < count ? *reinterpret_cast<const float2*>(x + part * step + D) : make_float2(-INFINITY, 0.f);
+    float m = warp_max(ml.x);
+    if (lane == 0) red[w] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float was = top;
+    top = fmaxf(fmaxf(top, m), from == 0 ? sink : -INFINITY);
+    const float base = top == -INFINITY ? 0.f : top, back = was == -INFINITY ? 0.f : ex2(was - base), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base);
+    factor_s[threadIdx.x] = f;
+    __syncthreads();                                                                 // (factors are there, and the maxima have been read)
+    total = total * back + block_sum(ml.x == -INFINITY ? 0.f : ml.y * f, red) + (from == 0 && p.sinks ? ex2(sink - base) : 0.f);
+    acc.x *= back; acc.y *= back;
+    if (has) {
+      int i = mine;
+      if (from == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc += y[j] * factor_s[i + j];
+        for (int j = 0; j < AHEAD; ++j) {
+          const float g = j * lanes + mine < min(count, JOIN) ? factor_s[j * lanes + mine] : 0.f;
+          if (j * lanes + mine < min(count, JOIN)) { acc.x += ahead[j].x * g; acc.y += ahead[j].y * g; }
+        }
+        i += AHEAD * lanes;
+      }
+      for (; i < JOIN && from + i < count; i += lanes) {
+        const float2 y = out[(from + i) * (step / 2)];
+        acc.x += y.x * factor_s[i]; acc.y += y.y * factor_s[i];
+      }
     }
-    for (; i < count; ++i) acc += x[i * step + d] * (i < FACTORS ? factor_s[i] : x[i * step + D] == -INFINITY ? 0.f : ex2(x[i * step + D] - top));
-    uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D + d;
-    if (p.bf16) *reinterpret_cast<__nv_bfloat16*>(to) = from_f32<__nv_bfloat16>(acc * f);
-    else *reinterpret_cast<__half*>(to) = from_f32<__half>(acc * f);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = total > 0.f ? ((top == -INFINITY ? 0.f : top) + log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
+  __shared__ float2 sums[JOIN];
+  sums[threadIdx.x] = acc;
+  __syncthreads();
+  const float f = total == 0.f ? 0.f : p.out_scale / total;
+  for (int i = threadIdx.x; i < pairs; i += JOIN) {
+    float2 y = sums[i];
+    for (int j = 1; j < lanes; ++j) { y.x += sums[j * pairs + i].x; y.y += sums[j * pairs + i].y; }
+    uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D + 2 * i;
+    *reinterpret_cast<uint32_t*>(to) = p.bf16 ? pack2<__nv_bfloat16>(y.x * f, y.y * f) : pack2<__half>(y.x * f, y.y * f);
   }
 }
 
 constexpr int ctas_of(int D, int NT) { return D <= 128 ? (NT == 1 ? 4 : 3) : 2; }            // of an SM
 
 // `clusters`: nothing is launched, the clusters of a row that the device runs at a time are counted.
-template <int D, int NT>
+template <int D, int NT, bool BF16>
 static int launch(const Params& p, cudaStream_t st, int* clusters, int* ctas) {
   using F = Form<D>;
-  auto k = attention_kernel<D, NT, ctas_of(D, NT)>;
+  auto k = attention_kernel<D, NT, BF16, ctas_of(D, NT)>;
   static std::atomic<uint64_t> devices{0};
-  if (vb_allow_smem(reinterpret_cast<const void*>(k), F::SMEM, devices) != cudaSuccess) return (int)cudaGetLastError();
+  constexpr int MOST = F::FIXED + (F::lists(MAX_REQUESTS) > F::PART ? F::lists(MAX_REQUESTS) : F::PART);
+  if (vb_allow_smem(reinterpret_cast<const void*>(k), MOST, devices) != cudaSuccess) return (int)cudaGetLastError();
   if (ctas) { *ctas = ctas_of(D, NT); return 0; }
   if (clusters) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = p.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = F::SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = F::FIXED + F::PART; cfg.attrs = &attr; cfg.numAttrs = 1;
     return (int)cudaOccupancyMaxActiveClusters(clusters, k, &cfg);
   }
   const int rows = p.B * p.Hkv * p.chunks;
   if (p.parts > 0) {
-    vb_launch_parts(k, dim3(rows * p.parts), dim3(THREADS), (size_t)F::SMEM, st, (unsigned)p.parts, p);
+    vb_launch_parts(k, dim3(rows * p.parts), dim3(THREADS), (size_t)(F::FIXED + F::PART), st, (unsigned)p.parts, p);
     return (int)cudaGetLastError();
   }
-  vb_launch(k, dim3(p.ctas), dim3(THREADS), (size_t)F::SMEM, st, p);
+  vb_launch(k, dim3(p.ctas), dim3(THREADS), (size_t)(F::FIXED + F::lists(p.B)), st, p);
   vb_launch(join_kernel, dim3(min(8 * NT, p.few * p.G), rows), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
   return (int)cudaGetLastError();
 }
 template <int D>
 static int pick(const Params& p, int nt, cudaStream_t st, int* clusters, int* ctas) {
-  return nt == 2 ? launch<D, 2>(p, st, clusters, ctas) : launch<D, 1>(p, st, clusters, ctas);
+  if (p.bf16) return nt == 2 ? launch<D, 2, true>(p, st, clusters, ctas) : launch<D, 1, true>(p, st, clusters, ctas);
+  return nt == 2 ? launch<D, 2, false>(p, st, clusters, ctas) : launch<D, 1, false>(p, st, clusters, ctas);
 }
 static int go(const Params& p, int D, int nt, cudaStream_t st, int* clusters = nullptr, int* ctas = nullptr) {
   switch (D) {

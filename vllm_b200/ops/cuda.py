@@ -800,7 +800,7 @@ _attention_fp4 = _sig("vb_attention_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _v
                       _i, _vp)
 _attention_fp4_plan = _sig("vb_attention_fp4_plan", _i, _i, _i, ctypes.POINTER(_i), ctypes.POINTER(_i), ctypes.POINTER(_i))
 FP4_HEADS = (32, 64, 80, 96, 128, 192, 256)
-FP4_EXTRA = 6                                # tiles that a row counts for beside its own, as its end costs about as much
+FP4_EXTRA = 3                                # tiles that a row counts for beside its own, as its end costs about as much
 
 
 @functools.lru_cache(maxsize=None)
