@@ -313,9 +313,6 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     ++fetched;
     cp_async_commit();
   };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
-
   const int r0 = lane >> 2, t4 = lane & 3, q0 = t4 * 2;
   // rows of a product in front of slots of the next: row r is key r ^ (r >> 1 & 1), so that the keys of neighbouring lanes lie in both halves of the banks
   const int key0 = r0 ^ (r0 >> 1 & 1);
@@ -324,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
   uint32_t q[KD][NT][2];
   float mult[NT][2];                                                        // of a column's sums: to powers of two, or to the cap
   int hi[NT][2];                                                            // last key that a column sees
-  auto load_q = [&]() {
+  auto read_q = [&]() {                      // as they are
     const int first_q = p.qsl ? p.qsl[row.b] : row.b;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -344,6 +341,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
           q[k][nt][0] = x.x; q[k][nt][1] = x.y;
         }
       }
+    }
+  };
+  auto convert_q = [&]() {                   // to fp16, with the factor of their products
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       float mine = 1.f;
       if (BF16) {
         float top = 0.f;
@@ -375,8 +377,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       }
     }
   };
-  load_q();
+  read_q();                                  // (on their way together with the first strips)
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
   while (true) {
+    convert_q();
     const int seg_end = min(row.end, t1) * PER_TILE, n = req.n, tile0 = req.first_tile(p), low = req.first_key(p);
     float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
     bool huge = false;                       // products of scores and their factor have to be rounded before a reference is taken off: its rounding is above 1
@@ -570,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     if (more) {                              // (the next row's queries are on their way meanwhile)
       next_row(p, COLS, first, reqs, row);
       req = Request{reqs[row.b].x, reqs[row.b].y};
-      load_q();
+      read_q();
     }
     if (!empty) {
 #pragma unroll
@@ -687,77 +692,74 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
 }
 
 // Grid (columns of a row, rows): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
-constexpr int JOIN = 128, AHEAD = 16;
+constexpr int JOIN = 128, JOINERS = JOIN / 32, PAIRS = 4, AHEAD = 4;
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, int D) {
-  __shared__ float factor_s[JOIN];
-  __shared__ float red[32];
+  __shared__ float2 sums[JOINERS][32 * PAIRS];
   pdl_trigger();
   pdl_wait();
   const int index = blockIdx.y, c = index % p.chunks, h = index / p.chunks % p.Hkv, b = index / p.chunks / p.Hkv, PD = D + 2;
+  const int2 at = p.info[index];                         // (says something where the request has keys and the row is one)
   const Request req = request(p, b);
   const int r = c * cols + blockIdx.x, tok = r / p.G;
   if (tok >= req.t) return;
-  const int2 at = req.n > 0 ? p.info[index] : make_int2(0, 0);
-  const int count = at.y;
-  if (req.n > 0 && count == 1) return;                   // done where its keys were
-  const int head = h * p.G + r - tok * p.G, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t step = (int64_t)cols * PD;
-  const float* x = p.part + ((int64_t)(index + at.x) * cols + blockIdx.x) * PD;
+  const int count = req.n > 0 ? at.y : 0;
+  if (count == 1) return;                                // done where its keys were
+  const int head = h * p.G + r - tok * p.G, lane = threadIdx.x & 31, w = threadIdx.x >> 5, pairs = D / 2;
+  const int step = cols * PD;                            // (a part's floats)
+  const float* x = p.part + ((int64_t)(index + (count ? at.x : 0)) * cols + blockIdx.x) * PD;
   const int64_t token = (p.qsl ? p.qsl[b] : b) + tok;
   const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
-  // a thread: two dimensions of every second part (heads above 128: of every part); the first parts' are read before their factors are known
-  const int pairs = D / 2, lanes = JOIN / pairs < 1 ? 1 : JOIN / pairs, mine = threadIdx.x / pairs;      // parts that a block takes at once
-  const float2* out = reinterpret_cast<const float2*>(x) + threadIdx.x % pairs;
-  const bool has = mine < lanes;
-  float2 ahead[AHEAD];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    const int part = i * lanes + mine;
-    ahead[i] = has && part < count ? out[part * (step / 2)] : make_float2(0.f, 0.f);
+  // every warp: the maximum and the sum; then its own parts, every fourth
+  float top = sink;
+  float2 ml = lane < count ? *reinterpret_cast<const float2*>(x + (int64_t)lane * step + D) : make_float2(-INFINITY, 0.f);
+  top = fmaxf(top, ml.x);
+  for (int i = 32 + lane; i < count; i += 32) top = fmaxf(top, x[(int64_t)i * step + D]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base), total = ml.x == -INFINITY ? 0.f : ml.y * f;
+  for (int i = 32 + lane; i < count; i += 32) {
+    const float2 y = *reinterpret_cast<const float2*>(x + (int64_t)i * step + D);
+    if (y.x > -INFINITY) total += y.y * ex2(y.x - base);
   }
-  float top = -INFINITY, total = 0.f;
-  float2 acc = make_float2(0.f, 0.f);
-  for (int from = 0; from == 0 || from < count; from += JOIN) {                      // (nearly always one round)
-    const int part = from + threadIdx.x;
-    const float2 ml = part < count ? *reinterpret_cast<const float2*>(x + part * step + D) : make_float2(-INFINITY, 0.f);
-    float m = warp_max(ml.x);
-    if (lane == 0) red[w] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float was = top;
-    top = fmaxf(fmaxf(top, m), from == 0 ? sink : -INFINITY);
-    const float base = top == -INFINITY ? 0.f : top, back = was == -INFINITY ? 0.f : ex2(was - base), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base);
-    factor_s[threadIdx.x] = f;
-    __syncthreads();                                                                 // (factors are there, and the maxima have been read)
-    total = total * back + block_sum(ml.x == -INFINITY ? 0.f : ml.y * f, red) + (from == 0 && p.sinks ? ex2(sink - base) : 0.f);
-    acc.x *= back; acc.y *= back;
-    if (has) {
-      int i = mine;
-      if (from == 0) {
+  total = warp_sum(total) + (p.sinks ? ex2(sink - base) : 0.f);
+  float2 acc[PAIRS];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          const float g = j * lanes + mine < min(count, JOIN) ? factor_s[j * lanes + mine] : 0.f;
-          if (j * lanes + mine < min(count, JOIN)) { acc.x += ahead[j].x * g; acc.y += ahead[j].y * g; }
-        }
-        i += AHEAD * lanes;
-      }
-      for (; i < JOIN && from + i < count; i += lanes) {
-        const float2 y = out[(from + i) * (step / 2)];
-        acc.x += y.x * factor_s[i]; acc.y += y.y * factor_s[i];
+  for (int j = 0; j < PAIRS; ++j) acc[j] = make_float2(0.f, 0.f);
+  for (int from = 0; from < count; from += 32) {
+    if (from > 0) {
+      const float m = from + lane < count ? x[(int64_t)(from + lane) * step + D] : -INFINITY;
+      f = m == -INFINITY ? 0.f : ex2(m - base);
+    }
+    const int end = min(32, count - from);
+    for (int i = w; i < end; i += JOINERS * AHEAD) {
+      float2 y[AHEAD][PAIRS];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j)
+          if (i + k * JOINERS < end && lane + 32 * j < pairs) y[k][j] = *reinterpret_cast<const float2*>(x + (int64_t)(from + i + k * JOINERS) * step + 2 * (lane + 32 * j));
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float g = __shfl_sync(0xffffffffu, f, (i + k * JOINERS) & 31);
+        if (i + k * JOINERS < end)
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j)
+            if (lane + 32 * j < pairs) { acc[j].x += y[k][j].x * g; acc[j].y += y[k][j].y * g; }
       }
     }
-    __syncthreads();
   }
-  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = total > 0.f ? ((top == -INFINITY ? 0.f : top) + log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
-  __shared__ float2 sums[JOIN];
-  sums[threadIdx.x] = acc;
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j)
+    if (lane + 32 * j < pairs) sums[w][lane + 32 * j] = acc[j];
   __syncthreads();
-  const float f = total == 0.f ? 0.f : p.out_scale / total;
+  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = total > 0.f ? (base + log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
+  const float by = total == 0.f ? 0.f : p.out_scale / total;
   for (int i = threadIdx.x; i < pairs; i += JOIN) {
-    float2 y = sums[i];
-    for (int j = 1; j < lanes; ++j) { y.x += sums[j * pairs + i].x; y.y += sums[j * pairs + i].y; }
+    float2 y = sums[0][i];
+#pragma unroll
+    for (int j = 1; j < JOINERS; ++j) { y.x += sums[j][i].x; y.y += sums[j][i].y; }
     uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D + 2 * i;
-    *reinterpret_cast<uint32_t*>(to) = p.bf16 ? pack2<__nv_bfloat16>(y.x * f, y.y * f) : pack2<__half>(y.x * f, y.y * f);
+    *reinterpret_cast<uint32_t*>(to) = p.bf16 ? pack2<__nv_bfloat16>(y.x * by, y.y * by) : pack2<__half>(y.x * by, y.y * by);
   }
 }
 
