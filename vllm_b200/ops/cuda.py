@@ -841,6 +841,37 @@ def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scal
 FP4_FEW_ROWS = 64                            # query rows (new tokens x query heads of a kv head) of requests that are attended straight from the cache
 
 
+_rows_fp4 = _sig("vb_rows_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _f, _f, _f, _i, _vp)
+_rows_fp4_ctas = _sig("vb_rows_fp4_ctas", _i, ctypes.POINTER(_i))
+FP4_PART_BYTES = 1 << 28                     # of the parts of split keys
+
+
+@functools.lru_cache(maxsize=None)
+def fp4_rows_ctas(D: int) -> int:
+    n = ctypes.c_int(0)
+    _check(_rows_fp4_ctas(D, ctypes.byref(n)), "rows_fp4_ctas", 0)
+    return n.value
+
+
+def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
+    """Attention of the requests with more than ``few`` new tokens, straight from the cache (csrc/attention_fp4_rows.cu)."""
+    (T, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
+    B, bt, G, max_q = md.num_reqs, md.block_table, Hq // kv_cache.shape[2], min(md.max_query_len, q.shape[0])
+    max_rows = max(1, min(bt.shape[1] * BS, md.max_seq_len))
+    tiles, lens = B * -(-max_q * G // 128), getattr(md, "host_lens", None)
+    if lens is not None:
+        cu = lens[0]
+        tiles = sum(-(-int(cu[b + 1] - cu[b]) * G // 128) for b in range(B) if cu[b + 1] - cu[b] > few)
+        if not tiles:
+            return
+    # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), max_rows // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
+    ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=q.device)
+    _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
+                     _p(ws), B, T, max_q, Hq, H, D, BS, max_rows, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
+                     _DT[q.dtype], _st()), "rows_fp4", 1 if splits == 1 else 2)
+
+
 # of 16-bit pages that a prompt's cache is read back to at a time: requests that want more are taken in several goes
 FP4_PAGES_BYTES = 1 << 30
 
@@ -922,10 +953,14 @@ def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causa
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     few, longest, G = 0, 1 if md.decode_only else md.max_query_len, Hq // kv_cache.shape[2]
-    if D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant():
+    straight = D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant()
+    if straight:
         few = min(longest, max(1, FP4_FEW_ROWS // G))
     if B and few < longest:
-        _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few)
+        if straight and not tc_attention_ok(D, D, G):
+            _fp4_rows_attention(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
+        else:
+            _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few)
     if B and few:
         _fp4_few(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
     if out is not None and to is not out:
