@@ -30,7 +30,7 @@ struct Params {
   void* out;
   float* lse;
   const float* sinks;
-  float* part;               // [split][token, head][D + 2]: output, maximum, sum
+  float* part;               // [split][token, head][D + 4]: output, maximum, sum of the weights as they were multiplied and before they were rounded
   int64_t q_stride, out_stride, bt_stride, num_blocks, tokens;
   int Hkv, G, BS, max_rows, few, splits, window, bf16;
   float scale_log2, ku, c2, out_scale;
@@ -66,9 +66,13 @@ VB_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+VB_DEVICE uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+
+VB_DEVICE float log_of(float base, float sum) { return sum > 0.f ? (base + log2f(sum)) * LN2 : sum == 0.f ? -INFINITY : sum; }
+
 template <int D_> struct Form {
   static constexpr int D = D_, MT = D <= 96 ? 2 : 1, WARPS = ROWS / (16 * MT), THREADS = WARPS * 32;
-  static constexpr int CTAS = D <= 64 ? 3 : D <= 96 ? 2 : 1;             // of an SM
+  static constexpr int CTAS = D <= 96 ? 2 : 1;             // of an SM
   static constexpr int LD = 2 * D + 16;                                  // bytes of a row in shared memory: an odd number of 16, so that neighbouring rows begin in different banks
   static constexpr int SIDE = TILE * LD, BUF = 2 * SIDE, SMEM = 2 * BUF;
   static constexpr int GROUPS = TILE * D / 16, MINE = (GROUPS + THREADS - 1) / THREADS;      // of a side; of a thread
@@ -92,25 +96,37 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 
   // ---- codes and scales of a tile: a thread's groups
   const int64_t page = fp4::page_bytes(p.BS, D), to_v = p.Hkv * page;
-  int blk[MINE];                                       // of the tile after the one that is on its way
+  int at_page[MINE], at_off[MINE];                     // of the tile that is looked up next
+  int blk[MINE], off[MINE];                            // of the tile that is read next
+  const int pages_on = TILE / p.BS, rest = TILE % p.BS;
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) {
+    const int tok = sp.lo * TILE + (j * F::THREADS + threadIdx.x) / KD;
+    at_page[j] = tok / p.BS;
+    at_off[j] = tok % p.BS;
+  }
   uint2 codes[2][MINE];
   uint32_t scales[2][MINE];
   auto look = [&](int tl) {
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
       const int gi = j * F::THREADS + threadIdx.x, tok = tl * TILE + gi / KD;
-      blk[j] = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n ? p.block_table[b * p.bt_stride + tok / p.BS] : -1;
+      blk[j] = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n ? p.block_table[b * p.bt_stride + at_page[j]] : -1;
+      off[j] = at_off[j];
+      at_page[j] += pages_on;
+      at_off[j] += rest;
+      if (at_off[j] >= p.BS) { at_off[j] -= p.BS; ++at_page[j]; }
     }
   };
   auto read = [&](int tl) {
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-      const int gi = j * F::THREADS + threadIdx.x, r = gi / KD, c = gi - r * KD, tok = tl * TILE + r, off = tok % p.BS;
+      const int gi = j * F::THREADS + threadIdx.x, r = gi / KD, c = gi - r * KD, tok = tl * TILE + r;
       const bool there = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n;
-      const int64_t at = (uint64_t)blk[j] < (uint64_t)p.num_blocks ? blk[j] : 0;       // (a table may not say that; nothing is read outside the cache)
-      const uint8_t* k = p.cache + (at * 2 * p.Hkv + h) * page;
-      const uint8_t* x = k + (int64_t)off * (D / 2) + c * 8;
-      const uint8_t* s = k + (int64_t)p.BS * (D / 2) + off * (D / 16) + c;
+      const uint64_t at = (uint64_t)blk[j] < (uint64_t)p.num_blocks ? blk[j] : 0;      // (a table may not say that; nothing is read outside the cache)
+      const uint8_t* k = p.cache + (uint32_t)(at * 2 * p.Hkv + h) * (uint64_t)(uint32_t)page;      // (pages of heads: below 2^31)
+      const uint8_t* x = k + off[j] * (D / 2) + c * 8;
+      const uint8_t* s = k + p.BS * (D / 2) + off[j] * (D / 16) + c;
       codes[0][j] = there ? *reinterpret_cast<const uint2*>(x) : make_uint2(0u, 0u);
       codes[1][j] = there ? *reinterpret_cast<const uint2*>(x + to_v) : make_uint2(0u, 0u);
       scales[0][j] = there ? s[0] : 0u;
@@ -189,7 +205,8 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
     }
   const int warp_first = n - sp.t + (sp.r0 + wr) / p.G, warp_last = wr < sp.rows ? n - sp.t + (sp.r0 + min(wr + 16 * MT, sp.rows) - 1) / p.G : -1;
 
-  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
+  float o[MT][D / 8][4], m_run[MT][2], sum[MT][4];       // sum: of the weights as they are multiplied, rows g and g + 8, in each of two columns
+  float exact[MT][2];                                  // the lane's, before they are rounded: for log-sum-exps
   bool huge = false;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -198,7 +215,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[m][i][j] = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) { m_run[m][u] = NONE; l_run[m][u] = 0.f; }
+    for (int u = 0; u < 2; ++u) { m_run[m][u] = NONE; sum[m][2 * u] = sum[m][2 * u + 1] = exact[m][u] = 0.f; }
   }
   if (sp.lo < sp.hi) store(0);
   const uint32_t base = smem_u32(smem);
@@ -251,13 +268,15 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
             }
           f[0] = f[1] = 1.f;
         }
-        float most = -INFINITY;
+        uint32_t most = 0u;                              // the largest weights, two halves
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaf(s[m][i][j], f[j >> 1], -m_run[m][j >> 1]));
-        const bool grow = __any_sync(0xffffffffu, most > 8.f + SHIFT) != 0;
-        if (grow) {
+          for (int u = 0; u < 2; ++u) {
+            w[m][i][u] = pack2<__half>(ex2(fmaf(s[m][i][2 * u], f[u], -m_run[m][u])), ex2(fmaf(s[m][i][2 * u + 1], f[u], -m_run[m][u])));
+            most = max2(most, w[m][i][u]);
+          }
+        if (__any_sync(0xffffffffu, (most & 0xffffu) > 0x7800u || most > 0x7800ffffu)) {          // above 2^15
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             float mx = -INFINITY;
@@ -269,7 +288,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
             const bool up = at > was + 8.f;
             const float alpha = up ? ex2(was - at) : 1.f;
             m_run[m][u] = up ? at : was;
-            l_run[m][u] *= alpha;
+            sum[m][2 * u] *= alpha; sum[m][2 * u + 1] *= alpha; exact[m][u] *= alpha;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) { o[m][i][2 * u] *= alpha; o[m][i][2 * u + 1] *= alpha; }
           }
@@ -277,17 +296,20 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[m][i][j] = __fmul_rn(s[m][i][j], f[j >> 1]);
-          f[0] = f[1] = 1.f;                           // (the difference of two rounded numbers: nothing is left over where scores are huge)
+            for (int u = 0; u < 2; ++u)                  // (the difference of two rounded numbers: nothing is left over where scores are huge)
+              w[m][i][u] = pack2<__half>(ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u], f[u]), m_run[m][u])), ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u + 1], f[u]), m_run[m][u])));
+        }
+        if (p.lse) {                                     // (asked for seldom: the exponentials once more)
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) exact[m][j >> 1] += ex2(__fsub_rn(__fmul_rn(s[m][i][j], f[j >> 1]), m_run[m][j >> 1]));
         }
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float x = ex2(fmaf(s[m][i][2 * u], f[u], -m_run[m][u])), y = ex2(fmaf(s[m][i][2 * u + 1], f[u], -m_run[m][u]));
-            l_run[m][u] += x + y;
-            w[m][i][u] = pack2<__half>(x, y);
-          }
+        for (int kk = 0; kk < SUB / 16; ++kk) {          // sums of the weights, as a product with ones
+          const uint32_t a[4] = {w[m][2 * kk][0], w[m][2 * kk][1], w[m][2 * kk + 1][0], w[m][2 * kk + 1][1]};
+          mma16816(sum[m], a, 0x3c003c00u, 0x3c003c00u);
+        }
       }
       // ---- O += P V
       const uint32_t vs = base + buf * F::BUF + F::SIDE + (k0 + (mi & 1) * 8 + l7) * F::LD + (mi >> 1) * 16;
@@ -312,47 +334,49 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float l = l_run[m][u];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      const float l = sum[m][2 * u];
+      float l32 = exact[m][u];
+      l32 += __shfl_xor_sync(0xffffffffu, l32, 1);
+      l32 += __shfl_xor_sync(0xffffffffu, l32, 2);
       const int i = wr + m * 16 + u * 8 + g, r = sp.r0 + i, tok = r / p.G, head = h * p.G + r - tok * p.G;
       if (i >= sp.rows) continue;
       const bool none = m_run[m][u] == NONE;
       const int64_t at = (int64_t)(first_q + tok) * p.Hkv * p.G + head;
       if (p.splits > 1) {
-        float* to = p.part + (split * p.tokens * p.Hkv * p.G + at) * (D + 2);
+        float* to = p.part + (split * p.tokens * p.Hkv * p.G + at) * (D + 4);
         if (!none)
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(to + j * 8 + t4 * 2) = make_float2(o[m][j][2 * u], o[m][j][2 * u + 1]);
-        if (t4 == 0) *reinterpret_cast<float2*>(to + D) = make_float2(none ? -INFINITY : m_run[m][u], l);
+        if (t4 == 0) *reinterpret_cast<float4*>(to + D) = make_float4(none ? -INFINITY : m_run[m][u], l, l32, 0.f);
         continue;
       }
       const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = none ? sink : fmaxf(m_run[m][u], sink), base2 = top == -INFINITY ? 0.f : top;
-      const float back = none ? 0.f : ex2(m_run[m][u] - base2), sum = (none ? 0.f : l * back) + (p.sinks ? ex2(sink - base2) : 0.f), f = sum == 0.f ? 0.f : back / sum * p.out_scale;
+      const float back = none ? 0.f : ex2(m_run[m][u] - base2), all = (none ? 0.f : l * back) + (p.sinks ? ex2(sink - base2) : 0.f), f = all == 0.f ? 0.f : back / all * p.out_scale;
       uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(first_q + tok) * p.out_stride + (int64_t)head * D + t4 * 2;
 #pragma unroll
       for (int j = 0; j < D / 8; ++j) {
         const float x = none ? 0.f : o[m][j][2 * u] * f, y = none ? 0.f : o[m][j][2 * u + 1] * f;
         *reinterpret_cast<uint32_t*>(to + j * 8) = BF16 ? pack2<__nv_bfloat16>(x, y) : pack2<__half>(x, y);
       }
-      if (t4 == 0 && p.lse) p.lse[at] = sum > 0.f ? (base2 + log2f(sum)) * LN2 : sum == 0.f ? -INFINITY : sum;
+      if (t4 == 0 && p.lse) p.lse[at] = log_of(base2, (none ? 0.f : l32 * back) + (p.sinks ? ex2(sink - base2) : 0.f));
     }
 }
 
-// Grid (tiles of rows, kv heads, requests): joins the parts of split keys.  A warp has a row.
-constexpr int JOIN = 256, MOST_SPLITS = 16;
+// Grid (runs of JOIN / 32 rows, kv heads, requests): joins the parts of split keys.  A warp has a row.
+constexpr int JOIN = 256, PER_TILE = ROWS / (JOIN / 32), MOST_SPLITS = 16;
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int D) {
   pdl_trigger();
   pdl_wait();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const Span sp = span_of(p, b, blockIdx.x, 0);
+  const Span sp = span_of(p, b, blockIdx.x / PER_TILE, 0);
   const int first_q = p.qsl[b];
-  const int64_t step = p.tokens * p.Hkv * p.G * (D + 2);
-  for (int i = threadIdx.x >> 5; i < sp.rows; i += JOIN / 32) {
+  const int64_t step = p.tokens * p.Hkv * p.G * (D + 4);
+  const int i = blockIdx.x % PER_TILE * (JOIN / 32) + (threadIdx.x >> 5);
+  if (i < sp.rows) {
     const int r = sp.r0 + i, tok = r / p.G, head = h * p.G + r - tok * p.G;
     const int64_t at = (int64_t)(first_q + tok) * p.Hkv * p.G + head;
-    const float* x = p.part + at * (D + 2);
-    const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(x + lane * step + D) : make_float2(-INFINITY, 0.f);
+    const float* x = p.part + at * (D + 4);
+    const float4 ml = lane < p.splits ? *reinterpret_cast<const float4*>(x + lane * step + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
     const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
     const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base);
     const float sum = warp_sum(ml.x == -INFINITY ? 0.f : ml.y * f) + (p.sinks ? ex2(sink - base) : 0.f), by = sum == 0.f ? 0.f : p.out_scale / sum;
@@ -370,7 +394,8 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int D) {
       }
       if (d < D) *reinterpret_cast<uint32_t*>(to + d) = p.bf16 ? pack2<__nv_bfloat16>(acc.x * by, acc.y * by) : pack2<__half>(acc.x * by, acc.y * by);
     }
-    if (lane == 0 && p.lse) p.lse[at] = sum > 0.f ? (base + log2f(sum)) * LN2 : sum == 0.f ? -INFINITY : sum;
+    const float l32 = warp_sum(ml.x == -INFINITY ? 0.f : ml.z * f) + (p.sinks ? ex2(sink - base) : 0.f);
+    if (lane == 0 && p.lse) p.lse[at] = log_of(base, l32);
   }
 }
 
@@ -382,7 +407,7 @@ static int launch(const Params& p, dim3 grid, cudaStream_t st, int* ctas) {
   static std::atomic<uint64_t> devices{0};
   if (vb_allow_smem(reinterpret_cast<const void*>(k), F::SMEM, devices) != cudaSuccess) return (int)cudaGetLastError();
   vb_launch(k, dim3(grid.x * p.splits, grid.y, grid.z), dim3(F::THREADS), (size_t)F::SMEM, st, p);
-  if (p.splits > 1) vb_launch(join_kernel, grid, dim3(JOIN), (size_t)0, st, p, D);
+  if (p.splits > 1) vb_launch(join_kernel, dim3(grid.x * PER_TILE, grid.y, grid.z), dim3(JOIN), (size_t)0, st, p, D);
   return (int)cudaGetLastError();
 }
 static int go(const Params& p, int D, dim3 grid, cudaStream_t st, int* ctas = nullptr) {
@@ -402,7 +427,7 @@ EXPORT int vb_rows_fp4_ctas(int D, int* ctas) {
   return rfp4::go(p, D, dim3(1), nullptr, ctas);
 }
 
-// Causal attention of requests of more than `few` new tokens, at most max_q; rows of q and out [tokens] of the others are not touched.  ws: for splits > 1, splits tokens Hq (D + 2)
+// Causal attention of requests of more than `few` new tokens, at most max_q; rows of q and out [tokens] of the others are not touched.  ws: for splits > 1, splits tokens Hq (D + 4)
 // floats.  lse [tokens, Hq] or null.
 EXPORT int vb_rows_fp4(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, void* out, float* lse,
                        const float* sinks, float* ws, int B, int64_t tokens, int max_q, int Hq, int Hkv, int D, int BS, int max_rows, int few, int64_t q_stride, int64_t out_stride,

@@ -865,8 +865,8 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
         if not tiles:
             return
     # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
-    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), max_rows // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
-    ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=q.device)
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), max_rows // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 4))))
+    ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 4), dtype=torch.float32, device=q.device)
     _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
                      _p(ws), B, T, max_q, Hq, H, D, BS, max_rows, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
                      _DT[q.dtype], _st()), "rows_fp4", 1 if splits == 1 else 2)
@@ -961,6 +961,9 @@ def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causa
             _fp4_rows_attention(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
         else:
             _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few)
+        lens = getattr(md, "host_lens", None)
+        if lens is not None and all(lens[0][b + 1] - lens[0][b] > few for b in range(B)):
+            few = 0                          # (no request has so few)
     if B and few:
         _fp4_few(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
     if out is not None and to is not out:
