@@ -187,17 +187,18 @@ __global__ void __launch_bounds__(READERS) gather_kernel(Source s, const int* __
   }
 }
 
-// Grid (pages of PS rows, kv heads, requests): the rows of requests with more than `few` new tokens as pages [pages, 2, Hkv, PS, D] of a workspace (VT: values of
-// a page transposed, heads of 128 and pages of 64), with the block table [B, gridDim.x] and the lengths that say so.  A request has as many pages as its rows need,
-// behind those of the requests in front of it; the others have none, and a length of 0.  Rows behind the last one are zeros.
+// Grid (pages of PS rows, kv heads, requests): the rows of requests with more than `few` new tokens as pages [pages, 2, Hkv, PS, W] of a workspace (W >= D, zeros behind
+// the rows' values; VT: values of a page transposed, W = 128 and pages of 64), with the block table [B, gridDim.x] and the lengths that say so.  A request has as many pages
+// as its rows need, behind those of the requests in front of it; the others have none, and a length of 0.  Rows behind the last one are zeros.
 template <typename T, bool VT>
 __global__ void __launch_bounds__(READERS) pages_kernel(Source s, const int* __restrict__ seq_lens, const int* __restrict__ qsl, int few, T* __restrict__ pages, int num_pages,
-                                                        int PS, int* __restrict__ table, int* __restrict__ lens) {
+                                                        int PS, int W, int* __restrict__ table, int* __restrict__ lens) {
   __shared__ float red[32];
   __shared__ __align__(16) T tile[VT ? 64 * 130 : 1];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, h = blockIdx.y, p = blockIdx.x, chunks = s.D / N, width = gridDim.x;
+  const int b = blockIdx.z, h = blockIdx.y, p = blockIdx.x, real = s.D / N, width = gridDim.x;
+  const int chunks = VT ? 128 / N : W / N;
   auto rows_of = [&](int i) {
     const int n = min(max(seq_lens[i], 0), s.width * s.BS);
     return qsl && qsl[i + 1] - qsl[i] <= few ? 0 : n;
@@ -219,22 +220,23 @@ __global__ void __launch_bounds__(READERS) pages_kernel(Source s, const int* __r
     table[(int64_t)b * width + p] = p < room ? page : 0;
   }
   if (p >= room) return;
-  T* kp = pages + ((int64_t)page * 2 * s.Hkv + h) * PS * s.D;
-  T* vp = kp + (int64_t)s.Hkv * PS * s.D;
+  const int w = VT ? 128 : W;
+  T* kp = pages + ((int64_t)page * 2 * s.Hkv + h) * PS * w;
+  T* vp = kp + (int64_t)s.Hkv * PS * w;
   for (int i = threadIdx.x; i < PS * chunks; i += READERS) {
     const int r = i / chunks, c = i % chunks, tok = p * PS + r;
     uint32_t codes[2] = {0u, 0u}, scale[2] = {0u, 0u};
-    if (tok < n) {
+    if (tok < n && c < real) {
       load_chunk(s, b, 0, h, tok, c, codes[0], scale[0]);
       load_chunk(s, b, 1, h, tok, c, codes[1], scale[1]);
     }
-    st16(kp + r * s.D + c * N, row_chunk<T>(codes[0], scale[0], 1.f));
+    st16(kp + r * w + c * N, row_chunk<T>(codes[0], scale[0], 1.f));
     const Vec16<T> x = row_chunk<T>(codes[1], scale[1], 1.f);
     if (VT) {
       uint32_t* dst = reinterpret_cast<uint32_t*>(tile + r * 130 + c * N);
       dst[0] = x.u.x; dst[1] = x.u.y; dst[2] = x.u.z; dst[3] = x.u.w;
     } else {
-      st16(vp + r * s.D + c * N, x);
+      st16(vp + r * w + c * N, x);
     }
   }
   if (VT) {
@@ -246,6 +248,22 @@ __global__ void __launch_bounds__(READERS) pages_kernel(Source s, const int* __r
       for (int e = 0; e < N; ++e) o.e[e] = tile[(r + e) * 130 + d];
       st16(vp + d * 64 + r, o);
     }
+  }
+}
+
+// Rows [T, H, G, D] to [T, H, G2, D2] (chunks of eight values; zeros where there are none), or back
+template <typename T>
+__global__ void __launch_bounds__(READERS) fit_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t n, int G, int G2, int from, int to, int64_t x_stride, int64_t y_stride,
+                                                      int heads) {
+  pdl_trigger();
+  pdl_wait();
+  for (int64_t i = (int64_t)blockIdx.x * READERS + threadIdx.x; i < n; i += (int64_t)gridDim.x * READERS) {
+    const int c = (int)(i % to), hg = (int)(i / to % heads), h = hg / G2, g = hg - h * G2;      // (heads: of a row of y)
+    const int64_t t = i / to / heads;
+    Vec16<T> v;
+    v.u = make_uint4(0u, 0u, 0u, 0u);
+    if (c < from && g < G) v = ld16(x + t * x_stride + ((int64_t)(h * G + g) * from + c) * N);
+    st16(y + t * y_stride + ((int64_t)hg * to + c) * N, v);
   }
 }
 
@@ -283,16 +301,28 @@ EXPORT int vb_gather_fp4(const void* cache, int64_t num_blocks, const int* block
   return (int)cudaGetLastError();
 }
 
-// Pages of a workspace [num_pages, 2, Hkv, PS, D] with table [B, table_width] and lens [B] of them, without the factors of keys and values.  few: requests of at most
+// Pages of a workspace [num_pages, 2, Hkv, PS, W] with table [B, table_width] and lens [B] of them, without the factors of keys and values.  few: requests of at most
 // so many new tokens (qsl [B + 1]; null: all take part) are left out.
 EXPORT int vb_pages_fp4(const void* cache, int64_t num_blocks, const int* block_table, int64_t bt_stride, int width, const int* seq_lens, const int* qsl, int few, void* pages,
-                        int num_pages, int PS, int vt, int* table, int table_width, int* lens, int B, int Hkv, int D, int BS, int dtype, cudaStream_t st) {
+                        int num_pages, int PS, int W, int vt, int* table, int table_width, int* lens, int B, int Hkv, int D, int BS, int dtype, cudaStream_t st) {
   if (B <= 0) return 0;
-  if (bad_shape(D, BS, dtype) || Hkv < 1 || Hkv > 65535 || B > 65535 || width < 0 || table_width < 1 || PS < 1 || num_pages < 0 || (vt && (D != 128 || PS != 64))) return -1;
+  if (bad_shape(D, BS, dtype) || Hkv < 1 || Hkv > 65535 || B > 65535 || width < 0 || table_width < 1 || PS < 1 || num_pages < 0 || W < D || W % N ||
+      (vt && (W != 128 || PS != 64)))
+    return -1;
   const Source s{(const uint8_t*)cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv};
   DISPATCH_HALF(dtype, TT, {
     auto kernel = vt ? pages_kernel<TT, true> : pages_kernel<TT, false>;
-    vb_launch(kernel, dim3(table_width, Hkv, B), dim3(READERS), 0, st, s, seq_lens, qsl, few, (TT*)pages, num_pages, PS, table, lens);
+    vb_launch(kernel, dim3(table_width, Hkv, B), dim3(READERS), 0, st, s, seq_lens, qsl, few, (TT*)pages, num_pages, PS, W, table, lens);
   });
+  return (int)cudaGetLastError();
+}
+
+// x [T, H, G, D] (row stride x_stride) to y [T, H, G2, D2]: values and heads behind the last are zeros, or left out.
+EXPORT int vb_fit_rows(const void* x, void* y, int T, int H, int G, int D, int G2, int D2, int64_t x_stride, int64_t y_stride, int sms, int dtype, cudaStream_t st) {
+  if (T <= 0) return 0;
+  if ((dtype != DT_BF16 && dtype != DT_F16) || D % N || D2 % N || H < 1 || G < 1 || G2 < 1) return -1;
+  const int64_t n = (int64_t)T * H * G2 * (D2 / N), blocks = (n + READERS - 1) / READERS;
+  DISPATCH_HALF(dtype, TT, vb_launch(fit_kernel<TT>, dim3((unsigned)(blocks < 8 * sms ? blocks : 8 * sms)), dim3(READERS), 0, st, (const TT*)x, (TT*)y, n, G, G2, D / N, D2 / N,
+                                     x_stride, y_stride, H * G2));
   return (int)cudaGetLastError();
 }

@@ -748,7 +748,8 @@ def evict_keys(kv_cache, md, scores, keep: int, first: int, recent: int, positio
 # ------------------------------------------------------------------ a cache in 4 bits (csrc/cache_fp4.cu, csrc/attention_fp4.cu)
 _write_fp4 = _sig("vb_write_fp4", _vp, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i, _f, _f, _i, _vp)
 _gather_fp4 = _sig("vb_gather_fp4", _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _i, _i, _f, _f, _i, _vp)
-_pages_fp4 = _sig("vb_pages_fp4", _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp)
+_pages_fp4 = _sig("vb_pages_fp4", _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp)
+_fit_rows = _sig("vb_fit_rows", _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64, _i, _i, _vp)
 
 
 def _fp4_half(x, kv_cache, op: str) -> int:
@@ -838,7 +839,26 @@ def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scal
                           window or 0, scale, soft_cap, out_scale, _DT[q.dtype], _st()), "attention_fp4", 1 if parts else 2 * -(-B // group))
 
 
-FP4_FEW_ROWS = 64                            # query rows (new tokens x query heads of a kv head) of requests that are attended straight from the cache
+FP4_FEW_ROWS = 64                            # query rows (new tokens x query heads of a kv head) of requests that always take the kernel of single tokens
+
+
+def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int) -> tuple[int, bool]:
+    """(new tokens up to which a request takes the kernel of single tokens, whether the others' prompts go straight from the cache or through 16-bit pages), for T
+    tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: the kernel of single tokens 3.5 TB/s of the cache for every 16
+    query rows; the one of prompts 190 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
+    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 32, 41, 203; 160 there 96, 78, 123; 320 there
+    179, 164, 126; 500 there -, 235, 198; 160 behind 1200 30, 28, 35; 640 there 76, 50, 41; of 128, 80 behind 12 000 81, 90, 183; 160 there 149, 168, 121."""
+    base = max(1, FP4_FEW_ROWS // G)
+    if longest <= base:
+        return longest, True
+    pairs = T * H * max(rows - longest / 2, 1)
+    single = 6 + (T * G / 16 + B) * rows * H * D * 1.125 / 3.5e6
+    straight = 20 + pairs * G * 4 * D / 190e6
+    pages = float("inf")
+    if D <= 128:
+        pages = 20 + B * rows * H * 1024 / 4.5e6 + max(rows * 0.0085, pairs * (1 << (G - 1).bit_length()) * 512 / 800e6)
+    few = longest if longest * G <= 1024 and single < min(straight, pages) else base
+    return few, straight < pages
 
 
 _rows_fp4 = _sig("vb_rows_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _f, _f, _f, _i, _vp)
@@ -897,39 +917,57 @@ def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[i
     return runs
 
 
-def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, lse, alibi, sinks, chunk, out_scale, few: int) -> None:
+def fit_rows(x, y, H: int) -> None:
+    """x [T, heads, D] to y [T, more or fewer heads of each of the H kv heads, D2]: what x does not have is zeros."""
+    T, (hx, dx), (hy, dy) = x.shape[0], x.shape[1:], y.shape[1:]
+    _check(_fit_rows(x.data_ptr(), y.data_ptr(), T, H, hx // H, dx, hy // H, dy, x.stride(0), y.stride(0), num_sms(), _DT[x.dtype], _st()), "fit_rows")
+
+
+def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, lse, alibi, sinks, chunk, out_scale, few: int, wide: bool) -> None:
     """Attention of the requests with more than ``few`` new tokens: their cache is read back to 16-bit pages, which the attention kernels over those take.  Rows of
-    the other requests hold anything afterwards."""
-    (_, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
-    bt, sl = md.block_table, md.seq_lens
-    vt = tc_attention_ok(D, D, Hq // H) and alibi is None
-    PS = 32 if D == 256 else 64
+    the other requests hold anything afterwards.  ``wide``: heads become 128 wide, and a power of two for each kv head, as the tcgen05 kernel takes them."""
+    (T, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
+    bt, sl, W, to, norm = md.block_table, md.seq_lens, D, out, lse
+    if wide:
+        W, G = 128, 1 << (Hq // H - 1).bit_length()
+        if W != D or G != Hq // H:
+            q, narrow = q.new_empty((T, H * G, W)), q
+            fit_rows(narrow, q, H)
+            to, norm = torch.empty_like(q), None if lse is None else lse.new_empty((T, H * G))
+            if sinks is not None:
+                sinks = torch.nn.functional.pad(sinks.view(H, Hq // H), (0, G - Hq // H)).flatten()
+    vt = tc_attention_ok(W, W, q.shape[1] // H) and alibi is None
+    PS = 32 if W == 256 else 64
     qsl = None if md.decode_only else md.query_start_loc
     most = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS)
-    for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * D):
+    for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * W):
         n = b1 - b0
         if total == 0:                       # (none of them has more than `few`)
             continue
-        pages = torch.empty((total, 2, H, PS, D), dtype=q.dtype, device=q.device)
+        pages = torch.empty((total, 2, H, PS, W), dtype=q.dtype, device=q.device)
         table, lens = sl.new_empty((n, longest)), sl.new_empty(n)
         _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt[b0:].data_ptr(), bt.stride(0), bt.shape[1], sl[b0:].data_ptr(), None if qsl is None else qsl[b0:].data_ptr(), few,
-                          pages.data_ptr(), pages.shape[0], PS, int(vt), table.data_ptr(), table.shape[1], lens.data_ptr(), n, H, D, BS, _DT[q.dtype], _st()), "pages_fp4")
+                          pages.data_ptr(), pages.shape[0], PS, W, int(vt), table.data_ptr(), table.shape[1], lens.data_ptr(), n, H, D, BS, _DT[q.dtype], _st()), "pages_fp4")
         part = copy.copy(md)
         part.num_reqs, part.block_table, part.seq_lens, part.max_seq_len, part.kv_vt, part.flat, part.cascade = n, table, lens, longest * PS, vt, False, None
         if md.decode_only:
             rows = slice(b0, b1)
             part.query_start_loc = None if md.query_start_loc is None else md.query_start_loc[:n + 1]
         else:
-            rows = slice(0, q.shape[0])
+            rows = slice(0, T)
             part.query_start_loc = qsl[b0:b1 + 1]
-        got = paged_attention(q[rows], pages, part, scale, window, soft_cap, causal, out[rows], return_lse=lse is not None, alibi_slopes=alibi, sinks=sinks, chunk_size=chunk,
+        got = paged_attention(q[rows], pages, part, scale, window, soft_cap, causal, to[rows], return_lse=lse is not None, alibi_slopes=alibi, sinks=sinks, chunk_size=chunk,
                               out_scale=out_scale)
         if lse is not None:
             if md.decode_only or n == md.num_reqs:
-                lse[rows] = got[1]
+                norm[rows] = got[1]
             else:
-                t = torch.arange(q.shape[0], device=q.device)
-                lse.copy_(torch.where(((t >= qsl[b0]) & (t < qsl[b1]))[:, None], got[1], lse))
+                t = torch.arange(T, device=q.device)
+                norm.copy_(torch.where(((t >= qsl[b0]) & (t < qsl[b1]))[:, None], got[1], norm))
+    if to is not out:
+        fit_rows(to, out, H)
+        if lse is not None:
+            lse.view(T, H, -1).copy_(norm.view(T, H, -1)[:, :, :Hq // H])
 
 
 def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causal=True, out=None, alibi=None, sinks=None, chunk=0, return_lse: bool = False,
@@ -952,15 +990,15 @@ def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causa
         to[used:].zero_()
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
-    few, longest, G = 0, 1 if md.decode_only else md.max_query_len, Hq // kv_cache.shape[2]
-    straight = D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant()
-    if straight:
-        few = min(longest, max(1, FP4_FEW_ROWS // G))
+    few, longest, G, H = 0, 1 if md.decode_only else md.max_query_len, Hq // kv_cache.shape[2], kv_cache.shape[2]
+    direct = D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant()
+    if direct and longest:
+        few, straight = fp4_kernels(used, B, longest, min(md.max_seq_len, bt.shape[1] * kv_cache.shape[3]), H, G, D)
     if B and few < longest:
-        if straight and not tc_attention_ok(D, D, G):
+        if direct and straight:
             _fp4_rows_attention(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
         else:
-            _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few)
+            _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few, direct)
         lens = getattr(md, "host_lens", None)
         if lens is not None and all(lens[0][b + 1] - lens[0][b] > few for b in range(B)):
             few = 0                          # (no request has so few)
