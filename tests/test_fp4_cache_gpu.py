@@ -351,3 +351,104 @@ def test_refusals():
         ops.reshape_and_cache_fp4(x, x, cache, torch.zeros(2, dtype=torch.int64, device="cuda"))
     with pytest.raises(ValueError):
         ops.gather_cache_fp4(cache, md.block_table.int(), torch.tensor([0, 2], dtype=torch.int32, device="cuda"), x, x, 2)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("D", [32, 64, 80, 96, 128, 192, 256])
+def test_prompts_straight_from_the_cache(dtype, D):
+    """The kernel of prompts for every head, whatever the rule would choose: with and without parts of keys, with requests that are not its own."""
+    cu = cuda_ops()
+    for lens, queries, Hq, Hkv, BS in (([700, 130, 5], [150, 130, 2], 6, 2, 48), ([2100], [40], 5, 1, 64), ([1300, 9], [33, 9], 8, 4, 16)):
+        q, cache, md = step(lens, queries, Hq, Hkv, D, BS, dtype, "cuda", seed=D + len(lens), spread=2.0, host=Hq != 5)
+        for window, cap, sinks in ((None, 0.0, None), (65, 25.0, torch.randn(Hq).cuda())):
+            out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+            cu._fp4_rows_attention(q, cache, md, D ** -0.5, window, cap, out, lse, sinks, 1.0, 8)
+            want, norm, mass, terms, big = attend(q, cache, md, D ** -0.5, window, cap, sinks)
+            eps, u = (D / 8 + 16) * 2.0 ** -23 * terms + 8 * 2.0 ** -24 * 1.5 * terms + 2.0 ** -21, torch.finfo(dtype).eps / 2
+            bound = u * want.abs() + (2.0 ** -11 + 2 * eps + 2.0 ** -13) * mass + max(lens) * 2.0 ** -31 * big + 2.0 ** -25
+            mine = torch.cat([torch.full((n,), n > 8) for n in queries])
+            assert ((out.double().cpu() - want).abs() <= bound)[mine].all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs())[mine].all()
+            assert (out.cpu()[~mine] == 7.0).all() and (lse.cpu()[~mine] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("Hq,Hkv,D", [(6, 2, 64), (5, 1, 128), (8, 2, 80), (4, 4, 32)])
+def test_prompts_through_wider_pages(dtype, Hq, Hkv, D):
+    """Heads that the tensor-core kernel does not take become 128 wide, and a power of two for each kv head."""
+    cu = cuda_ops()
+    lens, queries = [700, 130, 5, 64], [150, 130, 2, 64]
+    q, cache, md = step(lens, queries, Hq, Hkv, D, 32, dtype, "cuda", seed=D, spread=2.0)
+    for window, cap, sinks in ((None, 0.0, None), (65, 25.0, torch.randn(Hq).cuda())):
+        out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+        cu._fp4_attention_pages(q, cache, md, D ** -0.5, window, cap, True, out, lse, None, sinks, 0, 1.0, 8, True)
+        want, norm, mass, terms, big = attend(q, cache, md, D ** -0.5, window, cap, sinks)
+        eps, u = (128 / 8 + 16) * 2.0 ** -23 * terms + 8 * 2.0 ** -24 * 1.5 * terms + 2.0 ** -21, torch.finfo(dtype).eps / 2
+        bound = u * want.abs() + (u + 2 * eps + 2.0 ** -13) * mass + max(lens) * 2.0 ** -31 * big + 2.0 ** -25
+        mine = torch.cat([torch.full((n,), n > 8) for n in queries])
+        assert ((out.double().cpu() - want).abs() <= bound)[mine].all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs())[mine].all()
+
+
+def test_prompts_in_more_than_one_go(monkeypatch):
+    """A workspace for one request at a time gives what one for all gives, also without lengths on the host."""
+    cu = cuda_ops()
+    for host in (True, False):
+        q, cache, md = step([300, 700, 90, 500], [100, 200, 1, 150], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=1, host=host)
+        monkeypatch.setattr(cu, "FP4_PAGES_BYTES", 1 << 30)
+        want = ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)
+        monkeypatch.setattr(cu, "FP4_PAGES_BYTES", 1 << 18)
+        got = ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_batch_invariant_rows(monkeypatch):
+    """In batch-invariant mode a request's rows do not depend on what else is in the step."""
+    monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
+    q, cache, md = step([300, 700, 90], [1, 1, 1], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=1)
+    want = ops.paged_attention_fp4(q, cache, md, 0.1)
+    for b in range(3):
+        _, _, one = step([300], [1], 8, 2, 128, 64, torch.bfloat16, "cuda")
+        one.seq_lens, one.block_table, one.max_seq_len, one.host_lens = md.seq_lens[b:b + 1], md.block_table[b:b + 1], 700, None
+        assert torch.equal(ops.paged_attention_fp4(q[b:b + 1], cache, one, 0.1), want[b:b + 1])
+
+
+def _llm(model, **kw):
+    from vllm_b200 import LLM
+    from vllm_b200.model_loader import initialize_dummy_weights
+    llm = LLM(model, **{**dict(max_model_len=512, max_num_seqs=16, max_num_batched_tokens=512, gpu_memory_utilization=0.2, load_format="dummy",
+                               cudagraph_capture_sizes=[1, 2, 4, 8], dtype="bfloat16"), **kw})
+    runner = llm.llm_engine.engine_core.engine_core.model_executor.worker.runner
+    with torch.no_grad():
+        initialize_dummy_weights(runner.model, 7, -0.05, 0.05)
+    return llm, runner
+
+
+def test_generation_with_a_cache_in_4_bits():
+    """Teacher-forced log-probabilities stay near those of a 16-bit cache; captured decode steps give what eager ones give."""
+    from vllm_b200 import SamplingParams
+    prompts = [{"prompt_token_ids": [(7 * i + j) % 4000 + 3 for j in range(90 + 31 * i)]} for i in range(5)]
+    tokens, lps = {}, {}
+    for name, kw in (("auto", {}), ("nvfp4", {"kv_cache_dtype": "nvfp4"}), ("eager", {"kv_cache_dtype": "nvfp4", "enforce_eager": True})):
+        llm, r = _llm("llama-small", max_num_batched_tokens=64, **kw)                   # chunked: prompts read the cache
+        outs = llm.generate(prompts, SamplingParams(max_tokens=12, temperature=0.0, ignore_eos=True, prompt_logprobs=0))
+        lps[name] = [list(d.values())[0].logprob for o in outs for d in o.prompt_logprobs[1:]]
+        tokens[name] = [o.outputs[0].token_ids for o in outs]
+        cache = next(iter(r.kv_caches.values()))
+        assert (cache.dtype == torch.uint8) == (name != "auto") and bool(r.graphs) == (name != "eager")
+        llm.shutdown()
+        del r
+    assert tokens["nvfp4"] == tokens["eager"]
+    d = sorted(abs(a - b) for a, b in zip(lps["auto"], lps["nvfp4"]))
+    assert 0 < d[-1] and d[len(d) // 2] < 0.2 and d[int(0.95 * len(d))] < 0.7, d[-5:]
+
+
+@pytest.mark.parametrize("model", ["gemma2-tiny", "gptoss-tiny", "qwen2vl-tiny", "qwen3moe-tiny", "bloom-tiny"])
+def test_families_with_a_cache_in_4_bits(model):
+    from vllm_b200 import SamplingParams
+    try:
+        llm, _ = _llm(model, kv_cache_dtype="nvfp4", max_model_len=256, max_num_batched_tokens=64, block_size=16)
+    except ValueError as e:
+        assert "4 bits" in str(e)
+        return
+    outs = llm.generate([{"prompt_token_ids": [5, 7, 11, 13] * n} for n in (3, 30)], SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True, logprobs=0))
+    assert all(len(o.outputs[0].token_ids) == 6 and all(math.isfinite(x.logprob) for d in o.outputs[0].logprobs for x in d.values()) for o in outs)
+    llm.shutdown()

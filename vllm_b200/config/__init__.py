@@ -43,7 +43,7 @@ class CacheConfig(_ConfigBase):
     block_size: int = 64  # tokens per KV page: a K page [64,128] / V^T page [128,64] is one 16 KB SW128 TMA box
     gpu_memory_utilization: float = 0.92
     swap_space_gb: float = 4.0
-    cache_dtype: str = "auto"  # auto|bfloat16|fp8|fp8_e4m3|fp8_e5m2
+    cache_dtype: str = "auto"  # auto|bfloat16|fp8|fp8_e4m3|fp8_e5m2|nvfp4
     num_gpu_blocks_override: Optional[int] = None
     enable_prefix_caching: bool = True
     prefix_caching_hash_algo: str = "sha256"  # sha256|builtin
@@ -60,8 +60,10 @@ class CacheConfig(_ConfigBase):
             raise ValueError(f"gpu_memory_utilization must be in (0,1], got {self.gpu_memory_utilization}")
         if self.block_size <= 0 or self.block_size & (self.block_size - 1):
             raise ValueError(f"block_size must be a positive power of two, got {self.block_size}")
-        if self.cache_dtype not in ("auto", "bfloat16", "float16", "fp8", "fp8_e4m3", "fp8_e5m2"):
+        if self.cache_dtype not in ("auto", "bfloat16", "float16", "fp8", "fp8_e4m3", "fp8_e5m2", "nvfp4"):
             raise ValueError(f"unknown cache_dtype {self.cache_dtype}")
+        if self.cache_dtype == "nvfp4" and self.block_size % 16:
+            raise ValueError(f"cache_dtype nvfp4 has pages of 16 tokens and multiples of it, got block_size {self.block_size}")
 
 
 @dataclass

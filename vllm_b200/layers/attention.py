@@ -8,17 +8,32 @@ RoPE + KV-write + attention call sequence over our own cache layout
 """
 from __future__ import annotations
 
+import dataclasses
 from typing import Optional
 
 import torch
 import torch.nn as nn
 
 from vllm_b200 import envs, ops
-from vllm_b200.core.kv_cache_manager import (FullAttentionSpec, KVCacheSpec, MLAAttentionSpec, SlidingWindowMLASpec,
+from vllm_b200.core.kv_cache_manager import (FullAttentionSpec, KVCacheSpec, MambaSpec, MLAAttentionSpec, SlidingWindowMLASpec,
                                             SlidingWindowSpec)
 from vllm_b200.forward_context import get_forward_context
 
 _LAYER_REGISTRY: dict[str, "Attention"] = {}
+
+
+def fp4_cache_spec(layer, name: str, spec: KVCacheSpec) -> KVCacheSpec:
+    """Spec of a layer whose keys and values are cached in 4 bits: rows of so many bytes.  Recurrent states stay as they are."""
+    if isinstance(spec, MambaSpec):
+        return spec
+    if not isinstance(layer, Attention) or isinstance(spec, MLAAttentionSpec):
+        raise ValueError(f"kv_cache_dtype nvfp4: layer {name!r} caches latents, not keys and values")
+    if layer.v_head_size != layer.head_size or layer.fused_prologue or layer.whole_qk_norm or layer.talk is not None or layer.v_rope is not None:
+        raise ValueError(f"kv_cache_dtype nvfp4: layer {name!r} writes its cache in a kernel of its own, in the model's type")
+    if getattr(spec, "dcp", 1) > 1:
+        raise ValueError("kv_cache_dtype nvfp4 does not cover decode context parallelism")
+    row = ops.fp4_cache_shape(1, layer.num_kv_heads, spec.block_size, layer.head_size)[-1]
+    return dataclasses.replace(spec, head_size=row, dtype_size=1)
 
 
 def attention_layers() -> dict[str, "Attention"]:
@@ -191,6 +206,7 @@ class Attention(nn.Module):
         if pcp is not None and (shared or self.whole_qk_norm or self.talk is not None or self.v_rope is not None):
             raise NotImplementedError("prefill context parallelism does not cover shared caches, norms over whole projections, mixed heads "
                                       "and rotated values")
+        fp4 = kv_cache.dtype is torch.uint8           # 4 bits: ops.fp4_cache_shape
         mpos = ctx.extra.get("mrope_positions") if (self.rope is not None and self.rope.mrope_section) else None
         first = positions
         if qk_norm is not None or self.fused_prologue:
@@ -240,9 +256,12 @@ class Attention(nn.Module):
         elif mpos is not None:
             # multimodal rotary ids differ per channel section for image tokens: rotate un-fused, then the ordinary
             # cache write (text-only steps take the fused path below with 1-D positions = index + per-request delta)
-            q, k = self.rope.forward_mrope(mpos, q, k)
-            ops.reshape_and_cache(k.view(T, self.num_kv_heads, D), v.view(T, self.num_kv_heads, D), kv_cache,
-                                  md.slot_mapping, vt=md.kv_vt)
+            if fp4:
+                q = ops.rope_and_cache_fp4(mpos.long(), q, k, v, self.rope.cos_sin_cache, D, True, kv_cache, md.slot_mapping, axes=self.rope.axes(q.device))
+            else:
+                q, k = self.rope.forward_mrope(mpos, q, k)
+                ops.reshape_and_cache(k.view(T, self.num_kv_heads, D), v.view(T, self.num_kv_heads, D), kv_cache,
+                                      md.slot_mapping, vt=md.kv_vt)
         elif pcp is not None:
             # prefill context parallelism: this rank holds a share of the step's tokens.  Rotate locally, all-gather
             # K / V of the whole step (global token order) so that every rank's cache stays complete, attend for the
@@ -251,15 +270,24 @@ class Attention(nn.Module):
                 q, k = self.rope(positions, q, k)
             Tg = pcp["num_tokens"]
             k_all, v_all = pcp["gather"](k.contiguous()), pcp["gather"](v.contiguous())
-            ops.reshape_and_cache(k_all.view(Tg, self.num_kv_heads, D), v_all.view(Tg, self.num_kv_heads, D), kv_cache,
-                                  pcp["slot_mappings"][ctx.layer_to_group.get(self.layer_name, 0)], vt=md.kv_vt)
+            k_all, v_all = k_all.view(Tg, self.num_kv_heads, D), v_all.view(Tg, self.num_kv_heads, D)
+            slots = pcp["slot_mappings"][ctx.layer_to_group.get(self.layer_name, 0)]
+            if fp4:
+                ops.reshape_and_cache_fp4(k_all, v_all, kv_cache, slots)
+            else:
+                ops.reshape_and_cache(k_all, v_all, kv_cache, slots, vt=md.kv_vt)
+        elif fp4:
+            if self.rope is not None and positions is not None:
+                q = ops.rope_and_cache_fp4(positions, q, k, v, self.rope.cos_sin_cache, D, self.rope.is_neox_style, kv_cache, md.slot_mapping)
+            else:
+                ops.reshape_and_cache_fp4(k.view(T, self.num_kv_heads, D), v.view(T, self.num_kv_heads, D), kv_cache, md.slot_mapping)
         elif self.rope is not None and positions is not None:
             q, k = ops.rope_and_cache(positions, q, k, v, self.rope.cos_sin_cache, D,
                                       self.rope.is_neox_style, kv_cache, md.slot_mapping, vt=md.kv_vt)
         else:
             ops.reshape_and_cache(k.view(T, self.num_kv_heads, D), v.view(T, self.num_kv_heads, D),
                                   kv_cache, md.slot_mapping, vt=md.kv_vt)
-        if (md.cascade is not None and self.causal and not self.sliding_window and self.alibi_slopes is None
+        if (md.cascade is not None and not fp4 and self.causal and not self.sliding_window and self.alibi_slopes is None
                 and self.sinks is None and not self.chunk_size and self.v_head_size == D and out is None):
             # shared prefix: its K/V are read once for the whole batch (all queries sit after it → no causal mask),
             # the per-request remainders are attended separately, the two partial softmaxes are merged by their LSE
@@ -275,6 +303,10 @@ class Attention(nn.Module):
             o = ops.talking_attention(q.view(T, self.num_heads, D), kv_cache, md, self.scale, self.sliding_window, self.logits_soft_cap,
                                       self.talk, self.sinks, self.v_head_size, self.v_rope, first, out=buf)
             return o.reshape(T, self.num_heads * self.v_head_size) if out is None else out
+        if fp4:
+            o = ops.paged_attention_fp4(q.view(T, self.num_heads, D), kv_cache, md, self.scale, self.sliding_window, self.logits_soft_cap, self.causal, out=buf,
+                                        alibi_slopes=self.alibi_slopes, sinks=self.sinks, chunk_size=self.chunk_size, out_scale=self.out_scale)
+            return o.reshape(T, self.num_heads * D) if out is None else out
         o = ops.paged_attention(q.view(T, self.num_heads, D), kv_cache, md, self.scale,
                                 self.sliding_window, self.logits_soft_cap, self.causal, out=buf,
                                 alibi_slopes=self.alibi_slopes, sinks=self.sinks, chunk_size=self.chunk_size,

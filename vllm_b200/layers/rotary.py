@@ -51,6 +51,7 @@ class RotaryEmbedding(nn.Module):
         self.rope_scaling = rope_scaling or {}
         self.mscale = 1.0
         self.mrope_section = self.rope_scaling.get("mrope_section")
+        self._axes: dict[torch.device, torch.Tensor] = {}
         cache = self._build()
         self.register_buffer("cos_sin_cache", cache, persistent=False)
 
@@ -110,23 +111,30 @@ class RotaryEmbedding(nn.Module):
         freqs = torch.outer(t, inv)
         return torch.cat((freqs.cos() * self.mscale, freqs.sin() * self.mscale), dim=-1).float().contiguous()
 
+    def axes(self, device) -> torch.Tensor:
+        """Axis (temporal, height, width) whose position turns pair j of a head, [rotary_dim / 2] int32."""
+        got = self._axes.get(device)
+        if got is None:
+            half, sec = self.rotary_dim // 2, list(self.mrope_section)
+            if self.rope_scaling.get("mrope_interleaved"):
+                # Qwen3-VL: frequency j belongs to axis j % 3 (t, h, w, t, h, w, …) while that axis still has channels left,
+                # the tail falls back to the temporal axis
+                j = torch.arange(half)
+                idx = torch.zeros(half, dtype=torch.int32)
+                for ax in (1, 2):
+                    idx[(j % 3 == ax) & (j < 3 * sec[ax])] = ax
+            else:
+                idx = torch.cat([torch.full((n,), i % 3, dtype=torch.int32) for i, n in enumerate(sec)])[:half]
+            got = self._axes[device] = idx.to(device)
+        return got
+
     def forward_mrope(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor):
         """positions [3, T] (temporal, height, width ids): channel section i of the rotary dims takes its angle from
         row i % 3 (reference: rotary_embedding/mrope.py; HF ``apply_multimodal_rotary_pos_emb``)."""
         half = self.rotary_dim // 2
         cs = self.cos_sin_cache[positions.long()]                              # [3, T, rot]
         cos3, sin3 = cs[..., :half], cs[..., half:]
-        sec = list(self.mrope_section)
-        if self.rope_scaling.get("mrope_interleaved"):
-            # Qwen3-VL: frequency j belongs to axis j % 3 (t, h, w, t, h, w, …) while that axis still has channels left,
-            # the tail falls back to the temporal axis
-            j = torch.arange(half)
-            idx = torch.zeros(half, dtype=torch.long)
-            for ax in (1, 2):
-                idx[(j % 3 == ax) & (j < 3 * sec[ax])] = ax
-            idx = idx.to(q.device)
-        else:
-            idx = torch.cat([torch.full((n,), i % 3, dtype=torch.long) for i, n in enumerate(sec)]).to(q.device)[:half]
+        idx = self.axes(q.device).long()
         ar = torch.arange(half, device=q.device)
         cos = cos3[idx, :, ar].t()                                              # [T, half]
         sin = sin3[idx, :, ar].t()

@@ -346,6 +346,11 @@ def _check_fp4(kv_cache, op: str, k_scale: float = 1.0, v_scale: float = 1.0) ->
     return shape[2], shape[4] * 16 // 9
 
 
+def fp4_decode_supported(D: int, G: int, dtype, other_masks: bool = False) -> bool:
+    """Decode steps of these heads go straight from a cache in 4 bits, without anything that depends on lengths on the host (and may be captured)."""
+    return dtype in _HALF and D in cuda_ops().FP4_HEADS and G <= 64 and not other_masks
+
+
 def _check_slots(slot_mapping, T: int, kv_cache, op: str) -> None:
     if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] < T or not slot_mapping.is_contiguous() \
             or slot_mapping.device != kv_cache.device:

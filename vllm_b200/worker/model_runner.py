@@ -34,7 +34,7 @@ from vllm_b200.config import VllmConfig
 from vllm_b200.core.kv_cache_manager import KVCacheConfig, KVCacheSpec
 from vllm_b200.core.sched_output import LogprobsTensors, ModelRunnerOutput, SchedulerOutput
 from vllm_b200.forward_context import AttentionMetadata, ForwardContext, set_forward_context
-from vllm_b200.layers.attention import attention_layers, clear_attention_layers
+from vllm_b200.layers.attention import attention_layers, clear_attention_layers, fp4_cache_spec
 from vllm_b200.logger import init_logger
 from vllm_b200.sample.sampler import RejectionSampler, Sampler, SamplingMetadata
 from vllm_b200.utils import cdiv
@@ -308,12 +308,19 @@ class ModelRunner:
 
     def get_kv_cache_specs(self) -> dict[str, KVCacheSpec]:
         dsz = self._kv_dtype().itemsize
-        return {name: layer.get_kv_cache_spec(self.block_size, dsz) for name, layer in attention_layers().items()}
+        specs = {name: layer.get_kv_cache_spec(self.block_size, dsz) for name, layer in attention_layers().items()}
+        if self.cc.cache_dtype == "nvfp4":
+            if self.is_cuda and self.dtype not in (torch.bfloat16, torch.float16):
+                raise ValueError(f"kv_cache_dtype nvfp4 takes models of 16 bits on the device, not {self.dtype}")
+            return {name: fp4_cache_spec(attention_layers()[name], name, spec) for name, spec in specs.items()}
+        return specs
 
     def _kv_dtype(self) -> torch.dtype:
         cd = self.cc.cache_dtype
         if cd == "auto":
             return self.dtype
+        if cd == "nvfp4":
+            return torch.uint8                    # rows of codes and scales: the specs count their bytes
         if cd.startswith("fp8"):
             return torch.float8_e5m2 if cd.endswith("e5m2") else torch.float8_e4m3fn
         return {"bfloat16": torch.bfloat16, "float16": torch.float16}[cd]
@@ -1533,13 +1540,17 @@ class ModelRunner:
     # -------------------------------------------------------- CUDA graphs
     def _attention_kernels_cover_model(self) -> bool:
         """False when some attention layer would fall back to the plain-PyTorch op (which syncs with the host)."""
-        from vllm_b200.ops import cuda_attention_supported, cuda_cache_write_supported
+        from vllm_b200.ops import cuda_attention_supported, cuda_cache_write_supported, fp4_decode_supported
         for name, cache in self.kv_caches.items():
             layer = attention_layers().get(name)
             if layer is None or cache.dim() != 5:
                 continue
             vt = self.kv_vt[self.layer_to_group[name]]
             d = layer.head_size
+            if cache.dtype is torch.uint8:
+                if not fp4_decode_supported(d, layer.num_heads // cache.shape[2], self.dtype, layer.alibi_slopes is not None or bool(layer.chunk_size)):
+                    return False
+                continue
             if not cuda_attention_supported(d, getattr(layer, "v_head_size", d), cache.shape[3],
                                             layer.num_heads // cache.shape[2], self.dtype, cache.dtype, vt):
                 return False
