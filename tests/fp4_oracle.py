@@ -29,7 +29,8 @@ def quantise(row, factor=1.0):
         e = nearest(min(max(abs(v) for v in y) / 6, 448.0), SCALES[:127].tolist())
         scales.append(e)
         for v in y:
-            codes.append(0 if e == 0 else nearest(min(abs(v) / float(SCALES[e]), 6.0), MAGNITUDES) + 8 * (v < 0))
+            code = 0 if e == 0 else nearest(min(abs(v) / float(SCALES[e]), 6.0), MAGNITUDES)
+            codes.append(code + 8 * (v < 0 and code > 0))
     return codes, scales
 
 

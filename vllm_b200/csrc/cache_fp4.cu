@@ -21,110 +21,193 @@ struct Turn {
   const float* table;               // [table_rows, rot]: cosines, sines
   int table_rows, rot, n_axes;
 };
-VB_DEVICE void angle(const Turn& r, int t, int pair, float& co, float& si) {
-  const int a = r.axes ? min(max(r.axes[pair], 0), r.n_axes - 1) : 0;
-  int64_t p = r.positions[a * r.pos_stride + t];
-  p = p < 0 ? 0 : p >= r.table_rows ? r.table_rows - 1 : p;       // (nothing is read outside the table)
-  const float* row = r.table + p * r.rot;
-  co = row[pair];
-  si = row[r.rot / 2 + pair];
+// Cosines and sines of the pairs of a block's tokens into shared memory, [tokens][2][rot / 2]: every head of a token takes them
+VB_DEVICE void angles(const Turn& r, int t0, int tokens, float* to) {
+  const int half = r.rot / 2;
+  for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
+    const int t = i / half, pair = i - t * half, a = r.axes ? min(max(r.axes[pair], 0), r.n_axes - 1) : 0;
+    int64_t p = r.positions[a * r.pos_stride + t0 + t];
+    p = p < 0 ? 0 : p >= r.table_rows ? r.table_rows - 1 : p;     // (nothing is read outside the table)
+    const float* row = r.table + p * r.rot + pair;
+    to[t * r.rot + pair] = row[0];
+    to[t * r.rot + half + pair] = row[half];
+  }
+  __syncthreads();
+}
+template <int M> VB_DEVICE void take(const float* at, float (&x)[M]) {          // M: 4 or 8; at a multiple of four
+#pragma unroll
+  for (int i = 0; i < M; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(at + i);
+    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+  }
 }
 VB_DEVICE float turn_a(float a, float b, float co, float si) { return __fsub_rn(__fmul_rn(a, co), __fmul_rn(b, si)); }
 VB_DEVICE float turn_b(float a, float b, float co, float si) { return __fadd_rn(__fmul_rn(b, co), __fmul_rn(a, si)); }
 
-// ROT: 0 none, 1 halves are pairs, 2 neighbours are pairs
-template <typename T, int ROT>
-__global__ void __launch_bounds__(256) write_kernel(T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Turn turn, int Hq, int Hkv, int D,
+// Quotients of values of 16 bits and a scale, for their codes: y r, r the rounded reciprocal, is off by less than 2^-20.  Borders of codes times a scale have seven significant
+// bits, y has at most eleven, so a quotient that is not on a border is 2^-13 or more from it: as multiples of 2^-13 all quotients are on their side.  (A division for each value
+// was a third of the kernel's instructions.)
+VB_DEVICE float on_side(float y, float r) {
+  constexpr float C = 1536.f;
+  return __fsub_rn(__fadd_rn(__fmul_rn(y, r), C), C);
+}
+
+// Eight codes without the signs of zeros
+VB_DEVICE uint32_t unsigned_zeros(uint32_t x) { return x & (0x77777777u | x << 1 | x << 2 | x << 3); }      // (the sign bit stays where one of the three below it is set)
+
+// ROT: 0 none, 1 halves are pairs, 2 neighbours are pairs.  DC: head size and rotated part, or 0.  A lane has a group of 16 values.  A block has some tokens one after the
+// other (several where there are many: their angles, which have to be waited for, come together); a thread's first rows are on their way before the angles are.
+template <typename T, int ROT, int DC>
+__global__ void __launch_bounds__(256) write_kernel(T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Turn turn, int Hq, int Hkv, int D_,
                                                     int64_t q_stride, int64_t k_stride, int64_t v_stride, uint8_t* __restrict__ cache, int64_t num_slots,
-                                                    const int64_t* __restrict__ slots, int BS, float k_factor, float v_factor) {
+                                                    const int64_t* __restrict__ slots, int BS, int shift, float k_factor, float v_factor, int T_, int tokens) {
+  extern __shared__ __align__(16) float angles_s[];
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x, half = turn.rot / 2;
-  const int64_t slot = slots[t];
-  if (slot >= 0 && slot < num_slots) {
-    const int64_t blk = slot / BS, bytes = fp4::page_bytes(BS, D);
-    const int off = (int)(slot - blk * BS), chunks = D / N, side = Hkv * chunks, n = 2 * side;
-    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
-      const int i = i0 + threadIdx.x, j = min(i, n - 1), part = j >= side, h = (j - part * side) / chunks, c = (j - part * side) - h * chunks;
-      if (i0 + (int)(threadIdx.x & ~31u) >= n) break;                 // (whole warps)
-      const T* row = (part ? v + t * v_stride : k + t * k_stride) + (int64_t)h * D;
-      const Vec16<T> x = ld16(row + c * N);
-      float y[N];
+  const int first_t = blockIdx.x * tokens, last_t = min(first_t + tokens, T_), D = DC ? DC : D_, rot = DC ? DC : turn.rot, half = rot / 2;
+  const int groups = D / 16, side = Hkv * groups, n = 2 * side, per = ROT == 0 ? 1 : (ROT == 1 ? half : rot) / N, nq = ROT && q ? Hq * per : 0;
+  struct Item { int part, h, g; };
+  auto item = [&](int i) {
+    const int part = i >= side, h = (i - part * side) / groups;
+    return Item{part, h, i - part * side - h * groups};
+  };
+  auto turned = [&](const Item& m, int u) { return ROT && !m.part && m.g * 16 + u * N < rot; };       // u: half of the group
+  auto load = [&](int t, const Item& m, Vec16<T> (&x)[2], Vec16<T> (&other)[2]) {
+    const T* row = (m.part ? v + t * v_stride : k + t * k_stride) + m.h * D + m.g * 16;
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = to_f32(x.e[e]);
-      if (ROT && !part && c * N < turn.rot) {
-        if (ROT == 1) {
-          const bool first = c * N < half;
-          const Vec16<T> o = ld16(row + c * N + (first ? half : -half));
+    for (int u = 0; u < 2; ++u) {
+      x[u] = ld16(row + u * N);
+      if (ROT == 1 && turned(m, u)) other[u] = ld16(row + u * N + (m.g * 16 + u * N < half ? half : -half));
+    }
+  };
+  auto q_row = [&](int t, int i) { const int h = i / per; return q + t * q_stride + h * D + (i - h * per) * N; };
+  const int64_t bytes = fp4::page_bytes(BS, D);
+  for (int t = first_t; t < last_t; ++t) {
+    const float* angle_s = angles_s + (t - first_t) * rot;
+    const int64_t slot = slots[t];
+    const bool kept = slot >= 0 && slot < num_slots;
+    Item m = item(threadIdx.x);
+    Vec16<T> x[2], other[2], qa, qb;
+    if (kept && threadIdx.x < n) load(t, m, x, other);
+    if (threadIdx.x < nq) {
+      qa = ld16(q_row(t, threadIdx.x));
+      if (ROT == 1) qb = ld16(q_row(t, threadIdx.x) + half);
+    }
+    if (ROT && t == first_t) angles(turn, first_t, last_t - first_t, angles_s);
+    if (kept) {
+      const int64_t blk = shift >= 0 ? slot >> shift : slot / BS;       // (a division of 64 bits was a fifth of the kernel)
+      const int off = (int)(slot - blk * BS);
+      uint8_t* block = cache + blk * 2 * Hkv * bytes;
+      for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        if (i >= (int)blockDim.x) {
+          m = item(i);
+          load(t, m, x, other);
+        }
+        float y[2][N];
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            float co, si;
-            angle(turn, t, c * N + e - (first ? 0 : half), co, si);
-            const float other = to_f32(o.e[e]);
-            y[e] = first ? turn_a(y[e], other, co, si) : turn_b(other, y[e], co, si);
-          }
-        } else {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int e = 0; e < N; e += 2) {
-            float co, si;
-            angle(turn, t, (c * N + e) / 2, co, si);
-            const float a = y[e], b = y[e + 1];
-            y[e] = turn_a(a, b, co, si);
-            y[e + 1] = turn_b(a, b, co, si);
+          for (int e = 0; e < N; ++e) y[u][e] = to_f32(x[u].e[e]);
+          if (turned(m, u)) {
+            const int c = m.g * 2 + u;
+            if (ROT == 1) {
+              const bool first = c * N < half;
+              const float* at = angle_s + c * N - (first ? 0 : half);
+              float co[N], si[N];
+              take(at, co);
+              take(at + half, si);
+#pragma unroll
+              for (int e = 0; e < N; ++e) y[u][e] = turn_b(to_f32(other[u].e[e]), y[u][e], co[e], first ? -si[e] : si[e]);      // (x - y is x + -y)
+            } else {
+              float co[N / 2], si[N / 2];
+              take(angle_s + c * (N / 2), co);
+              take(angle_s + half + c * (N / 2), si);
+#pragma unroll
+              for (int e = 0; e < N; e += 2) {
+                const float a = y[u][e], b = y[u][e + 1];
+                y[u][e] = turn_a(a, b, co[e / 2], si[e / 2]);
+                y[u][e + 1] = turn_b(a, b, co[e / 2], si[e / 2]);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+              const float2 r = unpack2<T>(pack2<T>(y[u][e], y[u][e + 1]));
+              y[u][e] = r.x;
+              y[u][e + 1] = r.y;
+            }
           }
         }
+        const float factor = m.part ? v_factor : k_factor;
+        if (factor != 1.f)
 #pragma unroll
-        for (int e = 0; e < N; ++e) y[e] = to_f32(from_f32<T>(y[e]));
-      }
-      const float factor = part ? v_factor : k_factor;
-      float top = 0.f;
-      bool nan = false;
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (factor != 1.f) y[e] = __fdiv_rn(y[e], factor);
-        top = fmaxf(top, fabsf(y[e]));
-        nan |= y[e] != y[e];
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));         // the other half of the group: D / 8 is even
-      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 1) != 0;
-      const uint32_t e8 = nan ? 0x7fu : fp4::scale_of(top);
-      const float e4 = fp4::scale_value(e8);
+            for (int e = 0; e < N; ++e) y[u][e] = __fdiv_rn(y[u][e], factor);
+        uint32_t top = 0u;                                              // (of the bits: a NaN is above all numbers)
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = e8 == 0u || nan ? 0.f : __fdiv_rn(y[e], e4) + 0.f;      // (no code of -0 for a -0)
-      if (i < n) {
-        uint8_t* page = cache + ((blk * 2 + part) * Hkv + h) * bytes;
-        *reinterpret_cast<uint32_t*>(page + (int64_t)off * (D / 2) + c * (N / 2)) = fp4::pack8(y);
-        if ((c & 1) == 0) page[(int64_t)BS * (D / 2) + (int64_t)off * (D / 16) + c / 2] = (uint8_t)e8;
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(y[u][e]) & 0x7fffffffu);
+        const bool nan = top > 0x7f800000u;
+        const uint32_t e8 = nan ? 0x7fu : fp4::scale_of(__uint_as_float(top));
+        const float e4 = fp4::scale_value(e8);
+        if (e8 == 0u || nan) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[u][e] = 0.f;
+        } else if (factor != 1.f) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[u][e] = __fdiv_rn(y[u][e], e4);
+        } else {
+          const float r = __frcp_rn(e4);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[u][e] = on_side(y[u][e], r);
+        }
+        uint2 codes = make_uint2(fp4::pack8(y[0]), fp4::pack8(y[1]));
+        codes.x = unsigned_zeros(codes.x);
+        codes.y = unsigned_zeros(codes.y);
+        uint8_t* page = block + (m.part * Hkv + m.h) * bytes;
+        *reinterpret_cast<uint2*>(page + off * (D / 2) + m.g * 8) = codes;
+        page[BS * (D / 2) + off * (D / 16) + m.g] = (uint8_t)e8;
       }
     }
-  }
-  if (ROT && q) {
-    const int per = (ROT == 1 ? half : turn.rot) / N;
-    for (int i = threadIdx.x; i < Hq * per; i += blockDim.x) {
-      T* row = q + t * q_stride + (int64_t)(i / per) * D + (i % per) * N;
-      Vec16<T> a = ld16(row), b;
-      if (ROT == 1) {
-        b = ld16(row + half);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          float co, si;
-          angle(turn, t, (i % per) * N + e, co, si);
-          const float x = to_f32(a.e[e]), y = to_f32(b.e[e]);
-          a.e[e] = from_f32<T>(turn_a(x, y, co, si));
-          b.e[e] = from_f32<T>(turn_b(x, y, co, si));
+    if (ROT) {
+      for (int i = threadIdx.x; i < nq; i += blockDim.x) {
+        T* row = q_row(t, i);
+        const int c = i % per;
+        if (i >= (int)blockDim.x) {
+          qa = ld16(row);
+          if (ROT == 1) qb = ld16(row + half);
         }
-        st16(row + half, b);
-      } else {
+        if (ROT == 1) {
+          float co[N], si[N];
+          take(angle_s + c * N, co);
+          take(angle_s + half + c * N, si);
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          float co, si;
-          angle(turn, t, ((i % per) * N + e) / 2, co, si);
-          const float x = to_f32(a.e[e]), y = to_f32(a.e[e + 1]);
-          a.e[e] = from_f32<T>(turn_a(x, y, co, si));
-          a.e[e + 1] = from_f32<T>(turn_b(x, y, co, si));
+          for (int e = 0; e < N; ++e) {
+            const float a = to_f32(qa.e[e]), b = to_f32(qb.e[e]);
+            qa.e[e] = from_f32<T>(turn_a(a, b, co[e], si[e]));
+            qb.e[e] = from_f32<T>(turn_b(a, b, co[e], si[e]));
+          }
+          st16(row + half, qb);
+        } else {
+          float co[N / 2], si[N / 2];
+          take(angle_s + c * (N / 2), co);
+          take(angle_s + half + c * (N / 2), si);
+#pragma unroll
+          for (int e = 0; e < N; e += 2) {
+            const float a = to_f32(qa.e[e]), b = to_f32(qa.e[e + 1]);
+            qa.e[e] = from_f32<T>(turn_a(a, b, co[e / 2], si[e / 2]));
+            qa.e[e + 1] = from_f32<T>(turn_b(a, b, co[e / 2], si[e / 2]));
+          }
         }
+        st16(row, qa);
       }
-      st16(row, a);
     }
   }
 }
@@ -135,11 +218,15 @@ template <typename T> VB_DEVICE Vec16<T> row_chunk(uint32_t codes, uint32_t scal
   fp4::unpack8(codes, r);
   const uint32_t s2 = fp4::low2(fp4::scales2(scale));
   Vec16<T> o;
+  uint32_t* w = &o.u.x;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 x = unpack2<__half>(fp4::mul2(r[i], s2));
-    o.e[2 * i] = from_f32<T>(x.x * factor);
-    o.e[2 * i + 1] = from_f32<T>(x.y * factor);
+    w[i] = fp4::mul2(r[i], s2);
+    if (DTypeOf<T>::v != DT_F16 || factor != 1.f) {
+      float2 x = unpack2<__half>(w[i]);
+      if (factor != 1.f) { x.x *= factor; x.y *= factor; }
+      w[i] = pack2<T>(x.x, x.y);
+    }
   }
   return o;
 }
@@ -149,41 +236,60 @@ struct Source {
   int64_t num_blocks;
   const int* block_table;
   int64_t bt_stride;
-  int width, BS, D, Hkv;
+  int width, BS, D, Hkv, shift;              // shift: of BS where that is a power of two, or -1
 };
-VB_DEVICE const uint8_t* page_of(const Source& s, int b, int part, int h, int tok) {
-  int64_t blk = s.block_table[b * s.bt_stride + tok / s.BS];
-  if ((uint64_t)blk >= (uint64_t)s.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
-  return s.cache + ((blk * 2 + part) * s.Hkv + h) * fp4::page_bytes(s.BS, s.D);
+int shift_of(int BS) {
+  int shift = 0;
+  while (1 << shift < BS) ++shift;
+  return 1 << shift == BS ? shift : -1;
 }
-VB_DEVICE void load_chunk(const Source& s, int b, int part, int h, int tok, int c, uint32_t& codes, uint32_t& scale) {
-  const uint8_t* page = page_of(s, b, part, h, tok);
-  const int off = tok % s.BS;
-  codes = *reinterpret_cast<const uint32_t*>(page + (int64_t)off * (s.D / 2) + c * 4);
-  scale = page[(int64_t)s.BS * (s.D / 2) + (int64_t)off * (s.D / 16) + c / 2];
+Source source(const void* cache, int64_t num_blocks, const int* block_table, int64_t bt_stride, int width, int BS, int D, int Hkv) {
+  return Source{(const uint8_t*)cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv, shift_of(BS)};
+}
+// Codes and scales of a chunk of a row's keys and values
+VB_DEVICE void load_chunk(const Source& s, int b, int h, int tok, int c, uint32_t (&codes)[2], uint32_t (&scale)[2]) {
+  const int p = s.shift >= 0 ? tok >> s.shift : tok / s.BS, off = tok - p * s.BS, bytes = (int)fp4::page_bytes(s.BS, s.D);
+  int64_t blk = s.block_table[b * s.bt_stride + p];
+  if ((uint64_t)blk >= (uint64_t)s.num_blocks) blk = 0;             // (a table may not say that; nothing is read outside the cache)
+  const uint8_t* k = s.cache + (uint32_t)(blk * 2 * s.Hkv + h) * (uint64_t)(uint32_t)bytes;      // (pages of heads have 144 bytes or more: below 2^31 of them)
+  const int64_t to_v = (int64_t)s.Hkv * bytes;
+  const int at = off * (s.D / 2) + c * 4, sc = s.BS * (s.D / 2) + off * (s.D / 16) + c / 2;
+  codes[0] = *reinterpret_cast<const uint32_t*>(k + at);
+  codes[1] = *reinterpret_cast<const uint32_t*>(k + to_v + at);
+  scale[0] = k[sc];
+  scale[1] = k[to_v + sc];
 }
 
-// Grid (runs of ROWS rows, kv heads, requests): rows [first, first + n) of a request to rows [cu[b], cu[b + 1]) of k and v
-constexpr int ROWS = 64, READERS = 256;
-template <typename T>
+// Grid (runs of rows, requests): rows [first, first + n) of a request to rows [cu[b], cu[b + 1]) of k and v.  A block has all heads of a run of rows, so that what it
+// writes lies together; a thread's loads are on their way before it writes.  EVEN: the chunks of a row divide the block, so that a thread stays with its chunk.
+constexpr int READERS = 256, AHEAD = 4;
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(READERS) gather_kernel(Source s, const int* __restrict__ cu, const int* __restrict__ starts, T* __restrict__ k, T* __restrict__ v,
-                                                         int64_t k_stride, int64_t v_stride, int64_t num_rows, float k_factor, float v_factor) {
+                                                         int64_t k_stride, int64_t v_stride, int64_t num_rows, int run, float k_factor, float v_factor) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, h = blockIdx.y, to = cu[b], n = cu[b + 1] - to, first = starts ? starts[b] : 0, chunks = s.D / N;
-  const int r0 = blockIdx.x * ROWS, r1 = min(r0 + ROWS, n);
-  for (int i = threadIdx.x; i < (r1 - r0) * chunks; i += READERS) {
-    const int r = r0 + i / chunks, c = i % chunks;
-    const int64_t tok = (int64_t)first + r;
-    if ((uint64_t)((int64_t)to + r) >= (uint64_t)num_rows) continue;
-    const bool real = tok >= 0 && tok < (int64_t)s.width * s.BS;
-    uint32_t codes[2] = {0u, 0u}, scale[2] = {0u, 0u};
-    if (real) {
-      load_chunk(s, b, 0, h, (int)tok, c, codes[0], scale[0]);
-      load_chunk(s, b, 1, h, (int)tok, c, codes[1], scale[1]);
+  const int b = blockIdx.y, to = cu[b], n = cu[b + 1] - to, first = starts ? starts[b] : 0, chunks = s.D / N, wide = s.Hkv * chunks;
+  const int r0 = blockIdx.x * run, rows = min(run, n - r0), items = rows * wide;
+  const int r1 = threadIdx.x / wide, hc = threadIdx.x - r1 * wide, step = READERS / (EVEN ? wide : 1);
+  for (int i0 = threadIdx.x, turn = 0; i0 < items; i0 += READERS * AHEAD, turn += AHEAD) {
+    uint32_t codes[AHEAD][2], scale[AHEAD][2];
+    auto row_of = [&](int j) { return EVEN ? r1 + (turn + j) * step : (i0 + j * READERS) / wide; };
+    auto place_of = [&](int j) { return EVEN ? hc : (i0 + j * READERS) % wide; };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = i0 + j * READERS, r = row_of(j), at = place_of(j), h = at / chunks;
+      const int64_t tok = (int64_t)first + r0 + r;
+      codes[j][0] = codes[j][1] = scale[j][0] = scale[j][1] = 0u;
+      if (i < items && tok >= 0 && tok < (int64_t)s.width * s.BS) load_chunk(s, b, h, (int)tok, at - h * chunks, codes[j], scale[j]);
     }
-    st16(k + (int64_t)(to + r) * k_stride + (int64_t)h * s.D + c * N, row_chunk<T>(codes[0], scale[0], k_factor));
-    st16(v + (int64_t)(to + r) * v_stride + (int64_t)h * s.D + c * N, row_chunk<T>(codes[1], scale[1], v_factor));
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = i0 + j * READERS, r = row_of(j), at = place_of(j);
+      const int64_t row = (int64_t)to + r0 + r;
+      if (i >= items || (uint64_t)row >= (uint64_t)num_rows) continue;
+      st16(k + row * k_stride + at * N, row_chunk<T>(codes[j][0], scale[j][0], k_factor));
+      st16(v + row * v_stride + at * N, row_chunk<T>(codes[j][1], scale[j][1], v_factor));
+    }
   }
 }
 
@@ -226,10 +332,7 @@ __global__ void __launch_bounds__(READERS) pages_kernel(Source s, const int* __r
   for (int i = threadIdx.x; i < PS * chunks; i += READERS) {
     const int r = i / chunks, c = i % chunks, tok = p * PS + r;
     uint32_t codes[2] = {0u, 0u}, scale[2] = {0u, 0u};
-    if (tok < n && c < real) {
-      load_chunk(s, b, 0, h, tok, c, codes[0], scale[0]);
-      load_chunk(s, b, 1, h, tok, c, codes[1], scale[1]);
-    }
+    if (tok < n && c < real) load_chunk(s, b, h, tok, c, codes, scale);
     st16(kp + r * w + c * N, row_chunk<T>(codes[0], scale[0], 1.f));
     const Vec16<T> x = row_chunk<T>(codes[1], scale[1], 1.f);
     if (VT) {
@@ -279,11 +382,12 @@ EXPORT int vb_write_fp4(const int64_t* positions, int64_t pos_stride, int n_axes
   if (T <= 0) return 0;
   if (bad_shape(D, BS, dtype) || Hkv < 1 || rot < 0 || rot > D || rot % 16 || (rot && (!positions || !table || table_rows < 1 || n_axes < 1))) return -1;
   const Turn turn{positions, pos_stride, axes, table, table_rows, rot, n_axes};
-  const int items = max(2 * Hkv * (D / N), rot ? Hq * (rot / (neox ? 2 * N : N)) : 0), threads = min(256, (items + 31) / 32 * 32);
+  const int items = max(2 * Hkv * (D / 16), rot ? Hq * (rot / (neox ? 2 * N : N)) : 0), threads = min(256, (items + 31) / 32 * 32);
+  const int tokens = T >= 2048 ? 4 : T >= 1024 ? 2 : 1;          // of a block: the SMs hold about a thousand blocks
   DISPATCH_HALF(dtype, TT, {
-    auto kernel = rot == 0 ? write_kernel<TT, 0> : neox ? write_kernel<TT, 1> : write_kernel<TT, 2>;
-    vb_launch(kernel, dim3(T), dim3(threads), 0, st, (TT*)q, (const TT*)k, (const TT*)v, turn, Hq, Hkv, D, q_stride, k_stride, v_stride, (uint8_t*)cache,
-              num_blocks * BS, slots, BS, k_factor, v_factor);
+    auto kernel = rot == 0 ? write_kernel<TT, 0, 0> : !neox ? write_kernel<TT, 2, 0> : rot == 128 && D == 128 ? write_kernel<TT, 1, 128> : write_kernel<TT, 1, 0>;
+    vb_launch(kernel, dim3((T + tokens - 1) / tokens), dim3(threads), (size_t)tokens * rot * 4, st, (TT*)q, (const TT*)k, (const TT*)v, turn, Hq, Hkv, D, q_stride, k_stride, v_stride,
+              (uint8_t*)cache, num_blocks * BS, slots, BS, shift_of(BS), k_factor, v_factor, T, tokens);
   });
   return (int)cudaGetLastError();
 }
@@ -295,9 +399,13 @@ EXPORT int vb_gather_fp4(const void* cache, int64_t num_blocks, const int* block
                          cudaStream_t st) {
   if (B <= 0 || max_rows <= 0 || num_rows <= 0) return 0;
   if (bad_shape(D, BS, dtype) || Hkv < 1 || Hkv > 65535 || B > 65535 || width < 0) return -1;
-  const Source s{(const uint8_t*)cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv};
-  DISPATCH_HALF(dtype, TT, vb_launch(gather_kernel<TT>, dim3((max_rows + ROWS - 1) / ROWS, Hkv, B), dim3(READERS), 0, st, s, cu, starts, (TT*)k, (TT*)v, k_stride, v_stride,
-                                     num_rows, k_factor, v_factor));
+  const Source s = source(cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv);
+  const int wide = Hkv * (D / N), run = max(1, 1024 / wide);          // (four items of keys and values for every thread)
+  if (((int64_t)max_rows + run - 1) / run > 0x7fffffff) return -1;
+  DISPATCH_HALF(dtype, TT, {
+    auto kernel = wide <= READERS && READERS % wide == 0 ? gather_kernel<TT, true> : gather_kernel<TT, false>;
+    vb_launch(kernel, dim3((max_rows + run - 1) / run, B), dim3(READERS), 0, st, s, cu, starts, (TT*)k, (TT*)v, k_stride, v_stride, num_rows, run, k_factor, v_factor);
+  });
   return (int)cudaGetLastError();
 }
 
@@ -309,7 +417,7 @@ EXPORT int vb_pages_fp4(const void* cache, int64_t num_blocks, const int* block_
   if (bad_shape(D, BS, dtype) || Hkv < 1 || Hkv > 65535 || B > 65535 || width < 0 || table_width < 1 || PS < 1 || num_pages < 0 || W < D || W % N ||
       (vt && (W != 128 || PS != 64)))
     return -1;
-  const Source s{(const uint8_t*)cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv};
+  const Source s = source(cache, num_blocks, block_table, bt_stride, width, BS, D, Hkv);
   DISPATCH_HALF(dtype, TT, {
     auto kernel = vt ? pages_kernel<TT, true> : pages_kernel<TT, false>;
     vb_launch(kernel, dim3(table_width, Hkv, B), dim3(READERS), 0, st, s, seq_lens, qsl, few, (TT*)pages, num_pages, PS, W, table, lens);

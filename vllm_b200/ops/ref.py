@@ -163,7 +163,7 @@ def fp4_quant_rows(x: torch.Tensor, factor: float = 1.0) -> tuple[torch.Tensor, 
     code = torch.zeros_like(m, dtype=torch.uint8)
     for border, up in ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)):
         code += m >= border if up else m > border
-    code = (code + 8 * (y < 0).to(torch.uint8)).flatten(-2)
+    code = (code + 8 * ((y < 0) & (code > 0)).to(torch.uint8)).flatten(-2)              # (a code of 0 has no sign)
     return code[..., 0::2] | (code[..., 1::2] << 4), e.view(torch.uint8)
 
 
