@@ -58,7 +58,7 @@ VB_DEVICE uint32_t unsigned_zeros(uint32_t x) { return x & (0x77777777u | x << 1
 // ROT: 0 none, 1 halves are pairs, 2 neighbours are pairs.  DC: head size and rotated part, or 0.  A lane has a group of 16 values.  A block has some tokens one after the
 // other (several where there are many: their angles, which have to be waited for, come together); a thread's first rows are on their way before the angles are.
 template <typename T, int ROT, int DC>
-__global__ void __launch_bounds__(256) write_kernel(T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Turn turn, int Hq, int Hkv, int D_,
+__global__ void __launch_bounds__(256, 4) write_kernel(T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Turn turn, int Hq, int Hkv, int D_,
                                                     int64_t q_stride, int64_t k_stride, int64_t v_stride, uint8_t* __restrict__ cache, int64_t num_slots,
                                                     const int64_t* __restrict__ slots, int BS, int shift, float k_factor, float v_factor, int T_, int tokens) {
   extern __shared__ __align__(16) float angles_s[];
@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(256) write_kernel(T* __restrict__ q, const T* 
     const bool kept = slot >= 0 && slot < num_slots;
     Item m = item(threadIdx.x);
     Vec16<T> x[2], other[2], qa, qb;
-    if (kept && threadIdx.x < n) load(t, m, x, other);
-    if (threadIdx.x < nq) {
+    if (kept && (int)threadIdx.x < n) load(t, m, x, other);
+    if ((int)threadIdx.x < nq) {
       qa = ld16(q_row(t, threadIdx.x));
       if (ROT == 1) qb = ld16(q_row(t, threadIdx.x) + half);
     }
@@ -383,7 +383,7 @@ EXPORT int vb_write_fp4(const int64_t* positions, int64_t pos_stride, int n_axes
   if (bad_shape(D, BS, dtype) || Hkv < 1 || rot < 0 || rot > D || rot % 16 || (rot && (!positions || !table || table_rows < 1 || n_axes < 1))) return -1;
   const Turn turn{positions, pos_stride, axes, table, table_rows, rot, n_axes};
   const int items = max(2 * Hkv * (D / 16), rot ? Hq * (rot / (neox ? 2 * N : N)) : 0), threads = min(256, (items + 31) / 32 * 32);
-  const int tokens = T >= 2048 ? 4 : T >= 1024 ? 2 : 1;          // of a block: the SMs hold about a thousand blocks
+  const int tokens = T >= 4096 ? 2 : 1;          // of a block: the SMs hold 592 blocks
   DISPATCH_HALF(dtype, TT, {
     auto kernel = rot == 0 ? write_kernel<TT, 0, 0> : !neox ? write_kernel<TT, 2, 0> : rot == 128 && D == 128 ? write_kernel<TT, 1, 128> : write_kernel<TT, 1, 0>;
     vb_launch(kernel, dim3((T + tokens - 1) / tokens), dim3(threads), (size_t)tokens * rot * 4, st, (TT*)q, (const TT*)k, (const TT*)v, turn, Hq, Hkv, D, q_stride, k_stride, v_stride,

@@ -813,11 +813,14 @@ def fp4_plan(device: int, D: int, rows: int, parts: int) -> tuple[int, int, int]
 
 
 def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
-    """CTAs of a cluster that has a row of the schedule, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel."""
-    if tiles > 64 or rows > 512:
-        return 0
-    parts = 8 if tiles > 8 else 4 if tiles > 4 else 2
-    return parts if rows <= fp4_plan(_device(), D, min(query_rows, 9), parts)[2] else 0
+    """CTAs of a cluster that has a row of the schedule, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel.  us with 8, 4, 2, 1 and 0,
+    heads of 128: 8 rows of 700 6.4, 6.7, 7.7, 9.5, 7.6; 32 of 2000 10.1, 9.9, 13.6, 21.0, 12.1; 64 of 2000 17.7, 13.4, 13.6, 21.1, 13.5; 512 of 250 71, 34, 22, 15.5, 18.8; 512 of
+    1000 85, 48, 36, 32, 32; of 64, 192 of 60 to 924 21, 16, 11.6, 12.4, 12.8."""
+    query_rows, sms = min(query_rows, 9), num_sms()
+    for parts in (8, 4, 2):
+        if parts // 2 < tiles <= 10 * parts and rows * parts <= 3 * sms and rows <= fp4_plan(_device(), D, query_rows, parts)[2]:
+            return parts
+    return int(tiles <= 8 and rows <= fp4_plan(_device(), D, query_rows, 0)[1] * sms)
 
 
 def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
@@ -830,7 +833,7 @@ def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scal
     chunks = -(-query_rows // cols)
     group = min(512, 65535 // (H * chunks))
     group = -(-B // -(-B // group))
-    parts = fp4_parts(B * H * chunks, tiles, D, query_rows) if group >= B else 0
+    parts = fp4_parts(B * H * chunks, tiles, D, query_rows) if B <= group else 0
     ctas, rows, ws = ctas * sms, group * H * chunks, None
     if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
         ws = torch.empty((rows + ctas) * cols * (D + 2) + 2 * rows, dtype=torch.float32, device=q.device)
