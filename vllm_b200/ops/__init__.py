@@ -8,6 +8,7 @@ missing raises — it never silently falls back to eager PyTorch.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -338,12 +339,14 @@ def fp4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int, head_si
 def _check_fp4(kv_cache, op: str, k_scale: float = 1.0, v_scale: float = 1.0) -> tuple[int, int]:
     """(kv heads, head size) of a cache in 4 bits."""
     shape = kv_cache.shape
-    if kv_cache.dtype is not torch.uint8 or len(shape) != 5 or shape[1] != 2 or shape[3] < 16 or shape[3] % 16 or shape[4] < 9 or shape[4] % 9 \
-            or not kv_cache.is_contiguous():
+    if len(shape) != 5 or kv_cache.dtype is not torch.uint8 or not kv_cache.is_contiguous():
         raise ValueError(f"{op}: a contiguous uint8 cache of fp4_cache_shape; got {tuple(shape)} of {kv_cache.dtype}")
-    if not (0.0 < k_scale < float("inf") and 0.0 < v_scale < float("inf")):
+    _, two, H, page, row = shape
+    if two != 2 or page < 16 or page % 16 or row < 9 or row % 9 or H < 1:
+        raise ValueError(f"{op}: a cache of fp4_cache_shape; got {tuple(shape)}")
+    if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
         raise ValueError(f"{op}: factors of keys and values above 0; got {k_scale} and {v_scale}")
-    return shape[2], shape[4] * 16 // 9
+    return H, row * 16 // 9
 
 
 def fp4_decode_supported(D: int, G: int, dtype, other_masks: bool = False) -> bool:
@@ -367,7 +370,7 @@ def reshape_and_cache_fp4(key, value, kv_cache, slot_mapping, k_scale: float = 1
         raise ValueError(f"{op}: keys {tuple(key.shape)} and values {tuple(value.shape)} for {H} heads of {D}")
     _check_slots(slot_mapping, key.shape[0], kv_cache, op)
     if _use_cuda(key):
-        return cuda_ops().write_fp4(None, None, None, key, value, None, D, True, kv_cache, slot_mapping, k_scale, v_scale)
+        return cuda_ops().write_fp4(None, None, None, key, value, None, H, D, True, kv_cache, slot_mapping, k_scale, v_scale)
     return ref.reshape_and_cache_fp4(key, value, kv_cache, slot_mapping[:key.shape[0]], k_scale, v_scale)
 
 
@@ -391,7 +394,7 @@ def rope_and_cache_fp4(positions, q, k, v, cos_sin_cache, head_dim: int, is_neox
         raise ValueError(f"{op}: axes int32 [{rot // 2}]; got {tuple(axes.shape)} of {axes.dtype}")
     _check_slots(slot_mapping, T, kv_cache, op)
     if _use_cuda(q) and rot % 16 == 0 and q.dtype in _HALF:
-        return cuda_ops().write_fp4(positions, axes, q, k, v, cos_sin_cache, D, is_neox, kv_cache, slot_mapping, k_scale, v_scale)
+        return cuda_ops().write_fp4(positions, axes, q, k, v, cos_sin_cache, H, D, is_neox, kv_cache, slot_mapping, k_scale, v_scale)
     at, table = (positions[:T], cos_sin_cache) if axes is None else (torch.arange(T, device=q.device), ref.axes_table(positions[:, :T], cos_sin_cache, axes))
     q2, k2 = ref.rotary_embedding(at, q, k, table, D, is_neox)
     q.copy_(q2)
@@ -416,7 +419,7 @@ def gather_cache_fp4(kv_cache, block_table, cu_seq_lens, k, v, max_tokens: int, 
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < B or block_table.device != dev:
         raise ValueError(f"{op}: an int32 block table of {B} requests; got {tuple(block_table.shape)} of {block_table.dtype}")
     if _use_cuda(kv_cache):
-        return cuda_ops().gather_fp4(kv_cache, block_table, cu_seq_lens, k, v, max_tokens, seq_starts, k_scale, v_scale)
+        return cuda_ops().gather_fp4(kv_cache, block_table, cu_seq_lens, k, v, H, D, max_tokens, seq_starts, k_scale, v_scale)
     return ref.gather_cache_fp4(kv_cache, block_table, cu_seq_lens, k, v, seq_starts, k_scale, v_scale)
 
 
@@ -427,19 +430,19 @@ def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft
     which the cache stands for."""
     op = "paged_attention_fp4"
     H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H or q.device != kv_cache.device:
-        raise ValueError(f"{op}: queries {tuple(q.shape)} of {q.dtype} for a cache of {H} heads of {D}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] % H or q.get_device() != kv_cache.get_device():
+        raise ValueError(f"{op}: queries {tuple(shape)} of {q.dtype} for a cache of {H} heads of {D}")
     if md.kv_vt:
         raise ValueError(f"{op}: a cache in 4 bits has no transposed values")
-    if q.shape[0] < (md.num_reqs if md.decode_only else md.num_actual_tokens):
-        raise ValueError(f"{op}: {q.shape[0]} queries for a step of {md.num_reqs if md.decode_only else md.num_actual_tokens}")
-    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != D):
+    if shape[0] < (md.num_reqs if md.decode_only else md.num_actual_tokens):
+        raise ValueError(f"{op}: {shape[0]} queries for a step of {md.num_reqs if md.decode_only else md.num_actual_tokens}")
+    if out is not None and (out.shape != shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != D):
         raise ValueError(f"{op}: out {tuple(out.shape)} of {out.dtype}, the heads of a row next to each other")
-    for name, t in (("sinks", sinks), ("alibi_slopes", alibi_slopes)):
-        if t is not None and t.numel() != q.shape[1]:
-            raise ValueError(f"{op}: {t.numel()} {name} for {q.shape[1]} heads")
+    if (sinks is not None and sinks.numel() != shape[1]) or (alibi_slopes is not None and alibi_slopes.numel() != shape[1]):
+        raise ValueError(f"{op}: a sink and a slope for each of {shape[1]} heads, where there are any")
     if _use_cuda(q):
-        return cuda_ops().paged_attention_fp4(q, kv_cache, md, scale, sliding_window, logits_soft_cap, causal, out, alibi_slopes, sinks, chunk_size, return_lse,
+        return cuda_ops().paged_attention_fp4(q, kv_cache, md, H, D, scale, sliding_window, logits_soft_cap, causal, out, alibi_slopes, sinks, chunk_size, return_lse,
                                               out_scale, k_scale, v_scale)
     sl = md.seq_lens_cpu if md.seq_lens_cpu is not None else md.seq_lens.cpu()
     if md.decode_only and md.query_start_loc is None:

@@ -763,38 +763,45 @@ def _fp4_half(x, kv_cache, op: str) -> int:
 def _fp4_rows(x, width: int):
     """Rows of ``width`` values next to each other, at 16-byte addresses."""
     if x.dim() == 3:
-        x = x.flatten(1) if x.stride(2) == 1 and x.stride(1) == x.shape[2] else x.reshape(x.shape[0], width)
-    return _heads(x if x.stride(1) == 1 else x.contiguous())
+        _, head, one = x.stride()
+        if one != 1 or head != x.shape[2]:
+            x = x.reshape(x.shape[0], width)
+    elif x.stride(1) != 1:
+        x = x.contiguous()
+    return _heads(x)
 
 
-def write_fp4(positions, axes, q, k, v, table, D: int, neox: bool, kv_cache, slots, k_scale: float, v_scale: float):
+def write_fp4(positions, axes, q, k, v, table, H: int, D: int, neox: bool, kv_cache, slots, k_scale: float, v_scale: float):
     """Rotation (positions None: none) and quantisation of new tokens; q in place."""
-    T, H = k.shape[0], kv_cache.shape[2]
-    dtype = _fp4_half(k, kv_cache, "write_fp4")
+    T, dtype, blocks, BS = k.shape[0], _fp4_half(k, kv_cache, "write_fp4"), kv_cache.shape[0], kv_cache.shape[3]
     if not T:
         return q
     k, v = _fp4_rows(k, H * D), _fp4_rows(v, H * D)
-    rot, Hq, turned = (0, 0, None) if positions is None else (table.shape[1], q.shape[1] // D, _fp4_rows(q, q.shape[1]))
-    if rot and positions.stride(-1) != 1:
+    if positions is None:
+        _check(_write_fp4(None, 0, 1, None, None, 0, 0, 1, None, k.data_ptr(), v.data_ptr(), T, 0, H, D, 0, k.stride(0), v.stride(0), kv_cache.data_ptr(), blocks, slots.data_ptr(),
+                          BS, k_scale, v_scale, dtype, _st()), "write_fp4")
+        return q
+    (rows, rot), width = table.shape, q.shape[1]
+    turned = _fp4_rows(q, width)
+    if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    _check(_write_fp4(_p(positions), 0 if axes is None else positions.stride(0), 1 if axes is None else positions.shape[0], _p(axes), _p(table),
-                      table.shape[0] if rot else 0, rot, int(neox), _p(turned), k.data_ptr(), v.data_ptr(), T, Hq, H, D, turned.stride(0) if rot else 0, k.stride(0),
-                      v.stride(0), kv_cache.data_ptr(), kv_cache.shape[0], slots.data_ptr(), kv_cache.shape[3], k_scale, v_scale, dtype, _st()), "write_fp4")
-    if turned is not None and turned.data_ptr() != q.data_ptr():
+    step, n = (0, 1) if axes is None else (positions.stride(0), positions.shape[0])
+    _check(_write_fp4(positions.data_ptr(), step, n, _p(axes), table.data_ptr(), rows, rot, int(neox), turned.data_ptr(), k.data_ptr(), v.data_ptr(), T, width // D, H, D,
+                      turned.stride(0), k.stride(0), v.stride(0), kv_cache.data_ptr(), blocks, slots.data_ptr(), BS, k_scale, v_scale, dtype, _st()), "write_fp4")
+    if turned is not q and turned.data_ptr() != q.data_ptr():
         q.copy_(turned)
     return q
 
 
-def gather_fp4(kv_cache, block_table, cu, k, v, max_tokens: int, starts, k_scale: float, v_scale: float) -> None:
-    _, _, H, BS, row = kv_cache.shape
-    D, dtype = row * 16 // 9, _fp4_half(k, kv_cache, "gather_cache_fp4")
-    for t in (k, v):
-        if t.stride(2) != 1 or t.stride(1) != D or t.data_ptr() % 16 or t.stride(0) % 8:
-            raise ValueError("gather_cache_fp4: rows of k and v at 16-byte addresses, their heads next to each other")
-    if block_table.stride(1) != 1:
+def gather_fp4(kv_cache, block_table, cu, k, v, H: int, D: int, max_tokens: int, starts, k_scale: float, v_scale: float) -> None:
+    dtype = _fp4_half(k, kv_cache, "gather_cache_fp4")
+    (kr, kh, ke), (vr, vh, ve), (br, be) = k.stride(), v.stride(), block_table.stride()
+    if ke != 1 or ve != 1 or kh != D or vh != D or kr % 8 or vr % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+        raise ValueError("gather_cache_fp4: rows of k and v at 16-byte addresses, their heads next to each other")
+    if be != 1:
         raise ValueError("gather_cache_fp4: a request's pages are next to each other in the block table")
-    _check(_gather_fp4(kv_cache.data_ptr(), kv_cache.shape[0], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu.data_ptr(), _p(starts), k.data_ptr(),
-                       v.data_ptr(), k.stride(0), v.stride(0), k.shape[0], cu.numel() - 1, max_tokens, H, D, BS, k_scale, v_scale, dtype, _st()), "gather_cache_fp4")
+    _check(_gather_fp4(kv_cache.data_ptr(), kv_cache.shape[0], block_table.data_ptr(), br, block_table.shape[1], cu.data_ptr(), _p(starts), k.data_ptr(), v.data_ptr(), kr, vr,
+                       k.shape[0], cu.shape[0] - 1, max_tokens, H, D, kv_cache.shape[3], k_scale, v_scale, dtype, _st()), "gather_cache_fp4")
 
 
 _attention_fp4 = _sig("vb_attention_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _f, _f, _f,
@@ -823,23 +830,29 @@ def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
     return int(tiles <= 8 and rows <= fp4_plan(_device(), D, query_rows, 0)[1] * sms)
 
 
-def _fp4_few(q, kv_cache, md, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
-    """Attention of the requests with at most ``few`` new tokens, straight from the cache; rows of the others are not touched."""
-    (_, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
-    bt, B, sms = md.block_table, md.num_reqs, num_sms()
-    max_rows = max(1, min(bt.shape[1] * BS, md.max_seq_len))
-    query_rows, tiles = few * (Hq // H), -(-max_rows // 64)
-    cols, ctas, _ = fp4_plan(_device(), D, min(query_rows, 9), 0)
+@functools.lru_cache(maxsize=4096)
+def fp4_schedule(device: int, B: int, H: int, G: int, D: int, few: int, max_rows: int) -> tuple[int, int, int, int, int]:
+    """(CTAs, CTAs of a cluster that has a row, requests of a launch, floats of the workspace, launches)."""
+    tiles, query_rows = -(-max_rows // 64), few * G
+    cols, ctas, _ = fp4_plan(device, D, min(query_rows, 9), 0)
     chunks = -(-query_rows // cols)
     group = min(512, 65535 // (H * chunks))
-    group = -(-B // -(-B // group))
-    parts = fp4_parts(B * H * chunks, tiles, D, query_rows) if B <= group else 0
-    ctas, rows, ws = ctas * sms, group * H * chunks, None
-    if not parts:                            # (of this call: two calls at once, or two captured graphs, share nothing)
-        ws = torch.empty((rows + ctas) * cols * (D + 2) + 2 * rows, dtype=torch.float32, device=q.device)
-    _check(_attention_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), None if md.decode_only else md.query_start_loc.data_ptr(),
-                          out.data_ptr(), _p(lse), _p(sinks), _p(ws), B, Hq, H, D, BS, max_rows, few, q.stride(0), out.stride(0), bt.stride(0), ctas, FP4_EXTRA, parts, group,
-                          window or 0, scale, soft_cap, out_scale, _DT[q.dtype], _st()), "attention_fp4", 1 if parts else 2 * -(-B // group))
+    launches = -(-B // group)
+    group = -(-B // launches)
+    parts, ctas = fp4_parts(B * H * chunks, tiles, D, query_rows) if launches == 1 else 0, ctas * num_sms()
+    rows = group * H * chunks
+    return ctas, parts, group, 0 if parts else (rows + ctas) * cols * (D + 2) + 2 * rows, 1 if parts else 2 * launches
+
+
+def _fp4_few(q, kv_cache, md, H: int, D: int, BS: int, max_rows: int, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
+    """Attention of the requests with at most ``few`` new tokens, straight from the cache; rows of the others are not touched."""
+    bt, B, Hq = md.block_table, md.num_reqs, q.shape[1]
+    ctas, parts, group, floats, launches = fp4_schedule(_device(), B, H, Hq // H, D, few, max(1, max_rows))
+    # (of this call: two calls at once, or two captured graphs, share nothing)
+    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    _check(_attention_fp4(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), md.seq_lens.data_ptr(), None if md.decode_only else md.query_start_loc.data_ptr(),
+                          out.data_ptr(), _p(lse), _p(sinks), _p(ws), B, Hq, H, D, BS, max(1, max_rows), few, q.stride(0), out.stride(0), bt.stride(0), ctas, FP4_EXTRA, parts, group,
+                          window or 0, scale, soft_cap, out_scale, _DT[q.dtype], _st()), "attention_fp4", launches)
 
 
 FP4_FEW_ROWS = 64                            # query rows (new tokens x query heads of a kv head) of requests that always take the kernel of single tokens
@@ -973,41 +986,44 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
             lse.view(T, H, -1).copy_(norm.view(T, H, -1)[:, :, :Hq // H])
 
 
-def paged_attention_fp4(q, kv_cache, md, scale, window=None, soft_cap=0.0, causal=True, out=None, alibi=None, sinks=None, chunk=0, return_lse: bool = False,
+def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, soft_cap=0.0, causal=True, out=None, alibi=None, sinks=None, chunk=0, return_lse: bool = False,
                         out_scale: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0):
-    T, Hq, D = q.shape
+    (T, Hq, _), BS = q.shape, kv_cache.shape[3]
     _fp4_half(q, kv_cache, "paged_attention_fp4")
-    bt, sl, B, dev = md.block_table, md.seq_lens, md.num_reqs, _device()
-    if bt.dtype is not _I32 or bt.dim() != 2 or bt.stride(1) != 1 or bt.shape[0] < B or sl.dtype is not _I32 or not sl.is_contiguous() or sl.numel() < B \
-            or bt.get_device() != dev or sl.get_device() != dev:
-        raise ValueError("paged_attention_fp4: int32 block tables with a request's pages next to each other and int32 lengths of all requests, on the current device")
-    if not md.decode_only:
+    bt, sl, B, dev, decode = md.block_table, md.seq_lens, md.num_reqs, _device(), md.decode_only
+    if bt.dtype is not _I32 or sl.dtype is not _I32 or bt.dim() != 2 or bt.get_device() != dev or sl.get_device() != dev or not sl.is_contiguous() or sl.numel() < B:
+        raise ValueError("paged_attention_fp4: int32 block tables and lengths of all requests on the current device")
+    n, width = bt.shape
+    if n < B or bt.stride(1) != 1:
+        raise ValueError("paged_attention_fp4: block tables of all requests, a request's pages next to each other")
+    if not decode:
         _query_offsets(md, dev)
-    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
+    if not q.is_contiguous() or q.data_ptr() % 16:
         q = _q_heads(q)
-    used, to = B if md.decode_only else md.num_actual_tokens, out
+    used, to = B if decode else md.num_actual_tokens, out
     if out is None or out.data_ptr() % 16 or out.stride(0) % 8:
-        to = torch.empty_like(q, memory_format=torch.contiguous_format)
+        to = torch.empty_like(q)
+        if T > used:                         # (padding rows are written by no CTA: keep them finite)
+            to[used:].zero_()
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    if T > used and out is None:             # (padding rows are written by no CTA: keep them finite)
-        to[used:].zero_()
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
-    few, longest, G, H = 0, 1 if md.decode_only else md.max_query_len, Hq // kv_cache.shape[2], kv_cache.shape[2]
-    direct = D in FP4_HEADS and alibi is None and not chunk and (causal or md.decode_only) and G <= 64 and not batch_invariant()
-    if direct and longest:
-        few, straight = fp4_kernels(used, B, longest, min(md.max_seq_len, bt.shape[1] * kv_cache.shape[3]), H, G, D)
+    few, longest, G, max_rows = 0, 1 if decode else md.max_query_len, Hq // H, min(md.max_seq_len, width * BS)
+    scale, out_scale = scale * k_scale, out_scale * v_scale
+    direct = D in FP4_HEADS and alibi is None and not chunk and (causal or decode) and G <= 64 and not batch_invariant()
+    if direct:
+        few, straight = (1, True) if longest == 1 else fp4_kernels(used, B, longest, max_rows, H, G, D)
     if B and few < longest:
         if direct and straight:
-            _fp4_rows_attention(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
+            _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, to, lse, sinks, out_scale, few)
         else:
-            _fp4_attention_pages(q, kv_cache, md, scale * k_scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale * v_scale, few, direct)
+            _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale, few, direct)
         lens = getattr(md, "host_lens", None)
         if lens is not None and all(lens[0][b + 1] - lens[0][b] > few for b in range(B)):
             few = 0                          # (no request has so few)
     if B and few:
-        _fp4_few(q, kv_cache, md, scale * k_scale, window, soft_cap, to, lse, sinks, out_scale * v_scale, few)
-    if out is not None and to is not out:
+        _fp4_few(q, kv_cache, md, H, D, BS, max_rows, scale, window, soft_cap, to, lse, sinks, out_scale, few)
+    if to is not out and out is not None:
         out[:used] = to[:used]
         to = out
     return (to, lse) if return_lse else to
