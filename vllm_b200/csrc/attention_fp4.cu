@@ -2,7 +2,7 @@
 //
 //   s[r, k] = c(scale q_r . K_k) for the keys k that row r sees,  lse_r = log(sum_k e^s[r, k] + e^sink),  out_r = sum_k e^(s[r, k] - lse_r) V_k
 //
-// Query rows are pairs (new token, query head of a kv head), 16 of them (or 8, where there are no more) at a time: with a request and a kv head they are a
+// Query rows are pairs (new token, query head of a kv head), 8, 16 or (heads of up to 128) 24 of them at a time: with a request and a kv head they are a
 // "row" of the schedule.  All rows' tiles of 64 keys, in order, are dealt to the CTAs in equal runs, so that ragged and few long requests keep all SMs as
 // busy as many equal ones; a row that one CTA has is finished there, one that several have is joined by a second kernel.  Where rows are few and short a cluster
 // has a row, and the parts meet in shared memory.
@@ -27,6 +27,7 @@ namespace afp4 {
 
 constexpr int TILE = 64, STRIP = 32, WARPS = 4, THREADS = WARPS * 32;
 constexpr int MAX_REQUESTS = 512;            // of a launch: their first tiles and lengths lie in shared memory
+constexpr int MOST_COLS = 24;               // query rows of a row of the schedule
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float SHIFT = 7.f;                 // the reference of a row's weights is its largest score less SHIFT, or up to 8 below that
 constexpr float NONE = -3e38f;               // the reference of a row that has seen no key: any score is far above it
@@ -183,9 +184,9 @@ template <int D_> struct Form {
   static constexpr int CODES = STRIP * D / 2, SIDE = CODES + STRIP * D / 16, STAGE = 2 * SIDE;       // bytes of a strip's keys, values behind them
   static constexpr int STAGES = D <= 64 ? 3 : 2;
   static constexpr int RING = WARPS * STAGES * STAGE;
-  static constexpr int EXCH = WARPS * KD * 4 * 128, MAXIMA = WARPS * 16 * 8;   // the warps' outputs of eight query rows; maxima and sums of 16
+  static constexpr int EXCH = WARPS * KD * 4 * 128, MAXIMA = WARPS * MOST_COLS * 8;   // the warps' outputs of eight query rows; maxima and sums of all
   static constexpr int lists(int B) { return ((3 * B + 2 + WARPS) * 4 + 15) & ~15; }                 // first tiles, lengths and new tokens of B requests
-  static constexpr int PART = 16 * (D + 2 + 9) * 4;                        // of a CTA of a cluster, instead of the lists
+  static constexpr int PART = MOST_COLS * (D + 2 + 9) * 4;                 // of a CTA of a cluster, instead of the lists
   static constexpr int FIXED = RING + EXCH + MAXIMA;
   // a lane's D / 4 values of a key lie in GK groups, its D / 8 values of a value row in GV
   static constexpr int SK = D / 4, SV = D / 8;
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
           if (m_run[nt][u] == NONE) m_run[nt][u] = -INFINITY;
-          if (r0 == 0) maxima[warp * 16 + nt * 8 + q0 + u] = make_float2(m_run[nt][u], l_run[nt][u]);
+          if (r0 == 0) maxima[warp * MOST_COLS + nt * 8 + q0 + u] = make_float2(m_run[nt][u], l_run[nt][u]);
         }
       __syncthreads();
 #pragma unroll
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
         for (int u = 0; u < 2; ++u) {
           float2 ml[WARPS];
 #pragma unroll
-          for (int w = 0; w < WARPS; ++w) ml[w] = maxima[w * 16 + nt * 8 + q0 + u];
+          for (int w = 0; w < WARPS; ++w) ml[w] = maxima[w * MOST_COLS + nt * 8 + q0 + u];
           top[u] = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
           total[u] = 0.f;
 #pragma unroll
@@ -653,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
             if (r0 == 0 && i0 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
           }
         }
-        if (NT > 1 && nt == 0) __syncthreads();          // (in front of the next row: the barrier behind the maxima)
+        if (nt + 1 < NT) __syncthreads();                // (in front of the next row: the barrier behind the maxima)
       }
     }
     if (!more) break;
@@ -763,7 +764,10 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, in
   }
 }
 
-constexpr int ctas_of(int D, int NT) { return D <= 128 ? (NT == 1 ? 4 : 3) : 2; }            // of an SM
+constexpr int ctas_of(int D, int NT) { return D <= 128 ? 5 - NT : 2; }            // of an SM
+
+// Groups of eight query rows of a row of the schedule, for requests of up to `rows` of them
+static int groups_of(int D, int rows) { return rows <= 8 ? 1 : rows <= 16 || D > 128 ? 2 : 3; }
 
 // `clusters`: nothing is launched, the clusters of a row that the device runs at a time are counted.
 template <int D, int NT, bool BF16>
@@ -793,6 +797,8 @@ static int launch(const Params& p, cudaStream_t st, int* clusters, int* ctas) {
 }
 template <int D>
 static int pick(const Params& p, int nt, cudaStream_t st, int* clusters, int* ctas) {
+  if constexpr (D <= 128)
+    if (nt == 3) return p.bf16 ? launch<D, 3, true>(p, st, clusters, ctas) : launch<D, 3, false>(p, st, clusters, ctas);
   if (p.bf16) return nt == 2 ? launch<D, 2, true>(p, st, clusters, ctas) : launch<D, 1, true>(p, st, clusters, ctas);
   return nt == 2 ? launch<D, 2, false>(p, st, clusters, ctas) : launch<D, 1, false>(p, st, clusters, ctas);
 }
@@ -817,7 +823,7 @@ EXPORT int vb_attention_fp4_plan(int D, int rows, int parts, int* cols, int* cta
   using namespace afp4;
   Params p{};
   p.parts = parts;
-  const int nt = rows > 8 ? 2 : 1;
+  const int nt = groups_of(D, rows);
   *cols = 8 * nt;
   int rc = go(p, D, nt, nullptr, nullptr, ctas);
   if (rc == 0 && parts > 0) rc = parts > 8 ? -1 : go(p, D, nt, nullptr, clusters);
@@ -840,7 +846,7 @@ EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks
   Params p;
   p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.extra = extra; p.parts = parts; p.window = window; p.bf16 = dtype == DT_BF16;
   if ((int64_t)few * p.G > 4096) return -1;
-  const int nt = few * p.G > 8 ? 2 : 1;
+  const int nt = groups_of(D, few * p.G);
   p.chunks = (few * p.G + 8 * nt - 1) / (8 * nt);
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.num_blocks = num_blocks; p.cache = (const uint8_t*)cache; p.sinks = sinks;
   p.scale_log2 = scale * LOG2E;

@@ -823,7 +823,7 @@ def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
     """CTAs of a cluster that has a row of the schedule, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel.  us with 8, 4, 2, 1 and 0,
     heads of 128: 8 rows of 700 6.4, 6.7, 7.7, 9.5, 7.6; 32 of 2000 10.1, 9.9, 13.6, 21.0, 12.1; 64 of 2000 17.7, 13.4, 13.6, 21.1, 13.5; 512 of 250 71, 34, 22, 15.5, 18.8; 512 of
     1000 85, 48, 36, 32, 32; of 64, 192 of 60 to 924 21, 16, 11.6, 12.4, 12.8."""
-    query_rows, sms = min(query_rows, 9), num_sms()
+    query_rows, sms = min(query_rows, 17), num_sms()
     for parts in (8, 4, 2):
         if parts // 2 < tiles <= 10 * parts and rows * parts <= 3 * sms and rows <= fp4_plan(_device(), D, query_rows, parts)[2]:
             return parts
@@ -834,7 +834,7 @@ def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
 def fp4_schedule(device: int, B: int, H: int, G: int, D: int, few: int, max_rows: int) -> tuple[int, int, int, int, int]:
     """(CTAs, CTAs of a cluster that has a row, requests of a launch, floats of the workspace, launches)."""
     tiles, query_rows = -(-max_rows // 64), few * G
-    cols, ctas, _ = fp4_plan(device, D, min(query_rows, 9), 0)
+    cols, ctas, _ = fp4_plan(device, D, min(query_rows, 17), 0)
     chunks = -(-query_rows // cols)
     group = min(512, 65535 // (H * chunks))
     launches = -(-B // group)
@@ -860,15 +860,15 @@ FP4_FEW_ROWS = 64                            # query rows (new tokens x query he
 
 def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int) -> tuple[int, bool]:
     """(new tokens up to which a request takes the kernel of single tokens, whether the others' prompts go straight from the cache or through 16-bit pages), for T
-    tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: the kernel of single tokens 3.5 TB/s of the cache for every 16
-    query rows; the one of prompts 190 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
-    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 32, 41, 203; 160 there 96, 78, 123; 320 there
-    179, 164, 126; 500 there -, 235, 198; 160 behind 1200 30, 28, 35; 640 there 76, 50, 41; of 128, 80 behind 12 000 81, 90, 183; 160 there 149, 168, 121."""
+    tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: the kernel of single tokens 2.6 TB/s of the cache for every 24
+    query rows (16 where heads are above 128); the one of prompts 190 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
+    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 33, 42, 202; 160 there 95, 78, 121; 320 there
+    175, 165, 124; 500 there 261, 238, 193; 160 behind 1200 32, 29, 35; 640 there 79, 49, 41; of 128, 80 behind 12 000 76, 91, 183; 160 there 135, 165, 119; of 192, 160 behind 4000 88, 84."""
     base = max(1, FP4_FEW_ROWS // G)
     if longest <= base:
         return longest, True
     pairs = T * H * max(rows - longest / 2, 1)
-    single = 6 + (T * G / 16 + B) * rows * H * D * 1.125 / 3.5e6
+    single = 6 + (T * G / (24 if D <= 128 else 16) + B) * rows * H * D * 1.125 / 2.6e6
     straight = 20 + pairs * G * 4 * D / 190e6
     pages = float("inf")
     if D <= 128:
