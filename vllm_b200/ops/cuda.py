@@ -954,7 +954,7 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
                 sinks = torch.nn.functional.pad(sinks.view(H, Hq // H), (0, G - Hq // H)).flatten()
     vt = tc_attention_ok(W, W, q.shape[1] // H) and alibi is None
     PS = 32 if W == 256 else 64
-    qsl = None if md.decode_only else md.query_start_loc
+    qsl, B = None if md.decode_only else md.query_start_loc, md.num_reqs
     most = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS)
     for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * W):
         n = b1 - b0
@@ -962,21 +962,25 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
             continue
         pages = torch.empty((total, 2, H, PS, W), dtype=q.dtype, device=q.device)
         table, lens = sl.new_empty((n, longest)), sl.new_empty(n)
-        _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt[b0:].data_ptr(), bt.stride(0), bt.shape[1], sl[b0:].data_ptr(), None if qsl is None else qsl[b0:].data_ptr(), few,
-                          pages.data_ptr(), pages.shape[0], PS, W, int(vt), table.data_ptr(), table.shape[1], lens.data_ptr(), n, H, D, BS, _DT[q.dtype], _st()), "pages_fp4")
-        part = copy.copy(md)
+        _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt.data_ptr() + 4 * b0 * bt.stride(0), bt.stride(0), bt.shape[1], sl.data_ptr() + 4 * b0,
+                          None if qsl is None else qsl.data_ptr() + 4 * b0, few, pages.data_ptr(), total, PS, W, int(vt), table.data_ptr(), longest, lens.data_ptr(), n, H, D, BS,
+                          _DT[q.dtype], _st()), "pages_fp4")
+        part, whole = copy.copy(md), n == B
         part.num_reqs, part.block_table, part.seq_lens, part.max_seq_len, part.kv_vt, part.flat, part.cascade = n, table, lens, longest * PS, vt, False, None
+        q_part, to_part = q, to
         if md.decode_only:
-            rows = slice(b0, b1)
+            if not whole or q.shape[0] != n:
+                q_part, to_part = q[b0:b1], to[b0:b1]
             part.query_start_loc = None if md.query_start_loc is None else md.query_start_loc[:n + 1]
-        else:
-            rows = slice(0, T)
+        elif not whole:
             part.query_start_loc = qsl[b0:b1 + 1]
-        got = paged_attention(q[rows], pages, part, scale, window, soft_cap, causal, to[rows], return_lse=lse is not None, alibi_slopes=alibi, sinks=sinks, chunk_size=chunk,
+        got = paged_attention(q_part, pages, part, scale, window, soft_cap, causal, to_part, return_lse=lse is not None, alibi_slopes=alibi, sinks=sinks, chunk_size=chunk,
                               out_scale=out_scale)
         if lse is not None:
-            if md.decode_only or n == md.num_reqs:
-                norm[rows] = got[1]
+            if md.decode_only:
+                norm[b0:b1] = got[1]
+            elif whole:
+                norm.copy_(got[1])
             else:
                 t = torch.arange(T, device=q.device)
                 norm.copy_(torch.where(((t >= qsl[b0]) & (t < qsl[b1]))[:, None], got[1], norm))
