@@ -44,9 +44,13 @@ struct Params {
   float* part;               // [segment][COLS][D + 2]: output, maximum, sum
   int2* info;                // [row]: its first CTA, and how many
   int64_t q_stride, out_stride, bt_stride, num_blocks;
-  int B, Hkv, G, BS, max_rows, few, ctas, chunks, extra, parts, window, bf16;
+  int B, Hkv, G, BS, max_rows, few, ctas, chunks, extra, parts, window, bf16, shift;      // shift: of BS where that is a power of two, or -1
+  uint32_t over_g;           // 2^32 / G, rounded up (0: G is 1)
   float scale_log2, ku, c2, out_scale;
 };
+
+// Token of a query row: r / G for r below 2^16 and G up to 2^6 (a dozen divisions a row were a fifth of its end)
+VB_DEVICE int token_of(const Params& p, int r) { return p.over_g ? (int)__umulhi((uint32_t)r, p.over_g) : r; }
 
 struct Request {
   int n, t;                  // rows in the cache, new tokens among them (0: none of this kernel's)
@@ -112,7 +116,7 @@ VB_DEVICE void row_at(const Params& p, int cols, const int* first, const int2* r
   const Request q{reqs[lo].x, reqs[lo].y};               // (it has slots: the last request that begins at or in front of the tile)
   const int n = slots_of(p, q), chunks = q.chunks(p, cols), i = (tile - first[lo] * p.Hkv) / n;
   r.b = lo;
-  r.h = i / chunks;
+  r.h = chunks == 1 ? i : i / chunks;
   r.c = i - r.h * chunks;
   r.begin = first[lo] * p.Hkv + i * n;
   r.end = r.begin + n;
@@ -214,12 +218,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
   int t0, t1, per;
   Row row;
   Request req;
-  const int rank = fused ? blockIdx.x % p.parts : 0;
+  const int rank = fused ? blockIdx.x : 0;
   if (fused) {
-    const int i = blockIdx.x / p.parts;
-    row.c = i % p.chunks;
-    row.h = i / p.chunks % p.Hkv;
-    row.b = i / p.chunks / p.Hkv;
+    row.b = blockIdx.z;
+    row.h = p.chunks == 1 ? blockIdx.y : blockIdx.y / p.chunks;
+    row.c = blockIdx.y - row.h * p.chunks;
     req = request(p, row.b);
     row.begin = 0;
     row.end = row.c < req.chunks(p, COLS) ? req.tiles(p) : 0;
@@ -283,10 +286,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
         for (int half = 0; half < 2; ++half) {
           const int at = tok + half * 16;
           if (at < q.n) {
-            int64_t blk = p.block_table[r.b * p.bt_stride + at / p.BS];
+            const int pg = p.shift >= 0 ? at >> p.shift : at / p.BS;
+            int64_t blk = p.block_table[r.b * p.bt_stride + pg];
             if ((uint64_t)blk >= (uint64_t)p.num_blocks) blk = 0;           // (a table may not say that; nothing is read outside the cache)
             my_page[half] = (uint32_t)(blk * 2 * p.Hkv + r.h);
-            my_off[half] = at % p.BS;
+            my_off[half] = at - pg * p.BS;
           }
         }
       }
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     const int first_q = p.qsl ? p.qsl[row.b] : row.b;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row.c * COLS + nt * 8 + r0, tok = r / p.G;
+      const int r = row.c * COLS + nt * 8 + r0, tok = token_of(p, r);
       const bool there = tok < req.t;
       const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(first_q + tok) * p.q_stride + (int64_t)(row.h * p.G + r - tok * p.G) * D + t4 * (D / 4);
       if constexpr (D % 32 == 0) {
@@ -349,17 +353,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     for (int nt = 0; nt < NT; ++nt) {
       float mine = 1.f;
       if (BF16) {
-        float top = 0.f;
+        uint32_t most = 0u;                  // of the halves' bits without their signs
 #pragma unroll
-        for (int k = 0; k < KD; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float2 x = unpack2<__nv_bfloat16>(q[k][nt][j]);
-            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 27), 254);                  // of the exponent's field; [2^-100, 2^127]
+        for (int k = 0; k < KD; ++k) most = __vmaxu2(most, __vmaxu2(q[k][nt][0] & 0x7fff7fffu, q[k][nt][1] & 0x7fff7fffu));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = min(max((int)(max(most & 0xffffu, most >> 16) >> 7), 27), 254);        // of the exponent's field; [2^-100, 2^127]
         const float f = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);               // 2^(14 - (e - 127)), at least 2^-113
         mine = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
@@ -374,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         mult[nt][u] = __shfl_sync(0xffffffffu, mine, (q0 + u) * 4);
-        hi[nt][u] = req.n - req.t + (row.c * COLS + nt * 8 + q0 + u) / p.G;
+        hi[nt][u] = req.n - req.t + token_of(p, row.c * COLS + nt * 8 + q0 + u);
       }
     }
   };
@@ -567,9 +566,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     // ---- the warps' results of the segment meet in shared memory
     const int index = (row.b * p.Hkv + row.h) * p.chunks + row.c, live = row.begin + req.tiles(p);       // (behind its tiles a row has further slots)
     const bool empty = !fused && max(row.begin, t0) >= live;
-    const int n_ctas = fused ? 1 : (live - 1) / per - row.begin / per + 1;
-    const bool whole = !fused && n_ctas == 1;
-    if (!fused && !empty && row.begin >= t0 && threadIdx.x == 0) p.info[index] = make_int2(blockIdx.x, n_ctas);
+    const bool whole = !fused && row.begin >= t0 && live <= t1;
+    if (!fused && !empty && row.begin >= t0 && threadIdx.x == 0) p.info[index] = make_int2(blockIdx.x, whole ? 1 : (live - 1) / per - (int)blockIdx.x + 1);
     const Row done = row;
     const Request done_req = req;
     const bool more = !fused && row.end < t1;
@@ -613,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
         __syncthreads();
         // a thread: a column's values of half of a lane's dimensions
         constexpr int HALF = (KD + 1) / 2;
-        const int u = warp & 1, i0 = warp >> 1 ? HALF : 0, g = nt * 8 + q0 + u, r = done.c * COLS + g, tok = r / p.G, d0 = r0 * (D / 8) + 2 * i0;
+        const int u = warp & 1, i0 = warp >> 1 ? HALF : 0, g = nt * 8 + q0 + u, r = done.c * COLS + g, tok = token_of(p, r), d0 = r0 * (D / 8) + 2 * i0;
         const float m = u ? top[1] : top[0], l = u ? total[1] : total[0];
         float2 x[HALF];
 #pragma unroll
@@ -666,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     const int live = min(max(req.t * p.G - row.c * COLS, 0), COLS), first_q = p.qsl ? p.qsl[row.b] : row.b;
     for (int g = warp; g < live; g += WARPS) {           // a warp: log-sum-exp of a column, its parts and the sink
       const uint32_t at = parts_at + (g * PD + D) * 4;
-      const int r = row.c * COLS + g, tok = r / p.G, head = row.h * p.G + r - tok * p.G;
+      const int r = row.c * COLS + g, tok = token_of(p, r), head = row.h * p.G + r - tok * p.G;
       const float m0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at, lane)) : -INFINITY, l0 = lane < p.parts ? ld_dsmem_f32(dsmem_addr(at + 4, lane)) : 0.f;
       const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
       const float m = warp_max(fmaxf(m0, sink)), top = m == -INFINITY ? 0.f : m;
@@ -676,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     }
     __syncthreads();
     for (int i = rank * THREADS + threadIdx.x; i < live * (D / 2); i += p.parts * THREADS) {
-      const int g = i / (D / 2), d = i % (D / 2) * 2, r = row.c * COLS + g, tok = r / p.G;
+      const int g = i / (D / 2), d = i % (D / 2) * 2, r = row.c * COLS + g, tok = token_of(p, r);
       float2 x[8], acc = make_float2(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < 8; ++c) x[c] = c < p.parts ? ld_dsmem_f32x2(dsmem_addr(parts_at + (g * PD + d) * 4, c)) : make_float2(0.f, 0.f);
@@ -692,16 +690,16 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
   }
 }
 
-// Grid (columns of a row, rows): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
+// Grid (columns of a row, rows of a request, requests): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
 constexpr int JOIN = 128, JOINERS = JOIN / 32, PAIRS = 4, AHEAD = 4;
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, int D) {
   __shared__ float2 sums[JOINERS][32 * PAIRS];
   pdl_trigger();
   pdl_wait();
-  const int index = blockIdx.y, c = index % p.chunks, h = index / p.chunks % p.Hkv, b = index / p.chunks / p.Hkv, PD = D + 2;
+  const int b = blockIdx.z, h = p.chunks == 1 ? blockIdx.y : blockIdx.y / p.chunks, c = blockIdx.y - h * p.chunks, index = b * p.Hkv * p.chunks + blockIdx.y, PD = D + 2;
   const int2 at = p.info[index];                         // (says something where the request has keys and the row is one)
   const Request req = request(p, b);
-  const int r = c * cols + blockIdx.x, tok = r / p.G;
+  const int r = c * cols + blockIdx.x, tok = token_of(p, r);
   if (tok >= req.t) return;
   const int count = req.n > 0 ? at.y : 0;
   if (count == 1) return;                                // done where its keys were
@@ -786,13 +784,12 @@ static int launch(const Params& p, cudaStream_t st, int* clusters, int* ctas) {
     cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = F::FIXED + F::PART; cfg.attrs = &attr; cfg.numAttrs = 1;
     return (int)cudaOccupancyMaxActiveClusters(clusters, k, &cfg);
   }
-  const int rows = p.B * p.Hkv * p.chunks;
   if (p.parts > 0) {
-    vb_launch_parts(k, dim3(rows * p.parts), dim3(THREADS), (size_t)(F::FIXED + F::PART), st, (unsigned)p.parts, p);
+    vb_launch_parts(k, dim3(p.parts, p.Hkv * p.chunks, p.B), dim3(THREADS), (size_t)(F::FIXED + F::PART), st, (unsigned)p.parts, p);
     return (int)cudaGetLastError();
   }
   vb_launch(k, dim3(p.ctas), dim3(THREADS), (size_t)(F::FIXED + F::lists(p.B)), st, p);
-  vb_launch(join_kernel, dim3(min(8 * NT, p.few * p.G), rows), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
+  vb_launch(join_kernel, dim3(min(8 * NT, p.few * p.G), p.Hkv * p.chunks, p.B), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
   return (int)cudaGetLastError();
 }
 template <int D>
@@ -845,13 +842,17 @@ EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks
   if (parts > 0 && B > group) return -1;
   Params p;
   p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.extra = extra; p.parts = parts; p.window = window; p.bf16 = dtype == DT_BF16;
-  if ((int64_t)few * p.G > 4096) return -1;
+  if ((int64_t)few * p.G > 4096 || p.G > 64) return -1;
   const int nt = groups_of(D, few * p.G);
   p.chunks = (few * p.G + 8 * nt - 1) / (8 * nt);
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.num_blocks = num_blocks; p.cache = (const uint8_t*)cache; p.sinks = sinks;
   p.scale_log2 = scale * LOG2E;
   p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E; p.out_scale = out_scale;
   p.lse = lse;
+  p.over_g = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0u;
+  p.shift = 0;
+  while (1 << p.shift < BS) ++p.shift;
+  if (1 << p.shift != BS) p.shift = -1;
   for (int b0 = 0; b0 < B; b0 += group) {
     p.B = B - b0 < group ? B - b0 : group;
     // with offsets, rows are where they say; without, request b0 + i has row b0 + i
