@@ -404,6 +404,30 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       if (tok >= n) continue;
       const unsigned char* ks = ring + stage * F::STAGE;
       const unsigned char* vs = ks + F::SIDE;
+      // ---- values of the strip as they are, on their way while the scores are computed
+      const int gv0 = r0 * F::SV / 16, crossv = (16 - r0 * F::SV % 16) / 2;
+      Bytes<D / 16> vc[2][4];
+      uint32_t sa[2][F::GV], sb[2][F::GV];                                           // scales of the keys of slots (0, 1) and (8, 9)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = r0 * (D / 16);
+          vc[m][j].load(vs + (m * 16 + vkey[j]) * (D / 2) + (D == 128 ? (((at >> 4) ^ (vkey[j] >> 1 & 2)) << 4 | (at & 15)) : at));
+        }
+#pragma unroll
+        for (int g = 0; g < F::GV; ++g) {
+          const unsigned char* at = vs + F::CODES + m * D + min(gv0 + g, D / 16 - 1);
+          uint32_t x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = at[vkey[j] * (D / 16)];
+          if (tok + STRIP > n || tok < low)      // rows of nobody, or that no query row sees, may hold what a weight of 0 does not cancel
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = tok + m * 16 + vkey[j] < n && tok + m * 16 + vkey[j] >= low ? x[j] : 0u;
+          sa[m][g] = fp4::scales2(x[0] | x[1] << 8);
+          sb[m][g] = fp4::scales2(x[2] | x[3] << 8);
+        }
+      }
       // ---- S^T = K Q^T, 16 keys at a time
       float sc[2][NT][4];
 #pragma unroll
@@ -517,41 +541,21 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
       // ---- O^T += V^T P^T, 16 keys at a time
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        Bytes<D / 16> c[4];
-        uint32_t sa[F::GV], sb[F::GV];                                               // scales of the keys of slots (0, 1) and (8, 9)
-        const int g0 = r0 * F::SV / 16, cross = (16 - r0 * F::SV % 16) / 2;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = r0 * (D / 16);
-          c[j].load(vs + (m * 16 + vkey[j]) * (D / 2) + (D == 128 ? (((at >> 4) ^ (vkey[j] >> 1 & 2)) << 4 | (at & 15)) : at));
-        }
-#pragma unroll
-        for (int g = 0; g < F::GV; ++g) {
-          const unsigned char* at = vs + F::CODES + m * D + min(g0 + g, D / 16 - 1);
-          uint32_t x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = at[vkey[j] * (D / 16)];
-          if (tok + STRIP > n || tok < low)      // rows of nobody, or that no query row sees, may hold what a weight of 0 does not cancel
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = tok + m * 16 + vkey[j] < n && tok + m * 16 + vkey[j] >= low ? x[j] : 0u;
-          sa[g] = fp4::scales2(x[0] | x[1] << 8);
-          sb[g] = fp4::scales2(x[2] | x[3] << 8);
-        }
 #pragma unroll
         for (int w = 0; w < Bytes<D / 16>::WORDS; ++w) {
           // the nibbles of two keys next to each other: bytes of even values, and of odd ones
           constexpr uint32_t LOW = 0x0f0f0f0fu;
           uint32_t e01[4], o01[4], e23[4], o23[4];
-          fp4::unpack8((c[0].w[w] & LOW) | ((c[1].w[w] << 4) & ~LOW), e01);
-          fp4::unpack8(((c[0].w[w] >> 4) & LOW) | (c[1].w[w] & ~LOW), o01);
-          fp4::unpack8((c[2].w[w] & LOW) | ((c[3].w[w] << 4) & ~LOW), e23);
-          fp4::unpack8(((c[2].w[w] >> 4) & LOW) | (c[3].w[w] & ~LOW), o23);
+          fp4::unpack8((vc[m][0].w[w] & LOW) | ((vc[m][1].w[w] << 4) & ~LOW), e01);
+          fp4::unpack8(((vc[m][0].w[w] >> 4) & LOW) | (vc[m][1].w[w] & ~LOW), o01);
+          fp4::unpack8((vc[m][2].w[w] & LOW) | ((vc[m][3].w[w] << 4) & ~LOW), e23);
+          fp4::unpack8(((vc[m][2].w[w] >> 4) & LOW) | (vc[m][3].w[w] & ~LOW), o23);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int i = 4 * w + j;
             if (i < KD) {
-              const uint32_t f0 = F::STRAIGHT_V ? sa[F::GV > 1 ? i / 8 : 0] : i < cross ? sa[0] : sa[F::GV - 1];
-              const uint32_t f1 = F::STRAIGHT_V ? sb[F::GV > 1 ? i / 8 : 0] : i < cross ? sb[0] : sb[F::GV - 1];
+              const uint32_t f0 = F::STRAIGHT_V ? sa[m][F::GV > 1 ? i / 8 : 0] : i < crossv ? sa[m][0] : sa[m][F::GV - 1];
+              const uint32_t f1 = F::STRAIGHT_V ? sb[m][F::GV > 1 ? i / 8 : 0] : i < crossv ? sb[m][0] : sb[m][F::GV - 1];
               const uint32_t a0 = fp4::mul2(e01[j], f0), a1 = fp4::mul2(o01[j], f0), a2 = fp4::mul2(e23[j], f1), a3 = fp4::mul2(o23[j], f1);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
@@ -690,79 +694,89 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
   }
 }
 
-// Grid (columns of a row, rows of a request, requests): the outputs of rows that several CTAs had, and of rows without keys.  One block has a column.
-constexpr int JOIN = 128, JOINERS = JOIN / 32, PAIRS = 4, AHEAD = 4;
+// Grid (columns of a row, rows of a request, requests): the outputs of rows that several CTAs had, and of rows without keys.  EACH: warps of a column; the block has JOINERS /
+// EACH columns.  The first parts are on their way before it is known what they count for.
+constexpr int JOINERS = 4, JOIN = JOINERS * 32, PAIRS = 4, AHEAD = 4;
+template <int EACH>
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, int D) {
-  __shared__ float2 sums[JOINERS][32 * PAIRS];
+  __shared__ float2 sums[EACH > 1 ? EACH : 1][EACH > 1 ? 32 * PAIRS : 1];
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.z, h = p.chunks == 1 ? blockIdx.y : blockIdx.y / p.chunks, c = blockIdx.y - h * p.chunks, index = b * p.Hkv * p.chunks + blockIdx.y, PD = D + 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = EACH > 1 ? warp : 0, col = blockIdx.x * (JOINERS / EACH) + (EACH > 1 ? 0 : warp), pairs = D / 2;
   const int2 at = p.info[index];                         // (says something where the request has keys and the row is one)
   const Request req = request(p, b);
-  const int r = c * cols + blockIdx.x, tok = token_of(p, r);
-  if (tok >= req.t) return;
+  const int r = c * cols + col, tok = token_of(p, r);
+  if (col >= cols || tok >= req.t) return;
   const int count = req.n > 0 ? at.y : 0;
   if (count == 1) return;                                // done where its keys were
-  const int head = h * p.G + r - tok * p.G, lane = threadIdx.x & 31, w = threadIdx.x >> 5, pairs = D / 2;
   const int step = cols * PD;                            // (a part's floats)
-  const float* x = p.part + ((int64_t)(index + (count ? at.x : 0)) * cols + blockIdx.x) * PD;
+  const float* x = p.part + ((int64_t)(index + (count ? at.x : 0)) * cols + col) * PD;
+  auto read = [&](int from, float2 (&y)[AHEAD][PAIRS]) { // parts from, from + EACH, ...
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+        if (from + k * EACH < count && lane + 32 * j < pairs) y[k][j] = *reinterpret_cast<const float2*>(x + (int64_t)(from + k * EACH) * step + 2 * (lane + 32 * j));
+  };
+  float2 y[AHEAD][PAIRS];
+  float2 ml = lane < count ? *reinterpret_cast<const float2*>(x + (int64_t)lane * step + D) : make_float2(-INFINITY, 0.f);
+  read(w, y);
+  const int head = h * p.G + r - tok * p.G;
   const int64_t token = (p.qsl ? p.qsl[b] : b) + tok;
   const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
-  // every warp: the maximum and the sum; then its own parts, every fourth
-  float top = sink;
-  float2 ml = lane < count ? *reinterpret_cast<const float2*>(x + (int64_t)lane * step + D) : make_float2(-INFINITY, 0.f);
-  top = fmaxf(top, ml.x);
+  float top = fmaxf(sink, ml.x);
   for (int i = 32 + lane; i < count; i += 32) top = fmaxf(top, x[(int64_t)i * step + D]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base), total = ml.x == -INFINITY ? 0.f : ml.y * f;
   for (int i = 32 + lane; i < count; i += 32) {
-    const float2 y = *reinterpret_cast<const float2*>(x + (int64_t)i * step + D);
-    if (y.x > -INFINITY) total += y.y * ex2(y.x - base);
+    const float2 v = *reinterpret_cast<const float2*>(x + (int64_t)i * step + D);
+    if (v.x > -INFINITY) total += v.y * ex2(v.x - base);
   }
   total = warp_sum(total) + (p.sinks ? ex2(sink - base) : 0.f);
   float2 acc[PAIRS];
 #pragma unroll
   for (int j = 0; j < PAIRS; ++j) acc[j] = make_float2(0.f, 0.f);
-  for (int from = 0; from < count; from += 32) {
-    if (from > 0) {
-      const float m = from + lane < count ? x[(int64_t)(from + lane) * step + D] : -INFINITY;
+  for (int i = w, block = 0; i < count; i += AHEAD * EACH) {
+    if (i / 32 != block) {                               // factors of the next 32 parts, a lane each (AHEAD EACH divides 32)
+      block = i / 32;
+      const float m = block * 32 + lane < count ? x[(int64_t)(block * 32 + lane) * step + D] : -INFINITY;
       f = m == -INFINITY ? 0.f : ex2(m - base);
     }
-    const int end = min(32, count - from);
-    for (int i = w; i < end; i += JOINERS * AHEAD) {
-      float2 y[AHEAD][PAIRS];
+    if (i != w) read(i, y);
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
+    for (int k = 0; k < AHEAD; ++k) {
+      const float g = __shfl_sync(0xffffffffu, f, (i + k * EACH) & 31);
+      if (i + k * EACH < count)
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j)
-          if (i + k * JOINERS < end && lane + 32 * j < pairs) y[k][j] = *reinterpret_cast<const float2*>(x + (int64_t)(from + i + k * JOINERS) * step + 2 * (lane + 32 * j));
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const float g = __shfl_sync(0xffffffffu, f, (i + k * JOINERS) & 31);
-        if (i + k * JOINERS < end)
-#pragma unroll
-          for (int j = 0; j < PAIRS; ++j)
-            if (lane + 32 * j < pairs) { acc[j].x += y[k][j].x * g; acc[j].y += y[k][j].y * g; }
-      }
+          if (lane + 32 * j < pairs) { acc[j].x += y[k][j].x * g; acc[j].y += y[k][j].y * g; }
     }
   }
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j)
-    if (lane + 32 * j < pairs) sums[w][lane + 32 * j] = acc[j];
-  __syncthreads();
-  if (threadIdx.x == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = total > 0.f ? (base + log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
+  if (lane == 0 && w == 0 && p.lse) p.lse[token * p.Hkv * p.G + head] = total > 0.f ? (base + log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
   const float by = total == 0.f ? 0.f : p.out_scale / total;
-  for (int i = threadIdx.x; i < pairs; i += JOIN) {
-    float2 y = sums[0][i];
+  uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D;
+  auto write = [&](int i, float2 v) { *reinterpret_cast<uint32_t*>(to + 2 * i) = p.bf16 ? pack2<__nv_bfloat16>(v.x * by, v.y * by) : pack2<__half>(v.x * by, v.y * by); };
+  if constexpr (EACH == 1) {
 #pragma unroll
-    for (int j = 1; j < JOINERS; ++j) { y.x += sums[j][i].x; y.y += sums[j][i].y; }
-    uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_stride + (int64_t)head * D + 2 * i;
-    *reinterpret_cast<uint32_t*>(to) = p.bf16 ? pack2<__nv_bfloat16>(y.x * by, y.y * by) : pack2<__half>(y.x * by, y.y * by);
+    for (int j = 0; j < PAIRS; ++j)
+      if (lane + 32 * j < pairs) write(lane + 32 * j, acc[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j)
+      if (lane + 32 * j < pairs) sums[w][lane + 32 * j] = acc[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs; i += JOIN) {
+      float2 v = sums[0][i];
+#pragma unroll
+      for (int j = 1; j < EACH; ++j) { v.x += sums[j][i].x; v.y += sums[j][i].y; }
+      write(i, v);
+    }
   }
 }
 
-constexpr int ctas_of(int D, int NT) { return D <= 128 ? 5 - NT : 2; }            // of an SM
+constexpr int ctas_of(int D, int NT) { return D <= 128 ? (NT == 1 ? 3 : 5 - NT) : 2; }            // of an SM
 
 // Groups of eight query rows of a row of the schedule, for requests of up to `rows` of them
 static int groups_of(int D, int rows) { return rows <= 8 ? 1 : rows <= 16 || D > 128 ? 2 : 3; }
@@ -789,7 +803,12 @@ static int launch(const Params& p, cudaStream_t st, int* clusters, int* ctas) {
     return (int)cudaGetLastError();
   }
   vb_launch(k, dim3(p.ctas), dim3(THREADS), (size_t)(F::FIXED + F::lists(p.B)), st, p);
-  vb_launch(join_kernel, dim3(min(8 * NT, p.few * p.G), p.Hkv * p.chunks, p.B), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
+  // many columns have few parts each, and a warp will do (behind 64 x 1000: 4.3 us, where four warps a column took 6.6)
+  const int cols = min(8 * NT, p.few * p.G);
+  if ((int64_t)cols * p.Hkv * p.chunks * p.B >= 1024)
+    vb_launch(join_kernel<1>, dim3((cols + JOINERS - 1) / JOINERS, p.Hkv * p.chunks, p.B), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
+  else
+    vb_launch(join_kernel<JOINERS>, dim3(cols, p.Hkv * p.chunks, p.B), dim3(JOIN), (size_t)0, st, p, 8 * NT, D);
   return (int)cudaGetLastError();
 }
 template <int D>
