@@ -452,3 +452,55 @@ def test_families_with_a_cache_in_4_bits(model):
     outs = llm.generate([{"prompt_token_ids": [5, 7, 11, 13] * n} for n in (3, 30)], SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True, logprobs=0))
     assert all(len(o.outputs[0].token_ids) == 6 and all(math.isfinite(x.logprob) for d in o.outputs[0].logprobs for x in d.values()) for o in outs)
     llm.shutdown()
+
+
+@pytest.mark.parametrize("queries", [[1, 1, 1], [200, 1, 90]])
+def test_rows_behind_the_last_token_stay(queries):
+    """A bucket's padding is left as it is in a given output, and finite in a new one, whichever kernels the step takes."""
+    for D, Hq in ((64, 6), (128, 8), (256, 4)):
+        q, cache, md = step([300, 90, 1000], queries, Hq, 2, D, 32, torch.bfloat16, "cuda", seed=D)
+        T = q.shape[0]
+        padded = torch.cat((q, torch.full((5, Hq, D), float("nan"), dtype=q.dtype, device="cuda")))
+        want = ops.paged_attention_fp4(q, cache, md, 0.1)
+        out = torch.full_like(padded, 7.0)
+        assert ops.paged_attention_fp4(padded, cache, md, 0.1, out=out) is out and torch.equal(out[:T], want) and (out[T:] == 7.0).all()
+        odd = torch.full((T + 5, Hq * D + 3), 7.0, dtype=q.dtype, device="cuda")
+        ops.paged_attention_fp4(padded, cache, md, 0.1, out=odd[:, 3:].unflatten(1, (Hq, D)))
+        assert torch.equal(odd[:T, 3:].unflatten(1, (Hq, D)), want) and (odd[T:] == 7.0).all() and (odd[:, :3] == 7.0).all()
+        got = ops.paged_attention_fp4(padded, cache, md, 0.1)
+        assert torch.equal(got[:T], want) and torch.isfinite(got).all()
+
+
+def test_max_seq_len_is_a_hint_for_single_tokens():
+    q, cache, md = step([5000, 64, 700], [1, 1, 1], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=4)
+    want = ops.paged_attention_fp4(q, cache, md, 0.1)
+    for hint in (1, 100, 100000):
+        md.max_seq_len = hint
+        got = ops.paged_attention_fp4(q, cache, md, 0.1)
+        assert (got.double() - want.double()).abs().max() < 0.02 and (got != 0).any()
+    md.block_table = md.block_table[:, :0]                       # tables without pages: requests without keys
+    assert (ops.paged_attention_fp4(q, cache, md, 0.1) == 0).all()
+
+
+@pytest.mark.parametrize("D,queries", [(128, [1, 1]), (64, [1, 1]), (256, [100, 100]), (128, [100, 100])])
+def test_nan_comes_out(D, queries):
+    """Of a query, and of keys that are seen; other rows stay as they are."""
+    q, cache, md = step([300, 200], queries, 4, 2, D, 64, torch.bfloat16, "cuda", seed=4)
+    want = ops.paged_attention_fp4(q, cache, md, 0.1)
+    q[0, 1] = float("nan")
+    got = ops.paged_attention_fp4(q, cache, md, 0.1)
+    assert torch.isnan(got[0, 1]).all()
+    got[0, 1] = want[0, 1]
+    same = torch.ones_like(got, dtype=torch.bool) if queries[0] == 1 else torch.arange(got.shape[0], device="cuda")[:, None, None] >= 100      # (rows of one warp grow together)
+    assert torch.equal(got[same.expand_as(got)], want[same.expand_as(got)]) and (got.double() - want.double()).abs().max() < 0.05
+
+
+def test_many_tables_with_much_room():
+    """Numbers of strips beyond 32 bits: several launches."""
+    q, cache, md = step([100] * 40, [1] * 40, 8, 8, 64, 16, torch.bfloat16, "cuda", seed=4)
+    want = ops.paged_attention_fp4(q, cache, md, 0.1)
+    wide = torch.full((40, 10_000_000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :md.block_table.shape[1]] = md.block_table
+    md.block_table, md.max_seq_len = wide, 160_000_000
+    got = ops.paged_attention_fp4(q, cache, md, 0.1)
+    assert (got.double() - want.double()).abs().max() < 0.02 and cuda_ops().fp4_schedule(0, 40, 8, 1, 64, 1, 2_500_000, 2_500_000)[4] > 2

@@ -14,8 +14,14 @@
 // instruction wants them: dimensions of K may go to the instruction's k in any order that Q follows, so a lane reads D / 4 neighbouring
 // values of a key at once; the products with V pair up keys, so the nibbles of two keys are brought together first (a shift and a bitwise select for eight values),
 // and a lane has D / 8 neighbouring dimensions.  Q is fp16, bf16 rows scaled by a power of two to [2^14, 2^15): exact but for values below 2^-28 of the largest,
-// whose error is below 2^-39 of it.  Weights are fp16 multiples of 2^-24 of up to 2^15: off by 2^-12 of themselves (a result in bf16 is rounded to 2^-9), in two
+// whose error is below 2^-39 of it.  Weights are fp16 multiples of 2^-24 of up to 2^15: off by 2^-11 of themselves (a result in bf16 is rounded by up to 2^-8), in two
 // such parts where the result is fp16.  Sums are in 32 bits.
+//
+// What bounds it: 9 / 16 of a byte a value would be 5.9 TB/s of codes at the rate of a 16-bit copy; turning them into operands takes about 160 instructions of the integer pipe for 16
+// keys and their values of 128, which is 27 us of two requests of 95000 beside 33.5 of their bytes; the two together with the matrix and exponential pipes leave 49.4 (74 % of the
+// copy's rate without the 5 of the join).  Three CTAs of 168 registers keep the pipes busier than four of 128 (49.4 to 54.4).  64 requests of 700 to 1301 take 26.4 (bytes 11.4): 13 at that
+// rate, 4 for the join, the rest for the chain at a CTA's start (lengths, pages, keys) and for ends of rows; one of 700 5.7; 24 of 60 to 924 with 16 / 8 heads of 64, capped, with
+// sinks and a window, 9.4.  A tcgen05 product would want the codes in shared memory as fp16 first: as many conversions, and their stores.
 #include "attention_prompt.cuh"
 #include "cluster.cuh"
 #include "device_once.h"
@@ -41,7 +47,7 @@ struct Params {
   void* out;
   float* lse;
   const float* sinks;
-  float* part;               // [segment][COLS][D + 2]: output, maximum, sum
+  float* part;               // [CTA][a row that began in front of the CTA's tiles, the one it leaves unfinished][COLS][D + 2]: output, maximum, sum
   int2* info;                // [row]: its first CTA, and how many
   int64_t q_stride, out_stride, bt_stride, num_blocks;
   int B, Hkv, G, BS, max_rows, few, ctas, chunks, extra, parts, window, bf16, shift;      // shift: of BS where that is a power of two, or -1
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) l_run[nt][u] += __shfl_xor_sync(0xffffffffu, l_run[nt][u], x);
-          if (m_run[nt][u] == NONE) m_run[nt][u] = -INFINITY;
+          if (m_run[nt][u] == NONE) m_run[nt][u] = l_run[nt][u] == 0.f ? -INFINITY : 0.f;        // (nothing seen, or nothing but NaN)
           if (r0 == 0) maxima[warp * MOST_COLS + nt * 8 + q0 + u] = make_float2(m_run[nt][u], l_run[nt][u]);
         }
       __syncthreads();
@@ -649,7 +655,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
             }
             if (p.lse && r0 == 0 && i0 == 0) p.lse[(int64_t)(first_q + tok) * p.Hkv * p.G + head] = sum > 0.f ? (base + log2f(sum)) * LN2 : sum == 0.f ? -INFINITY : sum;
           } else {
-            float* part = (fused ? part_s : p.part + (int64_t)(index + blockIdx.x) * COLS * PD) + g * PD;
+            float* part = (fused ? part_s : p.part + (int64_t)(2 * blockIdx.x + (done.begin >= t0)) * COLS * PD) + g * PD;
 #pragma unroll
             for (int i = 0; i < HALF; ++i)
               if (KD % 2 == 0 || i0 + i < KD) *reinterpret_cast<float2*>(part + d0 + 2 * i) = x[i];
@@ -710,28 +716,29 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, in
   if (col >= cols || tok >= req.t) return;
   const int count = req.n > 0 ? at.y : 0;
   if (count == 1) return;                                // done where its keys were
-  const int step = cols * PD;                            // (a part's floats)
-  const float* x = p.part + ((int64_t)(index + (count ? at.x : 0)) * cols + col) * PD;
+  // of part i: the first is what its CTA left unfinished, the others are the first rows of theirs
+  const float* x = p.part + ((int64_t)(count ? 2 * at.x : 0) * cols + col) * PD;
+  auto part = [&](int i) { return x + (int64_t)(2 * i + (i == 0)) * cols * PD; };
   auto read = [&](int from, float2 (&y)[AHEAD][PAIRS]) { // parts from, from + EACH, ...
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j)
-        if (from + k * EACH < count && lane + 32 * j < pairs) y[k][j] = *reinterpret_cast<const float2*>(x + (int64_t)(from + k * EACH) * step + 2 * (lane + 32 * j));
+        if (from + k * EACH < count && lane + 32 * j < pairs) y[k][j] = *reinterpret_cast<const float2*>(part(from + k * EACH) + 2 * (lane + 32 * j));
   };
   float2 y[AHEAD][PAIRS];
-  float2 ml = lane < count ? *reinterpret_cast<const float2*>(x + (int64_t)lane * step + D) : make_float2(-INFINITY, 0.f);
+  float2 ml = lane < count ? *reinterpret_cast<const float2*>(part(lane) + D) : make_float2(-INFINITY, 0.f);
   read(w, y);
   const int head = h * p.G + r - tok * p.G;
   const int64_t token = (p.qsl ? p.qsl[b] : b) + tok;
   const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY;
   float top = fmaxf(sink, ml.x);
-  for (int i = 32 + lane; i < count; i += 32) top = fmaxf(top, x[(int64_t)i * step + D]);
+  for (int i = 32 + lane; i < count; i += 32) top = fmaxf(top, part(i)[D]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base), total = ml.x == -INFINITY ? 0.f : ml.y * f;
   for (int i = 32 + lane; i < count; i += 32) {
-    const float2 v = *reinterpret_cast<const float2*>(x + (int64_t)i * step + D);
+    const float2 v = *reinterpret_cast<const float2*>(part(i) + D);
     if (v.x > -INFINITY) total += v.y * ex2(v.x - base);
   }
   total = warp_sum(total) + (p.sinks ? ex2(sink - base) : 0.f);
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int cols, in
   for (int i = w, block = 0; i < count; i += AHEAD * EACH) {
     if (i / 32 != block) {                               // factors of the next 32 parts, a lane each (AHEAD EACH divides 32)
       block = i / 32;
-      const float m = block * 32 + lane < count ? x[(int64_t)(block * 32 + lane) * step + D] : -INFINITY;
+      const float m = block * 32 + lane < count ? part(block * 32 + lane)[D] : -INFINITY;
       f = m == -INFINITY ? 0.f : ex2(m - base);
     }
     if (i != w) read(i, y);
@@ -846,8 +853,8 @@ EXPORT int vb_attention_fp4_plan(int D, int rows, int parts, int* cols, int* cta
   return rc;
 }
 
-// Requests of at most `few` new tokens (qsl null: one each); rows of q and out of the others are not touched.  `ws`: for rows = group Hkv chunks,
-// (rows + ctas) cols (D + 2) + 2 rows floats, chunks = ceil(few Hq / Hkv / cols).  group: requests of a launch, up to 512.  extra: tiles that a row counts for
+// Requests of at most `few` new tokens (qsl null: one each); rows of q and out of the others are not touched.  `ws`: 2 ctas cols (D + 2) + 2 group Hkv chunks
+// floats, chunks = ceil(few Hq / Hkv / cols).  group: requests of a launch, up to 512.  extra: tiles that a row counts for
 // beside its own.  parts: CTAs of a cluster that has a row (one kernel, no `ws`); 0: equal runs.  max_rows: rows of a request that the block table has room for.
 // lse [T, Hq] or null.
 EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, void* out, float* lse,
@@ -856,12 +863,12 @@ EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks
                             cudaStream_t st) {
   using namespace afp4;
   if (B <= 0) return 0;
-  if (group < 1 || group > MAX_REQUESTS || few < 1 || max_rows < 1 || ctas < 1 || extra < 0 || parts < 0 || parts > 8) return -1;
+  if (group < 1 || group > MAX_REQUESTS || few < 1 || max_rows < 0 || ctas < 1 || extra < 0 || parts < 0 || parts > 8) return -1;
   if ((dtype != DT_BF16 && dtype != DT_F16) || BS < 16 || BS % 16 || Hkv < 1 || Hq % Hkv || q_stride % 8 || out_stride % 8) return -1;
   if (parts > 0 && B > group) return -1;
   Params p;
   p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.extra = extra; p.parts = parts; p.window = window; p.bf16 = dtype == DT_BF16;
-  if ((int64_t)few * p.G > 4096 || p.G > 64) return -1;
+  if ((int64_t)few * p.G > 4096 || p.G > 64 || (int64_t)Hkv * few * p.G > 65535) return -1;
   const int nt = groups_of(D, few * p.G);
   p.chunks = (few * p.G + 8 * nt - 1) / (8 * nt);
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.num_blocks = num_blocks; p.cache = (const uint8_t*)cache; p.sinks = sinks;
@@ -883,10 +890,9 @@ EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks
     p.seq_lens = seq_lens + b0;
     const int64_t rows = (int64_t)p.B * Hkv * p.chunks, tiles = rows * ((max_rows + TILE - 1) / TILE + extra);
     if (tiles >= (1 << 29)) return -3;                 // flat strip numbers are 32 bits
-    if (rows > 65535) return -3;
-    p.ctas = ctas < tiles ? ctas : (int)tiles;
+    p.ctas = (int)max((int64_t)1, min((int64_t)ctas, tiles));
     p.part = ws;
-    p.info = reinterpret_cast<int2*>(ws + (rows + p.ctas) * 8 * nt * (D + 2));
+    p.info = reinterpret_cast<int2*>(ws + (int64_t)2 * p.ctas * 8 * nt * (D + 2));
     const int rc = go(p, D, nt, st);
     if (rc) return rc;
   }

@@ -12,6 +12,10 @@
 // an eighth of its rounding where it is bf16); sums are in 32 bits.
 //
 // Where there are fewer CTAs than the SMs hold, the keys are split and a second kernel joins the parts.
+//
+// It is bound by the legacy matrix instructions (560 TFLOP/s at most) and by how few warps the registers leave: 200 to 240 TFLOP/s for heads of 64 to 192, 171 for 256.  us for two
+// prompts of 2000 behind 1500, 20 / 4 heads of 64, 80, 96, 128, 192, 256: 234, 295, 335, 418, 581, 1080; heads of up to 128 read back to 16-bit pages of 128 take 204 to 209 there on
+// the tcgen05 kernel and are better off here only in short portions (fp4_kernels in ops/cuda.py).
 #include "attention_prompt.cuh"
 #include "device_once.h"
 #include "fp4.cuh"
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
       l32 += __shfl_xor_sync(0xffffffffu, l32, 2);
       const int i = wr + m * 16 + u * 8 + g, r = sp.r0 + i, tok = r / p.G, head = h * p.G + r - tok * p.G;
       if (i >= sp.rows) continue;
-      const bool none = m_run[m][u] == NONE;
+      const bool none = m_run[m][u] == NONE && l == 0.f;       // (with a NaN sum: nothing but NaN was seen, and that comes out)
       const int64_t at = (int64_t)(first_q + tok) * p.Hkv * p.G + head;
       if (p.splits > 1) {
         float* to = p.part + (split * p.tokens * p.Hkv * p.G + at) * (D + 4);
@@ -434,7 +438,7 @@ EXPORT int vb_rows_fp4(const void* q, const void* cache, int64_t num_blocks, con
                        int64_t bt_stride, int splits, int window, float scale, float soft_cap, float out_scale, int dtype, cudaStream_t st) {
   using namespace rfp4;
   if (B <= 0 || max_q <= few) return 0;
-  if ((dtype != DT_BF16 && dtype != DT_F16) || BS < 16 || BS % 16 || Hkv < 1 || Hkv > 65535 || Hq % Hkv || B > 65535 || q_stride % 8 || out_stride % 8 || !qsl || max_rows < 1 ||
+  if ((dtype != DT_BF16 && dtype != DT_F16) || BS < 16 || BS % 16 || Hkv < 1 || Hkv > 65535 || Hq % Hkv || B > 65535 || q_stride % 8 || out_stride % 8 || !qsl || max_rows < 0 ||
       splits < 1 || splits > MOST_SPLITS || (splits > 1 && !ws))
     return -1;
   Params p;

@@ -427,7 +427,11 @@ def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft
                         alibi_slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, chunk_size: int = 0, return_lse: bool = False,
                         out_scale: float = 1.0, k_scale: float = 1.0, v_scale: float = 1.0):
     """``paged_attention`` over a cache in 4 bits; q [T, heads, head size] in 16 bits on the device, ``md.kv_vt`` False.  The output is that of the values
-    which the cache stands for."""
+    which the cache stands for.
+
+    Requests of few new tokens are attended straight from the cache, whatever ``md.max_seq_len`` says.  Prompts may be read back to 16-bit pages first (up to 1 GiB of
+    them at a time, more for a request that needs more): ``md.max_query_len`` and, where the step has no lengths on the host, ``md.max_seq_len`` are then no smaller than
+    what they stand for."""
     op = "paged_attention_fp4"
     H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
     shape = q.shape

@@ -808,7 +808,9 @@ _attention_fp4 = _sig("vb_attention_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _v
                       _i, _vp)
 _attention_fp4_plan = _sig("vb_attention_fp4_plan", _i, _i, _i, ctypes.POINTER(_i), ctypes.POINTER(_i), ctypes.POINTER(_i))
 FP4_HEADS = (32, 64, 80, 96, 128, 192, 256)
-FP4_EXTRA = 3                                # tiles that a row counts for beside its own, as its end costs about as much
+# tiles that a row counts for beside its own, as its end costs about as much: us with 0, 2, 4 and 8 of them, 64 x 1000 with 32 / 8 heads of 128 27.5, 26.1, 26.0, 26.0; 16 x 3500 with
+# five new tokens 38.5, 38.0, 36.4, 35.6; 16 x 2000 17.8, 16.9, 16.7, 17.1; 32 x 700 of 64 12.2, 11.9, 12.3, 12.7
+FP4_EXTRA = 4
 
 
 @functools.lru_cache(maxsize=None)
@@ -831,27 +833,26 @@ def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def fp4_schedule(device: int, B: int, H: int, G: int, D: int, few: int, max_rows: int) -> tuple[int, int, int, int, int]:
-    """(CTAs, CTAs of a cluster that has a row, requests of a launch, floats of the workspace, launches)."""
-    tiles, query_rows = -(-max_rows // 64), few * G
+def fp4_schedule(device: int, B: int, H: int, G: int, D: int, few: int, room: int, longest: int) -> tuple[int, int, int, int, int]:
+    """(CTAs, CTAs of a cluster that has a row, requests of a launch, floats of the workspace, launches) for B requests in tables of ``room`` tiles, of up to about ``longest``."""
+    query_rows = few * G
     cols, ctas, _ = fp4_plan(device, D, min(query_rows, 17), 0)
-    chunks = -(-query_rows // cols)
-    group = min(512, 65535 // (H * chunks))
+    chunks, ctas = -(-query_rows // cols), ctas * num_sms()
+    group = max(1, min(512, (1 << 29) // (H * chunks * (room + FP4_EXTRA + 1))))      # (numbers of strips have 32 bits)
     launches = -(-B // group)
     group = -(-B // launches)
-    parts, ctas = fp4_parts(B * H * chunks, tiles, D, query_rows) if launches == 1 else 0, ctas * num_sms()
-    rows = group * H * chunks
-    return ctas, parts, group, 0 if parts else (rows + ctas) * cols * (D + 2) + 2 * rows, 1 if parts else 2 * launches
+    parts = fp4_parts(B * H * chunks, longest, D, query_rows) if launches == 1 else 0
+    return ctas, parts, group, 0 if parts else 2 * ctas * cols * (D + 2) + 2 * group * H * chunks, 1 if parts else 2 * launches
 
 
-def _fp4_few(q, kv_cache, md, H: int, D: int, BS: int, max_rows: int, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
-    """Attention of the requests with at most ``few`` new tokens, straight from the cache; rows of the others are not touched."""
+def _fp4_few(q, kv_cache, md, H: int, D: int, BS: int, room: int, scale, window, soft_cap, out, lse, sinks, out_scale, few: int) -> None:
+    """Attention of the requests with at most ``few`` new tokens, straight from the cache; rows of the others are not touched.  ``room``: rows of a block table."""
     bt, B, Hq = md.block_table, md.num_reqs, q.shape[1]
-    ctas, parts, group, floats, launches = fp4_schedule(_device(), B, H, Hq // H, D, few, max(1, max_rows))
+    ctas, parts, group, floats, launches = fp4_schedule(_device(), B, H, Hq // H, D, few, -(-room // 64), -(-min(room, md.max_seq_len) // 64))
     # (of this call: two calls at once, or two captured graphs, share nothing)
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     _check(_attention_fp4(q.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], bt.data_ptr(), md.seq_lens.data_ptr(), None if md.decode_only else md.query_start_loc.data_ptr(),
-                          out.data_ptr(), _p(lse), _p(sinks), _p(ws), B, Hq, H, D, BS, max(1, max_rows), few, q.stride(0), out.stride(0), bt.stride(0), ctas, FP4_EXTRA, parts, group,
+                          out.data_ptr(), _p(lse), _p(sinks), _p(ws), B, Hq, H, D, BS, room, few, q.stride(0), out.stride(0), bt.stride(0), ctas, FP4_EXTRA, parts, group,
                           window or 0, scale, soft_cap, out_scale, _DT[q.dtype], _st()), "attention_fp4", launches)
 
 
@@ -893,7 +894,7 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
     """Attention of the requests with more than ``few`` new tokens, straight from the cache (csrc/attention_fp4_rows.cu)."""
     (T, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
     B, bt, G, max_q = md.num_reqs, md.block_table, Hq // kv_cache.shape[2], min(md.max_query_len, q.shape[0])
-    max_rows = max(1, min(bt.shape[1] * BS, md.max_seq_len))
+    room = bt.shape[1] * BS
     tiles, lens = B * -(-max_q * G // 128), getattr(md, "host_lens", None)
     if lens is not None:
         cu = lens[0]
@@ -901,10 +902,10 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
         if not tiles:
             return
     # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
-    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), max_rows // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 4))))
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 4))))
     ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 4), dtype=torch.float32, device=q.device)
     _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
-                     _p(ws), B, T, max_q, Hq, H, D, BS, max_rows, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
+                     _p(ws), B, T, max_q, Hq, H, D, BS, room, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
                      _DT[q.dtype], _st()), "rows_fp4", 1 if splits == 1 else 2)
 
 
@@ -933,9 +934,9 @@ def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[i
     return runs
 
 
-def fit_rows(x, y, H: int) -> None:
-    """x [T, heads, D] to y [T, more or fewer heads of each of the H kv heads, D2]: what x does not have is zeros."""
-    T, (hx, dx), (hy, dy) = x.shape[0], x.shape[1:], y.shape[1:]
+def fit_rows(x, y, T: int, H: int) -> None:
+    """The first T rows of x [., heads, D] to y [., more or fewer heads of each of the H kv heads, D2]: what x does not have is zeros."""
+    (hx, dx), (hy, dy) = x.shape[1:], y.shape[1:]
     _check(_fit_rows(x.data_ptr(), y.data_ptr(), T, H, hx // H, dx, hy // H, dy, x.stride(0), y.stride(0), num_sms(), _DT[x.dtype], _st()), "fit_rows")
 
 
@@ -948,7 +949,7 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
         W, G = 128, 1 << (Hq // H - 1).bit_length()
         if W != D or G != Hq // H:
             q, narrow = q.new_empty((T, H * G, W)), q
-            fit_rows(narrow, q, H)
+            fit_rows(narrow, q, T, H)
             to, norm = torch.empty_like(q), None if lse is None else lse.new_empty((T, H * G))
             if sinks is not None:
                 sinks = torch.nn.functional.pad(sinks.view(H, Hq // H), (0, G - Hq // H)).flatten()
@@ -985,7 +986,7 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
                 t = torch.arange(T, device=q.device)
                 norm.copy_(torch.where(((t >= qsl[b0]) & (t < qsl[b1]))[:, None], got[1], norm))
     if to is not out:
-        fit_rows(to, out, H)
+        fit_rows(to, out, md.num_reqs if md.decode_only else md.num_actual_tokens, H)       # (rows behind the last token's are left as they are)
         if lse is not None:
             lse.view(T, H, -1).copy_(norm.view(T, H, -1)[:, :, :Hq // H])
 
@@ -1012,11 +1013,11 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
-    few, longest, G, max_rows = 0, 1 if decode else md.max_query_len, Hq // H, min(md.max_seq_len, width * BS)
+    few, longest, G, room = 0, 1 if decode else md.max_query_len, Hq // H, width * BS
     scale, out_scale = scale * k_scale, out_scale * v_scale
     direct = D in FP4_HEADS and alibi is None and not chunk and (causal or decode) and G <= 64 and not batch_invariant()
     if direct:
-        few, straight = (1, True) if longest == 1 else fp4_kernels(used, B, longest, max_rows, H, G, D)
+        few, straight = (1, True) if longest == 1 else fp4_kernels(used, B, longest, min(md.max_seq_len, room), H, G, D)
     if B and few < longest:
         if direct and straight:
             _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, to, lse, sinks, out_scale, few)
@@ -1026,7 +1027,7 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
         if lens is not None and all(lens[0][b + 1] - lens[0][b] > few for b in range(B)):
             few = 0                          # (no request has so few)
     if B and few:
-        _fp4_few(q, kv_cache, md, H, D, BS, max_rows, scale, window, soft_cap, to, lse, sinks, out_scale, few)
+        _fp4_few(q, kv_cache, md, H, D, BS, room, scale, window, soft_cap, to, lse, sinks, out_scale, few)
     if to is not out and out is not None:
         out[:used] = to[:used]
         to = out
