@@ -34,7 +34,7 @@ struct Params {
   void* out;
   float* lse;
   const float* sinks;
-  float* part;               // [split][token, head][D + 4]: output, maximum, sum of the weights as they were multiplied and before they were rounded
+  float* part;               // [split][token, head][D + 2]: output, maximum, sum
   int64_t q_stride, out_stride, bt_stride, num_blocks, tokens;
   int Hkv, G, BS, max_rows, few, splits, window, bf16;
   float scale_log2, ku, c2, out_scale;
@@ -209,8 +209,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
     }
   const int warp_first = n - sp.t + (sp.r0 + wr) / p.G, warp_last = wr < sp.rows ? n - sp.t + (sp.r0 + min(wr + 16 * MT, sp.rows) - 1) / p.G : -1;
 
-  float o[MT][D / 8][4], m_run[MT][2], sum[MT][4];       // sum: of the weights as they are multiplied, rows g and g + 8, in each of two columns
-  float exact[MT][2];                                  // the lane's, before they are rounded: for log-sum-exps
+  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
   bool huge = false;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -219,7 +218,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[m][i][j] = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) { m_run[m][u] = NONE; sum[m][2 * u] = sum[m][2 * u + 1] = exact[m][u] = 0.f; }
+    for (int u = 0; u < 2; ++u) { m_run[m][u] = NONE; l_run[m][u] = 0.f; }
   }
   if (sp.lo < sp.hi) store(0);
   const uint32_t base = smem_u32(smem);
@@ -273,11 +272,14 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
           f[0] = f[1] = 1.f;
         }
         uint32_t most = 0u;                              // the largest weights, two halves
+        float add[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            w[m][i][u] = pack2<__half>(ex2(fmaf(s[m][i][2 * u], f[u], -m_run[m][u])), ex2(fmaf(s[m][i][2 * u + 1], f[u], -m_run[m][u])));
+            const float x = ex2(fmaf(s[m][i][2 * u], f[u], -m_run[m][u])), y = ex2(fmaf(s[m][i][2 * u + 1], f[u], -m_run[m][u]));
+            add[u] += x + y;
+            w[m][i][u] = pack2<__half>(x, y);
             most = max2(most, w[m][i][u]);
           }
         if (__any_sync(0xffffffffu, (most & 0xffffu) > 0x7800u || most > 0x7800ffffu)) {          // above 2^15
@@ -292,7 +294,8 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
             const bool up = at > was + 8.f;
             const float alpha = up ? ex2(was - at) : 1.f;
             m_run[m][u] = up ? at : was;
-            sum[m][2 * u] *= alpha; sum[m][2 * u + 1] *= alpha; exact[m][u] *= alpha;
+            l_run[m][u] *= alpha;
+            add[u] = 0.f;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) { o[m][i][2 * u] *= alpha; o[m][i][2 * u + 1] *= alpha; }
           }
@@ -300,20 +303,14 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)                  // (the difference of two rounded numbers: nothing is left over where scores are huge)
-              w[m][i][u] = pack2<__half>(ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u], f[u]), m_run[m][u])), ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u + 1], f[u]), m_run[m][u])));
+            for (int u = 0; u < 2; ++u) {                // (the difference of two rounded numbers: nothing is left over where scores are huge)
+              const float x = ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u], f[u]), m_run[m][u])), y = ex2(__fsub_rn(__fmul_rn(s[m][i][2 * u + 1], f[u]), m_run[m][u]));
+              add[u] += x + y;
+              w[m][i][u] = pack2<__half>(x, y);
+            }
         }
-        if (p.lse) {                                     // (asked for seldom: the exponentials once more)
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) exact[m][j >> 1] += ex2(__fsub_rn(__fmul_rn(s[m][i][j], f[j >> 1]), m_run[m][j >> 1]));
-        }
-#pragma unroll
-        for (int kk = 0; kk < SUB / 16; ++kk) {          // sums of the weights, as a product with ones
-          const uint32_t a[4] = {w[m][2 * kk][0], w[m][2 * kk][1], w[m][2 * kk + 1][0], w[m][2 * kk + 1][1]};
-          mma16816(sum[m], a, 0x3c003c00u, 0x3c003c00u);
-        }
+        l_run[m][0] += add[0];
+        l_run[m][1] += add[1];
       }
       // ---- O += P V
       const uint32_t vs = base + buf * F::BUF + F::SIDE + (k0 + (mi & 1) * 8 + l7) * F::LD + (mi >> 1) * 16;
@@ -338,20 +335,19 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float l = sum[m][2 * u];
-      float l32 = exact[m][u];
-      l32 += __shfl_xor_sync(0xffffffffu, l32, 1);
-      l32 += __shfl_xor_sync(0xffffffffu, l32, 2);
+      float l = l_run[m][u];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
       const int i = wr + m * 16 + u * 8 + g, r = sp.r0 + i, tok = r / p.G, head = h * p.G + r - tok * p.G;
       if (i >= sp.rows) continue;
       const bool none = m_run[m][u] == NONE && l == 0.f;       // (with a NaN sum: nothing but NaN was seen, and that comes out)
       const int64_t at = (int64_t)(first_q + tok) * p.Hkv * p.G + head;
       if (p.splits > 1) {
-        float* to = p.part + (split * p.tokens * p.Hkv * p.G + at) * (D + 4);
+        float* to = p.part + (split * p.tokens * p.Hkv * p.G + at) * (D + 2);
         if (!none)
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(to + j * 8 + t4 * 2) = make_float2(o[m][j][2 * u], o[m][j][2 * u + 1]);
-        if (t4 == 0) *reinterpret_cast<float4*>(to + D) = make_float4(none ? -INFINITY : m_run[m][u], l, l32, 0.f);
+        if (t4 == 0) *reinterpret_cast<float2*>(to + D) = make_float2(none ? -INFINITY : m_run[m][u], l);
         continue;
       }
       const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = none ? sink : fmaxf(m_run[m][u], sink), base2 = top == -INFINITY ? 0.f : top;
@@ -362,7 +358,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
         const float x = none ? 0.f : o[m][j][2 * u] * f, y = none ? 0.f : o[m][j][2 * u + 1] * f;
         *reinterpret_cast<uint32_t*>(to + j * 8) = BF16 ? pack2<__nv_bfloat16>(x, y) : pack2<__half>(x, y);
       }
-      if (t4 == 0 && p.lse) p.lse[at] = log_of(base2, (none ? 0.f : l32 * back) + (p.sinks ? ex2(sink - base2) : 0.f));
+      if (t4 == 0 && p.lse) p.lse[at] = log_of(base2, all);
     }
 }
 
@@ -374,13 +370,13 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int D) {
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
   const Span sp = span_of(p, b, blockIdx.x / PER_TILE, 0);
   const int first_q = p.qsl[b];
-  const int64_t step = p.tokens * p.Hkv * p.G * (D + 4);
+  const int64_t step = p.tokens * p.Hkv * p.G * (D + 2);
   const int i = blockIdx.x % PER_TILE * (JOIN / 32) + (threadIdx.x >> 5);
   if (i < sp.rows) {
     const int r = sp.r0 + i, tok = r / p.G, head = h * p.G + r - tok * p.G;
     const int64_t at = (int64_t)(first_q + tok) * p.Hkv * p.G + head;
-    const float* x = p.part + at * (D + 4);
-    const float4 ml = lane < p.splits ? *reinterpret_cast<const float4*>(x + lane * step + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const float* x = p.part + at * (D + 2);
+    const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(x + lane * step + D) : make_float2(-INFINITY, 0.f);
     const float sink = p.sinks ? p.sinks[head] * LOG2E : -INFINITY, top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
     const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - base);
     const float sum = warp_sum(ml.x == -INFINITY ? 0.f : ml.y * f) + (p.sinks ? ex2(sink - base) : 0.f), by = sum == 0.f ? 0.f : p.out_scale / sum;
@@ -398,8 +394,7 @@ __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int D) {
       }
       if (d < D) *reinterpret_cast<uint32_t*>(to + d) = p.bf16 ? pack2<__nv_bfloat16>(acc.x * by, acc.y * by) : pack2<__half>(acc.x * by, acc.y * by);
     }
-    const float l32 = warp_sum(ml.x == -INFINITY ? 0.f : ml.z * f) + (p.sinks ? ex2(sink - base) : 0.f);
-    if (lane == 0 && p.lse) p.lse[at] = log_of(base, l32);
+    if (lane == 0 && p.lse) p.lse[at] = log_of(base, sum);
   }
 }
 
@@ -431,7 +426,7 @@ EXPORT int vb_rows_fp4_ctas(int D, int* ctas) {
   return rfp4::go(p, D, dim3(1), nullptr, ctas);
 }
 
-// Causal attention of requests of more than `few` new tokens, at most max_q; rows of q and out [tokens] of the others are not touched.  ws: for splits > 1, splits tokens Hq (D + 4)
+// Causal attention of requests of more than `few` new tokens, at most max_q; rows of q and out [tokens] of the others are not touched.  ws: for splits > 1, splits tokens Hq (D + 2)
 // floats.  lse [tokens, Hq] or null.
 EXPORT int vb_rows_fp4(const void* q, const void* cache, int64_t num_blocks, const int* block_table, const int* seq_lens, const int* qsl, void* out, float* lse,
                        const float* sinks, float* ws, int B, int64_t tokens, int max_q, int Hq, int Hkv, int D, int BS, int max_rows, int few, int64_t q_stride, int64_t out_stride,

@@ -902,8 +902,8 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
         if not tiles:
             return
     # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
-    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 4))))
-    ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 4), dtype=torch.float32, device=q.device)
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
+    ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=q.device)
     _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
                      _p(ws), B, T, max_q, Hq, H, D, BS, room, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
                      _DT[q.dtype], _st()), "rows_fp4", 1 if splits == 1 else 2)
