@@ -5,7 +5,7 @@
 // A CTA has 128 query rows of a request and a kv head (pairs of a new token and a query head, so all heads of the kv head share its keys) and goes through the keys in tiles
 // of 64.  Codes and scales of the next tile are on their way into registers while this one is worked on; then every thread turns its groups of 16 into fp16 (exact)
 // in shared memory, where two tiles take turns: one barrier a tile.  S = Q K^T and O += P V are m16n8k16 products; a warp has 32 rows (heads of up to 96: a
-// fragment of keys or values then serves two products) or 16, and takes 32 keys at a time: weights go from the accumulators of the first
+// fragment of keys or values then serves two products) or 16, and takes 64 or 32 keys at a time: weights go from the accumulators of the first
 // product into the operands of the second.  The reference of a row's weights stays until a weight would be above 2^15 (attention_fp4.cu).
 //
 // Q is fp16, bf16 rows scaled by a power of two (exact, attention_fp4.cu).  Weights are fp16 (off by at most 2^-11 of themselves: as the result where that is fp16,
@@ -13,16 +13,17 @@
 //
 // Where there are fewer CTAs than the SMs hold, the keys are split and a second kernel joins the parts.
 //
-// It is bound by the legacy matrix instructions (560 TFLOP/s at most) and by how few warps the registers leave: 200 to 240 TFLOP/s for heads of 64 to 192, 171 for 256.  us for two
-// prompts of 2000 behind 1500, 20 / 4 heads of 64, 80, 96, 128, 192, 256: 234, 295, 335, 418, 581, 1080; heads of up to 128 read back to 16-bit pages of 128 take 204 to 209 there on
-// the tcgen05 kernel and are better off here only in short portions (fp4_kernels in ops/cuda.py).
+// It is bound by the legacy matrix instructions (560 TFLOP/s at most) and by how few warps the registers leave: 220 to 240 TFLOP/s for heads of 64 to 192, 173 for 256.  us for two
+// prompts of 2000 behind 1500, 20 / 4 heads of 64, 80, 96, 128, 192, 256: 206, 282, 310, 394, 575, 1063 (64 keys at a time; 32: 224, 282, 310, 416, 575, 1063, and 64 for 96 357); heads of
+// up to 128 read back to 16-bit pages of 128 take 204 to 209 there on the tcgen05 kernel and are better off here only in short portions (fp4_kernels in ops/cuda.py).  256 rows of a CTA
+// share the keys' conversion but wait for one another: 251 where 128 took 226 (500 new tokens behind 11 500, 16 / 4 heads of 64, now 204).
 #include "attention_prompt.cuh"
 #include "device_once.h"
 #include "fp4.cuh"
 
 namespace rfp4 {
 
-constexpr int TILE = 64, ROWS = 128, SUB = 32;
+constexpr int TILE = 64, ROWS = 128;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, SHIFT = 7.f, NONE = -3e38f;
 
 struct Params {
@@ -77,6 +78,7 @@ VB_DEVICE float log_of(float base, float sum) { return sum > 0.f ? (base + log2f
 template <int D_> struct Form {
   static constexpr int D = D_, MT = D <= 96 ? 2 : 1, WARPS = ROWS / (16 * MT), THREADS = WARPS * 32;
   static constexpr int CTAS = D <= 96 ? 2 : 1;             // of an SM
+  static constexpr int SUB = D <= 64 || D == 128 ? 64 : 32;              // keys that a warp takes at a time: as many as the registers hold scores of
   static constexpr int LD = 2 * D + 16;                                  // bytes of a row in shared memory: an odd number of 16, so that neighbouring rows begin in different banks
   static constexpr int SIDE = TILE * LD, BUF = 2 * SIDE, SMEM = 2 * BUF;
   static constexpr int GROUPS = TILE * D / 16, MINE = (GROUPS + THREADS - 1) / THREADS;      // of a side; of a thread
@@ -85,7 +87,7 @@ template <int D_> struct Form {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(const Params p) {
   using F = Form<D>;
-  constexpr int MT = F::MT, KD = D / 16, NT = SUB / 8, MINE = F::MINE;
+  constexpr int MT = F::MT, KD = D / 16, SUB = F::SUB, NT = SUB / 8, MINE = F::MINE;
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
     __syncthreads();                                   // the tile is there, and nobody reads the other one
     read(tl + 1);
     look(tl + 2);
-#pragma unroll 1
+#pragma unroll
     for (int k0 = 0; k0 < TILE; k0 += SUB) {
       const int key0 = tl * TILE + k0;
       if (key0 > warp_last || (p.window > 0 && key0 + SUB <= warp_first - p.window + 1)) continue;

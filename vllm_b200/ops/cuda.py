@@ -862,15 +862,15 @@ FP4_FEW_ROWS = 64                            # query rows (new tokens x query he
 def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int) -> tuple[int, bool]:
     """(new tokens up to which a request takes the kernel of single tokens, whether the others' prompts go straight from the cache or through 16-bit pages), for T
     tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: the kernel of single tokens 2.6 TB/s of the cache for every 24
-    query rows (16 where heads are above 128); the one of prompts 190 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
-    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 33, 42, 202; 160 there 95, 78, 121; 320 there
-    175, 165, 124; 500 there 261, 238, 193; 160 behind 1200 32, 29, 35; 640 there 79, 49, 41; of 128, 80 behind 12 000 76, 91, 183; 160 there 135, 165, 119; of 192, 160 behind 4000 88, 84."""
+    query rows (16 where heads are above 128); the one of prompts 235 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
+    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 31, 38, 202; 160 there 83, 68, 121; 320 there
+    156, 138, 124; 500 there 239, 201, 193; 160 behind 1200 23, 26, 34; 640 there 60, 44, 42; of 128, 80 behind 12 000 70, 84, 180; 160 there 123, 151, 119; of 192, 160 behind 4000 80, 84."""
     base = max(1, FP4_FEW_ROWS // G)
     if longest <= base:
         return longest, True
     pairs = T * H * max(rows - longest / 2, 1)
     single = 6 + (T * G / (24 if D <= 128 else 16) + B) * rows * H * D * 1.125 / 2.6e6
-    straight = 20 + pairs * G * 4 * D / 190e6
+    straight = 10 + pairs * G * 4 * D / 235e6
     pages = float("inf")
     if D <= 128:
         pages = 20 + B * rows * H * 1024 / 4.5e6 + max(rows * 0.0085, pairs * (1 << (G - 1).bit_length()) * 512 / 800e6)
