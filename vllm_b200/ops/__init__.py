@@ -341,8 +341,8 @@ def _check_fp4(kv_cache, op: str, k_scale: float = 1.0, v_scale: float = 1.0) ->
     shape = kv_cache.shape
     if len(shape) != 5 or kv_cache.dtype is not torch.uint8 or not kv_cache.is_contiguous():
         raise ValueError(f"{op}: a contiguous uint8 cache of fp4_cache_shape; got {tuple(shape)} of {kv_cache.dtype}")
-    _, two, H, page, row = shape
-    if two != 2 or page < 16 or page % 16 or row < 9 or row % 9 or H < 1:
+    blocks, two, H, page, row = shape
+    if two != 2 or page < 16 or page % 16 or row < 9 or row % 9 or H < 1 or blocks < 1:
         raise ValueError(f"{op}: a cache of fp4_cache_shape; got {tuple(shape)}")
     if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
         raise ValueError(f"{op}: factors of keys and values above 0; got {k_scale} and {v_scale}")

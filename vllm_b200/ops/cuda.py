@@ -15,6 +15,7 @@ import functools
 import os
 from typing import Optional
 
+import numpy as np
 import torch
 
 from vllm_b200 import envs
@@ -895,10 +896,10 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
     (T, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
     B, bt, G, max_q = md.num_reqs, md.block_table, Hq // kv_cache.shape[2], min(md.max_query_len, q.shape[0])
     room = bt.shape[1] * BS
-    tiles, lens = B * -(-max_q * G // 128), getattr(md, "host_lens", None)
+    tiles, lens = B * -(-max_q * G // 128), _host_lens(md)
     if lens is not None:
-        cu = lens[0]
-        tiles = sum(-(-int(cu[b + 1] - cu[b]) * G // 128) for b in range(B) if cu[b + 1] - cu[b] > few)
+        new = lens[0]
+        tiles = int((-(-new[new > few] * G // 128)).sum())
         if not tiles:
             return
     # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
@@ -913,17 +914,32 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
 FP4_PAGES_BYTES = 1 << 30
 
 
+def _host_lens(md):
+    """(new tokens of each request, rows of each) where the step has them on the host, or None."""
+    lens = getattr(md, "host_lens", None)
+    if lens is None:
+        return None
+    cu, sl = (np.asarray(x, dtype=np.int64) for x in lens)
+    return np.diff(cu[:md.num_reqs + 1]), sl[:md.num_reqs]
+
+
 def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[int, int, int, int]]:
     """Runs of requests whose 16-bit pages fit into the workspace: (first, behind the last, pages of all, pages of the longest).  Lengths are those that the step
     has on the host; without them every request counts with ``most`` pages."""
-    B = md.num_reqs
-    need = [max(most, 1)] * B
-    lens = getattr(md, "host_lens", None)
+    B, most = md.num_reqs, max(most, 1)
+    lens = _host_lens(md)
     if lens is not None:
-        cu, sl = lens
-        need = [0 if not md.decode_only and cu[b + 1] - cu[b] <= few else max(min(-(-int(sl[b]) // PS), most), 1) for b in range(B)]
+        need = (-(-lens[1] // PS)).clip(1, most)
+        if not md.decode_only:
+            need[lens[0] <= few] = 0
     elif md.seq_lens_cpu is not None:
-        need = [max(min(-(-n // PS), most), 1) for n in md.seq_lens_cpu[:B].tolist()]
+        need = (-(-md.seq_lens_cpu[:B].long() // PS)).clamp(1, most).numpy()
+    else:
+        need = None
+    total = most * B if need is None else int(need.sum())
+    if total * page_bytes <= FP4_PAGES_BYTES:                # (nearly always)
+        return [(0, B, total, most if need is None else int(need.max(initial=0)))]
+    need = [most] * B if need is None else need.tolist()
     runs, first, total = [], 0, 0
     for b, n in enumerate(need):
         if total and (total + n) * page_bytes > FP4_PAGES_BYTES:
@@ -1023,8 +1039,8 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
             _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, to, lse, sinks, out_scale, few)
         else:
             _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale, few, direct)
-        lens = getattr(md, "host_lens", None)
-        if lens is not None and all(lens[0][b + 1] - lens[0][b] > few for b in range(B)):
+        lens = _host_lens(md)
+        if lens is not None and (lens[0] > few).all():
             few = 0                          # (no request has so few)
     if B and few:
         _fp4_few(q, kv_cache, md, H, D, BS, room, scale, window, soft_cap, to, lse, sinks, out_scale, few)
