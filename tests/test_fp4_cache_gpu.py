@@ -504,3 +504,20 @@ def test_many_tables_with_much_room():
     md.block_table, md.max_seq_len = wide, 160_000_000
     got = ops.paged_attention_fp4(q, cache, md, 0.1)
     assert (got.double() - want.double()).abs().max() < 0.02 and cuda_ops().fp4_schedule(0, 40, 8, 1, 64, 1, 2_500_000, 2_500_000)[4] > 2
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("D,lens,queries,few", [(64, [4500, 9], [24, 9], 0), (192, [4500], [20], 0), (128, [900, 256], [256, 250], 256), (192, [500, 700], [256, 33], 256), (80, [1300], [128], 128)])
+def test_most_parts_and_most_rows(dtype, D, lens, queries, few):
+    """Prompts in as many parts of keys as there may be (few = 0), and the kernel of single tokens with as many rows as the rule gives it."""
+    cu, G = cuda_ops(), 2048 // few if few else 4
+    q, cache, md = step(lens, queries, G, 1, D, 32, dtype, "cuda", seed=D, spread=2.0)
+    out, lse, scale = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda"), D ** -0.5
+    if few:
+        cu._fp4_few(q, cache, md, 1, D, 32, md.block_table.shape[1] * 32, scale, None, 0.0, out, lse, None, 1.0, few)
+    else:
+        cu._fp4_rows_attention(q, cache, md, scale, None, 0.0, out, lse, None, 1.0, few)
+    want, norm, mass, terms, big = attend(q, cache, md, scale, None, 0.0, None)
+    eps, u = (D / 8 + 16) * 2.0 ** -23 * terms + 8 * 2.0 ** -24 * 1.5 * terms + 2.0 ** -21, torch.finfo(dtype).eps / 2
+    bound = u * want.abs() + (2.0 ** -11 + 2 * eps + 2.0 ** -13) * mass + max(lens) * 2.0 ** -31 * big + 2.0 ** -25
+    assert ((out.double().cpu() - want).abs() <= bound).all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs()).all()

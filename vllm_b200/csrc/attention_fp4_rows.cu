@@ -37,7 +37,7 @@ struct Params {
   const float* sinks;
   float* part;               // [split][token, head][D + 2]: output, maximum, sum
   int64_t q_stride, out_stride, bt_stride, num_blocks, tokens;
-  int Hkv, G, BS, max_rows, few, splits, window, bf16, shift;      // shift: of BS where that is a power of two, or -1
+  int Hkv, G, BS, max_rows, few, splits, window, bf16;
   float scale_log2, ku, c2, out_scale;
 };
 
@@ -102,30 +102,41 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 
   // ---- codes and scales of a tile: a thread's groups
   const int64_t page = fp4::page_bytes(p.BS, D), to_v = p.Hkv * page;
-  int blk[MINE];                                       // of the tile that is read next
+  int at_page[MINE], at_off[MINE];                     // of the tile that is looked up next
+  int blk[MINE], off[MINE];                            // of the tile that is read next
+  const int pages_on = TILE / p.BS, rest = TILE % p.BS;
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) {
+    const int tok = sp.lo * TILE + (j * F::THREADS + threadIdx.x) / KD;
+    at_page[j] = tok / p.BS;
+    at_off[j] = tok % p.BS;
+  }
   uint2 codes[2][MINE];
-  uint32_t scales[MINE];
+  uint32_t scales[2][MINE];
   auto look = [&](int tl) {
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
       const int gi = j * F::THREADS + threadIdx.x, tok = tl * TILE + gi / KD;
-      const bool there = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n;
-      blk[j] = there ? p.block_table[b * p.bt_stride + (p.shift >= 0 ? tok >> p.shift : tok / p.BS)] : -1;
+      blk[j] = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n ? p.block_table[b * p.bt_stride + at_page[j]] : -1;
+      off[j] = at_off[j];
+      at_page[j] += pages_on;
+      at_off[j] += rest;
+      if (at_off[j] >= p.BS) { at_off[j] -= p.BS; ++at_page[j]; }
     }
   };
   auto read = [&](int tl) {
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-      const int gi = j * F::THREADS + threadIdx.x, r = gi / KD, c = gi - r * KD, tok = tl * TILE + r, off = p.shift >= 0 ? tok & (p.BS - 1) : tok % p.BS;
+      const int gi = j * F::THREADS + threadIdx.x, r = gi / KD, c = gi - r * KD, tok = tl * TILE + r;
       const bool there = (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) && tl < sp.hi && tok < n;
       const uint64_t at = (uint64_t)blk[j] < (uint64_t)p.num_blocks ? blk[j] : 0;      // (a table may not say that; nothing is read outside the cache)
       const uint8_t* k = p.cache + (uint32_t)(at * 2 * p.Hkv + h) * (uint64_t)(uint32_t)page;      // (pages of heads: below 2^31)
-      const uint8_t* x = k + off * (D / 2) + c * 8;
-      const uint8_t* s = k + p.BS * (D / 2) + off * (D / 16) + c;
+      const uint8_t* x = k + off[j] * (D / 2) + c * 8;
+      const uint8_t* s = k + p.BS * (D / 2) + off[j] * (D / 16) + c;
       codes[0][j] = there ? *reinterpret_cast<const uint2*>(x) : make_uint2(0u, 0u);
       codes[1][j] = there ? *reinterpret_cast<const uint2*>(x + to_v) : make_uint2(0u, 0u);
-      // keys' below, values' above; values that no row sees may be what a weight of 0 does not cancel
-      scales[j] = there ? s[0] | (tok >= low ? (uint32_t)s[to_v] << 8 : 0u) : 0u;
+      scales[0][j] = there ? s[0] : 0u;
+      scales[1][j] = there && tok >= low ? s[to_v] : 0u;            // values that no row sees may be what a weight of 0 does not cancel
     }
   };
   auto store = [&](int buf) {
@@ -133,7 +144,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
     for (int j = 0; j < MINE; ++j) {
       const int gi = j * F::THREADS + threadIdx.x, r = gi / KD, c = gi - r * KD;
       if (F::GROUPS % F::THREADS == 0 || gi < F::GROUPS) {
-        const uint32_t two = fp4::scales2(scales[j]);
+        const uint32_t two = fp4::scales2(scales[0][j] | scales[1][j] << 8);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
           const uint32_t f = side ? fp4::high2(two) : fp4::low2(two);
@@ -354,7 +365,7 @@ __global__ void __launch_bounds__(Form<D>::THREADS, Form<D>::CTAS) rows_kernel(c
 }
 
 // Grid (runs of JOIN / 32 rows, kv heads, requests): joins the parts of split keys.  A warp has a row.
-constexpr int JOIN = 256, PER_TILE = ROWS / (JOIN / 32), MOST_SPLITS = 16;
+constexpr int JOIN = 256, PER_TILE = ROWS / (JOIN / 32), MOST_SPLITS = 32;       // (a lane of the join each)
 __global__ void __launch_bounds__(JOIN) join_kernel(const Params p, int D) {
   pdl_trigger();
   pdl_wait();
@@ -433,9 +444,6 @@ EXPORT int vb_rows_fp4(const void* q, const void* cache, int64_t num_blocks, con
   p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.splits = splits; p.window = window; p.bf16 = dtype == DT_BF16;
   p.scale_log2 = scale * LOG2E;
   p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E; p.out_scale = out_scale;
-  p.shift = 0;
-  while (1 << p.shift < BS) ++p.shift;
-  if (1 << p.shift != BS) p.shift = -1;
   if ((int64_t)max_q * p.G > (1 << 30)) return -3;
   return go(p, D, dim3((max_q * p.G + ROWS - 1) / ROWS, Hkv, B), st);
 }

@@ -862,26 +862,29 @@ FP4_FEW_ROWS = 64                            # query rows (new tokens x query he
 
 def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int) -> tuple[int, bool]:
     """(new tokens up to which a request takes the kernel of single tokens, whether the others' prompts go straight from the cache or through 16-bit pages), for T
-    tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: the kernel of single tokens 2.6 TB/s of the cache for every 24
-    query rows (16 where heads are above 128); the one of prompts 235 TFLOP/s; through pages 4.5 TB/s of 16-bit values, then a walk from key to key that is not split, or 800 TFLOP/s of heads of 128, a
-    power of two for each kv head.  Measured with 2 requests, 16 / 4 heads, in this order: of 64, 40 new tokens behind 12 000 31, 38, 202; 160 there 83, 68, 121; 320 there
-    156, 138, 124; 500 there 239, 201, 193; 160 behind 1200 23, 26, 34; 640 there 60, 44, 42; of 128, 80 behind 12 000 70, 84, 180; 160 there 123, 151, 119; of 192, 160 behind 4000 80, 84."""
+    tokens of B requests of up to ``longest`` new tokens and ``rows`` rows, by what each costs in us: launches; for the kernel of single tokens every key for every 24
+    query rows (16 where heads are above 128); for the one of prompts 290 TFLOP/s of tiles of 128 query rows; through pages 4.5 TB/s of 16-bit values, then a walk from key
+    to key that is not split, or 700 TFLOP/s of heads of 128, a power of two for each kv head.  The rates are fitted to 600 shapes that were timed all three ways
+    (heads of 64, 128 and 192, 1 to 8 query heads a kv head, 1 to 6 requests of 24 to 800 new tokens behind 200 to 9000): the choice is 1.5% above the best of the three in
+    the mean, 32% at worst.  Of them, in this order, 2 requests, 4 kv heads, 4 query heads each: of 64, 24 behind 9000 23, 27, 135; 256 behind 700 30, 23, 34; of 128, 256 behind
+    200 34, 24, 19; of 192, 24 behind 9000 40, 49; 128 behind 200 20, 26."""
     base = max(1, FP4_FEW_ROWS // G)
     if longest <= base:
         return longest, True
-    pairs = T * H * max(rows - longest / 2, 1)
-    single = 6 + (T * G / (24 if D <= 128 else 16) + B) * rows * H * D * 1.125 / 2.6e6
-    straight = 10 + pairs * G * 4 * D / 235e6
+    keys = max(rows - longest / 2, 1)
+    single = 13 + (T * G / (24 if D <= 128 else 16) + B / 2) * (keys + 350) * H * (D + 26) / 2.75e6
+    straight = (13 if D <= 128 else 24) + min(rows, 1000) * 0.0035 + (T * G + 64 * B) * H * keys * 4 * (D + 4) / 290e6
     pages = float("inf")
     if D <= 128:
-        pages = 20 + B * rows * H * 1024 / 4.5e6 + max(rows * 0.0085, pairs * (1 << (G - 1).bit_length()) * 512 / 800e6)
-    few = longest if longest * G <= 1024 and single < min(straight, pages) else base
+        pages = 18 + B * rows * H * 1024 / 4.5e6 + max(rows * 0.0085, T * H * keys * (1 << (G - 1).bit_length()) * 512 / 700e6)
+    few = longest if longest * G <= 2048 and single < min(straight, pages) else base
     return few, straight < pages
 
 
 _rows_fp4 = _sig("vb_rows_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _f, _f, _f, _i, _vp)
 _rows_fp4_ctas = _sig("vb_rows_fp4_ctas", _i, ctypes.POINTER(_i))
 FP4_PART_BYTES = 1 << 28                     # of the parts of split keys
+FP4_PART_KEYS = 128                          # of a part, at least: parts of 512 took 20 to 30% more where a few tiles of rows see 500 to 2000 keys, and the same above 8000
 
 
 @functools.lru_cache(maxsize=None)
@@ -902,8 +905,8 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
         tiles = int((-(-new[new > few] * G // 128)).sum())
         if not tiles:
             return
-    # the keys are split where the SMs would hold twice as many CTAs, in parts of 512 or more
-    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // 512, 16, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
+    # the keys are split where the SMs would hold twice as many CTAs, in parts of FP4_PART_KEYS or more
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // FP4_PART_KEYS, 32, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
     ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=q.device)
     _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
                      _p(ws), B, T, max_q, Hq, H, D, BS, room, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
