@@ -183,3 +183,24 @@ def test_layers_that_write_their_own_caches_refuse(preset):
 def test_pages_that_are_no_multiple_of_16_refuse():
     with pytest.raises(ValueError, match="nvfp4"):
         make_llm("llama-tiny", kv_cache_dtype="nvfp4", load_format="dummy", block_size=8)
+
+
+def test_the_choice_of_kernel_looks_at_prompts_alone(monkeypatch):
+    """Single tokens beside a prompt, whatever their number and their lengths, do not move the choice for it where lengths are on the host."""
+    monkeypatch.setattr(cuda, "fp4_kernels", lambda T, B, longest, rows, H, G, D: (longest, (T, B, longest, rows)))
+
+    def asked(queries, lens, room, host=True):
+        cu = [sum(queries[:i]) for i in range(len(lens) + 1)]
+        md = types.SimpleNamespace(num_reqs=len(lens), max_seq_len=max(lens), host_lens=(cu, lens) if host else None)
+        return cuda._fp4_choice(md, max(queries), 4, cu[-1], room, 2, 128)
+
+    assert asked([400], [700], 1 << 20) == (400, (400, 1, 400, 700))
+    assert asked([1, 400, 1, 1], [90000, 700, 5, 800], 1 << 20) == (16, (400, 1, 400, 700))
+    assert asked([100, 300], [4000, 400], 1 << 20) == (300, (400, 2, 300, 1300)) and asked([100, 300], [4000, 400], 1000)[1][3] == 1000
+    assert asked([100, 300], [4000, 400], 5000, host=False) == (300, (400, 2, 300, 4000)) and asked([3, 2], [4000, 9], 5000) == (3, (5, 2, 3, 4000))
+
+
+def test_range_of_prompts():
+    import numpy as np
+    for new, few, want in (([1, 1, 40, 2, 90, 1], 4, (2, 3)), ([5], 4, (0, 1)), ([4, 4], 4, (0, 0)), ([], 0, (0, 0)), ([0, 0, 1], 0, (2, 1)), ([9, 1], 1, (0, 1))):
+        assert cuda._fp4_range(np.array(new, dtype=np.int64), few) == want

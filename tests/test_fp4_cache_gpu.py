@@ -521,3 +521,25 @@ def test_most_parts_and_most_rows(dtype, D, lens, queries, few):
     eps, u = (D / 8 + 16) * 2.0 ** -23 * terms + 8 * 2.0 ** -24 * 1.5 * terms + 2.0 ** -21, torch.finfo(dtype).eps / 2
     bound = u * want.abs() + (2.0 ** -11 + 2 * eps + 2.0 ** -13) * mass + max(lens) * 2.0 ** -31 * big + 2.0 ** -25
     assert ((out.double().cpu() - want).abs() <= bound).all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("D", [64, 128, 192])
+@pytest.mark.parametrize("lens,queries", [([300, 700, 5, 400, 90], [1, 150, 1, 90, 2]), ([40, 2100, 9], [1, 300, 3]), ([600, 30, 30], [500, 1, 1]), ([3, 7, 130], [1, 1, 130])])
+def test_prompts_among_single_tokens(dtype, D, lens, queries):
+    """Prompts first, last and in the middle, the kernels' grids over them alone; lengths on the host and not."""
+    for host in (True, False):
+        q, cache, md = step(lens, queries, 8, 2, D, 32, dtype, "cuda", seed=D, spread=2.0, host=host)
+        _check(q, cache, md, pages=D <= 128)
+        _check(q, cache, md, window=70, cap=20.0, sinks=torch.linspace(-2, 2, 8).cuda(), pages=D <= 128)
+
+
+def test_prompts_among_single_tokens_through_pages(monkeypatch):
+    """The same with every prompt through 16-bit pages, in one go and in several."""
+    cu = cuda_ops()
+    monkeypatch.setattr(cu, "fp4_kernels", lambda T, B, longest, rows, H, G, D: (min(longest, max(1, 64 // G)), False))
+    for most in (1 << 30, 1 << 19):
+        monkeypatch.setattr(cu, "FP4_PAGES_BYTES", most)
+        for D in (64, 128):
+            q, cache, md = step([300, 700, 5, 400, 90], [1, 150, 1, 90, 2], 6, 2, D, 32, torch.bfloat16, "cuda", seed=D, spread=2.0)
+            _check(q, cache, md, pages=True)

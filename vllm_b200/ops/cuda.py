@@ -881,6 +881,21 @@ def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int)
     return few, straight < pages
 
 
+def _fp4_choice(md, longest: int, G: int, T: int, room: int, H: int, D: int) -> tuple[int, bool]:
+    """fp4_kernels for the requests of a step that may take either kernel, with their rows in the mean over new tokens, where the step has its lengths on the host.  Beside
+    other requests they never take the kernel of single tokens, whose form for many rows would be the others' as well: 63 single tokens behind 1000 and 100 new tokens behind 500, 4
+    kv heads of 64, 31 us in two kernels and 49 in one (of 192, 49 and 58; 4 behind 20000 with a prompt of 128, 40 and 36).  Without lengths all requests count, with the longest's rows."""
+    lens = _host_lens(md) if longest * G > FP4_FEW_ROWS else None
+    if lens is not None:
+        base = max(1, FP4_FEW_ROWS // G)
+        either = lens[0] > base
+        new = lens[0][either]
+        if new.size:
+            few, straight = fp4_kernels(int(new.sum()), new.size, longest, min(int((new * lens[1][either]).sum() // new.sum()), room), H, G, D)
+            return (few if new.size == md.num_reqs else base), straight
+    return fp4_kernels(T, md.num_reqs, longest, min(md.max_seq_len, room), H, G, D)
+
+
 _rows_fp4 = _sig("vb_rows_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _f, _f, _f, _i, _vp)
 _rows_fp4_ctas = _sig("vb_rows_fp4_ctas", _i, ctypes.POINTER(_i))
 FP4_PART_BYTES = 1 << 28                     # of the parts of split keys
@@ -899,16 +914,19 @@ def _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, out, lse, sink
     (T, Hq, D), (blocks, _, H, BS, _) = q.shape, kv_cache.shape
     B, bt, G, max_q = md.num_reqs, md.block_table, Hq // kv_cache.shape[2], min(md.max_query_len, q.shape[0])
     room = bt.shape[1] * BS
-    tiles, lens = B * -(-max_q * G // 128), _host_lens(md)
+    b0, most, tiles, lens = 0, min(room, md.max_seq_len), B * -(-max_q * G // 128), _host_lens(md)
     if lens is not None:
-        new = lens[0]
-        tiles = int((-(-new[new > few] * G // 128)).sum())
-        if not tiles:
+        b0, B = _fp4_range(lens[0], few)
+        if not B:
             return
+        new, rows = (x[b0:b0 + B] for x in lens)
+        mine = new > few
+        tiles, max_q, most = int((-(-new[mine] * G // 128)).sum()), min(max_q, int(new.max())), min(room, int(rows[mine].max()))
     # the keys are split where the SMs would hold twice as many CTAs, in parts of FP4_PART_KEYS or more
-    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), min(room, md.max_seq_len) // FP4_PART_KEYS, 32, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
+    splits = max(1, min(fp4_rows_ctas(D) * num_sms() // (tiles * H), most // FP4_PART_KEYS, 32, FP4_PART_BYTES // (4 * T * Hq * (D + 2))))
     ws = None if splits == 1 else torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=q.device)
-    _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr(), md.seq_lens.data_ptr(), md.query_start_loc.data_ptr(), out.data_ptr(), _p(lse), _p(sinks),
+    _check(_rows_fp4(q.data_ptr(), kv_cache.data_ptr(), blocks, bt.data_ptr() + 4 * b0 * bt.stride(0), md.seq_lens.data_ptr() + 4 * b0, md.query_start_loc.data_ptr() + 4 * b0,
+                     out.data_ptr(), _p(lse), _p(sinks),
                      _p(ws), B, T, max_q, Hq, H, D, BS, room, few, q.stride(0), out.stride(0), bt.stride(0), splits, window or 0, scale, soft_cap, out_scale,
                      _DT[q.dtype], _st()), "rows_fp4", 1 if splits == 1 else 2)
 
@@ -924,6 +942,13 @@ def _host_lens(md):
         return None
     cu, sl = (np.asarray(x, dtype=np.int64) for x in lens)
     return np.diff(cu[:md.num_reqs + 1]), sl[:md.num_reqs]
+
+
+def _fp4_range(new, few: int) -> tuple[int, int]:
+    """(first request of more than ``few`` new tokens, how many from there to the last): a step has its prompts next to each other, and CTAs for the other requests, whose
+    number is that of the longest prompt, cost more than a prompt's work (63 single tokens behind 1000 beside 100 new tokens behind 500: 94 us, and 45 without them)."""
+    at = np.flatnonzero(new > few)
+    return (int(at[0]), int(at[-1] - at[0]) + 1) if at.size else (0, 0)
 
 
 def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[int, int, int, int]]:
@@ -975,11 +1000,14 @@ def _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, out, 
     vt = tc_attention_ok(W, W, q.shape[1] // H) and alibi is None
     PS = 32 if W == 256 else 64
     qsl, B = None if md.decode_only else md.query_start_loc, md.num_reqs
-    most = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS)
+    most, host = -(-min(md.max_seq_len, bt.shape[1] * BS) // PS), _host_lens(md)
     for b0, b1, total, longest in _fp4_runs(md, few, PS, most, 4 * H * PS * W):
-        n = b1 - b0
         if total == 0:                       # (none of them has more than `few`)
             continue
+        if host is not None and not md.decode_only:
+            first, n = _fp4_range(host[0][b0:b1], few)
+            b0, b1 = b0 + first, b0 + first + n
+        n = b1 - b0
         pages = torch.empty((total, 2, H, PS, W), dtype=q.dtype, device=q.device)
         table, lens = sl.new_empty((n, longest)), sl.new_empty(n)
         _check(_pages_fp4(kv_cache.data_ptr(), blocks, bt.data_ptr() + 4 * b0 * bt.stride(0), bt.stride(0), bt.shape[1], sl.data_ptr() + 4 * b0,
@@ -1036,15 +1064,15 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
     scale, out_scale = scale * k_scale, out_scale * v_scale
     direct = D in FP4_HEADS and alibi is None and not chunk and (causal or decode) and G <= 64 and not batch_invariant()
     if direct:
-        few, straight = (1, True) if longest == 1 else fp4_kernels(used, B, longest, min(md.max_seq_len, room), H, G, D)
+        few, straight = (1, True) if longest == 1 else _fp4_choice(md, longest, G, used, room, H, D)
     if B and few < longest:
         if direct and straight:
             _fp4_rows_attention(q, kv_cache, md, scale, window, soft_cap, to, lse, sinks, out_scale, few)
         else:
             _fp4_attention_pages(q, kv_cache, md, scale, window, soft_cap, causal, to, lse, alibi, sinks, chunk, out_scale, few, direct)
         lens = _host_lens(md)
-        if lens is not None and (lens[0] > few).all():
-            few = 0                          # (no request has so few)
+        if lens is not None:                 # as many as one of them has, if any: the kernel of single tokens has a form for each number
+            few = int(lens[0][lens[0] <= few].max(initial=0))
     if B and few:
         _fp4_few(q, kv_cache, md, H, D, BS, room, scale, window, soft_cap, to, lse, sinks, out_scale, few)
     if to is not out and out is not None:
