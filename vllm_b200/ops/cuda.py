@@ -761,12 +761,11 @@ def _fp4_half(x, kv_cache, op: str) -> int:
     return _DT[x.dtype]
 
 
-def _fp4_rows(x, width: int):
-    """Rows of ``width`` values next to each other, at 16-byte addresses."""
+def _fp4_rows(x):
+    """Rows of values next to each other, at 16-byte addresses."""
     if x.dim() == 3:
-        _, head, one = x.stride()
-        if one != 1 or head != x.shape[2]:
-            x = x.reshape(x.shape[0], width)
+        if x.stride(2) != 1 or x.stride(1) != x.shape[2]:
+            x = x.clone(memory_format=torch.contiguous_format)       # (a reshape may be a view whose values are still apart)
     elif x.stride(1) != 1:
         x = x.contiguous()
     return _heads(x)
@@ -777,13 +776,13 @@ def write_fp4(positions, axes, q, k, v, table, H: int, D: int, neox: bool, kv_ca
     T, dtype, blocks, BS = k.shape[0], _fp4_half(k, kv_cache, "write_fp4"), kv_cache.shape[0], kv_cache.shape[3]
     if not T:
         return q
-    k, v = _fp4_rows(k, H * D), _fp4_rows(v, H * D)
+    k, v = _fp4_rows(k), _fp4_rows(v)
     if positions is None:
         _check(_write_fp4(None, 0, 1, None, None, 0, 0, 1, None, k.data_ptr(), v.data_ptr(), T, 0, H, D, 0, k.stride(0), v.stride(0), kv_cache.data_ptr(), blocks, slots.data_ptr(),
                           BS, k_scale, v_scale, dtype, _st()), "write_fp4")
         return q
     (rows, rot), width = table.shape, q.shape[1]
-    turned = _fp4_rows(q, width)
+    turned = _fp4_rows(q)
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
     step, n = (0, 1) if axes is None else (positions.stride(0), positions.shape[0])
