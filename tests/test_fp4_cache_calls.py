@@ -1,4 +1,8 @@
 """A key-value cache in 4 bits: calls that its documentation allows, as far as they show without a device."""
+import random
+import types
+
+import numpy as np
 import pytest
 import torch
 
@@ -31,3 +35,39 @@ def test_rows_lie_as_the_kernel_reads_them(layout, H):
     assert rows.data_ptr() % 16 == 0 and step % 8 == 0
     assert rows.storage_offset() + (T - 1) * step + H * D <= rows.untyped_storage().nbytes() // 2
     assert torch.equal(rows.as_strided((T, H * D), (step, 1)), x.reshape(T, H * D))
+
+
+def _entry_takes(D, H, G, few, room):
+    """Limits of the kernel of single tokens (vb_attention_fp4): query rows of a request and a kv head, blocks of them in its grid, strips of a launch of one request."""
+    cols = 8 if few * G <= 8 else 16 if few * G <= 16 or D > 128 else 24
+    blocks = H * -(-few * G // cols)
+    return few * G <= 4096 and G <= 64 and blocks <= 65535 and blocks * (-(-room // 64) + cuda.FP4_EXTRA) < 1 << 29
+
+
+def _choice(queries, lens, room, H, G, D, host):
+    md = types.SimpleNamespace(num_reqs=len(lens), max_seq_len=max(lens), host_lens=(np.concatenate(([0], np.cumsum(queries))), np.array(lens)) if host else None)
+    return cuda._fp4_choice(md, max(queries), G, sum(queries), room, H, D)[0]
+
+
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("H,G,D,longest,others,each,rows,room", [(40, 1, 128, 1639, 31, 65, 9000, 10000), (32, 1, 128, 2048, 31, 65, 9000, 10000), (32, 4, 128, 512, 63, 17, 4000, 10000),
+                                                                  (1024, 1, 128, 1100, 63, 65, 9000, 10000), (64, 1, 128, 1500, 63, 65, 3000, 1 << 23)])
+def test_a_long_request_among_many_short_ones(H, G, D, longest, others, each, rows, room, host):
+    """Steps whose mean makes the kernel of single tokens the cheapest: its entry takes what the rule gives it."""
+    few = _choice([longest] + [each] * others, [rows] * (others + 1), room, H, G, D, host)
+    assert min(longest, max(1, 64 // G)) <= few <= longest and _entry_takes(D, H, G, few, room)
+    assert (few == longest) == (room == 10000 and H < 1024)                # (what it can take, it still gets)
+
+
+def test_the_rule_keeps_to_the_kernels_limits():
+    rng = random.Random(0)
+    asked = 0
+    for _ in range(5000):
+        H, G, D = rng.choice([1, 2, 8, 32, 40, 64, 128, 512, 2000]), rng.choice([1, 2, 4, 8, 16, 64]), rng.choice(cuda.FP4_HEADS)
+        longest, B, rows = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 7)), int(2 ** rng.uniform(0, 15))
+        queries = [longest, *(rng.randint(1, longest) for _ in range(B - 1))]
+        room = max(rows, int(2 ** rng.uniform(10, 20)))
+        few = _choice(queries, [max(rows, n) for n in queries], room, H, G, D, rng.random() < 0.5)
+        asked += few > max(1, 64 // G)
+        assert _entry_takes(D, H, G, few, room), (queries, H, G, D, few)
+    assert asked > 100                                   # (of steps that all take it)

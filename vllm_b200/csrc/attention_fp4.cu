@@ -868,9 +868,10 @@ EXPORT int vb_attention_fp4(const void* q, const void* cache, int64_t num_blocks
   if (parts > 0 && B > group) return -1;
   Params p;
   p.Hkv = Hkv; p.G = Hq / Hkv; p.BS = BS; p.max_rows = max_rows; p.few = few; p.extra = extra; p.parts = parts; p.window = window; p.bf16 = dtype == DT_BF16;
-  if ((int64_t)few * p.G > 4096 || p.G > 64 || (int64_t)Hkv * few * p.G > 65535) return -1;
+  if ((int64_t)few * p.G > 4096 || p.G > 64) return -1;
   const int nt = groups_of(D, few * p.G);
   p.chunks = (few * p.G + 8 * nt - 1) / (8 * nt);
+  if ((int64_t)Hkv * p.chunks > 65535) return -1;      // (a dimension of the grids)
   p.q_stride = q_stride; p.out_stride = out_stride; p.bt_stride = bt_stride; p.num_blocks = num_blocks; p.cache = (const uint8_t*)cache; p.sinks = sinks;
   p.scale_log2 = scale * LOG2E;
   p.ku = soft_cap > 0.f ? scale / soft_cap : 0.f; p.c2 = soft_cap * LOG2E; p.out_scale = out_scale;

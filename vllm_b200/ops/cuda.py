@@ -880,6 +880,13 @@ def fp4_kernels(T: int, B: int, longest: int, rows: int, H: int, G: int, D: int)
     return few, straight < pages
 
 
+def fp4_few_fits(few: int, room: int, H: int, G: int) -> bool:
+    """The kernel of single tokens takes requests of ``few`` new tokens in tables of ``room`` rows: blocks of 16 query rows or more of all kv heads are a dimension of its grid, and
+    numbers of their strips have 32 bits."""
+    blocks = H * -(-few * G // 16)
+    return blocks <= 65535 and blocks * (-(-room // 64) + FP4_EXTRA + 1) <= 1 << 29
+
+
 def _fp4_choice(md, longest: int, G: int, T: int, room: int, H: int, D: int) -> tuple[int, bool]:
     """fp4_kernels for the requests of a step that may take either kernel, with their rows in the mean over new tokens, where the step has its lengths on the host.  Beside
     other requests they never take the kernel of single tokens, whose form for many rows would be the others' as well: 63 single tokens behind 1000 and 100 new tokens behind 500, 4
@@ -891,8 +898,9 @@ def _fp4_choice(md, longest: int, G: int, T: int, room: int, H: int, D: int) -> 
         new = lens[0][either]
         if new.size:
             few, straight = fp4_kernels(int(new.sum()), new.size, longest, min(int((new * lens[1][either]).sum() // new.sum()), room), H, G, D)
-            return (few if new.size == md.num_reqs else base), straight
-    return fp4_kernels(T, md.num_reqs, longest, min(md.max_seq_len, room), H, G, D)
+            return (few if new.size == md.num_reqs and fp4_few_fits(few, room, H, G) else base), straight
+    few, straight = fp4_kernels(T, md.num_reqs, longest, min(md.max_seq_len, room), H, G, D)
+    return (few if few * G <= FP4_FEW_ROWS or fp4_few_fits(few, room, H, G) else max(1, FP4_FEW_ROWS // G)), straight
 
 
 _rows_fp4 = _sig("vb_rows_fp4", _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _f, _f, _f, _i, _vp)
