@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from vllm_b200 import envs, ops
 from vllm_b200.ops import cuda
 
 
@@ -71,3 +72,14 @@ def test_the_rule_keeps_to_the_kernels_limits():
         asked += few > max(1, 64 // G)
         assert _entry_takes(D, H, G, few, room), (queries, H, G, D, few)
     assert asked > 100                                   # (of steps that all take it)
+
+
+def test_decode_steps_in_batch_invariant_mode_are_not_captured(monkeypatch):
+    """They go through 16-bit pages, whose number depends on lengths that a captured step does not know."""
+    assert ops.fp4_decode_supported(128, 8, torch.bfloat16)
+    monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
+    envs._cache.clear()
+    assert cuda.batch_invariant() and not ops.fp4_decode_supported(128, 8, torch.bfloat16)
+    monkeypatch.undo()
+    envs._cache.clear()
+    assert ops.fp4_decode_supported(128, 8, torch.bfloat16)

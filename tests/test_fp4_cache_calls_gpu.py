@@ -4,7 +4,8 @@ import torch
 
 from tests.fp4_oracle import attend, step
 from tests.test_fp4_cache_calls import LAYOUTS
-from vllm_b200 import ops
+from tests.test_fp4_cache_gpu import _llm
+from vllm_b200 import envs, ops
 from vllm_b200.ops import cuda_ops
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +36,25 @@ def test_many_heads_and_a_long_request_in_one_kernel(Hkv, G, D, few):
     eps = (D / 8 + 16) * 2.0 ** -23 * terms + 8 * 2.0 ** -24 * 1.5 * terms + 2.0 ** -21
     bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2 * eps + 2.0 ** -13) * mass + 90 * 2.0 ** -31 * big + 2.0 ** -25
     assert ((out.double().cpu() - want).abs() <= bound).all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs()).all()
+
+
+def test_generation_in_batch_invariant_mode(monkeypatch):
+    """Runs without captured steps, and a request's tokens and log-probabilities are those that it has alone."""
+    from vllm_b200 import SamplingParams
+    monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
+    envs._cache.clear()
+    try:
+        llm, r = _llm("llama-small", kv_cache_dtype="nvfp4", max_num_batched_tokens=64, enable_prefix_caching=False)
+        assert not r.graphs and not r.mixed_graphs
+        sp = SamplingParams(max_tokens=8, temperature=0.0, ignore_eos=True, logprobs=0)
+        prompts = [{"prompt_token_ids": [(7 * i + j) % 4000 + 3 for j in range(20 + 41 * i)]} for i in range(4)]
+
+        def run(some):
+            return [(o.outputs[0].token_ids, [x.logprob for d in o.outputs[0].logprobs for x in d.values()]) for o in llm.generate(some, sp)]
+
+        together = run(prompts)
+        assert [run([p])[0] for p in prompts] == together
+        llm.shutdown()
+    finally:
+        monkeypatch.undo()
+        envs._cache.clear()

@@ -350,8 +350,10 @@ def _check_fp4(kv_cache, op: str, k_scale: float = 1.0, v_scale: float = 1.0) ->
 
 
 def fp4_decode_supported(D: int, G: int, dtype, other_masks: bool = False) -> bool:
-    """Decode steps of these heads go straight from a cache in 4 bits, without anything that depends on lengths on the host (and may be captured)."""
-    return dtype in _HALF and D in cuda_ops().FP4_HEADS and G <= 64 and not other_masks
+    """Decode steps of these heads go straight from a cache in 4 bits, without anything that depends on lengths on the host (and may be captured).  In batch-invariant mode they go
+    through 16-bit pages: a captured step would have to hold them for requests of the longest length that there may be."""
+    cu = cuda_ops()
+    return dtype in _HALF and D in cu.FP4_HEADS and G <= 64 and not other_masks and not cu.batch_invariant()
 
 
 def _check_slots(slot_mapping, T: int, kv_cache, op: str) -> None:
