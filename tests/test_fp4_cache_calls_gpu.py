@@ -58,3 +58,20 @@ def test_generation_in_batch_invariant_mode(monkeypatch):
     finally:
         monkeypatch.undo()
         envs._cache.clear()
+
+
+@pytest.mark.parametrize("queries", [[1], [40]])
+@pytest.mark.parametrize("odd", [1001, 1004])
+def test_queries_out_of_rows_of_any_width(queries, odd):
+    """One token's queries in a row whose width is no multiple of 16 bytes: their distance to the next row counts as contiguous."""
+    q, cache, md = step([300], queries, 6, 2, 64, 32, torch.bfloat16, "cuda", seed=9)
+    want, norm = ops.paged_attention_fp4(q, cache, md, 0.125, return_lse=True)
+    n = queries[0]
+    wide = torch.zeros(n + 1, odd, dtype=q.dtype, device="cuda")
+    wide[:n, :384] = q.flatten(1)
+    one = wide[:, :384].unflatten(1, (6, 64))[:n]
+    assert one.stride(0) == odd and one.is_contiguous() == (n == 1)
+    got, lse = ops.paged_attention_fp4(one, cache, md, 0.125, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(lse, norm)
+    out = torch.full_like(wide, 7.0)
+    assert torch.equal(ops.paged_attention_fp4(one, cache, md, 0.125, out=out[:, :384].unflatten(1, (6, 64))[:n]), want) and (out[:, 384:] == 7.0).all() and (out[n] == 7.0).all()

@@ -1057,11 +1057,11 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
         raise ValueError("paged_attention_fp4: block tables of all requests, a request's pages next to each other")
     if not decode:
         _query_offsets(md, dev)
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
         q = _q_heads(q)
     used, to = B if decode else md.num_actual_tokens, out
     if out is None or out.data_ptr() % 16 or out.stride(0) % 8:
-        to = torch.empty_like(q)
+        to = torch.empty_like(q, memory_format=torch.contiguous_format)
         if T > used:                         # (padding rows are written by no CTA: keep them finite)
             to[used:].zero_()
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
