@@ -75,3 +75,24 @@ def test_queries_out_of_rows_of_any_width(queries, odd):
     assert torch.equal(got, want) and torch.equal(lse, norm)
     out = torch.full_like(wide, 7.0)
     assert torch.equal(ops.paged_attention_fp4(one, cache, md, 0.125, out=out[:, :384].unflatten(1, (6, 64))[:n]), want) and (out[:, 384:] == 7.0).all() and (out[n] == 7.0).all()
+
+
+def test_one_row_is_read_into_rows_of_any_width():
+    """A row's distance to the next says nothing where there is one row; of more rows each has to lie at a 16-byte address."""
+    H, D, BS = 2, 64, 32
+    _, cache, md = step([300], [1], H, H, D, BS, torch.bfloat16, "cuda", seed=9)
+    kv = torch.full((2, 2, 133), 7.0, dtype=torch.bfloat16, device="cuda")
+    k, v = kv[0, :, :128].unflatten(1, (H, D)), torch.empty(2, H, D, dtype=torch.bfloat16, device="cuda")
+    cu, first = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1], [299]))
+    ops.gather_cache_fp4(cache, md.block_table, cu, k[:1], v[:1], 1, first)
+    want = [torch.empty(1, H, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.gather_cache_fp4(cache, md.block_table, cu, *want, 1, first)
+    assert torch.equal(k[:1], want[0]) and torch.equal(v[:1], want[1]) and (kv[0, 0, 128:] == 7.0).all() and (kv[0, 1] == 7.0).all()
+    with pytest.raises(ValueError):
+        ops.gather_cache_fp4(cache, md.block_table, cu, k, v, 1, first)
+    _, cache, md = step([300], [1], 1, 1, D, BS, torch.bfloat16, "cuda", seed=9)
+    heads_first = [torch.empty(1, 2, D, dtype=torch.bfloat16, device="cuda").transpose(0, 1) for _ in range(2)]              # one head
+    want = [torch.empty(2, 1, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for got in (heads_first, want):
+        ops.gather_cache_fp4(cache, md.block_table, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), *got, 2)
+    assert all(torch.equal(a, b) for a, b in zip(heads_first, want))

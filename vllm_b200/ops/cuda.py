@@ -796,7 +796,9 @@ def write_fp4(positions, axes, q, k, v, table, H: int, D: int, neox: bool, kv_ca
 def gather_fp4(kv_cache, block_table, cu, k, v, H: int, D: int, max_tokens: int, starts, k_scale: float, v_scale: float) -> None:
     dtype = _fp4_half(k, kv_cache, "gather_cache_fp4")
     (kr, kh, ke), (vr, vh, ve), (br, be) = k.stride(), v.stride(), block_table.stride()
-    if ke != 1 or ve != 1 or kh != D or vh != D or kr % 8 or vr % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+    if k.shape[0] == 1:                      # (the distance to another row says nothing, nor that to another head)
+        kr = vr = H * D
+    if ke != 1 or ve != 1 or (H > 1 and (kh != D or vh != D)) or kr % 8 or vr % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
         raise ValueError("gather_cache_fp4: rows of k and v at 16-byte addresses, their heads next to each other")
     if be != 1:
         raise ValueError("gather_cache_fp4: a request's pages are next to each other in the block table")
