@@ -96,3 +96,17 @@ def test_one_row_is_read_into_rows_of_any_width():
     for got in (heads_first, want):
         ops.gather_cache_fp4(cache, md.block_table, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), *got, 2)
     assert all(torch.equal(a, b) for a, b in zip(heads_first, want))
+
+
+@pytest.mark.parametrize("D,Hq", [(128, 8), (192, 8), (48, 8)])
+@pytest.mark.parametrize("padding", [0, 3])
+def test_a_step_without_tokens(D, Hq, padding):
+    """Requests wait, none has new tokens; ``max_query_len`` is a bound."""
+    _, cache, md = step([40, 0], [0, 0], Hq, 2, D, 32, torch.bfloat16, "cuda")
+    md.decode_only = False
+    for md.max_query_len in (0, 1, 500):
+        q = torch.full((padding, Hq, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        got, lse = ops.paged_attention_fp4(q, cache, md, 1.0, return_lse=True)
+        assert got.shape == q.shape and lse.shape == (padding, Hq) and (got == 0).all()
+        out = torch.full_like(q, 7.0)
+        assert ops.paged_attention_fp4(q, cache, md, 1.0, out=out) is out and (out == 7.0).all()

@@ -1069,7 +1069,7 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
-    few, longest, G, room = 0, 1 if decode else md.max_query_len, Hq // H, width * BS
+    few, longest, G, room = 0, 1 if decode else md.max_query_len if used else 0, Hq // H, width * BS
     scale, out_scale = scale * k_scale, out_scale * v_scale
     direct = D in FP4_HEADS and alibi is None and not chunk and (causal or decode) and G <= 64 and not batch_invariant()
     if direct:
