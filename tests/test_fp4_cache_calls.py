@@ -83,3 +83,21 @@ def test_decode_steps_in_batch_invariant_mode_are_not_captured(monkeypatch):
     monkeypatch.undo()
     envs._cache.clear()
     assert ops.fp4_decode_supported(128, 8, torch.bfloat16)
+
+
+@pytest.mark.parametrize("axes", [False, True])
+def test_positions_outside_the_table(axes, device="cpu", dtype=torch.float32, rots=(16, 24)):
+    """They take its first or last row, whether the rotation is the kernel's (multiples of 16) or not."""
+    T, Hq, H, D, far = 4, 4, 2, 32, 9
+    for rot in rots:
+        g = torch.Generator().manual_seed(rot)
+        table = torch.randn(far, rot, generator=g).to(device)
+        of_pair = (torch.arange(rot // 2, dtype=torch.int32) % 2).to(device)
+        got = []
+        for positions in ([-3, 0, 8, 50], [0, 0, 8, 8]):
+            q, k, v = (torch.randn(T, n * D, generator=torch.Generator().manual_seed(n)).to(dtype).to(device) for n in (Hq, H, H))
+            at = torch.tensor(positions, device=device)
+            cache = torch.zeros(ops.fp4_cache_shape(1, H, 16, D), dtype=torch.uint8, device=device)
+            ops.rope_and_cache_fp4(torch.stack((at, at.flip(0))) if axes else at, q, k, v, table, D, True, cache, torch.arange(T, device=device), axes=of_pair if axes else None)
+            got.append((q, cache))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])

@@ -4,6 +4,7 @@ import torch
 
 from tests.fp4_oracle import attend, step
 from tests.test_fp4_cache_calls import LAYOUTS
+from tests.test_fp4_cache_calls import test_positions_outside_the_table as on_host
 from tests.test_fp4_cache_gpu import _llm
 from vllm_b200 import envs, ops
 from vllm_b200.ops import cuda_ops
@@ -110,3 +111,8 @@ def test_a_step_without_tokens(D, Hq, padding):
         assert got.shape == q.shape and lse.shape == (padding, Hq) and (got == 0).all()
         out = torch.full_like(q, 7.0)
         assert ops.paged_attention_fp4(q, cache, md, 1.0, out=out) is out and (out == 7.0).all()
+
+
+@pytest.mark.parametrize("axes", [False, True])
+def test_positions_outside_the_table(axes):
+    on_host(axes, "cuda", torch.bfloat16)

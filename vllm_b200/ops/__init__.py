@@ -381,7 +381,7 @@ def rope_and_cache_fp4(positions, q, k, v, cos_sin_cache, head_dim: int, is_neox
     """``rope_and_cache`` into a cache in 4 bits: q [T, heads * head_dim] is rotated in place (and returned), k rotated on its way into the cache and left as it is.
 
     ``positions`` [T], or [n, T] with ``axes`` [rot / 2] int32: a token has a position on each of n axes (time, height, width), and pair j of a head turns by that on
-    axis axes[j].  Rotated values are rounded to the type of q before they are quantised, as a cache of that type would hold them."""
+    axis axes[j].  A position outside the table [positions, rot] takes its first or last row.  Rotated values are rounded to the type of q before they are quantised, as a cache of that type would hold them."""
     op = "rope_and_cache_fp4"
     H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
     T, rot = q.shape[0], cos_sin_cache.shape[-1]
@@ -397,7 +397,8 @@ def rope_and_cache_fp4(positions, q, k, v, cos_sin_cache, head_dim: int, is_neox
     _check_slots(slot_mapping, T, kv_cache, op)
     if _use_cuda(q) and rot % 16 == 0 and q.dtype in _HALF:
         return cuda_ops().write_fp4(positions, axes, q, k, v, cos_sin_cache, H, D, is_neox, kv_cache, slot_mapping, k_scale, v_scale)
-    at, table = (positions[:T], cos_sin_cache) if axes is None else (torch.arange(T, device=q.device), ref.axes_table(positions[:, :T], cos_sin_cache, axes))
+    positions = positions[..., :T].clamp(0, cos_sin_cache.shape[0] - 1)              # (as in the kernel; indexing outside the table would fault the device)
+    at, table = (positions, cos_sin_cache) if axes is None else (torch.arange(T, device=q.device), ref.axes_table(positions, cos_sin_cache, axes))
     q2, k2 = ref.rotary_embedding(at, q, k, table, D, is_neox)
     q.copy_(q2)
     reshape_and_cache_fp4(k2.reshape(T, H, D), v.unflatten(1, (H, D)), kv_cache, slot_mapping, k_scale, v_scale)
