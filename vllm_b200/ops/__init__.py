@@ -432,9 +432,10 @@ def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft
     """``paged_attention`` over a cache in 4 bits; q [T, heads, head size] in 16 bits on the device, ``md.kv_vt`` False.  The output is that of the values
     which the cache stands for.
 
-    Requests of few new tokens are attended straight from the cache, whatever ``md.max_seq_len`` says.  Prompts may be read back to 16-bit pages first (up to 1 GiB of
-    them at a time, more for a request that needs more): ``md.max_query_len`` and, where the step has no lengths on the host, ``md.max_seq_len`` are then no smaller than
-    what they stand for."""
+    Requests of few new tokens are attended straight from the cache, whatever ``md.max_seq_len`` says, where ``fp4_decode_supported`` holds for the call.  All others, and prompts, may be
+    read back to 16-bit pages first (up to 1 GiB of them at a time, more for a request that needs more): ``md.max_query_len`` and, where the step has no lengths on the host,
+    ``md.max_seq_len`` are then no smaller than what they stand for, and a step that is captured has none on the host (``host_lens``, ``seq_lens_cpu``), as its kernels' grids and the
+    pages are sized by them."""
     op = "paged_attention_fp4"
     H, D = _check_fp4(kv_cache, op, k_scale, v_scale)
     shape = q.shape
