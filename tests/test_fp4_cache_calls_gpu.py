@@ -1,4 +1,6 @@
 """A key-value cache in 4 bits on the device: calls that its documentation allows beside the usual ones."""
+import math
+
 import pytest
 import torch
 
@@ -6,6 +8,7 @@ from tests.fp4_oracle import attend, step
 from tests.test_fp4_cache_calls import LAYOUTS
 from tests.test_fp4_cache_calls import test_positions_outside_the_table as on_host
 from tests.test_fp4_cache_gpu import _llm
+from tests.test_fp4_cache_models import count_axes, image_prompts, logprobs
 from vllm_b200 import envs, ops
 from vllm_b200.ops import cuda_ops
 
@@ -116,3 +119,27 @@ def test_a_step_without_tokens(D, Hq, padding):
 @pytest.mark.parametrize("axes", [False, True])
 def test_positions_outside_the_table(axes):
     on_host(axes, "cuda", torch.bfloat16)
+
+
+@pytest.mark.parametrize("model", ["gemma2-tiny", "gptoss-tiny", "qwen2vl-tiny", "qwen3moe-tiny", "bloom-tiny"])
+def test_families_take_a_cache_in_4_bits(model):
+    """Heads of 16 or 32, pages of 16: nothing to refuse."""
+    llm, r = _llm(model, kv_cache_dtype="nvfp4", max_model_len=256, max_num_batched_tokens=64, block_size=16, kv_cache_memory_bytes=32 << 20)
+    assert any(c.dtype == torch.uint8 for c in r.kv_caches.values())
+    llm.shutdown()
+
+
+@pytest.mark.parametrize("preset", ["qwen2vl-tiny", "qwen3vl-tiny", "qwen35vl-tiny"])
+def test_an_image_turns_keys_by_three_axes(monkeypatch, preset):
+    """Beside a text in a step, then single tokens; text alone in front of it gives the tokens that it has without the image."""
+    from vllm_b200 import SamplingParams
+    calls = count_axes(monkeypatch)
+    llm, _ = _llm(preset, kv_cache_dtype="nvfp4", max_model_len=256, max_num_batched_tokens=64, block_size=16, kv_cache_memory_bytes=32 << 20, hf_overrides={"min_pixels": 32 * 32}, enable_prefix_caching=False)
+    sp = SamplingParams(max_tokens=4, temperature=0.0, ignore_eos=True, logprobs=0)
+    image, text = image_prompts()
+    outs = llm.generate([image, text], sp)
+    assert 3 in calls and all(len(x) == 4 and all(map(math.isfinite, x)) for x in logprobs(outs))
+    calls.clear()
+    alone = llm.generate([text], sp)
+    assert 3 not in calls and max(abs(a - b) for a, b in zip(logprobs(alone)[0], logprobs(outs)[1])) < 0.05       # (some steps of bf16 in the logits, below 4)
+    llm.shutdown()
