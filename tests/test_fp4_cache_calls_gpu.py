@@ -143,3 +143,11 @@ def test_an_image_turns_keys_by_three_axes(monkeypatch, preset):
     alone = llm.generate([text], sp)
     assert 3 not in calls and max(abs(a - b) for a, b in zip(logprobs(alone)[0], logprobs(outs)[1])) < 0.05       # (some steps of bf16 in the logits, below 4)
     llm.shutdown()
+
+
+def test_refused_offsets_name_the_call():
+    q, cache, md = step([40, 90], [3, 70], 8, 2, 64, 32, torch.bfloat16, "cuda")
+    good = md.query_start_loc
+    for md.query_start_loc in (None, good.long(), good[:2], good.cpu(), good.repeat_interleave(2)[::2]):
+        with pytest.raises(ValueError, match="paged_attention_fp4"):
+            ops.paged_attention_fp4(q, cache, md, 1.0)

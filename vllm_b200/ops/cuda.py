@@ -668,10 +668,10 @@ def key_weights(q, kv_cache, md, scale, lse, scores, soft_cap: float = 0.0, last
     return _add_weights(q, kv_cache, md, scale, lse.contiguous(), scores, soft_cap, last, pages)
 
 
-def _query_offsets(md, device: int):
+def _query_offsets(md, device: int, op: str = "key weights"):
     qsl = md.query_start_loc
     if qsl is None or qsl.dtype is not _I32 or not qsl.is_contiguous() or qsl.get_device() != device or qsl.numel() <= md.num_reqs:
-        raise ValueError("key weights: int32 query offsets of all requests, on the device")
+        raise ValueError(f"{op}: int32 query offsets of all requests, on the device")
     return qsl
 
 
@@ -1058,7 +1058,7 @@ def paged_attention_fp4(q, kv_cache, md, H: int, D: int, scale, window=None, sof
     if n < B or bt.stride(1) != 1:
         raise ValueError("paged_attention_fp4: block tables of all requests, a request's pages next to each other")
     if not decode:
-        _query_offsets(md, dev)
+        _query_offsets(md, dev, "paged_attention_fp4")
     if not q.is_contiguous() or q.data_ptr() % 16 or q.stride(0) % 8:
         q = _q_heads(q)
     used, to = B if decode else md.num_actual_tokens, out
