@@ -18,8 +18,8 @@
 // such parts where the result is fp16.  Sums are in 32 bits.
 //
 // What bounds it: 9 / 16 of a byte a value would be 5.9 TB/s of codes at the rate of a 16-bit copy; turning them into operands takes about 160 instructions of the integer pipe for 16
-// keys and their values of 128, which is 27 us of two requests of 95000 beside 33.5 of their bytes; the two together with the matrix and exponential pipes leave 49.4 (74 % of the
-// copy's rate without the 5 of the join).  Three CTAs of 168 registers keep the pipes busier than four of 128 (49.4 to 54.4).  64 requests of 700 to 1301 take 26.4 (bytes 11.4): 13 at that
+// keys and their values of 128, which is 27 us of two requests of 95000 beside 33.5 of their bytes.  They take 49.4 (74 % of the copy's rate without the 5 of the join): the integer pipe is
+// busy in 55 % of the cycles and instructions issue in 60 %, so what is left are the waits of a strip's chain (copy, conversion, product, exponential, product), which 12 warps do not cover.  Three CTAs of 168 registers keep the pipes busier than four of 128 (49.4 to 54.4).  64 requests of 700 to 1301 take 26.4 (bytes 11.4): 13 at that
 // rate, 4 for the join, the rest for the chain at a CTA's start (lengths, pages, keys) and for ends of rows; one of 700 5.7; 24 of 60 to 924 with 16 / 8 heads of 64, capped, with
 // sinks and a window, 9.4.  A tcgen05 product would want the codes in shared memory as fp16 first: as many conversions, and their stores.
 #include "attention_prompt.cuh"
@@ -390,7 +390,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) attention_kernel(const Params p
     convert_q();
     const int seg_end = min(row.end, t1) * PER_TILE, n = req.n, tile0 = req.first_tile(p), low = req.first_key(p);
     float o[KD][NT][4], m_run[NT][2], l_run[NT][2];
-    bool huge = false;                       // products of scores and their factor have to be rounded before a reference is taken off: its rounding is above 1
+    // a reference of 2^20 or more: products of scores and their factor are rounded before it is taken off, as the reference was.  What a fused subtraction would keep of them, up to 1/16
+    // there, grows with them, and as an exponent becomes a weight of its own
+    bool huge = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

@@ -13,7 +13,9 @@
 //
 // Where there are fewer CTAs than the SMs hold, the keys are split and a second kernel joins the parts.
 //
-// It is bound by the legacy matrix instructions (560 TFLOP/s at most) and by how few warps the registers leave: 220 to 240 TFLOP/s for heads of 64 to 192, 173 for 256.  us for two
+// It is bound by how few warps the registers leave, 8 on an SM: the matrix pipe, whose legacy instructions would give 560 TFLOP/s, is busy in 46 % of the cycles for heads of 64 and 35 %
+// for 256, and instructions issue in 35 and 21 %.  A warp that has issued waits for the latency of its own instruction (64: 2.3 of 5.3 cycles an instruction) or for shared memory (256:
+// 3.2 of 9.3).  220 to 240 TFLOP/s for heads of 64 to 192, 173 for 256.  us for two
 // prompts of 2000 behind 1500, 20 / 4 heads of 64, 80, 96, 128, 192, 256: 206, 282, 310, 394, 575, 1063 (64 keys at a time; 32: 224, 282, 310, 416, 575, 1063, and 64 for 96 357); heads of
 // up to 128 read back to 16-bit pages of 128 take 204 to 209 there on the tcgen05 kernel and are better off here only in short portions (fp4_kernels in ops/cuda.py).  256 rows of a CTA
 // share the keys' conversion but wait for one another: 251 where 128 took 226 (500 new tokens behind 11 500, 16 / 4 heads of 64, now 204).

@@ -8,7 +8,8 @@
 // Read: rows of requests one after the other, or (for the attention kernels over 16-bit pages) as pages of a workspace.
 //
 // Both are bound by the bytes they move: cached rows of 64 requests of 700 to 1301, 8 heads of 128, 60 us (bytes 51, 5.6 TB/s); a prompt of 8000 with 32 / 8 heads of
-// 128 44 us for the write (173 MB, 3.9 TB/s; queries, which only turn, are three quarters of it, and its 27 M instructions of a warp issue 55 % of the time) and 12 for the read.
+// 128 44 us for the write (173 MB, 3.9 TB/s; 47 where nothing is in L2) and 12 for the read.  Queries, which only turn, are three quarters of the write's bytes; its 30.7 M instructions of
+// a warp issue in 63 % of the cycles, the integer pipe is busy in 41 %, and the 64 registers of four blocks an SM spill some: no one thing bounds it.
 #include "fp4.cuh"
 
 namespace {
@@ -384,7 +385,10 @@ EXPORT int vb_write_fp4(const int64_t* positions, int64_t pos_stride, int n_axes
   if (bad_shape(D, BS, dtype) || Hkv < 1 || rot < 0 || rot > D || rot % 16 || (rot && (!positions || !table || table_rows < 1 || n_axes < 1))) return -1;
   const Turn turn{positions, pos_stride, axes, table, table_rows, rot, n_axes};
   const int items = max(2 * Hkv * (D / 16), rot ? Hq * (rot / (neox ? 2 * N : N)) : 0), threads = min(256, (items + 31) / 32 * 32);
-  const int tokens = T >= 4096 ? 2 : 1;          // of a block: the SMs hold 592 blocks
+  // tokens of a block: two halve the waits for angles, but need many blocks to fill the SMs, which hold 592.  us with 1 and 2 of them (4), 2000, 4000, 5331, 8000 and 16000 tokens: 32 / 8
+  // heads of 128 14.5 and 13.4 (14.2), 25.8 and 24.5, 34.9 and 31.8 (34.0), 55.0 and 47.4 (47.0), 105 and 90 (85); 12 / 12 of 128 on three axes 12.1 and 12.7, 21.6 and 20.7, 28.8 and 26.6,
+  // 44.9 and 39.8, 87 and 76; 16 / 4 of 64 6.1 and 9.6, 9.9 and 10.8, 12.8 and 13.2, 17.8 and 17.1, 33.3 and 31.2; 1000 tokens 8.2 and 8.2, 7.9 and 8.8, 5.5 and 8.9
+  const int tokens = T >= 4096 ? 2 : 1;
   DISPATCH_HALF(dtype, TT, {
     auto kernel = rot == 0 ? write_kernel<TT, 0, 0> : !neox ? write_kernel<TT, 2, 0> : rot == 128 && D == 128 ? write_kernel<TT, 1, 128> : write_kernel<TT, 1, 0>;
     vb_launch(kernel, dim3((T + tokens - 1) / tokens), dim3(threads), (size_t)tokens * rot * 4, st, (TT*)q, (const TT*)k, (const TT*)v, turn, Hq, Hkv, D, q_stride, k_stride, v_stride,

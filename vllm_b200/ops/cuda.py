@@ -826,7 +826,11 @@ def fp4_plan(device: int, D: int, rows: int, parts: int) -> tuple[int, int, int]
 def fp4_parts(rows: int, tiles: int, D: int, query_rows: int) -> int:
     """CTAs of a cluster that has a row of the schedule, where rows have few tiles and the clusters run at a time; 0: equal runs and a second kernel.  us with 8, 4, 2, 1 and 0,
     heads of 128: 8 rows of 700 6.4, 6.7, 7.7, 9.5, 7.6; 32 of 2000 10.1, 9.9, 13.6, 21.0, 12.1; 64 of 2000 17.7, 13.4, 13.6, 21.1, 13.5; 512 of 250 71, 34, 22, 15.5, 18.8; 512 of
-    1000 85, 48, 36, 32, 32; of 64, 192 of 60 to 924 21, 16, 11.6, 12.4, 12.8."""
+    1000 85, 48, 36, 32, 32; of 64, 192 of 60 to 924 21, 16, 11.6, 12.4, 12.8.  Where the bounds lie, rows of one length, heads of 128, us: 8 CTAs and runs, 8 rows of 80, 96 and 128 tiles 9.7
+    and 11.7, 10.5 and 11.8, 12.1 and 13.0; 24 rows 11.7 and 13.3, 12.8 and 13.8, 15.1 and 15.0; 4 CTAs and runs, 64 rows of 40, 48 and 64 tiles 13.6 and 14.4, 15.0 and 15.0, 18.0 and 16.8; 2
+    and runs, 160 rows of 20, 24 and 40 tiles 13.9 and 16.0, 15.7 and 17.5, 21.8 and 21.5; 8 and 4 CTAs of 64 rows (8 x 64 is above three CTAs an SM) of 8 tiles 13.5 and 7.7; 1 and runs, 384 rows
+    of 8, 12, 24, 48 and 64 tiles 12.3 and 17.0, 15.6 and 24.0, 25.2 and 28.4, 44.0 and 44.9, 55.3 and 55.1 (one length, which suits a CTA a row best).  Over the 262 such shapes that were timed the
+    choice is 4% above the best of the five in the mean, 54% at worst (384 rows of 12 tiles)."""
     query_rows, sms = min(query_rows, 17), num_sms()
     for parts in (8, 4, 2):
         if parts // 2 < tiles <= 10 * parts and rows * parts <= 3 * sms and rows <= fp4_plan(_device(), D, query_rows, parts)[2]:
