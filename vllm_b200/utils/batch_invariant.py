@@ -51,8 +51,11 @@ def apply_env_overrides() -> bool:
         return False
     for k, v in _NCCL.items():
         os.environ[k] = v
-    os.environ.setdefault("CUBLAS_WORKSPACE_CONFIG", ":4096:8")
     import torch
+    # a process that has used the device may have workspaces of the size that held until now, and later calls would take them for as large as the variable then says: products would
+    # write behind them.  (The workspaces that torch hands to the library are of a fixed size per stream either way.)
+    if not torch.cuda.is_initialized():
+        os.environ.setdefault("CUBLAS_WORKSPACE_CONFIG", ":4096:8")
     torch.backends.cuda.matmul.allow_tf32 = False
     torch.backends.cudnn.allow_tf32 = False
     torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
