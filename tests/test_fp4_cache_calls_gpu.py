@@ -1,5 +1,9 @@
 """A key-value cache in 4 bits on the device: calls that its documentation allows beside the usual ones."""
 import math
+import os
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -9,7 +13,7 @@ from tests.test_fp4_cache_calls import LAYOUTS
 from tests.test_fp4_cache_calls import test_positions_outside_the_table as on_host
 from tests.test_fp4_cache_gpu import _llm
 from tests.test_fp4_cache_models import count_axes, image_prompts, logprobs
-from vllm_b200 import envs, ops
+from vllm_b200 import ops
 from vllm_b200.ops import cuda_ops
 
 pytestmark = pytest.mark.gpu
@@ -42,26 +46,27 @@ def test_many_heads_and_a_long_request_in_one_kernel(Hkv, G, D, few):
     assert ((out.double().cpu() - want).abs() <= bound).all() and ((lse.double().cpu() - norm).abs() <= eps + 2.0 ** -20 + 2.0 ** -22 * norm.abs()).all()
 
 
-def test_generation_in_batch_invariant_mode(monkeypatch):
-    """Runs without captured steps, and a request's tokens and log-probabilities are those that it has alone."""
+def invariant_generation():
     from vllm_b200 import SamplingParams
-    monkeypatch.setenv("VLLM_BATCH_INVARIANT", "1")
-    envs._cache.clear()
-    try:
-        llm, r = _llm("llama-small", kv_cache_dtype="nvfp4", max_num_batched_tokens=64, enable_prefix_caching=False)
-        assert not r.graphs and not r.mixed_graphs
-        sp = SamplingParams(max_tokens=8, temperature=0.0, ignore_eos=True, logprobs=0)
-        prompts = [{"prompt_token_ids": [(7 * i + j) % 4000 + 3 for j in range(20 + 41 * i)]} for i in range(4)]
+    llm, r = _llm("llama-small", kv_cache_dtype="nvfp4", max_num_batched_tokens=64, enable_prefix_caching=False)
+    assert cuda_ops().batch_invariant() and not r.graphs and not r.mixed_graphs
+    sp = SamplingParams(max_tokens=8, temperature=0.0, ignore_eos=True, logprobs=0)
+    prompts = [{"prompt_token_ids": [(7 * i + j) % 4000 + 3 for j in range(20 + 41 * i)]} for i in range(4)]
 
-        def run(some):
-            return [(o.outputs[0].token_ids, [x.logprob for d in o.outputs[0].logprobs for x in d.values()]) for o in llm.generate(some, sp)]
+    def run(some):
+        return [(o.outputs[0].token_ids, [x.logprob for d in o.outputs[0].logprobs for x in d.values()]) for o in llm.generate(some, sp)]
 
-        together = run(prompts)
-        assert [run([p])[0] for p in prompts] == together
-        llm.shutdown()
-    finally:
-        monkeypatch.undo()
-        envs._cache.clear()
+    together = run(prompts)
+    assert [run([p])[0] for p in prompts] == together
+    llm.shutdown()
+    print("as alone")
+
+
+def test_generation_in_batch_invariant_mode():
+    """Runs without captured steps, and a request's tokens and log-probabilities are those that it has alone.  (A process of its own: the mode changes settings of the whole process.)"""
+    got = subprocess.run([sys.executable, "-c", f"import {__name__} as t; t.invariant_generation()"], env={**os.environ, "VLLM_BATCH_INVARIANT": "1"}, capture_output=True, text=True,
+                         timeout=300, cwd=pathlib.Path(__file__).parents[1])
+    assert got.returncode == 0 and "as alone" in got.stdout, got.stdout[-2000:] + got.stderr[-2000:]
 
 
 @pytest.mark.parametrize("queries", [[1], [40]])
