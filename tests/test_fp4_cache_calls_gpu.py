@@ -11,6 +11,7 @@ import torch
 from tests.fp4_oracle import attend, step
 from tests.test_fp4_cache_calls import LAYOUTS
 from tests.test_fp4_cache_calls import test_positions_outside_the_table as on_host
+from tests.test_fp4_cache_gpu import _check as check
 from tests.test_fp4_cache_gpu import _llm
 from tests.test_fp4_cache_models import count_axes, image_prompts, logprobs
 from vllm_b200 import ops
@@ -156,3 +157,21 @@ def test_refused_offsets_name_the_call():
     for md.query_start_loc in (None, good.long(), good[:2], good.cpu(), good.repeat_interleave(2)[::2]):
         with pytest.raises(ValueError, match="paged_attention_fp4"):
             ops.paged_attention_fp4(q, cache, md, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries", [[1, 1, 1, 1], [3, 1, 40, 5]])
+@pytest.mark.parametrize("Hq,Hkv,D,kw", [(4, 2, 128, {}), (6, 2, 64, {}), (4, 2, 192, {}), (4, 2, 48, {}), (3, 1, 160, {"window": 64}), (8, 2, 512, {"cap": 5.0}), (80, 1, 128, {}), (80, 1, 16, {}),
+                                         (4, 2, 128, {"alibi_slopes": 1}), (4, 2, 96, {"alibi_slopes": 1}), (4, 2, 128, {"chunk_size": 32}), (6, 2, 64, {"chunk_size": 32}),
+                                         (4, 2, 128, {"causal": False}), (4, 2, 80, {"causal": False}), (32, 2, 64, {"causal": False})])
+def test_rows_without_keys(dtype, queries, Hq, Hkv, D, kw):
+    """Requests with no rows in the cache, or fewer than new tokens: rows in front of the cache's first see no key (all of them where the mask is not causal), whatever was in memory."""
+    if "alibi_slopes" in kw:
+        kw = {"alibi_slopes": torch.linspace(0.01, 0.2, Hq).cuda()}
+    for host in (True, False):
+        for sinks in (None, torch.randn(Hq).cuda()):
+            q, cache, md = step([0, 70, 33, 2], queries, Hq, Hkv, D, 32, dtype, "cuda", seed=D, spread=2.0, host=host)
+            for x in [torch.full(q.shape, math.nan, dtype=dtype, device="cuda"), torch.full(q.shape[:2], math.nan, device="cuda")]:
+                del x                        # (what an allocation without values finds next)
+            got = check(q, cache, md, sinks=sinks, pages=True, **kw)
+            assert (got[:queries[0]] == 0).all()

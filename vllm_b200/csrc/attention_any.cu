@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(WARPS * 32) any_attn_kernel(const Params p) {
       float x = s[j] * p.scale_log2;
       if (p.soft_cap > 0.f) x = p.soft_cap * tanhf(x / (LOG2E * p.soft_cap)) * LOG2E;
       if (p.alibi) x += p.alibi[head[j]] * LOG2E * (float)(kpos - qpos[j]);
-      bool ok = qpos[j] >= 0 && lane < nk;
+      bool ok = lane < nk;
       if (p.causal) ok = ok && kpos <= qpos[j];
       if (p.window > 0) ok = ok && kpos > qpos[j] - p.window && (p.causal || kpos < qpos[j] + p.window);
       if (p.chunk > 0) ok = ok && qpos[j] >= 0 && kpos / p.chunk == qpos[j] / p.chunk;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(WARPS * 32) any_attn_kernel(const Params p) {
   }
 #pragma unroll
   for (int j = 0; j < RPW; ++j) {
-    if (qpos[j] < 0) continue;
+    if (w * RPW + j >= n_rows) continue;         // (a row in front of the cache's first has its zeros written, too)
     float sum = warp_sum(l[j]);
     float top = m[j];
     if (p.sinks) top = fmaxf(top, p.sinks[head[j]] * LOG2E);

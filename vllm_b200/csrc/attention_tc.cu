@@ -129,11 +129,20 @@ fmha_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
   const int n_pages_total = (kv_end + BS - 1) / BS;   // pages that hold valid tokens
 
   if (n_tiles == 0) {
-    // nothing to attend to (can happen for empty splits): emit a neutral partial
-    if (p.num_splits > 1 && (int)threadIdx.x < p.G * n_tok) {
-      const int64_t pi = ((int64_t)(q0 + tok0 + threadIdx.x / p.G) * p.Hq + (h * p.G + threadIdx.x % p.G)) * p.num_splits + split;
-      for (int d = 0; d < D; ++d) p.part_out[pi * D + d] = 0.f;
-      p.part_lse[pi] = -INFINITY;
+    // nothing to attend to (an empty split, a request without keys for these rows): a neutral partial, or zeros
+    if (p.num_splits > 1) {
+      if ((int)threadIdx.x < p.G * n_tok) {
+        const int64_t pi = ((int64_t)(q0 + tok0 + threadIdx.x / p.G) * p.Hq + (h * p.G + threadIdx.x % p.G)) * p.num_splits + split;
+        for (int d = 0; d < D; ++d) p.part_out[pi * D + d] = 0.f;
+        p.part_lse[pi] = -INFINITY;
+      }
+      return;
+    }
+    for (int i = threadIdx.x; i < n_tok * p.G * (D / 8); i += NUM_THREADS) {
+      const int r = i / (D / 8), hq = h * p.G + r % p.G;
+      const int64_t tok = q0 + tok0 + r / p.G;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + tok * p.out_stride + (int64_t)hq * D + i % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+      if (i % (D / 8) == 0 && p.lse_out) p.lse_out[tok * p.Hq + hq] = p.sinks ? p.sinks[hq] : -INFINITY;
     }
     return;
   }
