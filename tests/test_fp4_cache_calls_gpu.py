@@ -175,3 +175,43 @@ def test_rows_without_keys(dtype, queries, Hq, Hkv, D, kw):
                 del x                        # (what an allocation without values finds next)
             got = check(q, cache, md, sinks=sinks, pages=True, **kw)
             assert (got[:queries[0]] == 0).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (192, torch.bfloat16), (48, torch.bfloat16)])
+@pytest.mark.parametrize("window", [1, 63, 64, 65, 700])
+def test_windows_far_shorter_than_the_cache(D, dtype, window):
+    q, cache, md = step([20000, 7001, 20000, 9000], [100, 30, 3, 1], 2, 1, D, 64, dtype, "cuda", seed=window, spread=2.0)
+    check(q, cache, md, window=window, pages=True)
+
+
+@pytest.mark.parametrize("queries", [[1, 1, 1], [5, 4, 5], [100, 1, 90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 48])
+def test_the_same_call_gives_the_same_bits(D, queries):
+    q, cache, md = step([3000, 90, 1000], queries, 8, 2, D, 32, torch.bfloat16, "cuda", seed=D, spread=2.0)
+    first = ops.paged_attention_fp4(q, cache, md, D ** -0.5, return_lse=True)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(ops.paged_attention_fp4(q, cache, md, D ** -0.5, return_lse=True), first))
+
+
+@pytest.mark.parametrize("D,Hq", [(64, 6), (128, 8), (192, 4), (48, 4)])
+@pytest.mark.parametrize("path", ["rule", "straight", "pages", "few"])
+def test_a_captured_step_of_prompts_follows_its_lengths(monkeypatch, D, Hq, path):
+    """Without lengths on the host a step may be captured: replayed with other lengths and other new tokens of each request it gives what an eager call does."""
+    if path != "rule":
+        few = {"straight": 8, "pages": 8, "few": 200}[path]
+        monkeypatch.setattr(cuda_ops(), "fp4_kernels", lambda T, B, longest, rows, H, G, D: (min(longest, few), path == "straight" or D > 128))
+    q, cache, md = step([700, 300, 900], [150, 1, 40], Hq, 2, D, 32, torch.bfloat16, "cuda", seed=D, spread=2.0, host=False)
+    md.max_query_len, md.max_seq_len = 200, 900
+    other = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 10, 190, 191], [60, 300, 33])]
+    ops.paged_attention_fp4(q, cache, md, 0.1)       # (what a first call sets up)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)
+    for qsl, lens in ((md.query_start_loc.clone(), md.seq_lens.clone()), other):
+        md.query_start_loc.copy_(qsl)
+        md.seq_lens.copy_(lens)
+        graph.replay()
+        want, norm = ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, norm)
+    check(q, cache, md, pages=True)
