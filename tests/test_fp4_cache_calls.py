@@ -6,8 +6,9 @@ import numpy as np
 import pytest
 import torch
 
+from tests.fp4_oracle import step
 from vllm_b200 import envs, ops
-from vllm_b200.ops import cuda
+from vllm_b200.ops import cuda, ref
 
 
 def _rnd(*shape):
@@ -101,3 +102,22 @@ def test_positions_outside_the_table(axes, device="cpu", dtype=torch.float32, ro
             ops.rope_and_cache_fp4(torch.stack((at, at.flip(0))) if axes else at, q, k, v, table, D, True, cache, torch.arange(T, device=device), axes=of_pair if axes else None)
             got.append((q, cache))
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_the_plain_form_takes_the_pages_of_the_step(monkeypatch):
+    """Not the whole cache, which would be seven times its bytes in 32 bits."""
+    q, cache, md = step([5, 40, 0, 33], [1, 3, 0, 33], 4, 2, 32, 16, torch.float32, "cpu", seed=3, spread=2.0)
+    want = ops.paged_attention_fp4(q, cache, md, 0.2)
+    many = torch.full((1000, *cache.shape[1:]), 127, dtype=torch.uint8)
+    places = torch.randperm(1000, generator=torch.Generator().manual_seed(0))[:cache.shape[0]]
+    many[places] = cache
+    seen, values_of = [], ref.fp4_cache_values
+    monkeypatch.setattr(ref, "fp4_cache_values", lambda kv, *a: seen.append(kv.shape[0]) or values_of(kv, *a))
+    table = md.block_table.clone()
+    md.block_table = places[table.long()].int()
+    assert torch.equal(ops.paged_attention_fp4(q, many, md, 0.2), want) and seen == [1 + 3 + 3]
+    for b, n in enumerate(md.seq_lens.tolist()):     # what stands behind a request's pages says nothing
+        md.block_table[b, -(-n // 16):] = -7
+    assert torch.equal(ops.paged_attention_fp4(q, many, md, 0.2), want)
+    md.seq_lens.zero_()                              # no pages at all
+    assert (ops.paged_attention_fp4(q, many, md, 0.2) == 0).all()

@@ -457,7 +457,8 @@ def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft
         qsl = torch.arange(md.num_reqs + 1)
     else:
         qsl = md.query_start_loc_cpu if md.query_start_loc_cpu is not None else md.query_start_loc.cpu()
-    o, lse = ref.paged_attention(q, ref.fp4_cache_values(kv_cache, k_scale, v_scale), md.block_table, sl, qsl, scale, causal=causal, sliding_window=sliding_window,
+    pages, table = ref.fp4_step_values(kv_cache, md.block_table, sl[:md.num_reqs], k_scale, v_scale)
+    o, lse = ref.paged_attention(q, pages, table, sl[:md.num_reqs], qsl, scale, causal=causal, sliding_window=sliding_window,
                                  logits_soft_cap=logits_soft_cap, alibi_slopes=alibi_slopes, sinks=sinks, chunk_size=chunk_size, return_lse=True)
     if out_scale != 1.0:
         o = o * out_scale

@@ -181,6 +181,16 @@ def fp4_cache_values(kv_cache: torch.Tensor, k_scale: float = 1.0, v_scale: floa
     return torch.stack([fp4_rows(codes[:, i], scales[:, i], f) for i, f in enumerate((k_scale, v_scale))], dim=1)
 
 
+def fp4_step_values(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(the pages that requests of these lengths have, in 32 bits, the block table that says where each of them is): a whole cache would be seven times its bytes."""
+    bs, lens = kv_cache.shape[3], seq_lens.to(block_table.device)
+    there = torch.arange(block_table.shape[1], device=block_table.device) < ((lens + bs - 1) // bs)[:, None]
+    used, place = torch.unique(block_table[:len(lens)][there], return_inverse=True)
+    table = torch.zeros(there.shape, dtype=torch.long, device=block_table.device)
+    table[there] = place
+    return fp4_cache_values(kv_cache[used.long()], k_scale, v_scale), table
+
+
 def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: float = 1.0,
                           v_scale: float = 1.0) -> None:
     bs = kv_cache.shape[3]
