@@ -121,3 +121,16 @@ def test_the_plain_form_takes_the_pages_of_the_step(monkeypatch):
     assert torch.equal(ops.paged_attention_fp4(q, many, md, 0.2), want)
     md.seq_lens.zero_()                              # no pages at all
     assert (ops.paged_attention_fp4(q, many, md, 0.2) == 0).all()
+
+
+@pytest.mark.parametrize("queries", [[1, 1], [3, 2]])
+def test_rows_behind_the_last_token_stay_in_the_plain_form(queries):
+    """A bucket's padding is left as it is in a given output, and finite in a new one, as by the kernels."""
+    q, cache, md = step([5, 40], queries, 4, 2, 32, 16, torch.float32, "cpu", seed=3)
+    T = q.shape[0]
+    want = ops.paged_attention_fp4(q, cache, md, 0.2)
+    padded = torch.cat((q, torch.full((3, 4, 32), float("nan"))))
+    out = torch.full_like(padded, 7.0)
+    assert ops.paged_attention_fp4(padded, cache, md, 0.2, out=out) is out and torch.equal(out[:T], want) and (out[T:] == 7.0).all()
+    got = ops.paged_attention_fp4(padded, cache, md, 0.2, out_scale=0.5)
+    assert torch.equal(got[:T], want * 0.5) and (got[T:] == 0).all()

@@ -462,8 +462,12 @@ def paged_attention_fp4(q, kv_cache, md, scale, sliding_window=None, logits_soft
                                  logits_soft_cap=logits_soft_cap, alibi_slopes=alibi_slopes, sinks=sinks, chunk_size=chunk_size, return_lse=True)
     if out_scale != 1.0:
         o = o * out_scale
+    used = md.num_reqs if md.decode_only else md.num_actual_tokens
     if out is not None:
-        o = out.copy_(o)
+        out[:used] = o[:used]
+        o = out
+    else:
+        o[used:] = 0
     return (o, lse) if return_lse else o
 
 
