@@ -7,7 +7,9 @@ import pytest
 import torch
 
 from tests.fp4_oracle import step
+from tests.utils import make_llm
 from vllm_b200 import envs, ops
+from vllm_b200.layers.attention import attention_layers
 from vllm_b200.ops import cuda, ref
 
 
@@ -134,3 +136,18 @@ def test_rows_behind_the_last_token_stay_in_the_plain_form(queries):
     assert ops.paged_attention_fp4(padded, cache, md, 0.2, out=out) is out and torch.equal(out[:T], want) and (out[T:] == 7.0).all()
     got = ops.paged_attention_fp4(padded, cache, md, 0.2, out_scale=0.5)
     assert torch.equal(got[:T], want * 0.5) and (got[T:] == 0).all()
+
+
+def test_memory_of_a_step_is_kept_free():
+    """Of the budget of a device, for steps over a cache in 4 bits."""
+    for kvd in ("auto", "nvfp4"):
+        llm = make_llm("qwen3moe-tiny", kv_cache_dtype=kvd, load_format="dummy", max_num_seqs=3, max_model_len=200, max_num_batched_tokens=64)
+        runner = llm.llm_engine.engine_core.engine_core.model_executor.worker.runner
+        layer = next(iter(attention_layers().values()))
+        want = cuda.fp4_step_bytes(64, 3, 200, layer.num_heads, layer.num_kv_heads, layer.head_size) if kvd == "nvfp4" else 0
+        assert runner.cache_workspace_bytes() == want and want >= (cuda.FP4_PART_BYTES if want else 0)
+        llm.shutdown()
+    one = cuda.fp4_step_bytes(1, 1, 64, 1, 1, 128)
+    assert one == cuda.FP4_PART_BYTES + (64 << 20)                                                       # a page: below the parts
+    assert cuda.fp4_step_bytes(8192, 256, 131072, 32, 8, 128) == (1 << 30) + 8192 * 32 * 520 + (64 << 20)      # many requests: a gigabyte of pages at a time
+    assert cuda.fp4_step_bytes(8192, 1, 1 << 20, 32, 8, 128) == (1 << 32) + 8192 * 32 * 520 + (64 << 20)       # a long one: all of its own

@@ -215,3 +215,26 @@ def test_a_captured_step_of_prompts_follows_its_lengths(monkeypatch, D, Hq, path
         want, norm = ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)
         assert torch.equal(out, want) and torch.equal(lse, norm)
     check(q, cache, md, pages=True)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,lens,queries", [(6, 2, 64, [3000, 500], [900, 40]), (8, 2, 128, [30000], [700]), (4, 2, 256, [9000], [100]), (4, 2, 48, [4000, 4000], [1, 30]), (40, 1, 64, [900] * 30, [5] * 30),
+                                                   (5, 1, 96, [2000] * 9, [90] * 9)])
+@pytest.mark.parametrize("host", [True, False])
+def test_memory_of_a_step(monkeypatch, Hq, Hkv, D, lens, queries, host):
+    """What a call takes beside its outputs is within what the engine keeps free, whichever kernels it goes to."""
+    cu = cuda_ops()
+    q, cache, md = step(lens, queries, Hq, Hkv, D, 64, torch.bfloat16, "cuda", host=host)
+    for path in ("rule", "straight", "pages"):
+        if path != "rule":
+            monkeypatch.setattr(cu, "fp4_kernels", lambda T, B, longest, rows, H, G, D: (min(longest, 4), path == "straight" or D > 128))
+        for most in (1 << 30, 1 << 22):
+            monkeypatch.setattr(cu, "FP4_PAGES_BYTES", most)
+            out = torch.empty_like(q)
+            ops.paged_attention_fp4(q, cache, md, 0.1, out=out)
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            ops.paged_attention_fp4(q, cache, md, 0.1, out=out)
+            torch.cuda.synchronize()
+            # (beside 512 bytes for each allocation)
+            assert torch.cuda.max_memory_allocated() - before <= cu.fp4_step_bytes(q.shape[0], len(lens), max(lens), Hq, Hkv, D) + (1 << 16)

@@ -991,6 +991,15 @@ def _fp4_runs(md, few: int, PS: int, most: int, page_bytes: int) -> list[tuple[i
     return runs
 
 
+def fp4_step_bytes(tokens: int, requests: int, longest: int, Hq: int, H: int, D: int) -> int:
+    """Bytes that a call of paged_attention_fp4 takes beside its queries, outputs and cache at most, in steps of so many tokens of so many requests of up to ``longest`` rows: 16-bit
+    pages with widened queries, outputs and log-sum-exps, or parts of split keys or of rows."""
+    W, G = max(D, 128), 1 << (Hq // H - 1).bit_length()
+    one = 4 * H * W * (-(-longest // 64) * 64)
+    pages = min(max(FP4_PAGES_BYTES, one), requests * one) + tokens * H * G * (4 * W + 8)
+    return max(pages, FP4_PART_BYTES) + (64 << 20)
+
+
 def fit_rows(x, y, T: int, H: int) -> None:
     """The first T rows of x [., heads, D] to y [., more or fewer heads of each of the H kv heads, D2]: what x does not have is zeros."""
     (hx, dx), (hy, dy) = x.shape[1:], y.shape[1:]

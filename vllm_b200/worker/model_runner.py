@@ -34,7 +34,7 @@ from vllm_b200.config import VllmConfig
 from vllm_b200.core.kv_cache_manager import KVCacheConfig, KVCacheSpec
 from vllm_b200.core.sched_output import LogprobsTensors, ModelRunnerOutput, SchedulerOutput
 from vllm_b200.forward_context import AttentionMetadata, ForwardContext, set_forward_context
-from vllm_b200.layers.attention import attention_layers, clear_attention_layers, fp4_cache_spec
+from vllm_b200.layers.attention import Attention, attention_layers, clear_attention_layers, fp4_cache_spec
 from vllm_b200.logger import init_logger
 from vllm_b200.sample.sampler import RejectionSampler, Sampler, SamplingMetadata
 from vllm_b200.utils import cdiv
@@ -314,6 +314,14 @@ class ModelRunner:
                 raise ValueError(f"kv_cache_dtype nvfp4 takes models of 16 bits on the device, not {self.dtype}")
             return {name: fp4_cache_spec(attention_layers()[name], name, spec) for name, spec in specs.items()}
         return specs
+
+    def cache_workspace_bytes(self) -> int:
+        """Device memory that attention over the cache takes during a step, which a profiling run, without a cache, does not see."""
+        if self.cc.cache_dtype != "nvfp4":
+            return 0
+        from vllm_b200.ops import cuda_ops
+        return max((cuda_ops().fp4_step_bytes(self.max_num_tokens, self.max_num_reqs, self.max_model_len, layer.num_heads, layer.num_kv_heads, layer.head_size)
+                    for layer in attention_layers().values() if isinstance(layer, Attention)), default=0)
 
     def _kv_dtype(self) -> torch.dtype:
         cd = self.cc.cache_dtype

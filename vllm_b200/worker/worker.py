@@ -111,7 +111,7 @@ class Worker:
         non_torch = max((self.init_free_bytes - free) - torch.cuda.memory_reserved(self.device), 0)
         budget = min(int(total * cc.gpu_memory_utilization), self.init_free_bytes)
         graph_reserve = 0 if self.vllm_config.model_config.enforce_eager else (2 << 30)
-        avail = budget - peak_torch - non_torch - graph_reserve
+        avail = budget - peak_torch - non_torch - graph_reserve - self.runner.cache_workspace_bytes()
         gc.collect()
         torch.cuda.empty_cache()
         logger.info("memory: total %.1f GiB, budget %.1f, torch peak %.1f, non-torch %.1f → KV %.1f GiB",
