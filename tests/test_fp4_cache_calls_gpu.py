@@ -238,3 +238,38 @@ def test_memory_of_a_step(monkeypatch, Hq, Hkv, D, lens, queries, host):
             torch.cuda.synchronize()
             # (beside 512 bytes for each allocation)
             assert torch.cuda.max_memory_allocated() - before <= cu.fp4_step_bytes(q.shape[0], len(lens), max(lens), Hq, Hkv, D) + (1 << 16)
+
+
+CAPTURED_FIRST = """
+import torch
+from tests.fp4_oracle import step
+from vllm_b200 import ops
+runs = []
+for D, lens, queries in ((128, [70, 2000], [1, 1]), (64, [300] * 200, [1] * 200), (64, [400, 90], [5, 2]), (192, [700, 90], [300, 1]), (128, [700, 90], [300, 1]), (48, [70, 90], [1, 1])):
+    q, cache, md = step(lens, queries, 8, 2, D, 32, torch.bfloat16, "cuda", host=False)
+    runs.append((q, cache, md, D))
+k = torch.randn(6, 2, 64, device="cuda").bfloat16()
+to, slots, table = torch.zeros(ops.fp4_cache_shape(1, 2, 16, 64), dtype=torch.uint8, device="cuda"), torch.arange(6, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+cu = torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+
+def run():
+    out = [x for q, cache, md, D in runs for x in ops.paged_attention_fp4(q, cache, md, 0.1, return_lse=True)]
+    ops.reshape_and_cache_fp4(k, -k, to, slots)
+    back = [torch.empty_like(k) for _ in range(2)]
+    ops.gather_cache_fp4(to, table, cu, *back, 6)
+    return out + back
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in got]
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+"""
+
+
+def test_first_calls_in_a_capture():
+    """Before anything has run on the device."""
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], capture_output=True, text=True, timeout=300, cwd=pathlib.Path(__file__).parents[1])
+    assert r.returncode == 0, r.stderr[-2000:]
